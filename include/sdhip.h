@@ -263,6 +263,73 @@ int sd_op_attention(const void* big, int stride, const void* qw, const void* kw,
                     int HK, int HD, int RD, void* Q, void* Kc, void* Vt, int ctx, void* out, void* stream, char* err,
                     size_t errlen);
 
+/* ---- a K/V cache in pages, shared by many requests (no counterpart in the reference, whose cache holds
+ * one sequence): sd_op_page_plan gives a step's new tokens their pages, sd_op_paged_prep writes their keys
+ * and values there, sd_op_paged_attention lets their queries attend them.
+ *
+ * A page holds page_size cache rows (a power of two from 32) of all kv heads, in the blocks of 32 rows of
+ * sd_op_attention's caches: K page [HK][page_size/32][HD/32][32 rows][32 dims], V page, transposed,
+ * [HK][page_size/32][HD][32].  Page p starts page_stride elements after page p - 1 (0: back to back; else a
+ * multiple of 8).  Row j of request b lies in page table[b][j / page_size] (i32) at row j % page_size; its
+ * slot is page * page_size + j % page_size.  A table entry outside [0, n_pages) is a hole: nothing reads or
+ * writes its rows.  n_pages * page_size and max_blocks * page_size stay below 2^31.
+ *
+ * These calls allocate nothing, wait for nothing and keep nothing: they may be captured, and calls on
+ * several streams or threads run at once where they share no output and no workspace.  All counts, tables
+ * and lengths are device arrays of i32, read when the kernels run; what they hold cannot make a kernel
+ * leave the given buffers.  The buffers belong to the calling thread's current device. ---- */
+
+/* Types of the rows and caches below. */
+enum { SD_F16 = 0, SD_BF16 = 1 };
+
+/* Pages and rows of one step, from lengths: request b of B (at most 8192) has lens[b] tokens in its pages
+ * and brings news[b] more (0: none).  Requests are admitted in order until one does not fit: all admitted
+ * rows together at most T, new pages at most the free ones, a request's pages at most max_blocks, no count
+ * negative; that one and all behind it get nothing.  free_pages [n_pages] holds the free pages' numbers in
+ * its first *n_free entries, a stack: new pages are taken from its end on, request by request.
+ *   table   [B][max_blocks]: the entries of new pages are written, the others left as they are
+ *   cu      [B + 1]: request b's rows are cu[b] .. cu[b + 1] - 1
+ *   kv_lens [B]: lens[b] plus the admitted new tokens (the next step's lens)
+ *   slots   [T], pos [T]: each row's slot and its position in its request; -1 and 0 behind the last row,
+ *           the slot -1 also where the page's number is out of range
+ *   status  [4]: requests admitted, rows, pages taken, free pages left (the next step's n_free)
+ * No output may overlap an input or another output. */
+int sd_op_page_plan(const void* lens, const void* news, int B, int T, int page_size, int n_pages, const void* free_pages,
+                    const void* n_free, void* table, int max_blocks, void* cu, void* kv_lens, void* slots, void* pos,
+                    void* status, void* stream, char* err, size_t errlen);
+
+/* q and k RMSNorm, rotation and the cache write of T rows big [T][stride] (a multiple of 8, 16-byte aligned):
+ * HQ query heads of HD (64, 128 or 256), each followed by its HD gates when `gated` (sd_op_attention's
+ * layout), then HK key and HK value heads.  q and k become x rsqrt(mean(x^2) + 1e-6) w (qw, kw [HD] f32;
+ * both null: no norm), then dims j and j + RD/2 (j < RD/2, RD even, 0 for none) turn by the angle whose
+ * cosine and sine are rope[p][j] (f32 pairs, [rope_len][RD/2][2]), p = pos[a][t] the row's position on pair
+ * j's axis a = pair_axis[j] (u8; null with one axis), pos [axes][T] (1 to 4 axes: time, height and width of
+ * an image's patches, say).  Positions outside the table take its nearest row, axes past the last the last.
+ * All in f32, rounded once: q to Q [T][HQ][HD], k and v to their rows' slots.  A row whose slot is outside
+ * [0, n_pages * page_size) is passed over (Q too); two rows of one slot give either's values. */
+int sd_op_paged_prep(const void* big, int stride, int gated, const void* qw, const void* kw, const void* rope, int rope_len,
+                     const void* pos, int axes, const void* pair_axis, const void* slots, int T, int HQ, int HK, int HD,
+                     int RD, int page_size, int n_pages, size_t page_stride, void* Q, void* Kp, void* Vp, int type,
+                     void* stream, char* err, size_t errlen);
+
+/* Workspace of an sd_op_paged_attention call with these sizes, in bytes (0: none). */
+int sd_op_paged_attention_ws(int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, size_t* bytes, char* err,
+                             size_t errlen);
+
+/* Causal attention of every request's new rows over its pages: row t = cu[b] + i of request b with n =
+ * cu[b + 1] - cu[b] rows has position p = kv_lens[b] - n + i and sees the cache rows j <= p, with a window
+ * (> 0) those above p - window, holes left out.  out [T][HQ*HD] = softmax(scale q . k) v over the seen rows
+ * of kv head h / (HQ/HK), in f32, times sigmoid(gate) when big (rows as in sd_op_paged_prep, gated) is
+ * given; zeros where no row is seen or every seen score is -inf.  Values in rows that are not seen, NaN and
+ * infinities among them, change nothing.  Rows of out outside every request are left as they are.
+ * max_new and max_kv are upper bounds of n and kv_lens that the launch is made for (rows and keys past them
+ * are left out).  ws holds what sd_op_paged_attention_ws says, 16-byte aligned, and is free again when the
+ * call's kernels have run: calls that may overlap, captured graphs among them, need one each. */
+int sd_op_paged_attention(const void* Q, const void* big, int stride, const void* Kp, const void* Vp, const void* table,
+                          int max_blocks, const void* cu, const void* kv_lens, int B, int T, int max_new, int max_kv, int HQ,
+                          int HK, int HD, int page_size, int n_pages, size_t page_stride, int window, float scale, void* out,
+                          void* ws, size_t ws_bytes, int type, void* stream, char* err, size_t errlen);
+
 /* No counterpart in the reference (a test hook for per-layer parity): the forward of ids from cache
  * (nullable) run step by step; after every residual add + RMSNorm of the layers (each layer's
  * in_norm, then its post_norm) the residual x (f32) and the normalized h (f16 bits) of rows[0..n_rows)

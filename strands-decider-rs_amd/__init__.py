@@ -30,7 +30,8 @@ SYMBOLS = [
     "sd_ask_ids", "sd_op_matmul", "sd_op_gdn", "sd_engine_forward_batch", "sd_engine_ask_batch",
     "sd_op_repack_w4", "sd_decode_scale_codes", "sd_op_matmul_fmt", "sd_op_matmul_split", "sd_op_gate_up_silu",
     "sd_op_embed", "sd_op_add_norm", "sd_op_silu_mul", "sd_op_add_bias", "sd_op_conv", "sd_op_gnorm",
-    "sd_op_attention", "sd_engine_trace", "sd_op_matmul_noalloc",
+    "sd_op_attention", "sd_engine_trace", "sd_op_matmul_noalloc", "sd_op_page_plan", "sd_op_paged_prep",
+    "sd_op_paged_attention_ws", "sd_op_paged_attention",
 ]
 VOID_SYMBOLS = ("sd_engine_free", "sd_snapshot_free", "sd_head_free", "sd_engine_hidden_size", "sd_engine_adapter",
                 "sd_snapshot_len")
@@ -115,6 +116,12 @@ def lib():
         L.sd_op_attention.argtypes = [vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp, vp, err, sz]
         L.sd_engine_trace.argtypes = [vp, vp, sz, vp, vp, sz, vp, vp, sz, C.POINTER(sz), err, sz]
         L.sd_op_matmul_noalloc.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp, err, sz]
+        L.sd_op_page_plan.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, err, sz]
+        L.sd_op_paged_prep.argtypes = [vp, i32, i32, vp, vp, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, i32, sz,
+                                       vp, vp, vp, i32, vp, err, sz]
+        L.sd_op_paged_attention_ws.argtypes = [i32, i32, i32, i32, i32, i32, i32, C.POINTER(sz), err, sz]
+        L.sd_op_paged_attention.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32,
+                                            sz, i32, C.c_float, vp, vp, sz, i32, vp, err, sz]
         for name in SYMBOLS:
             if name not in VOID_SYMBOLS:
                 getattr(L, name).restype = i32
@@ -477,6 +484,41 @@ def op_matmul_noalloc(A, Wq, Sc, Y, M, N, K, exact=False, stream=None):
     """sd_op_matmul_noalloc: sd_op_matmul (engine plan, pre-packed weights) with no device allocation."""
     _call(lib().sd_op_matmul_noalloc, C.c_void_p(A), C.c_void_p(Wq), C.c_void_p(Sc), C.c_void_p(Y), M, N, K,
           int(exact), _sp(stream))
+
+
+# ---- a K/V cache in pages, shared by many requests ------------------------------------------------
+
+F16, BF16 = 0, 1  # the rows' and caches' type
+
+
+def op_page_plan(lens, news, B, T, page_size, n_pages, free_pages, n_free, table, max_blocks, cu, kv_lens, slots, pos,
+                 status, stream=None):
+    """sd_op_page_plan: the pages and rows of a step's new tokens, from the requests' lengths."""
+    _call(lib().sd_op_page_plan, lens, news, B, T, page_size, n_pages, free_pages, n_free, table, max_blocks, cu, kv_lens,
+          slots, pos, status, stream)
+
+
+def op_paged_prep(big, stride, gated, qw, kw, rope, rope_len, pos, axes, pair_axis, slots, T, HQ, HK, HD, RD, page_size,
+                  n_pages, Q, Kp, Vp, type, page_stride=0, stream=None):
+    """sd_op_paged_prep: q and k norm, rotary positions of one or several axes, K and V into their slots."""
+    _call(lib().sd_op_paged_prep, big, stride, int(gated), qw, kw, rope, rope_len, pos, axes, pair_axis, slots, T, HQ, HK,
+          HD, RD, page_size, n_pages, page_stride, Q, Kp, Vp, type, stream)
+
+
+def paged_attention_ws(B, T, max_new, max_kv, HQ, HK, HD) -> int:
+    """sd_op_paged_attention_ws: bytes of the workspace of an op_paged_attention call with these sizes."""
+    n = C.c_size_t()
+    _call(lib().sd_op_paged_attention_ws, B, T, max_new, max_kv, HQ, HK, HD, C.byref(n))
+    return n.value
+
+
+def op_paged_attention(Q, big, stride, Kp, Vp, table, max_blocks, cu, kv_lens, B, T, max_new, max_kv, HQ, HK, HD, page_size,
+                       n_pages, out, ws, ws_bytes, type, window=0, scale=None, page_stride=0, stream=None):
+    """sd_op_paged_attention: the new rows' attention over their requests' pages (scale None: 1/sqrt(HD); big None:
+    no gates)."""
+    _call(lib().sd_op_paged_attention, Q, big, stride, Kp, Vp, table, max_blocks, cu, kv_lens, B, T, max_new, max_kv, HQ,
+          HK, HD, page_size, n_pages, page_stride, window, HD ** -0.5 if scale is None else scale, out, ws, ws_bytes, type,
+          stream)
 
 
 # ---- achievable-peak microbenchmarks (libsdpeak.so, include/sdpeak.h; used by bench.py) ----------

@@ -592,6 +592,147 @@ int sd_op_attention(const void* big, int stride, const void* qw, const void* kw,
     });
 }
 
+namespace {
+
+bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The checks that the paged entry points share: page geometry, and (HK > 0) heads, type and page stride.
+sd::PagedShape paged_shape(const std::string& who, int HQ, int HK, int HD, int page_size, int n_pages, size_t page_stride,
+                           int type) {
+    if (page_size < 32 || (page_size & (page_size - 1))) throw sd::Error(who + ": the page size must be a power of two from 32");
+    if (n_pages < 1 || (long long)n_pages * page_size > INT32_MAX)
+        throw sd::Error(who + ": need at least one page and fewer than 2^31 cache rows");
+    sd::PagedShape s{HQ, HK, HD, page_size, n_pages, page_stride, type == SD_BF16};
+    if (HQ < 1 || HK < 1 || HQ % HK || HQ > 1024) throw sd::Error(who + ": q heads (1 to 1024) must be a multiple of kv heads");
+    if (HD != 64 && HD != 128 && HD != 256) throw sd::Error(who + ": head_dim must be 64, 128 or 256");
+    if (type != SD_F16 && type != SD_BF16) throw sd::Error(who + ": the type must be SD_F16 or SD_BF16");
+    const size_t page = (size_t)HK * page_size * HD;
+    if (!page_stride) s.pstride = page;
+    else if (page_stride < page || page_stride % 8)
+        throw sd::Error(who + ": the page stride must be a multiple of 8 that holds a page (" + std::to_string(page) + " elements)");
+    return s;
+}
+
+void paged_attn_sizes(const std::string& who, int B, int T, int max_new, int max_kv, int HQ) {
+    if (B < 1 || B > sd::PAGE_PLAN_MAX_B) throw sd::Error(who + ": 1 to " + std::to_string(sd::PAGE_PLAN_MAX_B) + " requests");
+    if (T < 1 || (long long)T * HQ > INT32_MAX / 2) throw sd::Error(who + ": need at least one row, and rows * q heads below 2^30");
+    if (max_new < 1 || max_kv < 1) throw sd::Error(who + ": max_new and max_kv must be at least 1");
+}
+
+}  // namespace
+
+int sd_op_page_plan(const void* lens, const void* news, int B, int T, int page_size, int n_pages, const void* free_pages,
+                    const void* n_free, void* table, int max_blocks, void* cu, void* kv_lens, void* slots, void* pos,
+                    void* status, void* stream, char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_page_plan";
+        if (!lens || !news || !free_pages || !n_free || !table || !cu || !kv_lens || !slots || !pos || !status)
+            throw sd::Error(who + ": null argument");
+        paged_shape(who, 1, 1, 64, page_size, n_pages, 0, SD_F16);
+        if (B < 1 || B > sd::PAGE_PLAN_MAX_B) throw sd::Error(who + ": 1 to " + std::to_string(sd::PAGE_PLAN_MAX_B) + " requests");
+        if (T < 1 || T > (1 << 30)) throw sd::Error(who + ": 1 to 2^30 rows");
+        if (max_blocks < 1 || (long long)max_blocks * page_size > INT32_MAX)
+            throw sd::Error(who + ": a table row must hold at least one page and fewer than 2^31 cache rows");
+        const std::pair<const void*, size_t> in[] = {{lens, (size_t)B * 4}, {news, (size_t)B * 4},
+                                                     {free_pages, (size_t)n_pages * 4}, {n_free, 4}};
+        const std::pair<const void*, size_t> out[] = {{table, (size_t)B * max_blocks * 4}, {cu, (size_t)(B + 1) * 4},
+                                                      {kv_lens, (size_t)B * 4}, {slots, (size_t)T * 4},
+                                                      {pos, (size_t)T * 4}, {status, 16}};
+        for (const auto& i : in)
+            if (!aligned(i.first, 4)) throw sd::Error(who + ": the arrays must be aligned to 4 bytes");
+        for (size_t o = 0; o < 6; o++) {
+            if (!aligned(out[o].first, 4)) throw sd::Error(who + ": the arrays must be aligned to 4 bytes");
+            for (const auto& i : in)
+                if (overlap(i.first, i.second, out[o].first, out[o].second)) throw sd::Error(who + ": an output overlaps an input");
+            for (size_t q = 0; q < o; q++)
+                if (overlap(out[q].first, out[q].second, out[o].first, out[o].second)) throw sd::Error(who + ": two outputs overlap");
+        }
+        sd::page_plan({static_cast<const int*>(lens), static_cast<const int*>(news), B, T, page_size, n_pages,
+                       static_cast<const int*>(free_pages), static_cast<const int*>(n_free), static_cast<int*>(table),
+                       max_blocks, static_cast<int*>(cu), static_cast<int*>(kv_lens), static_cast<int*>(slots),
+                       static_cast<int*>(pos), static_cast<int*>(status)},
+                      static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_paged_prep(const void* big, int stride, int gated, const void* qw, const void* kw, const void* rope, int rope_len,
+                     const void* pos, int axes, const void* pair_axis, const void* slots, int T, int HQ, int HK, int HD,
+                     int RD, int page_size, int n_pages, size_t page_stride, void* Q, void* Kp, void* Vp, int type,
+                     void* stream, char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_paged_prep";
+        if (!big || !slots || !Q || !Kp || !Vp) throw sd::Error(who + ": null argument");
+        const sd::PagedShape s = paged_shape(who, HQ, HK, HD, page_size, n_pages, page_stride, type);
+        if (T < 1 || (long long)T * (HQ + 2 * HK) > INT32_MAX / 2)
+            throw sd::Error(who + ": need at least one row, and rows * heads below 2^30");
+        if (!qw != !kw) throw sd::Error(who + ": norm weights for both q and k, or for neither");
+        if (RD < 0 || RD % 2 || RD > HD) throw sd::Error(who + ": rotary_dim must be even and at most head_dim");
+        if (RD && (!rope || !pos || rope_len < 1)) throw sd::Error(who + ": a rotation needs the table and the positions");
+        if (axes < 1 || axes > 4) throw sd::Error(who + ": 1 to 4 position axes");
+        if (RD && axes > 1 && !pair_axis) throw sd::Error(who + ": several axes need each pair's axis");
+        const long long width = (long long)(gated ? 2 : 1) * HQ * HD + 2ll * HK * HD;
+        if (stride < width || stride % 8)
+            throw sd::Error(who + ": the row stride must be a multiple of 8 and at least " + std::to_string(width));
+        if (!aligned(big, 16) || !aligned(Q, 16) || !aligned(Kp, 16) || !aligned(Vp, 16))
+            throw sd::Error(who + ": big, Q and the caches must be aligned to 16 bytes");
+        if (!aligned(rope, 8) || !aligned(qw, 4) || !aligned(kw, 4) || !aligned(pos, 4) || !aligned(slots, 4))
+            throw sd::Error(who + ": the table must be aligned to 8 bytes, weights, positions and slots to 4");
+        sd::paged_prep(s, {big, stride, gated != 0, static_cast<const float*>(qw), static_cast<const float*>(kw),
+                           static_cast<const float*>(rope), rope_len, static_cast<const int*>(pos), axes,
+                           static_cast<const uint8_t*>(pair_axis), static_cast<const int*>(slots), T, RD, Q, Kp, Vp},
+                       static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_paged_attention_ws(int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, size_t* bytes, char* err,
+                             size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_paged_attention_ws";
+        if (!bytes) throw sd::Error(who + ": null argument");
+        const sd::PagedShape s = paged_shape(who, HQ, HK, HD, 32, 1, 0, SD_F16);
+        paged_attn_sizes(who, B, T, max_new, max_kv, HQ);
+        *bytes = sd::paged_attn_ws(s, B, T, max_new, max_kv);
+    });
+}
+
+int sd_op_paged_attention(const void* Q, const void* big, int stride, const void* Kp, const void* Vp, const void* table,
+                          int max_blocks, const void* cu, const void* kv_lens, int B, int T, int max_new, int max_kv, int HQ,
+                          int HK, int HD, int page_size, int n_pages, size_t page_stride, int window, float scale, void* out,
+                          void* ws, size_t ws_bytes, int type, void* stream, char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_paged_attention";
+        if (!Q || !Kp || !Vp || !table || !cu || !kv_lens || !out) throw sd::Error(who + ": null argument");
+        const sd::PagedShape s = paged_shape(who, HQ, HK, HD, page_size, n_pages, page_stride, type);
+        paged_attn_sizes(who, B, T, max_new, max_kv, HQ);
+        if (max_blocks < 1 || (long long)max_blocks * page_size > INT32_MAX)
+            throw sd::Error(who + ": a table row must hold at least one page and fewer than 2^31 cache rows");
+        if (max_kv > (long long)max_blocks * page_size) throw sd::Error(who + ": max_kv is more than a table row's pages hold");
+        if (window < 0) throw sd::Error(who + ": the window must be at least 1, or 0 for none");
+        if (!(scale > 0.f) || !std::isfinite(scale)) throw sd::Error(who + ": the scale must be positive and finite");
+        if (big && (stride < 2ll * HQ * HD || stride % 8))
+            throw sd::Error(who + ": the gates' row stride must be a multiple of 8 and at least 2 * q heads * head_dim");
+        for (const void* p : {Q, big, Kp, Vp, static_cast<const void*>(out), static_cast<const void*>(ws)})
+            if (!aligned(p, 16)) throw sd::Error(who + ": Q, big, the caches, out and ws must be aligned to 16 bytes");
+        if (!aligned(table, 4) || !aligned(cu, 4) || !aligned(kv_lens, 4))
+            throw sd::Error(who + ": table, cu and kv_lens must be aligned to 4 bytes");
+        const size_t rows = (size_t)T * HQ * HD * 2, need = sd::paged_attn_ws(s, B, T, max_new, max_kv);
+        if (overlap(out, rows, Q, rows)) throw sd::Error(who + ": out overlaps Q");
+        if (big && overlap(out, rows, big, ((size_t)(T - 1) * stride + 2 * (size_t)HQ * HD) * 2))
+            throw sd::Error(who + ": out overlaps the gates' rows");
+        if (need && (!ws || ws_bytes < need))
+            throw sd::Error(who + ": needs a workspace of " + std::to_string(need) + " bytes, got " +
+                            std::to_string(ws ? ws_bytes : 0));
+        sd::paged_attn(s, {Q, big, stride, Kp, Vp, static_cast<const int*>(table), max_blocks, static_cast<const int*>(cu),
+                           static_cast<const int*>(kv_lens), B, T, max_new, max_kv, window, scale, out, ws},
+                       static_cast<hipStream_t>(stream));
+    });
+}
+
 int sd_engine_trace(sd_engine* e, const uint32_t* ids, size_t n, const sd_snapshot* cache, const size_t* rows,
                     size_t n_rows, float* x_out, uint16_t* h_out, size_t cap, size_t* n_taps, char* err, size_t errlen) {
     return guarded(err, errlen, [&] {

@@ -261,4 +261,49 @@ void attention_split(const f16* Q, const f16* Kc, const f16* Vc, const f16* big,
                      const uint32_t* lu, const Segs& sg, const AttnPlan& p, float* ws, f16* out, hipStream_t st,
                      const float* qw = nullptr, const float* rope = nullptr);
 
+// ---- paged cache (paged.hip) -----------------------------------------------------------------
+// The entry points (capi.cpp) check every argument; the layouts are described there and in paged.hip.
+constexpr int PAGE_PLAN_MAX_B = 8192;  // requests of a plan: their prefix sums stay in LDS
+struct PagedShape {
+    int HQ, HK, HD, PS, n_pages;
+    size_t pstride;  // elements from a page to the next
+    bool bf16;       // else f16
+};
+struct PagePlan {
+    const int *lens, *news;
+    int B, T, PS, n_pages;
+    const int *free_pages, *n_free;
+    int* table;
+    int max_blocks;
+    int *cu, *kv_lens, *slots, *pos, *status;
+};
+void page_plan(const PagePlan& a, hipStream_t st);
+struct PagedPrep {
+    const void* big;
+    int stride;
+    bool gated;
+    const float *qw, *kw, *rope;
+    int rope_len;
+    const int* pos;
+    int axes;
+    const uint8_t* axis;
+    const int* slots;
+    int rows, RD;
+    void *Q, *Kp, *Vp;
+};
+void paged_prep(const PagedShape& s, const PagedPrep& a, hipStream_t st);
+struct PagedAttn {
+    const void *Q, *big;  // big: the rows whose gates scale the output, or null
+    int stride;
+    const void *Kp, *Vp;
+    const int* table;
+    int max_blocks;
+    const int *cu, *kv_lens;
+    int B, rows, max_new, max_kv, window;
+    float scale;
+    void *out, *ws;
+};
+size_t paged_attn_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv);
+void paged_attn(const PagedShape& s, const PagedAttn& a, hipStream_t st);
+
 }  // namespace sd
