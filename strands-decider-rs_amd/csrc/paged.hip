@@ -6,6 +6,7 @@
 // elements after page p - 1.  Row j of a request lies in page table[j / PS] at row j % PS; a table entry outside
 // [0, n_pages) is a hole, whose rows nothing reads or writes.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -285,56 +286,726 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------
+//
+// A kv head's rows are its request's (token, query head) pairs, token-major: row r is token r / G and head kh G + r % G,
+// G = HQ / HK, so that all query heads of a kv head share each key that is fetched.  Scores are S^T = K Q^T (keys x
+// rows) on MFMA with the keys of a 32-row block ordered so that S^T's accumulator layout is the B operand's of O^T +=
+// V^T P^T: probabilities never move between lanes, and both operands come out of the cache's blocks 16 bytes at a time.
+//
+// The online softmax is in base 2 and f32: p = 2^(c s - m + 8), c = scale log2(e), m the running maximum of c s.  P is
+// rounded to the rows' type before the second product (f32 sums; the row sum takes the unrounded values): half a step
+// of the type relative to each weight, as the result's own rounding.  The 8 puts f16's normal range at weights down to
+// 2^-22 of the largest (30000 keys of 2^-22 each are 0.7 % of a result); m is raised, and O and the sum rescaled, only
+// when a block's maximum exceeds it by more than 6, so p stays below 2^14 and most blocks rescale nothing.
+//
+// A masked product is 0 times the value, which is NaN where that is not finite.  Blocks that some row does not see
+// whole (the diagonal, a window's edge, the last block) look at their values first; where one is not finite, the
+// products take it as 0, and at the end the rows that see it add it, element by element (add_seen).
 
-// One wave per (row, q head), lanes over the dims, key after key.
-template <class T, int HD>
-__global__ __launch_bounds__(256) void k_paged_attn(const T* __restrict__ Q, const T* __restrict__ big, int stride,
-                                                    const T* __restrict__ Kp, const T* __restrict__ Vp,
-                                                    const int* __restrict__ table, int max_blocks,
-                                                    const int* __restrict__ cu, const int* __restrict__ kv_lens, int B,
-                                                    int rows, int HQ, int HK, int lps, int n_pages, size_t pstride,
-                                                    int window, float scale, T* __restrict__ out) {
-    constexpr int E = HD / 64;
-    const int lane = threadIdx.x & 63, unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = unit / HQ, h = unit % HQ, kh = h / (HQ / HK);
-    if (t >= rows || t >= cu[B]) return;
-    const int b = find_range(cu, B, t);
-    const int p = kv_lens[b] - (cu[b + 1] - t);  // the row's own position
-    const int last = min(p, (int)min((long long)max_blocks << lps, (long long)INT32_MAX) - 1);
-    float q[E], acc[E], m = -INFINITY, l = 0.f;
+// (left to itself the compiler keeps the larger lambdas as calls, and with them their captures in memory)
+#define INL __attribute__((always_inline))
+
+constexpr float P_UP = 8.0f, RAISE = 6.0f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <class T>
+struct Num;
+template <>
+struct Num<f16> {
+    static constexpr uint32_t EXP = 0x7C00;
+    static __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Num<bf16> {
+    static constexpr uint32_t EXP = 0x7F80;
+    typedef Vec8<bf16>::type B8;
+    static __device__ __forceinline__ f32x4 mfma16(B8 a, B8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(B8 a, B8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+// Nonzero where one of 8 values is not finite (its exponent's bits all set: one more carries into the sign's place).
+template <class T>
+__device__ __forceinline__ uint32_t not_finite(u32x4 v) {
+    constexpr uint32_t M = Num<T>::EXP * 0x10001u, A = (0x8000u - Num<T>::EXP) * 0x10001u;
+    uint32_t r = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) q[e] = (float)Q[((size_t)t * HQ + h) * HD + lane + 64 * e], acc[e] = 0.f;
-    for (int j = window > 0 ? max(0, p - window + 1) : 0; j <= last; j++) {
-        const int page = table[(size_t)b * max_blocks + (j >> lps)];
-        if (page < 0 || page >= n_pages) continue;
-        const int row = j & ((1 << lps) - 1);
-        const size_t at = (size_t)page * pstride + ((size_t)kh * (1 << (lps - 5)) + (row >> 5)) * (HD * 32);
-        float s = 0.f;
+    for (int i = 0; i < 4; i++) r |= (v[i] & M) + A;
+    return r & 0x80008000u;
+}
+// 8 values with 0 in the place of those that are not finite.
+template <class T>
+__device__ __forceinline__ u32x4 finite8(u32x4 v) {
+    constexpr uint32_t M = Num<T>::EXP * 0x10001u, A = (0x8000u - Num<T>::EXP) * 0x10001u;
+    u32x4 r;
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int d = lane + 64 * e;
-            s += q[e] * (float)Kp[at + (d / 32) * 1024 + (row & 31) * 32 + d % 32];
+    for (int i = 0; i < 4; i++) r[i] = v[i] & ~(((((v[i] & M) + A) & 0x80008000u) >> 15) * 0xFFFFu);
+    return r;
+}
+
+// One request's part in a launch, cut to the bounds that the launch is made for.
+struct Req {
+    int q0;        // its first row
+    int n;         // rows to do
+    int p0;        // position of its first row
+    int kcap;      // keys that may be read
+};
+__device__ __forceinline__ Req request(const int* __restrict__ cu, const int* __restrict__ kv_lens, int b, int rows,
+                                       int max_new, int kcap) {
+    const int a = cu[b], e = cu[b + 1], kv = max(kv_lens[b], -(1 << 30));
+    Req r;
+    r.q0 = min(max(a, 0), rows);
+    const int n = min(max(e, r.q0), rows) - r.q0;
+    r.n = min(n, max_new);
+    r.p0 = kv - n;
+    r.kcap = min(kcap, max(kv, 0));
+    return r;
+}
+
+// The launch's arguments that all attention kernels share.
+struct AttnArgs {
+    const int *table, *cu, *kv_lens;
+    int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, few, ks, span, stride;
+    float c;  // scale log2(e)
+    size_t pstride;
+};
+
+// Output of 4 dims of a row: unnormalised o over the sum l, times the gate's sigmoid, rounded once.
+template <class T>
+__device__ __forceinline__ void finish4(f32x4 o, float l, const T* gate, T* out) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const float inv = 1.0f / l;
+    float sg[4] = {1.f, 1.f, 1.f, 1.f};
+    if (gate) {
+        const T4 v = *reinterpret_cast<const T4*>(gate);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sg[e] = __builtin_amdgcn_rcpf(1.0f + exp2_fast((float)v[e] * -LOG2E));
+    }
+    T4 r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) r[e] = (T)((l == 0.f ? 0.f : o[e] * inv) * sg[e]);
+    *reinterpret_cast<T4*>(out) = r;
+}
+
+// ---- few rows: up to 16 NR rows per (request, kv head), one new token's heads or a short draft's ----
+//
+// Bound by the cache's bytes: each is read once and used for a handful of rows.  The keys are split over workgroups
+// (span blocks of 32 each) and inside one over its 4 waves, block by block; a wave loads a block's K and V straight
+// into registers in MFMA operand order, one block ahead of the one it works on.
+template <class T, int HD, int NR>
+__global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, const T* __restrict__ Kp,
+                                                   const T* __restrict__ Vp, AttnArgs a, const T* __restrict__ big,
+                                                   T* __restrict__ out, float* __restrict__ pacc,
+                                                   float* __restrict__ pml) {
+    typedef typename Vec8<T>::type T8;
+    constexpr int NS = HD / 32, ND = HD / 16, R = 16 * NR;
+    __shared__ float Om[4][R][HD + 4];
+    __shared__ float Mm[4][R], Lm[4][R];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int fq = lane & 15, fg = lane >> 4;
+    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
+    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    const int nrows = rq.n * a.G;
+    if (nrows == 0 || nrows > a.few) return;
+    // keys [lo, hi) are seen by some row; this workgroup's blocks of them
+    const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
+    const int blk0 = (lo >> 5) + z * a.span, blk1 = min((hi + 31) >> 5, blk0 + a.span);
+    const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + 3) >> 2 : 0;
+    int jlo[NR], jhi[NR];  // keys [jlo, jhi) are seen by this lane's row
+    T8 qf[NR][NS];
+#pragma unroll
+    for (int u = 0; u < NR; u++) {
+        const int r = min(16 * u + fq, nrows - 1), t = r / a.G, h = kh * a.G + r % a.G;
+        const int p = rq.p0 + t;
+        jlo[u] = a.window ? p - a.window + 1 : 0;
+        jhi[u] = min(p + 1, hi);
+        const T* q = Q + ((size_t)(rq.q0 + t) * a.HQ + h) * HD + 8 * fg;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[u][s] = *reinterpret_cast<const T8*>(q + 32 * s);
+    }
+    // blocks in [open0, open1) are seen whole by every row
+    const int open0 = a.window ? rq.p0 + rq.n - a.window : 0, open1 = min(rq.p0 + 1, hi);
+
+    const int lbpp = a.lps - 5;
+    const int* const tb = a.table + (size_t)b * a.max_blocks;
+    auto entries = [&](int i) {  // lane l: the table entry of the wave's block i + l
+        return tb[min((first + 4 * (i + lane)) >> lbpp, a.max_blocks - 1)];
+    };
+    int ids = cnt ? entries(0) : 0, ids2 = cnt > 64 ? entries(64) : 0;
+    const uint32_t kofs = ((8 * (fq >> 2) + (fq & 3)) * 32 + fg * 8) * 2, vofs = (fq * 32 + fg * 8) * 2;
+    f32x4 acc[NR][ND];
+    float m[NR], l[NR];
+#pragma unroll
+    for (int u = 0; u < NR; u++) {
+        m[u] = -INFINITY, l[u] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) acc[u][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bool rare = false;  // some value was taken as 0
+    struct Blk {
+        u32x4 k[2][NS], v[ND];
+        bool there;
+    };
+    auto load = [&](int i, Blk& x) {
+        const int page = __builtin_amdgcn_readlane(ids, i & 63), blk = first + 4 * i;
+        x.there = i < cnt && (unsigned)page < (unsigned)a.n_pages;
+        const size_t at = x.there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+        const Rsrc rk = make_rsrc(Kp + at, x.there ? HD * 64u : 0u), rv = make_rsrc(Vp + at, x.there ? HD * 64u : 0u);
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++) x.k[tt][s] = buf_b128(rk, kofs + tt * 256, s * 2048);
+#pragma unroll
+        for (int d = 0; d < ND; d++) x.v[d] = buf_b128(rv, vofs, d * 1024);
+    };
+    auto work = [&](int i, Blk& x) {
+        const int j0 = (first + 4 * i) * 32;
+        const bool open = x.there && j0 >= open0 && j0 + 32 <= open1;
+        T8 pf[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            f32x4 s2[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++)
+                    s2[tt] = Num<T>::mfma16(__builtin_bit_cast(T8, x.k[tt][s]), qf[u][s], s2[tt]);
+            float sv[8], tmax = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sv[e] = s2[e >> 2][e & 3] * a.c;
+            if (!open) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int j = j0 + 8 * fg + e;
+                    const bool keep = x.there & (j >= jlo[u]) & (j < jhi[u]);
+                    sv[e] = keep ? sv[e] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) tmax = fmaxf(tmax, sv[e]);
+            tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
+            tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
+            if (__any(tmax > m[u] + RAISE)) {
+                const float mn = fmaxf(m[u], tmax), f = m[u] == -INFINITY ? 0.f : exp2_fast(m[u] - mn);
+                m[u] = mn;
+                l[u] *= f;
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[u][d][e] *= f;
+            }
+            const float nm = m[u] == -INFINITY ? 0.f : P_UP - m[u];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = exp2_fast(sv[e] + nm);
+                l[u] += p;
+                pf[u][e] = (T)p;
+            }
+        }
+        if (!open) {
+            uint32_t odd = 0;
+#pragma unroll
+            for (int d = 0; d < ND; d++) odd |= not_finite<T>(x.v[d]);
+            if (__builtin_expect(__any(odd != 0), 0)) {
+                rare = true;
+#pragma unroll
+                for (int d = 0; d < ND; d++) x.v[d] = finite8<T>(x.v[d]);
+            }
         }
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-        s *= scale;
-        const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.f : exp2f((m - mn) * LOG2E);
-        const float pr = exp2f((s - (mn == -INFINITY ? 0.f : mn)) * LOG2E);
-        l = l * f + pr;
-        m = mn;
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * f + pr * (float)Vp[at + (lane + 64 * e) * 32 + (row & 31)];
+            for (int u = 0; u < NR; u++) acc[u][d] = Num<T>::mfma16(__builtin_bit_cast(T8, x.v[d]), pf[u], acc[u][d]);
+    };
+    Blk A, B2;
+    load(0, A);
+    auto ahead = [&](int i) {  // before block i's load: its window of table entries
+        if ((i & 63) == 0) {
+            ids = ids2;
+            if (i + 64 < cnt) ids2 = entries(i + 64);
+        }
+    };
+    for (int i = 0; i < cnt; i += 2) {
+        load(i + 1, B2);
+        __builtin_amdgcn_sched_barrier(0);
+        work(i, A);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 >= cnt) break;
+        ahead(i + 2);
+        load(i + 2, A);
+        __builtin_amdgcn_sched_barrier(0);
+        work(i + 1, B2);
+        __builtin_amdgcn_sched_barrier(0);
     }
+    if (__builtin_expect(rare, 0)) {  // add_seen: see above
+#pragma unroll 1
+        for (int i = 0; i < cnt; i++) {
+            // (every block: a second time what a product gave already changes neither an infinity nor a NaN)
+            const int blk = first + 4 * i, page = tb[blk >> lbpp], j0 = 32 * blk;
+            if ((unsigned)page >= (unsigned)a.n_pages) continue;
+            const T* const v = Vp + (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32);
+#pragma unroll 1
+            for (int j = j0; j < j0 + 32; j++)
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int d = lane + 64 * e;
-        float o = l == 0.f ? 0.f : acc[e] / l;
-        if (big) o *= 1.0f / (1.0f + exp2f(-LOG2E * (float)big[(size_t)t * stride + h * 2 * HD + HD + d]));
-        out[((size_t)t * HQ + h) * HD + d] = (T)o;
+                for (int u = 0; u < NR; u++)
+                    if (j >= jlo[u] && j < jhi[u]) {
+#pragma unroll
+                        for (int d = 0; d < ND; d++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float x = (float)v[(16 * d + 4 * fg + e) * 32 + (j & 31)];
+                                if (!__builtin_isfinite(x)) acc[u][d][e] += x;
+                            }
+                    }
+        }
+    }
+    // the 4 waves' states side by side: acc[u][d][e] is O[row 16 u + fq][dim 16 d + 4 fg + e]
+#pragma unroll
+    for (int u = 0; u < NR; u++) {
+        l[u] += __shfl_xor(l[u], 16);
+        l[u] += __shfl_xor(l[u], 32);
+#pragma unroll
+        for (int d = 0; d < ND; d++) *reinterpret_cast<f32x4*>(&Om[wv][16 * u + fq][16 * d + 4 * fg]) = acc[u][d];
+        if (fg == 0) Mm[wv][16 * u + fq] = m[u], Lm[wv][16 * u + fq] = l[u];
+    }
+    __syncthreads();
+    for (int i = tid; i < nrows * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
+        float mx = -INFINITY, ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) mx = fmaxf(mx, Mm[w][r]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float lw = Lm[w][r], f = lw == 0.f ? 0.f : exp2_fast(Mm[w][r] - mx);
+            ls += lw == 0.f ? 0.f : lw * f;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&Om[w][r][d]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] += lw == 0.f ? 0.f : x[e] * f;
+        }
+        const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G;
+        const size_t row = (size_t)t * a.HQ + h;
+        if (a.ks == 1) {
+            finish4<T>(o, ls, big ? big + (size_t)t * a.stride + h * 2 * HD + HD + d : nullptr, out + row * HD + d);
+        } else {
+            const size_t pr = (size_t)z * a.rows * a.HQ + row;
+            *reinterpret_cast<f32x4*>(pacc + pr * HD + d) = o;
+            if (d == 0) pml[2 * pr] = mx, pml[2 * pr + 1] = ls;
+        }
+    }
+}
+
+// Joins the splits of a row: HD / 4 threads, 4 dims each.
+template <class T, int HD>
+__device__ __forceinline__ void join(const AttnArgs& a, int t, int h, int d, int nz, const float* pacc, const float* pml,
+                                     const T* big, T* out) {
+    const size_t row = (size_t)t * a.HQ + h, zs = (size_t)a.rows * a.HQ;
+    float mx = -INFINITY;
+    for (int z = 0; z < nz; z++) mx = fmaxf(mx, pml[2 * (z * zs + row)]);
+    float ls = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int z = 0; z < nz; z++) {
+        const float2 ml = *reinterpret_cast<const float2*>(pml + 2 * (z * zs + row));
+        const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
+        const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - mx);
+        ls += ml.y == 0.f ? 0.f : ml.y * f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += ml.y == 0.f ? 0.f : x[e] * f;
+    }
+    finish4<T>(o, ls, big ? big + (size_t)t * a.stride + h * 2 * HD + HD + d : nullptr, out + row * HD + d);
+}
+
+template <class T, int HD>
+__global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float* __restrict__ pacc,
+                                                        const float* __restrict__ pml, const T* __restrict__ big,
+                                                        T* __restrict__ out) {
+    const int kh = blockIdx.x, b = blockIdx.y;
+    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    const int nrows = rq.n * a.G;
+    if (nrows == 0 || nrows > a.few) return;
+    const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
+    const int nz = min(max((((hi + 31) >> 5) - (lo >> 5) + a.span - 1) / a.span, 0), a.ks);
+    for (int i = threadIdx.x; i < nrows * (HD / 4); i += 256) {
+        const int r = i / (HD / 4);
+        join<T, HD>(a, rq.q0 + r / a.G, kh * a.G + r % a.G, 4 * (i % (HD / 4)), nz, pacc, pml, big, out);
+    }
+}
+
+// ---- many rows: 128 rows of a kv head per workgroup ----
+//
+// Bound by MFMA and the softmax beside it: each wave has 32 rows on v_mfma_f32_32x32x16, its queries and outputs in
+// registers, and all 4 share tiles of keys that arrive by LDS DMA, one tile ahead.
+// Workgroup x of the launch is kv head x % HK (with 8 heads, one per XCD's L2), split and tile; the tiles of all
+// requests with more than `few` rows are numbered through, and taken from the last on: a causal chunk's late tiles are
+// the long ones.
+struct Tile {
+    int b, i;  // request and tile in it; b < 0: none
+};
+__device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x, int tile_rows) {
+    const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
+    auto tiles = [&](int b) {
+        if (b >= a.B) return 0;
+        const int n = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap).n * a.G;
+        return n > a.few ? (n + tile_rows - 1) / tile_rows : 0;
+    };
+    int own = 0;
+    for (int i = 0; i < per; i++) own += tiles(lane * per + i);
+    int to = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(to, o);
+        if (lane >= o) to += y;
+    }
+    const int total = __builtin_amdgcn_readlane(to, 63);
+    if (x >= total) return {-1, 0};
+    x = total - 1 - x;
+    const int at = __ffsll((long long)__ballot(to > x)) - 1;
+    x -= __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(own, at);
+    int b = at * per;
+    for (int i = 0; i < per - 1; i++, b++) {
+        const int n = tiles(b);
+        if (x < n) break;
+        x -= n;
+    }
+    return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(x)};
+}
+
+constexpr int TILE_ROWS = 128;
+template <int HD>
+constexpr int tile_blocks() { return HD == 256 ? 1 : 2; }  // blocks of 32 keys in a tile
+
+template <class T, int HD>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_rows(const T* __restrict__ Q, const T* __restrict__ Kp,
+                                                                       const T* __restrict__ Vp, AttnArgs a,
+                                                                       const T* __restrict__ big, T* __restrict__ out,
+                                                                       float* __restrict__ pacc,
+                                                                       float* __restrict__ pml) {
+    typedef typename Vec8<T>::type T8;
+    constexpr int NS = HD / 16, ND = HD / 32, KBB = tile_blocks<HD>();
+    constexpr int BB = HD * 64;         // bytes of a block's K (or V)
+    constexpr int PART = KBB * BB / 4;  // bytes of a tile's K that one wave fetches
+    // (an array per buffer: the compiler then sees that the DMAs into one never alias the reads of another)
+    __shared__ __align__(1024) uint8_t K0[KBB * BB], K1[KBB * BB], V0[KBB * BB], V1[KBB * BB];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK % a.ks;
+    const Tile tl = find_tile(a, blockIdx.x / (a.HK * a.ks), TILE_ROWS);
+    if (tl.b < 0) return;
+    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    const int nrows = rq.n * a.G, r0 = tl.i * TILE_ROWS, r1 = min(nrows, r0 + TILE_ROWS);
+    const int w0 = r0 + 32 * wv, w1 = min(w0 + 32, r1);  // the wave's rows
+    const bool live = w0 < r1;
+    // keys seen by some row of the workgroup, and this split's blocks of them
+    const int hi = min(rq.p0 + (r1 - 1) / a.G + 1, rq.kcap);
+    const int lo = a.window ? max(0, rq.p0 + r0 / a.G - a.window + 1) : 0;
+    const int blk0 = (lo >> 5) + z * a.span * KBB, blk1 = min((hi + 31) >> 5, blk0 + a.span * KBB);
+    const int nb = max(blk1 - blk0, 0);
+    // the lane's row (one past the last is the last again, also in the output), the keys [jlo, jhi) that it sees, and
+    // those [all0, all1) that every row of the wave sees
+    const int r = min(w0 + c, r1 - 1), t = r / a.G, h = kh * a.G + r % a.G;
+    const int jlo = a.window ? rq.p0 + t - a.window + 1 : 0, jhi = min(rq.p0 + t + 1, hi);
+    const int all0 = a.window ? rq.p0 + (w1 - 1) / a.G - a.window + 1 : 0, all1 = min(rq.p0 + w0 / a.G + 1, hi);
+
+    const int lbpp = a.lps - 5;
+    const int* const tb = a.table + (size_t)tl.b * a.max_blocks;
+    // lane l: the table entries of block l of the window of 64 blocks that block `at` is in, and of the next window
+    int at = 0;
+    auto entries = [&](int j) INL { return tb[min((blk0 + j + lane) >> lbpp, a.max_blocks - 1)]; };
+    int ids = nb > 0 ? entries(0) : 0, ids2 = nb > 0 ? entries(64) : 0;
+    auto page_of = [&](int j) INL { return __builtin_amdgcn_readlane((j ^ at) >> 6 ? ids2 : ids, j & 63); };
+    const uint32_t dlane = (uint32_t)((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
+    // blocks j .. j + KBB - 1 of a cache into an LDS buffer: the wave's quarter, 16 bytes per lane, the 16-byte pieces
+    // of each 64-byte row at p ^ (row / 4) % 4 (fragment reads then meet no bank twice); nothing is read past the last
+    // block or in a hole
+    auto fetch = [&](int j, const T* C, uint8_t* buf) INL {
+        constexpr int KW = 4 / KBB;  // waves per block
+        const int kb = wv / KW, part = (wv % KW) * PART, blk = blk0 + j + kb, page = page_of(j + kb);
+        const bool there = (unsigned)page < (unsigned)a.n_pages && blk < blk1;
+        const size_t off = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+        const Rsrc rs = make_rsrc(C + off, there ? BB : 0);
+        uint8_t* const d = buf + kb * BB + part;
+        if constexpr (PART == 4096) buf_lds64(rs, dlane, part, d);
+        else {
+#pragma unroll
+            for (int o = 0; o < PART; o += 1024) buf_lds16(rs, dlane, part + o, d + o);
+        }
+    };
+    T8 qf[NS];
+    {
+        const T* q = Q + ((size_t)(rq.q0 + t) * a.HQ + h) * HD + 8 * g;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const T8*>(q + 16 * s);
+    }
+    // K runs one block ahead of V: buffer i & 1 holds K of blocks KBB i + 1 .. KBB i + KBB, and V of those before them
+    if (nb > 0) {
+        fetch(0, Kp, K1);  // (block 0's K, and with two blocks per tile block 1's, which is not used there)
+        fetch(1, Kp, K0);
+        fetch(0, Vp, V0);
+    }
+    // row i of S^T is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 of its block: lane (row c, half g) then
+    // has keys 16 k + 8 g + e in registers 8 k + e
+    const int kperm = 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
+    const int kfo = kperm * 64 + ((g ^ ((kperm >> 2) & 3)) << 4), vfo = c * 64 + ((g ^ ((c >> 2) & 3)) << 4);
+    f32x16 acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f, nm = 0.f, tmax = -INFINITY;
+    bool rare = false;  // some value was taken as 0
+    bool open = true;   // every row of the wave sees the block whose probabilities are next whole
+    T8 pf[2];
+    auto prob = [&](const f32x16& s, int e) INL {
+        const float p = exp2_fast(__builtin_fmaf(s[e], a.c, nm));
+        l += p;
+        pf[e >> 3][e & 7] = (T)p;
+    };
+    // S^T of the block in K, 4 fragments at a time, the next ones read while the products run; mid(i) is work beside
+    // product i
+    auto scores = [&](const uint8_t* K, f32x16& s, auto mid) INL {
+        T8 fr[2][4];
+        auto read = [&](int n) INL {
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const int st = 4 * n + f;
+                fr[n & 1][f] = *reinterpret_cast<const T8*>(K + (st >> 1) * 2048 + (kfo ^ ((st & 1) << 5)));
+            }
+        };
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = 0.f;
+        read(0);
+#pragma unroll
+        for (int n = 0; n < NS / 4; n++) {
+            if (n + 1 < NS / 4) read(n + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                s = Num<T>::mfma32(fr[n & 1][f], qf[4 * n + f], s);
+                mid(4 * n + f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    // masks the scores of block j and takes their maximum
+    auto mask_max = [&](f32x16& s, int j) INL {
+        const int j0 = (blk0 + j) * 32;
+        const bool there = (unsigned)page_of(j) < (unsigned)a.n_pages;
+        open = there && j0 >= all0 && j0 + 32 <= all1;
+        if (!open) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int key = j0 + 16 * (e >> 3) + 8 * g + (e & 7);
+                const bool keep = there & (key >= jlo) & (key < jhi);
+                s[e] = keep ? s[e] : -INFINITY;
+            }
+        }
+        float x = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) x = fmaxf(x, s[e]);
+        tmax = fmaxf(x, __shfl_xor(x, 32)) * a.c;
+    };
+    auto raise = [&]() INL {
+        if (__any(tmax > m + RAISE)) {
+            const float mn = fmaxf(m, tmax), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[d][e] *= f;
+        }
+        nm = m == -INFINITY ? 0.f : P_UP - m;
+    };
+    // O^T += V^T P^T of the block in V, 4 fragments (2 dim tiles, 2 key slices) at a time
+    auto output = [&](const uint8_t* V) INL {
+        auto vfrag = [&](int d, int k) INL { return *reinterpret_cast<const u32x4*>(V + d * 2048 + (vfo ^ (k << 5))); };
+        bool odd = false;
+        if (!open) {
+            uint32_t x = 0;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                x |= not_finite<T>(vfrag(d, 0)) | not_finite<T>(vfrag(d, 1));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            odd = __any(x != 0);
+            rare = rare || odd;
+        }
+        u32x4 fr[2][4];
+        auto read = [&](int n) INL {
+#pragma unroll
+            for (int f = 0; f < 4; f++) fr[n & 1][f] = vfrag(2 * n + (f & 1), f >> 1);
+        };
+        read(0);
+#pragma unroll
+        for (int n = 0; n < ND / 2; n++) {
+            if (n + 1 < ND / 2) read(n + 1);
+            if (__builtin_expect(odd, 0)) {
+#pragma unroll
+                for (int f = 0; f < 4; f++) fr[n & 1][f] = finite8<T>(fr[n & 1][f]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < 4; f++)
+                acc[2 * n + (f & 1)] = Num<T>::mfma32(__builtin_bit_cast(T8, fr[n & 1][f]), pf[f >> 1], acc[2 * n + (f & 1)]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // block j (scores s): its probabilities and output, beside the scores of block j + 1, whose keys are in K
+    auto step = [&](int j, f32x16& s, f32x16& s2, const uint8_t* K, const uint8_t* V) INL {
+        if (j >= nb) return;
+        raise();
+        if (j + 1 < nb) {
+            constexpr int PER = 16 / NS;  // probabilities beside a product
+            scores(K, s2, [&](int i) {
+#pragma unroll
+                for (int e = 0; e < PER; e++) prob(s, PER * i + e);
+            });
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) prob(s, e);
+        }
+        output(V);
+        if (j + 1 < nb) mask_max(s2, j + 1);
+    };
+    f32x16 sA, sB;
+    auto tile = [&](int i, uint8_t* K, uint8_t* Kx, uint8_t* V, uint8_t* Vx) INL {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        lds_barrier();  // this tile is there for every wave, and every wave is done with the other buffers
+        at = KBB * i + 1;
+        if (i > 0 && (at & 63) < KBB) ids = ids2, ids2 = entries((at & ~63) + 64);
+        if (KBB * (i + 1) < nb) {
+            fetch(KBB * (i + 1) + 1, Kp, Kx);
+            fetch(KBB * (i + 1), Vp, Vx);
+        }
+        if (!live) return;
+        if constexpr (KBB == 2) {
+            step(2 * i, sA, sB, K, V);
+            step(2 * i + 1, sB, sA, K + BB, V + BB);
+        } else if (i & 1) step(i, sB, sA, K, V);
+        else step(i, sA, sB, K, V);
+    };
+    if (nb > 0) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        lds_barrier();
+        if (live) {
+            scores(K1, sA, [](int) {});
+            mask_max(sA, 0);
+        }
+        for (int i = 0; KBB * i < nb; i += 2) {
+            tile(i, K0, K1, V0, V1);
+            if (KBB * (i + 1) < nb) tile(i + 1, K1, K0, V1, V0);
+        }
+    }
+    if (!live) return;
+    if (__builtin_expect(rare, 0)) {  // add_seen: see above
+#pragma unroll 1
+        for (int blk = blk0; blk < blk1; blk++) {
+            // (every block: a second time what a product gave already changes neither an infinity nor a NaN)
+            const int j0 = 32 * blk, page = tb[blk >> lbpp];
+            if ((unsigned)page >= (unsigned)a.n_pages) continue;
+            const T* const v = Vp + (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32);
+#pragma unroll 1
+            for (int j = j0; j < j0 + 32; j++)
+                if (j >= jlo && j < jhi) {
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const float x = (float)v[(32 * d + 8 * (e >> 2) + 4 * g + (e & 3)) * 32 + (j & 31)];
+                            if (!__builtin_isfinite(x)) acc[d][e] += x;
+                        }
+                }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    // acc[d][e] is O[row c][dim 32 d + 8 (e / 4) + 4 g + e % 4]
+    const size_t row = (size_t)(rq.q0 + t) * a.HQ + h, pr = (size_t)z * a.rows * a.HQ + row;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int dim = 32 * d + 8 * q + 4 * g;
+            const f32x4 o = {acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
+            if (a.ks == 1)
+                finish4<T>(o, l, big ? big + (size_t)(rq.q0 + t) * a.stride + h * 2 * HD + HD + dim : nullptr,
+                           out + row * HD + dim);
+            else *reinterpret_cast<f32x4*>(pacc + pr * HD + dim) = o;
+        }
+    if (a.ks > 1 && g == 0) pml[2 * pr] = m, pml[2 * pr + 1] = l;
+}
+
+template <class T, int HD>
+__global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float* __restrict__ pacc,
+                                                         const float* __restrict__ pml, const T* __restrict__ big,
+                                                         T* __restrict__ out) {
+    // a workgroup joins 16 rows of a tile
+    const Tile tl = find_tile(a, blockIdx.x, TILE_ROWS);
+    if (tl.b < 0) return;
+    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    const int nrows = rq.n * a.G, t0 = tl.i * TILE_ROWS, t1 = min(nrows, t0 + TILE_ROWS);
+    const int hi = min(rq.p0 + (t1 - 1) / a.G + 1, rq.kcap), lo = a.window ? max(0, rq.p0 + t0 / a.G - a.window + 1) : 0;
+    const int per = a.span * tile_blocks<HD>();
+    const int nz = min(max((((hi + 31) >> 5) - (lo >> 5) + per - 1) / per, 0), a.ks);
+    const int kh = blockIdx.y >> 3, r0 = t0 + 16 * (blockIdx.y & 7), r1 = min(t1, r0 + 16);
+    for (int i = threadIdx.x; i < (r1 - r0) * (HD / 4); i += 256) {
+        const int r = r0 + i / (HD / 4);
+        join<T, HD>(a, rq.q0 + r / a.G, kh * a.G + r % a.G, 4 * (i % (HD / 4)), nz, pacc, pml, big, out);
     }
 }
 
 int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
+
+// How a call runs, from its sizes alone (the lengths themselves are on the device).
+struct Plan {
+    int nr = 0;                            // 16-row groups of k_paged_few, 0: not launched
+    int few = 0;                           // requests with up to this many rows (new tokens times G) are its own
+    int few_ks = 1, few_span = 1;          // splits, and blocks of 32 keys in each
+    int tiles = 0;                         // of k_paged_rows (an upper bound), 0: not launched
+    int rows_ks = 1, rows_span = 1;        // splits, and key tiles in each
+    size_t slots = 0;                      // partial results of [rows][HQ] that both need at most
+};
+
+Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, int window) {
+    const int G = s.HQ / s.HK;
+    const long long most = (long long)std::min(max_new, rows) * G;
+    Plan p;
+    const int fits = s.HD == 256 ? 16 : 32;  // (a second group's outputs and queries do not fit the registers at 256)
+    if (most <= fits) p.nr = most <= 16 ? 1 : 2, p.few = 16 * p.nr;
+    else if (B > 1 && (long long)rows * 2 < (long long)max_new * B && G <= fits) p.nr = G <= 16 ? 1 : 2, p.few = 16 * p.nr;
+    auto blocks = [&](long long n) {  // of 32 keys that n adjacent rows may see
+        long long k = max_kv;
+        if (window) k = std::min(k, (long long)window + n + 31);
+        return (int)((k + 31) / 32);
+    };
+    if (p.nr) {
+        const int nb = blocks(std::max(1, p.few / G));
+        const int want = std::max(1, 1024 / (B * s.HK));
+        p.few_span = std::max(8, ((nb + want - 1) / want + 3) / 4 * 4);
+        p.few_ks = (nb + p.few_span - 1) / p.few_span;
+        if (p.few_ks > 1) p.slots = p.few_ks;
+    }
+    if (most > p.few) {
+        p.tiles = (int)((long long)rows * G / TILE_ROWS) + B;
+        const int kbb = s.HD == 256 ? 1 : 2;
+        const int nt = (blocks(TILE_ROWS / G + 1) + kbb - 1) / kbb;
+        const int busy = (int)std::max(1ll, (long long)rows * G / TILE_ROWS) * s.HK;
+        const int want = std::max(1, 256 / busy);
+        p.rows_span = std::max(4, (nt + want - 1) / want);
+        p.rows_ks = (nt + p.rows_span - 1) / p.rows_span;
+        if (p.rows_ks > 1) p.slots = std::max(p.slots, (size_t)p.rows_ks);
+    }
+    return p;
+}
 
 template <class T, int HD>
 void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
@@ -353,11 +1024,36 @@ void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
 
 template <class T, int HD>
 void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_attn<T, HD>), dim3((unsigned)(((size_t)a.rows * s.HQ + 3) / 4)), dim3(256), 0, st,
-                       static_cast<const T*>(a.Q), static_cast<const T*>(a.big), a.stride, static_cast<const T*>(a.Kp),
-                       static_cast<const T*>(a.Vp), a.table, a.max_blocks, a.cu, a.kv_lens, a.B, a.rows, s.HQ, s.HK,
-                       log2i(s.PS), s.n_pages, s.pstride, a.window, a.scale, static_cast<T*>(a.out));
-    launched("paged_attention");
+    const Plan p = plan_attn(s, a.B, a.rows, a.max_new, a.max_kv, a.window);
+    AttnArgs g{a.table, a.cu, a.kv_lens, a.max_blocks, a.B, a.rows, s.HQ, s.HK, s.HQ / s.HK, log2i(s.PS), s.n_pages,
+               a.max_new, a.max_kv, a.window, p.few, 1, 1, a.stride, a.scale * LOG2E, s.pstride};
+    const T *Q = static_cast<const T*>(a.Q), *K = static_cast<const T*>(a.Kp), *V = static_cast<const T*>(a.Vp),
+            *big = static_cast<const T*>(a.big);
+    T* const out = static_cast<T*>(a.out);
+    float* const pacc = static_cast<float*>(a.ws);
+    float* const pml = pacc + p.slots * a.rows * s.HQ * HD;
+    if (p.tiles) {
+        g.ks = p.rows_ks, g.span = p.rows_span;
+        hipLaunchKernelGGL((k_paged_rows<T, HD>), dim3((unsigned)((size_t)p.tiles * s.HK * g.ks)), dim3(256), 0, st, Q, K, V,
+                           g, big, out, pacc, pml);
+        launched("paged_attention");
+        if (g.ks > 1) {
+            hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, 8 * s.HK), dim3(256), 0, st, g, pacc, pml, big, out);
+            launched("paged_attention");
+        }
+    }
+    if (p.nr) {
+        g.ks = p.few_ks, g.span = p.few_span;
+        const dim3 grid(s.HK * g.ks, a.B);
+        if (p.nr == 1) hipLaunchKernelGGL((k_paged_few<T, HD, 1>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
+        else if constexpr (HD < 256)
+            hipLaunchKernelGGL((k_paged_few<T, HD, 2>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
+        launched("paged_attention");
+        if (g.ks > 1) {
+            hipLaunchKernelGGL((k_paged_join_few<T, HD>), dim3(s.HK, a.B), dim3(256), 0, st, g, pacc, pml, big, out);
+            launched("paged_attention");
+        }
+    }
 }
 
 // f(type tag, head_dim constant)
@@ -385,7 +1081,10 @@ void paged_prep(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
     by_type(s, [&](auto t, auto hd) { prep_as<decltype(t), decltype(hd)::value>(s, a, st); });
 }
 
-size_t paged_attn_ws(const PagedShape&, int, int, int, int) { return 0; }
+size_t paged_attn_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv) {
+    // (a window only lowers the number of splits)
+    return plan_attn(s, B, rows, max_new, max_kv, 0).slots * rows * s.HQ * (s.HD + 2) * 4;
+}
 
 void paged_attn(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
     by_type(s, [&](auto t, auto hd) { attn_as<decltype(t), decltype(hd)::value>(s, a, st); });
