@@ -304,10 +304,27 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 
 // (left to itself the compiler keeps the larger lambdas as calls, and with them their captures in memory)
 #define INL __attribute__((always_inline))
+// (and it moves work that the products are to cover out from between them: a volatile asm keeps its place)
+#if defined(__HIP_DEVICE_COMPILE__)
+#define PIN_V(x) asm volatile("" : "+v"(x))
+#else
+#define PIN_V(x) (void)(x)
+#endif
 
 constexpr float P_UP = 8.0f, RAISE = 6.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The larger of a value and the one 32 lanes away.
+__device__ __forceinline__ float max_halves(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t lo = sw[0], hi = sw[1];
+    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+#else
+    return x;
+#endif
+}
 
 template <class T>
 struct Num;
@@ -379,21 +396,23 @@ struct AttnArgs {
     size_t pstride;
 };
 
-// Output of 4 dims of a row: unnormalised o over the sum l, times the gate's sigmoid, rounded once.
+// Output of 4 dims of a row: unnormalised o over the sum l, times the sigmoid of its gates where it has some, rounded once.
 template <class T>
-__device__ __forceinline__ void finish4(f32x4 o, float l, const T* gate, T* out) {
+__device__ __forceinline__ void finish4(f32x4 o, float l, bool gated, u32x2 gate, T* out) {
     typedef T T4 __attribute__((ext_vector_type(4)));
-    const float inv = 1.0f / l;
-    float sg[4] = {1.f, 1.f, 1.f, 1.f};
-    if (gate) {
-        const T4 v = *reinterpret_cast<const T4*>(gate);
-#pragma unroll
-        for (int e = 0; e < 4; e++) sg[e] = __builtin_amdgcn_rcpf(1.0f + exp2_fast((float)v[e] * -LOG2E));
-    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const T4 v = __builtin_bit_cast(T4, gate);
     T4 r;
 #pragma unroll
-    for (int e = 0; e < 4; e++) r[e] = (T)((l == 0.f ? 0.f : o[e] * inv) * sg[e]);
+    for (int e = 0; e < 4; e++) {
+        const float sg = gated ? __builtin_amdgcn_rcpf(1.0f + exp2_fast((float)v[e] * -LOG2E)) : 1.f;
+        r[e] = (T)((l == 0.f ? 0.f : o[e] * inv) * sg);
+    }
     *reinterpret_cast<T4*>(out) = r;
+}
+template <class T>
+__device__ __forceinline__ u32x2 gate4(const T* big, size_t at) {
+    return big ? *reinterpret_cast<const u32x2*>(big + at) : u32x2{0, 0};
 }
 
 // ---- few rows: up to 16 NR rows per (request, kv head), one new token's heads or a short draft's ----
@@ -418,7 +437,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
     if (nrows == 0 || nrows > a.few) return;
     // keys [lo, hi) are seen by some row; this workgroup's blocks of them
     const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
-    const int blk0 = (lo >> 5) + z * a.span, blk1 = min((hi + 31) >> 5, blk0 + a.span);
+    const int blk0 = (lo >> 5) + z * a.span, blk1 = z + 1 < a.ks ? min((hi + 31) >> 5, blk0 + a.span) : (hi + 31) >> 5;
     const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + 3) >> 2 : 0;
     int jlo[NR], jhi[NR];  // keys [jlo, jhi) are seen by this lane's row
     T8 qf[NR][NS];
@@ -595,7 +614,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
         const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G;
         const size_t row = (size_t)t * a.HQ + h;
         if (a.ks == 1) {
-            finish4<T>(o, ls, big ? big + (size_t)t * a.stride + h * 2 * HD + HD + d : nullptr, out + row * HD + d);
+            finish4<T>(o, ls, big, gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d), out + row * HD + d);
         } else {
             const size_t pr = (size_t)z * a.rows * a.HQ + row;
             *reinterpret_cast<f32x4*>(pacc + pr * HD + d) = o;
@@ -604,41 +623,51 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
     }
 }
 
-// Joins the splits of a row: HD / 4 threads, 4 dims each.
-template <class T, int HD>
-__device__ __forceinline__ void join(const AttnArgs& a, int t, int h, int d, int nz, const float* pacc, const float* pml,
-                                     const T* big, T* out) {
-    const size_t row = (size_t)t * a.HQ + h, zs = (size_t)a.rows * a.HQ;
-    float mx = -INFINITY;
-    for (int z = 0; z < nz; z++) mx = fmaxf(mx, pml[2 * (z * zs + row)]);
-    float ls = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int z = 0; z < nz; z++) {
-        const float2 ml = *reinterpret_cast<const float2*>(pml + 2 * (z * zs + row));
-        const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
-        const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - mx);
-        ls += ml.y == 0.f ? 0.f : ml.y * f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] += ml.y == 0.f ? 0.f : x[e] * f;
-    }
-    finish4<T>(o, ls, big ? big + (size_t)t * a.stride + h * 2 * HD + HD + d : nullptr, out + row * HD + d);
-}
-
+// Joins up to 64 splits of one row and writes it: 256 threads, HD / 4 of them side by side (4 dims each), their groups
+// each every so many splits.  Every split of a row has written its maximum and sum, 0 where it had no key.
+constexpr int MAX_KS = 64;
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float* __restrict__ pacc,
                                                         const float* __restrict__ pml, const T* __restrict__ big,
-                                                        T* __restrict__ out) {
-    const int kh = blockIdx.x, b = blockIdx.y;
-    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+                                                        T* __restrict__ out, int rows_max) {
+    constexpr int W = HD / 4, NG = 256 / W;
+    __shared__ float wt[MAX_KS];
+    __shared__ f32x4 part[NG][W];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int kh = blockIdx.x / rows_max, r = blockIdx.x % rows_max;
+    const Req rq = request(a.cu, a.kv_lens, blockIdx.y, a.rows, a.max_new, a.kcap);
     const int nrows = rq.n * a.G;
-    if (nrows == 0 || nrows > a.few) return;
-    const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
-    const int nz = min(max((((hi + 31) >> 5) - (lo >> 5) + a.span - 1) / a.span, 0), a.ks);
-    for (int i = threadIdx.x; i < nrows * (HD / 4); i += 256) {
-        const int r = i / (HD / 4);
-        join<T, HD>(a, rq.q0 + r / a.G, kh * a.G + r % a.G, 4 * (i % (HD / 4)), nz, pacc, pml, big, out);
+    if (r >= nrows || nrows > a.few) return;
+    const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G, d = 4 * (tid % W);
+    const size_t row = (size_t)t * a.HQ + h, zs = (size_t)a.rows * a.HQ;
+    const u32x2 gate = gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d);
+    // (every wave for itself, the same)
+    const float2 ml = lane < a.ks ? *reinterpret_cast<const float2*>(pml + 2 * (lane * zs + row)) : float2{-INFINITY, 0.f};
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - mx);
+    float ls = ml.y == 0.f ? 0.f : ml.y * f;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) ls += __shfl_xor(ls, o);
+    if (tid < 64) wt[lane] = f;
+    __syncthreads();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int z = tid / W; z < a.ks; z += NG) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
+        const float w = wt[z];
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += w == 0.f ? 0.f : x[e] * w;
     }
+    part[tid / W][tid % W] = o;
+    __syncthreads();
+    if (tid >= W) return;
+#pragma unroll
+    for (int g = 1; g < NG; g++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += part[g][tid][e];
+    finish4<T>(o, ls, big, gate, out + row * HD + d);
 }
 
 // ---- many rows: 128 rows of a kv head per workgroup ----
@@ -648,15 +677,16 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
 // Workgroup x of the launch is kv head x % HK (with 8 heads, one per XCD's L2), split and tile; the tiles of all
 // requests with more than `few` rows are numbered through, and taken from the last on: a causal chunk's late tiles are
 // the long ones.
+constexpr int TILE_ROWS = 128;
 struct Tile {
     int b, i;  // request and tile in it; b < 0: none
 };
-__device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x, int tile_rows) {
+__device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
     const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
     auto tiles = [&](int b) {
         if (b >= a.B) return 0;
         const int n = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap).n * a.G;
-        return n > a.few ? (n + tile_rows - 1) / tile_rows : 0;
+        return n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
     };
     int own = 0;
     for (int i = 0; i < per; i++) own += tiles(lane * per + i);
@@ -680,26 +710,23 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x, int tile_row
     return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(x)};
 }
 
-constexpr int TILE_ROWS = 128;
-template <int HD>
-constexpr int tile_blocks() { return HD == 256 ? 1 : 2; }  // blocks of 32 keys in a tile
-
 template <class T, int HD>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_rows(const T* __restrict__ Q, const T* __restrict__ Kp,
-                                                                       const T* __restrict__ Vp, AttnArgs a,
-                                                                       const T* __restrict__ big, T* __restrict__ out,
-                                                                       float* __restrict__ pacc,
-                                                                       float* __restrict__ pml) {
+__global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* __restrict__ Q, const T* __restrict__ Kp,
+                                                       const T* __restrict__ Vp, AttnArgs a, const T* __restrict__ big,
+                                                       T* __restrict__ out, float* __restrict__ pacc,
+                                                       float* __restrict__ pml) {
     typedef typename Vec8<T>::type T8;
-    constexpr int NS = HD / 16, ND = HD / 32, KBB = tile_blocks<HD>();
-    constexpr int BB = HD * 64;         // bytes of a block's K (or V)
-    constexpr int PART = KBB * BB / 4;  // bytes of a tile's K that one wave fetches
+    constexpr int NS = HD / 16, ND = HD / 32, NB = 4;
+    constexpr int BB = HD * 64;        // bytes of a block's K (or V)
+    constexpr int PART = BB / 4;   // bytes of it that one wave fetches
+    constexpr int IW = PART / 1024;  // in so many DMAs
     // (an array per buffer: the compiler then sees that the DMAs into one never alias the reads of another)
-    __shared__ __align__(1024) uint8_t K0[KBB * BB], K1[KBB * BB], V0[KBB * BB], V1[KBB * BB];
+    __shared__ __align__(1024) uint8_t K0[BB], K1[BB], K2[BB], K3[BB], V0[BB], V1[BB], V2[BB], V3[BB];
+    __shared__ int rare;  // some value was taken as 0
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
     const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK % a.ks;
-    const Tile tl = find_tile(a, blockIdx.x / (a.HK * a.ks), TILE_ROWS);
+    const Tile tl = find_tile(a, blockIdx.x / (a.HK * a.ks));
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const int nrows = rq.n * a.G, r0 = tl.i * TILE_ROWS, r1 = min(nrows, r0 + TILE_ROWS);
@@ -708,111 +735,163 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_rows(const T* 
     // keys seen by some row of the workgroup, and this split's blocks of them
     const int hi = min(rq.p0 + (r1 - 1) / a.G + 1, rq.kcap);
     const int lo = a.window ? max(0, rq.p0 + r0 / a.G - a.window + 1) : 0;
-    const int blk0 = (lo >> 5) + z * a.span * KBB, blk1 = min((hi + 31) >> 5, blk0 + a.span * KBB);
+    const int blk0 = (lo >> 5) + z * a.span, blk1 = z + 1 < a.ks ? min((hi + 31) >> 5, blk0 + a.span) : (hi + 31) >> 5;
     const int nb = max(blk1 - blk0, 0);
-    // the lane's row (one past the last is the last again, also in the output), the keys [jlo, jhi) that it sees, and
-    // those [all0, all1) that every row of the wave sees
+    // the lane's row (one past the last is the last again, also in the output) and the keys [jlo, jhi) that it sees
     const int r = min(w0 + c, r1 - 1), t = r / a.G, h = kh * a.G + r % a.G;
     const int jlo = a.window ? rq.p0 + t - a.window + 1 : 0, jhi = min(rq.p0 + t + 1, hi);
+    // the keys that every row of the wave, and of the workgroup, sees
     const int all0 = a.window ? rq.p0 + (w1 - 1) / a.G - a.window + 1 : 0, all1 = min(rq.p0 + w0 / a.G + 1, hi);
+    const int wg0 = a.window ? rq.p0 + (r1 - 1) / a.G - a.window + 1 : 0, wg1 = min(rq.p0 + r0 / a.G + 1, hi);
+    if (tid == 0) rare = 0;
 
     const int lbpp = a.lps - 5;
     const int* const tb = a.table + (size_t)tl.b * a.max_blocks;
-    // lane l: the table entries of block l of the window of 64 blocks that block `at` is in, and of the next window
-    int at = 0;
-    auto entries = [&](int j) INL { return tb[min((blk0 + j + lane) >> lbpp, a.max_blocks - 1)]; };
-    int ids = nb > 0 ? entries(0) : 0, ids2 = nb > 0 ? entries(64) : 0;
-    auto page_of = [&](int j) INL { return __builtin_amdgcn_readlane((j ^ at) >> 6 ? ids2 : ids, j & 63); };
-    const uint32_t dlane = (uint32_t)((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
-    // blocks j .. j + KBB - 1 of a cache into an LDS buffer: the wave's quarter, 16 bytes per lane, the 16-byte pieces
-    // of each 64-byte row at p ^ (row / 4) % 4 (fragment reads then meet no bank twice); nothing is read past the last
-    // block or in a hole
-    auto fetch = [&](int j, const T* C, uint8_t* buf) INL {
-        constexpr int KW = 4 / KBB;  // waves per block
-        const int kb = wv / KW, part = (wv % KW) * PART, blk = blk0 + j + kb, page = page_of(j + kb);
+    // Lane l: where block `win` + l begins in a cache (bytes; the sign bit where it is not there: past the last block, in
+    // a hole), and the same 32 blocks on.  The blocks in use at a time are less than 32 apart.
+    int win = 0;
+    struct Where {
+        uint32_t lo, hi;
+    };
+    auto entries = [&](int j) INL {
+        const int blk = blk0 + j + lane, page = tb[min(blk >> lbpp, a.max_blocks - 1)];
         const bool there = (unsigned)page < (unsigned)a.n_pages && blk < blk1;
-        const size_t off = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
-        const Rsrc rs = make_rsrc(C + off, there ? BB : 0);
-        uint8_t* const d = buf + kb * BB + part;
-        if constexpr (PART == 4096) buf_lds64(rs, dlane, part, d);
-        else {
+        const size_t off = ((size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32)) * 2;
+        return Where{(uint32_t)off, there ? (uint32_t)(off >> 32) : 0x80000000u};
+    };
+    Where wh{0, 0x80000000u}, wh2{0, 0x80000000u};
+    if (nb > 0) wh = entries(0), wh2 = entries(32);
+    auto is_there = [&](int j) INL { return (int)__builtin_amdgcn_readlane(wh.hi, j - win) >= 0; };
+    // block j of a cache: where it is not there nothing is read, and zeros come
+    struct At {
+        uint32_t lo, hi;
+    };
+    auto find = [&](int j) INL { return At{(uint32_t)__builtin_amdgcn_readlane(wh.lo, j - win), (uint32_t)__builtin_amdgcn_readlane(wh.hi, j - win)}; };
+    auto block = [&](At w, const T* C) INL {
+        const uint32_t lo = __builtin_amdgcn_readfirstlane(w.lo), hi = __builtin_amdgcn_readfirstlane(w.hi);
+        return make_rsrc(reinterpret_cast<const uint8_t*>(C) + ((uint64_t)(hi & 0x7FFFFFFFu) << 32 | lo), (int)hi < 0 ? 0 : BB);
+    };
+    const uint32_t dlane = (uint32_t)((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
+    // A block of a cache into an LDS buffer: the wave's quarter, 16 bytes per lane, the 16-byte pieces
+    // of each 64-byte row at p ^ (row / 4) % 4 (fragment reads then meet no bank twice).  Every call is the same DMAs.
+    const int part = wv * PART;
+    auto dma = [&](Rsrc rs, int u, uint8_t* buf) INL { buf_lds16(rs, dlane, part + u * 1024, buf + part + u * 1024); };
+    auto fetch = [&](At w, const T* C, uint8_t* buf) INL {
+        const Rsrc rs = block(w, C);
 #pragma unroll
-            for (int o = 0; o < PART; o += 1024) buf_lds16(rs, dlane, part + o, d + o);
-        }
+        for (int u = 0; u < IW; u++) dma(rs, u, buf);
     };
     T8 qf[NS];
     {
-        const T* q = Q + ((size_t)(rq.q0 + t) * a.HQ + h) * HD + 8 * g;
+        const T* p = Q + ((size_t)(rq.q0 + t) * a.HQ + h) * HD + 8 * g;
 #pragma unroll
-        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const T8*>(q + 16 * s);
-    }
-    // K runs one block ahead of V: buffer i & 1 holds K of blocks KBB i + 1 .. KBB i + KBB, and V of those before them
-    if (nb > 0) {
-        fetch(0, Kp, K1);  // (block 0's K, and with two blocks per tile block 1's, which is not used there)
-        fetch(1, Kp, K0);
-        fetch(0, Vp, V0);
+        for (int s = 0; s < NS; s++) {
+            qf[s] = *reinterpret_cast<const T8*>(p + 16 * s);
+#if defined(__HIP_DEVICE_COMPILE__)
+            if constexpr (HD == 256) asm("" : "+a"(qf[s]));  // (an MFMA reads AGPRs as it reads VGPRs)
+#endif
+        }
     }
     // row i of S^T is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 of its block: lane (row c, half g) then
     // has keys 16 k + 8 g + e in registers 8 k + e
     const int kperm = 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
     const int kfo = kperm * 64 + ((g ^ ((kperm >> 2) & 3)) << 4), vfo = c * 64 + ((g ^ ((c >> 2) & 3)) << 4);
+    // K runs one block ahead of V: stage i is block i + 1's K and block i's V, in buffers i % NB; block 0's K begins in
+    // the last stage's.
+    auto stage = [&](int i, uint8_t* K, uint8_t* V) INL {
+        fetch(find(i + 1), Kp, K);
+        fetch(find(i), Vp, V);
+    };
+    constexpr int NK = NS / 4, NV = ND / 2, AHEAD = 2;
+    if (nb > 0) {
+        fetch(find(0), Kp, K3);
+        stage(0, K0, V0);
+        stage(1, K1, V1);
+        stage(2, K2, V2);
+    }
     f32x16 acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
     float m = -INFINITY, l = 0.f, nm = 0.f, tmax = -INFINITY;
-    bool rare = false;  // some value was taken as 0
-    bool open = true;   // every row of the wave sees the block whose probabilities are next whole
     T8 pf[2];
     auto prob = [&](const f32x16& s, int e) INL {
         const float p = exp2_fast(__builtin_fmaf(s[e], a.c, nm));
         l += p;
+        PIN_V(l);
         pf[e >> 3][e & 7] = (T)p;
     };
-    // S^T of the block in K, 4 fragments at a time, the next ones read while the products run; mid(i) is work beside
-    // product i
-    auto scores = [&](const uint8_t* K, f32x16& s, auto mid) INL {
-        T8 fr[2][4];
-        auto read = [&](int n) INL {
+    // A step's fragments come in groups of 4: NK groups of K, then NV of V (ND dim tiles of the first 16 keys, then of
+    // the others); group n is read while the groups up to AHEAD before it are in use.
+    u32x4 fr[AHEAD + 1][4];
+    auto read_k = [&](int n, int slot, const uint8_t* K) INL {
 #pragma unroll
-            for (int f = 0; f < 4; f++) {
-                const int st = 4 * n + f;
-                fr[n & 1][f] = *reinterpret_cast<const T8*>(K + (st >> 1) * 2048 + (kfo ^ ((st & 1) << 5)));
-            }
-        };
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = 0.f;
-        read(0);
-#pragma unroll
-        for (int n = 0; n < NS / 4; n++) {
-            if (n + 1 < NS / 4) read(n + 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int f = 0; f < 4; f++) {
-                s = Num<T>::mfma32(fr[n & 1][f], qf[4 * n + f], s);
-                mid(4 * n + f);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int f = 0; f < 4; f++) {
+            const int st = 4 * n + f;
+            fr[slot][f] = *reinterpret_cast<const u32x4*>(K + (st >> 1) * 2048 + (kfo ^ ((st & 1) << 5)));
         }
     };
-    // masks the scores of block j and takes their maximum
-    auto mask_max = [&](f32x16& s, int j) INL {
-        const int j0 = (blk0 + j) * 32;
-        const bool there = (unsigned)page_of(j) < (unsigned)a.n_pages;
-        open = there && j0 >= all0 && j0 + 32 <= all1;
-        if (!open) {
+    auto read_v = [&](int n, int slot, const uint8_t* V) INL {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int key = j0 + 16 * (e >> 3) + 8 * g + (e & 7);
-                const bool keep = there & (key >= jlo) & (key < jhi);
-                s[e] = keep ? s[e] : -INFINITY;
-            }
+        for (int f = 0; f < 4; f++) {
+            const int d = (4 * n + f) % ND, k = (4 * n + f) / ND;
+            fr[slot][f] = *reinterpret_cast<const u32x4*>(V + d * 2048 + (vfo ^ (k << 5)));
         }
-        float x = s[0];
+    };
+    auto read = [&](int n, const uint8_t* K, const uint8_t* V) INL {
+        if (n < NK) {
+            read_k(n, n % (AHEAD + 1), K);
+        } else if (n < NK + NV) read_v(n - NK, n % (AHEAD + 1), V);
+    };
+    // group n of S^T = K Q^T; mid(i) is work beside product i
+    auto k_group = [&](int n, int slot, f32x16& s, auto mid) INL {
 #pragma unroll
-        for (int e = 1; e < 16; e++) x = fmaxf(x, s[e]);
-        tmax = fmaxf(x, __shfl_xor(x, 32)) * a.c;
+        for (int f = 0; f < 4; f++) {
+            s = Num<T>::mfma32(__builtin_bit_cast(T8, fr[slot][f]), qf[4 * n + f], s);
+            mid(4 * n + f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // group n of O^T += V^T P^T
+    auto v_group = [&](int n, int slot, auto mid) INL {
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            const int d = (4 * n + f) % ND, k = (4 * n + f) / ND;
+            acc[d] = Num<T>::mfma32(__builtin_bit_cast(T8, fr[slot][f]), pf[k], acc[d]);
+            mid(4 * n + f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // The wave's part of the values of block i, which it has fetched itself: 0 in the place of what is not finite, where
+    // some row of the workgroup does not see all of them.
+    auto clean = [&](int i, uint8_t* V) INL {
+        const int j0 = (blk0 + i) * 32;
+        if (j0 >= wg0 && j0 + 32 <= wg1) return;
+        uint8_t* const p = V + part + lane * 16;
+        u32x4 v[IW];
+        uint32_t x = 0;
+#pragma unroll
+        for (int u = 0; u < IW; u++) v[u] = *reinterpret_cast<const u32x4*>(p + u * 1024);
+#pragma unroll
+        for (int u = 0; u < IW; u++) x |= not_finite<T>(v[u]);
+        if (__builtin_expect(__any(x != 0), 0)) {
+#pragma unroll
+            for (int u = 0; u < IW; u++) *reinterpret_cast<u32x4*>(p + u * 1024) = finite8<T>(v[u]);
+            rare = 1;
+        }
+    };
+    // masks the scores of block j
+    auto mask = [&](f32x16& s, int j) INL {
+        const int j0 = (blk0 + j) * 32;
+        const bool there = is_there(j);
+        if (there && j0 >= all0 && j0 + 32 <= all1) return;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int key = j0 + 16 * (e >> 3) + 8 * g + (e & 7);
+            const bool keep = there & (key >= jlo) & (key < jhi);
+            s[e] = keep ? s[e] : -INFINITY;
+        }
     };
     auto raise = [&]() INL {
         if (__any(tmax > m + RAISE)) {
@@ -826,88 +905,134 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_rows(const T* 
         }
         nm = m == -INFINITY ? 0.f : P_UP - m;
     };
-    // O^T += V^T P^T of the block in V, 4 fragments (2 dim tiles, 2 key slices) at a time
-    auto output = [&](const uint8_t* V) INL {
-        auto vfrag = [&](int d, int k) INL { return *reinterpret_cast<const u32x4*>(V + d * 2048 + (vfo ^ (k << 5))); };
-        bool odd = false;
-        if (!open) {
-            uint32_t x = 0;
+    auto zero = [](f32x16& s) INL {
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
-                x |= not_finite<T>(vfrag(d, 0)) | not_finite<T>(vfrag(d, 1));
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            odd = __any(x != 0);
-            rare = rare || odd;
-        }
-        u32x4 fr[2][4];
-        auto read = [&](int n) INL {
-#pragma unroll
-            for (int f = 0; f < 4; f++) fr[n & 1][f] = vfrag(2 * n + (f & 1), f >> 1);
-        };
-        read(0);
-#pragma unroll
-        for (int n = 0; n < ND / 2; n++) {
-            if (n + 1 < ND / 2) read(n + 1);
-            if (__builtin_expect(odd, 0)) {
-#pragma unroll
-                for (int f = 0; f < 4; f++) fr[n & 1][f] = finite8<T>(fr[n & 1][f]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int f = 0; f < 4; f++)
-                acc[2 * n + (f & 1)] = Num<T>::mfma32(__builtin_bit_cast(T8, fr[n & 1][f]), pf[f >> 1], acc[2 * n + (f & 1)]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int e = 0; e < 16; e++) s[e] = 0.f;
     };
-    // block j (scores s): its probabilities and output, beside the scores of block j + 1, whose keys are in K
-    auto step = [&](int j, f32x16& s, f32x16& s2, const uint8_t* K, const uint8_t* V) INL {
-        if (j >= nb) return;
+    auto none = [](int) {};
+    // Block i (scores s): its probabilities and output, beside the scores s2 of the next, whose keys are in K.  The first EARLY keys' probabilities run beside the scores' products, the others beside the first half of the
+    // output's, the new scores' maximum beside the second half.  The stage NB - 1 further on goes into (Kx, Vx).
+    // (the pins keep the compiler from sinking work behind the products that it runs beside)
+    constexpr int EARLY = 12;
+    At nk{0, 0}, nv{0, 0};  // the blocks that the next step fetches: found in the shadow of this one's products
+    auto find_next = [&](int i) INL { nk = find(i + NB), nv = find(i + NB - 1); };
+    auto step = [&](int i, f32x16& s, f32x16& s2, const uint8_t* K, const uint8_t* V, uint8_t* Kx, uint8_t* Vx) INL {
+#pragma unroll
+        for (int n = 0; n < AHEAD; n++) read(n, K, V);
+        __builtin_amdgcn_sched_barrier(0);
         raise();
-        if (j + 1 < nb) {
-            constexpr int PER = 16 / NS;  // probabilities beside a product
-            scores(K, s2, [&](int i) {
+        zero(s2);
+        const Rsrc rk = block(nk, Kp), rv = block(nv, Vp);
 #pragma unroll
-                for (int e = 0; e < PER; e++) prob(s, PER * i + e);
+        for (int n = 0; n < NK; n++) {
+            read(n + AHEAD, K, V);
+            __builtin_amdgcn_sched_barrier(0);
+            k_group(n, n % (AHEAD + 1), s2, [&](int i) INL {
+#pragma unroll
+                for (int x = i * EARLY / NS; x < (i + 1) * EARLY / NS; x++) prob(s, x);
+                // the DMAs one at a time: a burst of them holds up the wave
+                if (i % (NS / IW) == NS / IW / 2) dma(rk, i / (NS / IW), Kx);
             });
-        } else {
+        }
+        OPAQUE_V(pf[0]);
+        mask(s2, i + 1);
+        constexpr int H = ND;  // products of each half
 #pragma unroll
-            for (int e = 0; e < 16; e++) prob(s, e);
+        for (int n = 0; n < NV; n++) {
+            read(NK + n + AHEAD, K, V);
+            __builtin_amdgcn_sched_barrier(0);
+            v_group(n, (NK + n) % (AHEAD + 1), [&](int p) INL {
+                if (p % (2 * H / IW) == H / IW) dma(rv, p / (2 * H / IW), Vx);
+                if (p < H) {
+                    constexpr int LATE = 16 - EARLY;
+#pragma unroll
+                    for (int x = p * LATE / H; x < (p + 1) * LATE / H; x++) prob(s, EARLY + x);
+                    if (p == H - 1) OPAQUE_V(pf[1]);
+                    if (p == H / 2) find_next(i + 1);
+                } else {
+                    constexpr int M = H - 1;  // the maximum beside all but the last
+#pragma unroll
+                    for (int x = (p - H) * 16 / M; x < (p - H + 1) * 16 / M && x < 16; x++)
+                        tmax = x ? fmaxf(tmax, s2[x]) : s2[0];
+                    if (p == 2 * H - 1) tmax = max_halves(tmax) * a.c;
+                }
+            });
         }
-        output(V);
-        if (j + 1 < nb) mask_max(s2, j + 1);
+        OPAQUE_V(tmax);
     };
-    f32x16 sA, sB;
-    auto tile = [&](int i, uint8_t* K, uint8_t* Kx, uint8_t* V, uint8_t* Vx) INL {
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-        lds_barrier();  // this tile is there for every wave, and every wave is done with the other buffers
-        at = KBB * i + 1;
-        if (i > 0 && (at & 63) < KBB) ids = ids2, ids2 = entries((at & ~63) + 64);
-        if (KBB * (i + 1) < nb) {
-            fetch(KBB * (i + 1) + 1, Kp, Kx);
-            fetch(KBB * (i + 1), Vp, Vx);
+    // the wave's last block
+    auto last = [&](f32x16& s, const uint8_t* V) INL {
+        raise();
+#pragma unroll
+        for (int x = 0; x < 16; x++) prob(s, x);
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            read_v(n, 0, V);
+            v_group(n, 0, none);
         }
-        if (!live) return;
-        if constexpr (KBB == 2) {
-            step(2 * i, sA, sB, K, V);
-            step(2 * i + 1, sB, sA, K + BB, V + BB);
-        } else if (i & 1) step(i, sB, sA, K, V);
-        else step(i, sA, sB, K, V);
+    };
+    // Stage i is there for every wave, the one before is done with.  (DMAs issued after it: NB - 2 stages.)
+    auto arrive = [&](int i, uint8_t* V) INL {
+        wait_loads<vmcnt_imm((NB - 2) * 2 * IW)>();
+        clean(i, V);
+        lds_barrier();
+    };
+    auto advance = [&](int i) INL {  // before blocks from i on are found
+        if (i >= win + 32) win += 32, wh = wh2, wh2 = entries(win + 32);
     };
     if (nb > 0) {
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        wait_loads<vmcnt_imm((NB - 1) * 2 * IW)>();
         lds_barrier();
-        if (live) {
-            scores(K1, sA, [](int) {});
-            mask_max(sA, 0);
+    }
+    if (live && nb > 0) {
+        f32x16 sA, sB;
+        zero(sA);
+#pragma unroll
+        for (int n = 0; n < NK; n++) {
+            read_k(n, 0, K3);
+            k_group(n, 0, sA, none);
         }
-        for (int i = 0; KBB * i < nb; i += 2) {
-            tile(i, K0, K1, V0, V1);
-            if (KBB * (i + 1) < nb) tile(i + 1, K1, K0, V1, V0);
+        mask(sA, 0);
+        tmax = sA[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) tmax = fmaxf(tmax, sA[e]);
+        tmax = max_halves(tmax) * a.c;
+        find_next(0);
+        // block i, its stage in (K, V), the stage NB - 1 further into (Kx, Vx)
+        auto turn = [&](int i, f32x16& s, f32x16& s2, uint8_t* K, uint8_t* V, uint8_t* Kx, uint8_t* Vx) INL {
+            arrive(i, V);
+            advance(i);
+            step(i, s, s2, K, V, Kx, Vx);
+        };
+        int i = 0;
+        for (;;) {
+            if (i + 1 >= nb) break;
+            turn(i, sA, sB, K0, V0, K3, V3);
+            if (++i + 1 >= nb) break;
+            turn(i, sB, sA, K1, V1, K0, V0);
+            if (++i + 1 >= nb) break;
+            turn(i, sA, sB, K2, V2, K1, V1);
+            if (++i + 1 >= nb) break;
+            turn(i, sB, sA, K3, V3, K2, V2);
+            ++i;
+        }
+        uint8_t* const V = i & 2 ? (i & 1 ? V3 : V2) : (i & 1 ? V1 : V0);
+        arrive(i, V);
+        if (i & 1) sA = sB;
+        last(sA, V);
+    } else {  // no rows: its part of the fetching
+        auto buf = [&](int n, uint8_t* b0, uint8_t* b1, uint8_t* b2, uint8_t* b3) INL {
+            return n & 2 ? (n & 1 ? b3 : b2) : (n & 1 ? b1 : b0);
+        };
+        for (int i = 0; i < nb; i++) {
+            arrive(i, buf(i, V0, V1, V2, V3));
+            advance(i);
+            stage(i + NB - 1, buf(i + NB - 1, K0, K1, K2, K3), buf(i + NB - 1, V0, V1, V2, V3));
         }
     }
-    if (!live) return;
-    if (__builtin_expect(rare, 0)) {  // add_seen: see above
+    wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
+    lds_barrier();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(rare), 0)) {  // add_seen: see above
 #pragma unroll 1
         for (int blk = blk0; blk < blk1; blk++) {
             // (every block: a second time what a product gave already changes neither an infinity nor a NaN)
@@ -927,39 +1052,71 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_rows(const T* 
                 }
         }
     }
-    l += __shfl_xor(l, 32);
+    if (!live) return;
     // acc[d][e] is O[row c][dim 32 d + 8 (e / 4) + 4 g + e % 4]
+    l += __shfl_xor(l, 32);
     const size_t row = (size_t)(rq.q0 + t) * a.HQ + h, pr = (size_t)z * a.rows * a.HQ + row;
+    if (a.ks > 1) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<f32x4*>(pacc + pr * HD + 32 * d + 8 * i + 4 * g) =
+                    f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+        if (g == 0) pml[2 * pr] = m, pml[2 * pr + 1] = l;
+        return;
+    }
+    // (all gates are loaded before the first is used: one after the other they were 17 us of a 256-dim call)
+    u32x2 gate[ND][4];
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int dim = 32 * d + 8 * q + 4 * g;
-            const f32x4 o = {acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
-            if (a.ks == 1)
-                finish4<T>(o, l, big ? big + (size_t)(rq.q0 + t) * a.stride + h * 2 * HD + HD + dim : nullptr,
-                           out + row * HD + dim);
-            else *reinterpret_cast<f32x4*>(pacc + pr * HD + dim) = o;
-        }
-    if (a.ks > 1 && g == 0) pml[2 * pr] = m, pml[2 * pr + 1] = l;
+        for (int i = 0; i < 4; i++) gate[d][i] = u32x2{0, 0};
+    if (big) {
+        const T* const p = big + (size_t)(rq.q0 + t) * a.stride + h * 2 * HD + HD + 4 * g;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) gate[d][i] = *reinterpret_cast<const u32x2*>(p + 32 * d + 8 * i);
+    }
+    T* const o = out + row * HD + 4 * g;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            finish4<T>(f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]}, l, big, gate[d][i],
+                       o + 32 * d + 8 * i);
 }
 
+// Joins the splits of k_paged_rows (at most 8): HD / 4 threads per row, 4 dims each.
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float* __restrict__ pacc,
                                                          const float* __restrict__ pml, const T* __restrict__ big,
                                                          T* __restrict__ out) {
-    // a workgroup joins 16 rows of a tile
-    const Tile tl = find_tile(a, blockIdx.x, TILE_ROWS);
+    constexpr int W = HD / 4, PER = 16;  // a workgroup joins 16 rows of a tile
+    const Tile tl = find_tile(a, blockIdx.x);
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
-    const int nrows = rq.n * a.G, t0 = tl.i * TILE_ROWS, t1 = min(nrows, t0 + TILE_ROWS);
-    const int hi = min(rq.p0 + (t1 - 1) / a.G + 1, rq.kcap), lo = a.window ? max(0, rq.p0 + t0 / a.G - a.window + 1) : 0;
-    const int per = a.span * tile_blocks<HD>();
-    const int nz = min(max((((hi + 31) >> 5) - (lo >> 5) + per - 1) / per, 0), a.ks);
-    const int kh = blockIdx.y >> 3, r0 = t0 + 16 * (blockIdx.y & 7), r1 = min(t1, r0 + 16);
-    for (int i = threadIdx.x; i < (r1 - r0) * (HD / 4); i += 256) {
-        const int r = r0 + i / (HD / 4);
-        join<T, HD>(a, rq.q0 + r / a.G, kh * a.G + r % a.G, 4 * (i % (HD / 4)), nz, pacc, pml, big, out);
+    constexpr int parts = TILE_ROWS / PER;
+    const int kh = blockIdx.y / parts, r0 = tl.i * TILE_ROWS + PER * (blockIdx.y % parts);
+    const int r1 = min(min(rq.n * a.G, (tl.i + 1) * TILE_ROWS), r0 + PER);
+    const size_t zs = (size_t)a.rows * a.HQ;
+    for (int i = threadIdx.x; i < (r1 - r0) * W; i += 256) {
+        const int r = r0 + i / W, t = rq.q0 + r / a.G, h = kh * a.G + r % a.G, d = 4 * (i % W);
+        const size_t row = (size_t)t * a.HQ + h;
+        float mx = -INFINITY, ls = 0.f;
+        for (int z = 0; z < a.ks; z++) mx = fmaxf(mx, pml[2 * (z * zs + row)]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int z = 0; z < a.ks; z++) {
+            const float2 ml = *reinterpret_cast<const float2*>(pml + 2 * (z * zs + row));
+            const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
+            const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - mx);
+            ls += ml.y == 0.f ? 0.f : ml.y * f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] += ml.y == 0.f ? 0.f : x[e] * f;
+        }
+        finish4<T>(o, ls, big, gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d), out + row * HD + d);
     }
 }
 
@@ -967,12 +1124,12 @@ int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
 struct Plan {
-    int nr = 0;                            // 16-row groups of k_paged_few, 0: not launched
-    int few = 0;                           // requests with up to this many rows (new tokens times G) are its own
-    int few_ks = 1, few_span = 1;          // splits, and blocks of 32 keys in each
-    int tiles = 0;                         // of k_paged_rows (an upper bound), 0: not launched
-    int rows_ks = 1, rows_span = 1;        // splits, and key tiles in each
-    size_t slots = 0;                      // partial results of [rows][HQ] that both need at most
+    int nr = 0;                      // 16-row groups of k_paged_few, 0: not launched
+    int few = 0;                     // requests with up to this many rows (new tokens times G) are its own
+    int few_ks = 1, few_span = 1;    // splits, and blocks of 32 keys in each
+    int tiles = 0;                   // of k_paged_rows (an upper bound), 0: not launched
+    int rows_ks = 1, rows_span = 1;  // splits, and blocks in each
+    size_t slots = 0;                // partial results of [rows][HQ] that they need at most, whatever the window
 };
 
 Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, int window) {
@@ -989,21 +1146,21 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
     };
     if (p.nr) {
         const int nb = blocks(std::max(1, p.few / G));
-        const int want = std::max(1, 1024 / (B * s.HK));
+        const int want = std::min(MAX_KS, std::max(1, 256 / (B * s.HK)));
         p.few_span = std::max(8, ((nb + want - 1) / want + 3) / 4 * 4);
         p.few_ks = (nb + p.few_span - 1) / p.few_span;
-        if (p.few_ks > 1) p.slots = p.few_ks;
+        p.slots = std::min(want, (nb + 7) / 8);
     }
     if (most > p.few) {
-        p.tiles = (int)((long long)rows * G / TILE_ROWS) + B;
-        const int kbb = s.HD == 256 ? 1 : 2;
-        const int nt = (blocks(TILE_ROWS / G + 1) + kbb - 1) / kbb;
-        const int busy = (int)std::max(1ll, (long long)rows * G / TILE_ROWS) * s.HK;
-        const int want = std::max(1, 256 / busy);
-        p.rows_span = std::max(4, (nt + want - 1) / want);
-        p.rows_ks = (nt + p.rows_span - 1) / p.rows_span;
-        if (p.rows_ks > 1) p.slots = std::max(p.slots, (size_t)p.rows_ks);
+        const long long all = (long long)rows * G;
+        p.tiles = (int)(all / TILE_ROWS) + B;
+        const int nb = blocks(TILE_ROWS / G + 2);
+        const int want = (int)std::min(8ll, std::max(1ll, 256 / std::max(1ll, all / TILE_ROWS * s.HK)));
+        p.rows_span = std::max(8, ((nb + want - 1) / want + 1) / 2 * 2);
+        p.rows_ks = (nb + p.rows_span - 1) / p.rows_span;
+        p.slots = std::max(p.slots, (size_t)std::min(want, (nb + 7) / 8));
     }
+    if (p.slots == 1) p.slots = 0;
     return p;
 }
 
@@ -1034,11 +1191,12 @@ void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
     float* const pml = pacc + p.slots * a.rows * s.HQ * HD;
     if (p.tiles) {
         g.ks = p.rows_ks, g.span = p.rows_span;
-        hipLaunchKernelGGL((k_paged_rows<T, HD>), dim3((unsigned)((size_t)p.tiles * s.HK * g.ks)), dim3(256), 0, st, Q, K, V,
-                           g, big, out, pacc, pml);
+        const dim3 grid((unsigned)((size_t)p.tiles * s.HK * g.ks));
+        hipLaunchKernelGGL((k_paged_rows<T, HD>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
         launched("paged_attention");
         if (g.ks > 1) {
-            hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, 8 * s.HK), dim3(256), 0, st, g, pacc, pml, big, out);
+            hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, TILE_ROWS / 16 * s.HK), dim3(256), 0, st, g, pacc, pml,
+                               big, out);
             launched("paged_attention");
         }
     }
@@ -1050,7 +1208,9 @@ void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
             hipLaunchKernelGGL((k_paged_few<T, HD, 2>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
         launched("paged_attention");
         if (g.ks > 1) {
-            hipLaunchKernelGGL((k_paged_join_few<T, HD>), dim3(s.HK, a.B), dim3(256), 0, st, g, pacc, pml, big, out);
+            const int rows_max = (int)std::min((long long)p.few, (long long)std::min(a.max_new, a.rows) * g.G);
+            hipLaunchKernelGGL((k_paged_join_few<T, HD>), dim3(s.HK * rows_max, a.B), dim3(256), 0, st, g, pacc, pml, big, out,
+                               rows_max);
             launched("paged_attention");
         }
     }
