@@ -159,38 +159,49 @@ __device__ __forceinline__ size_t block_at(int slot, int kh, int lps, size_t pst
     return (size_t)(slot >> lps) * pstride + ((size_t)kh * (1 << (lps - 5)) + ((slot & ((1 << lps) - 1)) >> 5)) * (HD * 32);
 }
 
-constexpr int VT = 64;  // rows of a V workgroup
+constexpr int VT = 64, VD = 64;  // rows and dims of a V workgroup
 
-// Workgroups [0, nqk): q and k heads.  HD / 8 threads share a (row, head), 8 dims each; a thread takes `nh` heads of its
-// row one after the other with one set of cosines and sines (they are f32 and twice a row's bytes: fetched per head
-// they, not the rows, were what a chunk's time went to).  Workgroups from nqk: 64 rows of one kv head's V, transposed
-// through LDS so that 8 consecutive slots go out as 16 bytes.
-template <class T, int HD>
+// Workgroups [0, nv) transpose V, 64 rows of 64 dims of a kv head each, through LDS, so that 8 consecutive slots go out as
+// 16 bytes.  In the others HD / 8 threads share a row and `hpu` of its q or k heads, 8 dims each, with one set of cosines
+// and sines (they are f32 and twice a row's bytes), NH heads in flight; every load that depends on nothing is issued
+// before the first is used.
+template <class T, int HD, int NH>
 __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, int stride, int q_step,
                                                     const float* __restrict__ qw, const float* __restrict__ kw,
                                                     const float* __restrict__ rope, int rope_len,
                                                     const int* __restrict__ pos, int axes,
                                                     const uint8_t* __restrict__ axis, const int* __restrict__ slots,
                                                     int rows, int HQ, int HK, int RD, int lps, int n_pages,
-                                                    size_t pstride, int nh, int nqk, T* __restrict__ Q,
+                                                    size_t pstride, int hpu, int nv, T* __restrict__ Q,
                                                     T* __restrict__ Kp, T* __restrict__ Vp) {
     typedef typename Vec8<T>::type T8;
     constexpr int LPH = HD / 8;
     const int tid = threadIdx.x;
     const int k_off = HQ * q_step, v_off = k_off + HK * HD;
     const long long n_slots = (long long)n_pages << lps;
-    if ((int)blockIdx.x < nqk) {
-        const int gq = (HQ + nh - 1) / nh, gk = (HK + nh - 1) / nh;
-        const int unit = blockIdx.x * (256 / LPH) + tid / LPH, c = tid % LPH;
-        const int t = unit / (gq + gk), u = unit % (gq + gk);
+    if ((int)blockIdx.x >= nv) {
+        const int gq = (HQ + hpu - 1) / hpu, gk = (HK + hpu - 1) / hpu, per = gq + gk;
+        const int unit = (blockIdx.x - nv) * (256 / LPH) + tid / LPH, c = tid % LPH;
+        const int t = unit / per, u = unit % per;
         if (t >= rows) return;
-        const int slot = slots[t];
-        if (slot < 0 || slot >= n_slots) return;
         const bool isq = u < gq;
-        const int h0 = (isq ? u : u - gq) * nh, h1 = min(isq ? HQ : HK, h0 + nh);
-        const T* const src = big + (size_t)t * stride + (isq ? 0 : k_off) + 8 * c;
+        const int h0 = (isq ? u : u - gq) * hpu, heads = isq ? HQ : HK, h1 = min(heads, h0 + hpu);
+        const T* const src = big + (size_t)t * stride + (isq ? 0 : k_off);
         const int step = isq ? q_step : HD;
+        const int slot = slots[t];
+        T8 x8[NH];
+        auto load = [&](int h) {  // NH heads from h on
+#pragma unroll
+            for (int i = 0; i < NH; i++) x8[i] = *reinterpret_cast<const T8*>(src + (size_t)min(h + i, heads - 1) * step + 8 * c);
+        };
+        load(h0);
         const float* const nw = isq ? qw : kw;
+        int at[4] = {0, 0, 0, 0};  // the row's positions
+        if (RD) {
+#pragma unroll
+            for (int a = 0; a < 4; a++)
+                if (a < axes) at[a] = pos[(size_t)a * rows + t];
+        }
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) w[e] = nw ? nw[8 * c + e] : 1.f;
@@ -199,23 +210,53 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
         const bool whole = rd2 % 8 == 0;  // a chunk's partners are one other chunk
         float cs[8], sn[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int d = 8 * c + e;
-            cs[e] = 1.f, sn[e] = 0.f;
-            if (d < RD) {
-                const int j = d < rd2 ? d : d - rd2;
-                const int a = axes > 1 ? min((int)axis[j], axes - 1) : 0;
-                const int at = min(max(pos[(size_t)a * rows + t], 0), rope_len - 1);
-                const float2 v = *reinterpret_cast<const float2*>(rope + ((size_t)at * rd2 + j) * 2);
-                cs[e] = v.x;
-                sn[e] = d < rd2 ? -v.y : v.y;
+        for (int e = 0; e < 8; e++) cs[e] = 1.f, sn[e] = 0.f;
+#pragma unroll
+        for (int a = 0; a < 4; a++) at[a] = min(max(at[a], 0), rope_len - 1);
+        auto turn = [&](int e, float2 v) {
+            cs[e] = v.x;
+            sn[e] = 8 * c + e < rd2 ? -v.y : v.y;
+        };
+        if (8 * c < RD && whole) {
+            const int j = 8 * c < rd2 ? 8 * c : 8 * c - rd2;
+            if (axes == 1) {
+                typedef float F4 __attribute__((ext_vector_type(4), aligned(8)));
+                const F4* const p = reinterpret_cast<const F4*>(rope + ((size_t)at[0] * rd2 + j) * 2);
+                F4 v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = p[e];
+#pragma unroll
+                for (int e = 0; e < 4; e++) turn(2 * e, float2{v[e][0], v[e][1]}), turn(2 * e + 1, float2{v[e][2], v[e][3]});
+            } else {
+                uint64_t ax;
+                __builtin_memcpy(&ax, axis + j, 8);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int b = min((int)(ax >> (8 * e) & 255), axes - 1);
+                    const int p = b == 0 ? at[0] : b == 1 ? at[1] : b == 2 ? at[2] : at[3];
+                    turn(e, *reinterpret_cast<const float2*>(rope + ((size_t)p * rd2 + j + e) * 2));
+                }
+            }
+        } else if (8 * c < RD) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = min(8 * c + e, RD - 1), j = d < rd2 ? d : d - rd2, b = axes > 1 ? min((int)axis[j], axes - 1) : 0;
+                const int p = b == 0 ? at[0] : b == 1 ? at[1] : b == 2 ? at[2] : at[3];
+                turn(e, *reinterpret_cast<const float2*>(rope + ((size_t)p * rd2 + j) * 2));
             }
         }
-        for (int h = h0; h < h1; h++) {
-            const T8 x8 = *reinterpret_cast<const T8*>(src + (size_t)h * step);
+        if (slot < 0 || slot >= n_slots) return;
+        for (int hb = h0; hb < h1; hb += NH) {
+        T8 now[NH];
+#pragma unroll
+        for (int i = 0; i < NH; i++) now[i] = x8[i];
+        if (hb + NH < h1) load(hb + NH);
+#pragma unroll
+        for (int i = 0; i < NH; i++) {
+            const int h = hb + i;
             float x[8], ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = (float)x8[e], ss += x[e] * x[e];
+            for (int e = 0; e < 8; e++) x[e] = (float)now[i][e], ss += x[e] * x[e];
             float inv = 1.f;
             if (nw) {
 #pragma unroll
@@ -226,41 +267,43 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
             for (int e = 0; e < 8; e++) x[e] = x[e] * inv * w[e];
             T8 y8;
             if (whole) {
-                const int s = rd2 / 8;
+                const int s = rd2 / 8, from = c < s ? c + s : c - s;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float up = __shfl(x[e], c + s, LPH), dn = __shfl(x[e], c - s, LPH);
-                    y8[e] = (T)(8 * c + e < RD ? x[e] * cs[e] + (c < s ? up : dn) * sn[e] : x[e]);
+                    const float o = __shfl(x[e], from, LPH);
+                    y8[e] = (T)(8 * c + e < RD ? x[e] * cs[e] + o * sn[e] : x[e]);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int d = 8 * c + e, o = d < rd2 ? d + rd2 : d - rd2;
                     float r = x[e];
-                    if (d < RD) r = x[e] * cs[e] + (float)src[(size_t)h * step - 8 * c + o] * inv * (nw ? nw[o] : 1.f) * sn[e];
+                    if (d < RD) r = x[e] * cs[e] + (float)src[(size_t)min(h, heads - 1) * step + o] * inv * (nw ? nw[o] : 1.f) * sn[e];
                     y8[e] = (T)r;
                 }
             }
+            if (h >= h1) break;
             if (isq) *reinterpret_cast<T8*>(Q + ((size_t)t * HQ + h) * HD + 8 * c) = y8;
             else
                 *reinterpret_cast<T8*>(Kp + block_at<HD>(slot, h, lps, pstride) + (c / 4) * 1024 + (slot & 31) * 32 +
                                        8 * (c % 4)) = y8;
         }
+        }
         return;
     }
-    __shared__ __align__(16) T tile[VT][HD + 8];
+    __shared__ __align__(16) T tile[VT][VD + 8];
     __shared__ int sl[VT];
     __shared__ int first, whole8[VT / 8 + 1];
-    const int v = blockIdx.x - nqk, kh = v % HK, t0 = v / HK * VT, nt = min(VT, rows - t0);
+    const int v = blockIdx.x, d0 = v % (HD / VD) * VD, kh = v / (HD / VD) % HK, t0 = v / (HD / VD) / HK * VT, nt = min(VT, rows - t0);
     if (tid < VT) {
         const int s = tid < nt ? slots[t0 + tid] : -1;
         sl[tid] = s >= 0 && s < n_slots ? s : -1;
         const unsigned long long any = __ballot(sl[tid] >= 0);
         if (tid == 0) first = any ? __ffsll((long long)any) - 1 : 0;
     }
-    for (int i = tid; i < nt * LPH; i += 256)
-        *reinterpret_cast<T8*>(&tile[i / LPH][8 * (i % LPH)]) =
-            *reinterpret_cast<const T8*>(big + (size_t)(t0 + i / LPH) * stride + v_off + kh * HD + 8 * (i % LPH));
+    for (int i = tid; i < nt * (VD / 8); i += 256)
+        *reinterpret_cast<T8*>(&tile[i / (VD / 8)][8 * (i % (VD / 8))]) =
+            *reinterpret_cast<const T8*>(big + (size_t)(t0 + i / (VD / 8)) * stride + v_off + kh * HD + d0 + 8 * (i % (VD / 8)));
     __syncthreads();
     // octets of rows cut where the slots of the first request here are multiples of 8
     const int s0 = sl[first], cut = s0 < 0 ? 0 : ((first - s0) & 7) - 8;
@@ -271,16 +314,16 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
         whole8[tid] = ok;
     }
     __syncthreads();
-    for (int i = tid; i < HD * (VT / 8 + 1); i += 256) {
+    for (int i = tid; i < VD * (VT / 8 + 1); i += 256) {
         const int d = i / (VT / 8 + 1), o = i % (VT / 8 + 1), r0 = cut + 8 * o;
         if (whole8[o]) {
             T8 y;
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = tile[r0 + e][d];
-            *reinterpret_cast<T8*>(Vp + block_at<HD>(sl[r0], kh, lps, pstride) + d * 32 + (sl[r0] & 31)) = y;
+            *reinterpret_cast<T8*>(Vp + block_at<HD>(sl[r0], kh, lps, pstride) + (d0 + d) * 32 + (sl[r0] & 31)) = y;
         } else {
             for (int r = max(r0, 0); r < min(r0 + 8, nt); r++)
-                if (sl[r] >= 0) Vp[block_at<HD>(sl[r], kh, lps, pstride) + d * 32 + (sl[r] & 31)] = tile[r][d];
+                if (sl[r] >= 0) Vp[block_at<HD>(sl[r], kh, lps, pstride) + (d0 + d) * 32 + (sl[r] & 31)] = tile[r][d];
         }
     }
 }
@@ -1166,16 +1209,23 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
 
 template <class T, int HD>
 void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
-    constexpr int PER = 256 / (HD / 8);  // (row, head) units of a workgroup
-    // heads per thread: as many as leave about four workgroups per CU
-    int nh = 1;
-    while (nh < 8 && (size_t)a.rows * (s.HQ + s.HK) / (2 * nh) / PER >= 1024) nh *= 2;
-    const size_t units = (size_t)a.rows * ((s.HQ + nh - 1) / nh + (s.HK + nh - 1) / nh);
-    const size_t nqk = (units + PER - 1) / PER, nv = (size_t)((a.rows + VT - 1) / VT) * s.HK;
-    hipLaunchKernelGGL((k_paged_prep<T, HD>), dim3((unsigned)(nqk + nv)), dim3(256), 0, st, static_cast<const T*>(a.big),
-                       a.stride, a.gated ? 2 * HD : HD, a.qw, a.kw, a.rope, a.rope_len, a.pos, a.axes, a.axis, a.slots,
-                       a.rows, s.HQ, s.HK, a.RD, log2i(s.PS), s.n_pages, s.pstride, nh, (int)nqk, static_cast<T*>(a.Q),
-                       static_cast<T*>(a.Kp), static_cast<T*>(a.Vp));
+    constexpr int PER = 256 / (HD / 8);  // (row, heads) units of a workgroup
+    auto groups = [&](int hpu) { return ((size_t)a.rows * ((s.HQ + hpu - 1) / hpu + (s.HK + hpu - 1) / hpu) + PER - 1) / PER; };
+    // heads per thread: as many as leave a workgroup per CU (us at 1, 2, 4, 8: 32 and 8 heads of 128, three axes, 256 rows
+    // 8.4 7.1 7.0 9.3, 1024 rows 21.4 15.0 13.4 12.9, 4099 rows 71 45 36 31; the engine's heads, 2048 rows 18.0 13.4 13.0 12.4)
+    int hpu = 8;
+    while (hpu > 1 && groups(hpu) < 300) hpu /= 2;
+    const int nh = std::min(hpu, 4);
+    const size_t nv = (size_t)((a.rows + VT - 1) / VT) * s.HK * (HD / VD);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(nv + groups(hpu))), dim3(256), 0, st, static_cast<const T*>(a.big), a.stride,
+                           a.gated ? 2 * HD : HD, a.qw, a.kw, a.rope, a.rope_len, a.pos, a.axes, a.axis, a.slots, a.rows, s.HQ,
+                           s.HK, a.RD, log2i(s.PS), s.n_pages, s.pstride, hpu, (int)nv, static_cast<T*>(a.Q),
+                           static_cast<T*>(a.Kp), static_cast<T*>(a.Vp));
+    };
+    if (nh == 4) go(k_paged_prep<T, HD, 4>);
+    else if (nh == 2) go(k_paged_prep<T, HD, 2>);
+    else go(k_paged_prep<T, HD, 1>);
     launched("paged_prep");
 }
 
