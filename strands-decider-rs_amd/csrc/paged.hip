@@ -358,12 +358,22 @@ constexpr float P_UP = 8.0f, RAISE = 6.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The larger of a value and the one 32 lanes away.
+// The largest of a value and the one 32 lanes away, and of the four 16 lanes apart.  (The swap of a register with itself
+// leaves one half's values in both halves of each result.)
 __device__ __forceinline__ float max_halves(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
     const uint32_t lo = sw[0], hi = sw[1];
     return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+#else
+    return x;
+#endif
+}
+__device__ __forceinline__ float max_quarters(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto sw = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t lo = sw[0], hi = sw[1];
+    return max_halves(fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)));
 #else
     return x;
 #endif
@@ -461,17 +471,28 @@ __device__ __forceinline__ u32x2 gate4(const T* big, size_t at) {
 // ---- few rows: up to 16 NR rows per (request, kv head), one new token's heads or a short draft's ----
 //
 // Bound by the cache's bytes: each is read once and used for a handful of rows.  The keys are split over workgroups
-// (span blocks of 32 each) and inside one over its 4 waves, block by block; a wave loads a block's K and V straight
+// (span blocks of 32 each) and inside one over its NW waves, block by block; a wave loads a block's K and V straight
 // into registers in MFMA operand order, one block ahead of the one it works on.
-template <class T, int HD, int NR>
-__global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, const T* __restrict__ Kp,
+// 16 bytes per lane; ONCE: of data that nothing reads again before it has left the caches (the non-temporal hint).
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t voff, uint32_t soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (ONCE) return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 2));
+#endif
+    return buf_b128(r, voff, soff);
+}
+
+template <int HD, int NR>
+constexpr int few_waves() { return HD * NR <= 128 ? 8 : 4; }  // 8 where two fit a SIMD's registers
+template <class T, int HD, int NR, bool ONCE>
+__global__ __launch_bounds__((64 * few_waves<HD, NR>())) void k_paged_few(const T* __restrict__ Q, const T* __restrict__ Kp,
                                                    const T* __restrict__ Vp, AttnArgs a, const T* __restrict__ big,
                                                    T* __restrict__ out, float* __restrict__ pacc,
                                                    float* __restrict__ pml) {
     typedef typename Vec8<T>::type T8;
-    constexpr int NS = HD / 32, ND = HD / 16, R = 16 * NR;
-    __shared__ float Om[4][R][HD + 4];
-    __shared__ float Mm[4][R], Lm[4][R];
+    constexpr int NS = HD / 32, ND = HD / 16, R = 16 * NR, NW = few_waves<HD, NR>(), D = 2;
+    __shared__ float Om[NW][R][HD + 4];
+    __shared__ float Mm[NW][R], Lm[NW][R];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fq = lane & 15, fg = lane >> 4;
     const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
@@ -481,7 +502,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
     // keys [lo, hi) are seen by some row; this workgroup's blocks of them
     const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
     const int blk0 = (lo >> 5) + z * a.span, blk1 = z + 1 < a.ks ? min((hi + 31) >> 5, blk0 + a.span) : (hi + 31) >> 5;
-    const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + 3) >> 2 : 0;
+    const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + NW - 1) / NW : 0;
     int jlo[NR], jhi[NR];  // keys [jlo, jhi) are seen by this lane's row
     T8 qf[NR][NS];
 #pragma unroll
@@ -500,7 +521,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
     const int lbpp = a.lps - 5;
     const int* const tb = a.table + (size_t)b * a.max_blocks;
     auto entries = [&](int i) {  // lane l: the table entry of the wave's block i + l
-        return tb[min((first + 4 * (i + lane)) >> lbpp, a.max_blocks - 1)];
+        return tb[min((first + NW * (i + lane)) >> lbpp, a.max_blocks - 1)];
     };
     int ids = cnt ? entries(0) : 0, ids2 = cnt > 64 ? entries(64) : 0;
     const uint32_t kofs = ((8 * (fq >> 2) + (fq & 3)) * 32 + fg * 8) * 2, vofs = (fq * 32 + fg * 8) * 2;
@@ -517,47 +538,55 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
         u32x4 k[2][NS], v[ND];
         bool there;
     };
-    auto load = [&](int i, Blk& x) {
-        const int page = __builtin_amdgcn_readlane(ids, i & 63), blk = first + 4 * i;
+    auto load = [&](int i, Blk& x) INL {
+        const int page = __builtin_amdgcn_readlane(ids, i & 63), blk = first + NW * i;
         x.there = i < cnt && (unsigned)page < (unsigned)a.n_pages;
         const size_t at = x.there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
         const Rsrc rk = make_rsrc(Kp + at, x.there ? HD * 64u : 0u), rv = make_rsrc(Vp + at, x.there ? HD * 64u : 0u);
 #pragma unroll
         for (int s = 0; s < NS; s++)
 #pragma unroll
-            for (int tt = 0; tt < 2; tt++) x.k[tt][s] = buf_b128(rk, kofs + tt * 256, s * 2048);
+            for (int tt = 0; tt < 2; tt++) x.k[tt][s] = load16<ONCE>(rk, kofs + tt * 256, s * 2048);
 #pragma unroll
-        for (int d = 0; d < ND; d++) x.v[d] = buf_b128(rv, vofs, d * 1024);
+        for (int d = 0; d < ND; d++) x.v[d] = load16<ONCE>(rv, vofs, d * 1024);
     };
-    auto work = [&](int i, Blk& x) {
-        const int j0 = (first + 4 * i) * 32;
+    auto work = [&](int i, Blk& x) INL {
+        const int j0 = (first + NW * i) * 32;
         const bool open = x.there && j0 >= open0 && j0 + 32 <= open1;
-        T8 pf[NR];
+        f32x4 s2[NR][2];
 #pragma unroll
-        for (int u = 0; u < NR; u++) {
-            f32x4 s2[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        for (int u = 0; u < NR; u++) s2[u][0] = s2[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int s = 0; s < NS; s++)
+        for (int s = 0; s < NS; s++)
 #pragma unroll
-                for (int tt = 0; tt < 2; tt++)
-                    s2[tt] = Num<T>::mfma16(__builtin_bit_cast(T8, x.k[tt][s]), qf[u][s], s2[tt]);
-            float sv[8], tmax = -INFINITY;
+            for (int tt = 0; tt < 2; tt++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) sv[e] = s2[e >> 2][e & 3] * a.c;
-            if (!open) {
+                for (int u = 0; u < NR; u++)
+                    s2[u][tt] = Num<T>::mfma16(__builtin_bit_cast(T8, x.k[tt][s]), qf[u][s], s2[u][tt]);
+        if (!open) {
+#pragma unroll
+            for (int u = 0; u < NR; u++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int j = j0 + 8 * fg + e;
                     const bool keep = x.there & (j >= jlo[u]) & (j < jhi[u]);
-                    sv[e] = keep ? sv[e] : -INFINITY;
+                    s2[u][e >> 2][e & 3] = keep ? s2[u][e >> 2][e & 3] : -INFINITY;
                 }
-            }
+        }
+        float tmax[NR];
+        bool up = false;
 #pragma unroll
-            for (int e = 0; e < 8; e++) tmax = fmaxf(tmax, sv[e]);
-            tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
-            tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
-            if (__any(tmax > m[u] + RAISE)) {
-                const float mn = fmaxf(m[u], tmax), f = m[u] == -INFINITY ? 0.f : exp2_fast(m[u] - mn);
+        for (int u = 0; u < NR; u++) {
+            tmax[u] = s2[u][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) tmax[u] = fmaxf(tmax[u], s2[u][e >> 2][e & 3]);
+            tmax[u] = max_quarters(tmax[u]) * a.c;
+            up |= tmax[u] > m[u] + RAISE;
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (int u = 0; u < NR; u++) {
+                const float mn = fmaxf(m[u], tmax[u]), f = m[u] == -INFINITY ? 0.f : exp2_fast(m[u] - mn);
                 m[u] = mn;
                 l[u] *= f;
 #pragma unroll
@@ -565,10 +594,14 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[u][d][e] *= f;
             }
+        }
+        T8 pf[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
             const float nm = m[u] == -INFINITY ? 0.f : P_UP - m[u];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float p = exp2_fast(sv[e] + nm);
+                const float p = exp2_fast(__builtin_fmaf(s2[u][e >> 2][e & 3], a.c, nm));
                 l[u] += p;
                 pf[u][e] = (T)p;
             }
@@ -588,31 +621,32 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
 #pragma unroll
             for (int u = 0; u < NR; u++) acc[u][d] = Num<T>::mfma16(__builtin_bit_cast(T8, x.v[d]), pf[u], acc[u][d]);
     };
-    Blk A, B2;
-    load(0, A);
-    auto ahead = [&](int i) {  // before block i's load: its window of table entries
-        if ((i & 63) == 0) {
+    // D blocks' registers: block i is in set i % D, and while it is worked on the D - 1 after it are on their way
+    Blk set[D];
+    auto ahead = [&](int i) INL {  // before block i's load: its window of table entries
+        if ((i & 63) == 0 && i) {
             ids = ids2;
             if (i + 64 < cnt) ids2 = entries(i + 64);
         }
     };
-    for (int i = 0; i < cnt; i += 2) {
-        load(i + 1, B2);
-        __builtin_amdgcn_sched_barrier(0);
-        work(i, A);
-        __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 >= cnt) break;
-        ahead(i + 2);
-        load(i + 2, A);
-        __builtin_amdgcn_sched_barrier(0);
-        work(i + 1, B2);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < D - 1; u++) load(u, set[u]);
+    for (int i = 0; i < cnt; i += D) {
+#pragma unroll
+        for (int u = 0; u < D; u++) {
+            if (u && i + u >= cnt) break;
+            ahead(i + u + D - 1);
+            load(i + u + D - 1, set[(u + D - 1) % D]);
+            __builtin_amdgcn_sched_barrier(0);
+            work(i + u, set[u]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     if (__builtin_expect(rare, 0)) {  // add_seen: see above
 #pragma unroll 1
         for (int i = 0; i < cnt; i++) {
             // (every block: a second time what a product gave already changes neither an infinity nor a NaN)
-            const int blk = first + 4 * i, page = tb[blk >> lbpp], j0 = 32 * blk;
+            const int blk = first + NW * i, page = tb[blk >> lbpp], j0 = 32 * blk;
             if ((unsigned)page >= (unsigned)a.n_pages) continue;
             const T* const v = Vp + (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32);
 #pragma unroll 1
@@ -630,7 +664,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
                     }
         }
     }
-    // the 4 waves' states side by side: acc[u][d][e] is O[row 16 u + fq][dim 16 d + 4 fg + e]
+    // the waves' states side by side: acc[u][d][e] is O[row 16 u + fq][dim 16 d + 4 fg + e]
 #pragma unroll
     for (int u = 0; u < NR; u++) {
         l[u] += __shfl_xor(l[u], 16);
@@ -640,14 +674,14 @@ __global__ __launch_bounds__(256) void k_paged_few(const T* __restrict__ Q, cons
         if (fg == 0) Mm[wv][16 * u + fq] = m[u], Lm[wv][16 * u + fq] = l[u];
     }
     __syncthreads();
-    for (int i = tid; i < nrows * (HD / 4); i += 256) {
+    for (int i = tid; i < nrows * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
         float mx = -INFINITY, ls = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) mx = fmaxf(mx, Mm[w][r]);
+        for (int w = 0; w < NW; w++) mx = fmaxf(mx, Mm[w][r]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             const float lw = Lm[w][r], f = lw == 0.f ? 0.f : exp2_fast(Mm[w][r] - mx);
             ls += lw == 0.f ? 0.f : lw * f;
             const f32x4 x = *reinterpret_cast<const f32x4*>(&Om[w][r][d]);
@@ -726,6 +760,11 @@ struct Tile {
 };
 __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
     const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
+    if (a.B == 1) {
+        const int n = request(a.cu, a.kv_lens, 0, a.rows, a.max_new, a.kcap).n * a.G;
+        const int total = n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
+        return {x < total ? 0 : -1, total - 1 - x};
+    }
     auto tiles = [&](int b) {
         if (b >= a.B) return 0;
         const int n = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap).n * a.G;
@@ -1131,36 +1170,42 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
                        o + 32 * d + 8 * i);
 }
 
-// Joins the splits of k_paged_rows (at most 8): HD / 4 threads per row, 4 dims each.
+// Joins the splits of k_paged_rows: HD / 4 threads per row, 4 dims each, every load issued before the first is used.
+constexpr int MAX_ROWS_KS = 8;
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float* __restrict__ pacc,
                                                          const float* __restrict__ pml, const T* __restrict__ big,
                                                          T* __restrict__ out) {
-    constexpr int W = HD / 4, PER = 16;  // a workgroup joins 16 rows of a tile
+    constexpr int W = HD / 4, PER = 256 / W, PARTS = TILE_ROWS / PER;
     const Tile tl = find_tile(a, blockIdx.x);
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
-    constexpr int parts = TILE_ROWS / PER;
-    const int kh = blockIdx.y / parts, r0 = tl.i * TILE_ROWS + PER * (blockIdx.y % parts);
-    const int r1 = min(min(rq.n * a.G, (tl.i + 1) * TILE_ROWS), r0 + PER);
-    const size_t zs = (size_t)a.rows * a.HQ;
-    for (int i = threadIdx.x; i < (r1 - r0) * W; i += 256) {
-        const int r = r0 + i / W, t = rq.q0 + r / a.G, h = kh * a.G + r % a.G, d = 4 * (i % W);
-        const size_t row = (size_t)t * a.HQ + h;
-        float mx = -INFINITY, ls = 0.f;
-        for (int z = 0; z < a.ks; z++) mx = fmaxf(mx, pml[2 * (z * zs + row)]);
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int z = 0; z < a.ks; z++) {
-            const float2 ml = *reinterpret_cast<const float2*>(pml + 2 * (z * zs + row));
-            const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
-            const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - mx);
-            ls += ml.y == 0.f ? 0.f : ml.y * f;
+    const int kh = blockIdx.y / PARTS, r = tl.i * TILE_ROWS + PER * (blockIdx.y % PARTS) + threadIdx.x / W;
+    if (r >= rq.n * a.G) return;
+    const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G, d = 4 * (threadIdx.x % W);
+    const size_t row = (size_t)t * a.HQ + h, zs = (size_t)a.rows * a.HQ;
+    float2 ml[MAX_ROWS_KS];
+    f32x4 x[MAX_ROWS_KS];
+    const u32x2 gate = gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] += ml.y == 0.f ? 0.f : x[e] * f;
-        }
-        finish4<T>(o, ls, big, gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d), out + row * HD + d);
+    for (int z = 0; z < MAX_ROWS_KS; z++) {
+        const size_t at = min(z, a.ks - 1) * zs + row;
+        ml[z] = *reinterpret_cast<const float2*>(pml + 2 * at);
+        x[z] = *reinterpret_cast<const f32x4*>(pacc + at * HD + d);
     }
+    float mx = -INFINITY, ls = 0.f;
+#pragma unroll
+    for (int z = 0; z < MAX_ROWS_KS; z++) mx = fmaxf(mx, ml[z].x);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int z = 0; z < MAX_ROWS_KS; z++) {
+        if (z >= a.ks || ml[z].y == 0.f) continue;
+        const float f = exp2_fast(ml[z].x - mx);
+        ls += ml[z].y * f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += x[z][e] * f;
+    }
+    finish4<T>(o, ls, big, gate, out + row * HD + d);
 }
 
 int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
@@ -1170,6 +1215,7 @@ struct Plan {
     int nr = 0;                      // 16-row groups of k_paged_few, 0: not launched
     int few = 0;                     // requests with up to this many rows (new tokens times G) are its own
     int few_ks = 1, few_span = 1;    // splits, and blocks of 32 keys in each
+    bool once = false;               // its cache is read past the last-level cache
     int tiles = 0;                   // of k_paged_rows (an upper bound), 0: not launched
     int rows_ks = 1, rows_span = 1;  // splits, and blocks in each
     size_t slots = 0;                // partial results of [rows][HQ] that they need at most, whatever the window
@@ -1189,16 +1235,26 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
     };
     if (p.nr) {
         const int nb = blocks(std::max(1, p.few / G));
-        const int want = std::min(MAX_KS, std::max(1, 256 / (B * s.HK)));
+        // Two workgroups per CU want keys to read, but the parts cost a join: no split of few elements, and none where the
+        // unsplit workgroups draw most of the bandwidth already. us unsplit and split, at n keys of each request:
+        // 16 workgroups, dims 64: 1000 7.0 7.8, 2000 10.5 7.9; 128: 500 7.6 9.1, 1000 11.1 9.2; 256: 500 11.6 11.1
+        // 128 workgroups, dims 64: 8000 39 44; 128: 4000 40 46, 8000 90 81; 256: 2000 41 46, 4000 93 82
+        const int wgs = B * s.HK;
+        const double elems = 32.0 * nb * s.HD;
+        const int want = elems < (wgs < 128 ? 100e3 : 768e3) ? 1 : std::min(MAX_KS, std::max(1, 256 / wgs));
         p.few_span = std::max(8, ((nb + want - 1) / want + 3) / 4 * 4);
         p.few_ks = (nb + p.few_span - 1) / p.few_span;
         p.slots = std::min(want, (nb + 7) / 8);
+        // beyond the 256 MB that stay in the last-level cache a layer's keys are gone before they are read again (64
+        // requests of 1000 to 8191 rows 159 -> 142 us with the hint, two of 90 and 131 thousand 89 -> 78; 85 MB, read again
+        // and again, 22 -> 24)
+        p.once = (size_t)B * nb * s.HK * s.HD * 128 > (size_t(256) << 20);
     }
     if (most > p.few) {
         const long long all = (long long)rows * G;
         p.tiles = (int)(all / TILE_ROWS) + B;
         const int nb = blocks(TILE_ROWS / G + 2);
-        const int want = (int)std::min(8ll, std::max(1ll, 256 / std::max(1ll, all / TILE_ROWS * s.HK)));
+        const int want = (int)std::min((long long)MAX_ROWS_KS, std::max(1ll, 256ll / std::max(1ll, all / TILE_ROWS * s.HK)));
         p.rows_span = std::max(8, ((nb + want - 1) / want + 1) / 2 * 2);
         p.rows_ks = (nb + p.rows_span - 1) / p.rows_span;
         p.slots = std::max(p.slots, (size_t)std::min(want, (nb + 7) / 8));
@@ -1245,7 +1301,7 @@ void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
         hipLaunchKernelGGL((k_paged_rows<T, HD>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
         launched("paged_attention");
         if (g.ks > 1) {
-            hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, TILE_ROWS / 16 * s.HK), dim3(256), 0, st, g, pacc, pml,
+            hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, TILE_ROWS / (1024 / HD) * s.HK), dim3(256), 0, st, g, pacc, pml,
                                big, out);
             launched("paged_attention");
         }
@@ -1253,9 +1309,10 @@ void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
     if (p.nr) {
         g.ks = p.few_ks, g.span = p.few_span;
         const dim3 grid(s.HK * g.ks, a.B);
-        if (p.nr == 1) hipLaunchKernelGGL((k_paged_few<T, HD, 1>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
+        auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, Q, K, V, g, big, out, pacc, pml); };
+        if (p.nr == 1) p.once ? go(k_paged_few<T, HD, 1, true>, few_waves<HD, 1>()) : go(k_paged_few<T, HD, 1, false>, few_waves<HD, 1>());
         else if constexpr (HD < 256)
-            hipLaunchKernelGGL((k_paged_few<T, HD, 2>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
+            p.once ? go(k_paged_few<T, HD, 2, true>, few_waves<HD, 2>()) : go(k_paged_few<T, HD, 2, false>, few_waves<HD, 2>());
         launched("paged_attention");
         if (g.ks > 1) {
             const int rows_max = (int)std::min((long long)p.few, (long long)std::min(a.max_new, a.rows) * g.G);
