@@ -444,7 +444,9 @@ __device__ __forceinline__ Req request(const int* __restrict__ cu, const int* __
 // The launch's arguments that all attention kernels share.
 struct AttnArgs {
     const int *table, *cu, *kv_lens;
-    int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, few, ks, span, stride;
+    int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, stride;
+    int few, few_ks, few_span;       // rows of a request that k_paged_few does, its splits and the blocks in each
+    int tiles, rows_ks, rows_span;   // of k_paged_rows
     float c;  // scale log2(e)
     size_t pstride;
 };
@@ -484,24 +486,24 @@ __device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t voff, uint32_t soff) {
 
 template <int HD, int NR>
 constexpr int few_waves() { return HD * NR <= 128 ? 8 : 4; }  // 8 where two fit a SIMD's registers
-template <class T, int HD, int NR, bool ONCE>
-__global__ __launch_bounds__((64 * few_waves<HD, NR>())) void k_paged_few(const T* __restrict__ Q, const T* __restrict__ Kp,
-                                                   const T* __restrict__ Vp, AttnArgs a, const T* __restrict__ big,
-                                                   T* __restrict__ out, float* __restrict__ pacc,
-                                                   float* __restrict__ pml) {
+// Workgroup x of request b, of NW waves: om(w) gives LDS of R x HD floats for each wave, Ms and Ls are R of them per wave.
+template <class T, int HD, int NR, bool ONCE, int NW, class Om>
+__device__ __forceinline__ void few_part(const int x, const int b, const T* __restrict__ Q, const T* __restrict__ Kp,
+                                         const T* __restrict__ Vp, const AttnArgs& a, const T* __restrict__ big,
+                                         T* __restrict__ out, float* __restrict__ pacc, float* __restrict__ pml, Om om,
+                                         float* Ms, float* Ls) {
     typedef typename Vec8<T>::type T8;
-    constexpr int NS = HD / 32, ND = HD / 16, R = 16 * NR, NW = few_waves<HD, NR>(), D = 2;
-    __shared__ float Om[NW][R][HD + 4];
-    __shared__ float Mm[NW][R], Lm[NW][R];
+    constexpr int NS = HD / 32, ND = HD / 16, R = 16 * NR, D = 2;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fq = lane & 15, fg = lane >> 4;
-    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
+    const int kh = x % a.HK, z = x / a.HK;
     const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
     const int nrows = rq.n * a.G;
     if (nrows == 0 || nrows > a.few) return;
     // keys [lo, hi) are seen by some row; this workgroup's blocks of them
     const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
-    const int blk0 = (lo >> 5) + z * a.span, blk1 = z + 1 < a.ks ? min((hi + 31) >> 5, blk0 + a.span) : (hi + 31) >> 5;
+    const int blk0 = (lo >> 5) + z * a.few_span;
+    const int blk1 = z + 1 < a.few_ks ? min((hi + 31) >> 5, blk0 + a.few_span) : (hi + 31) >> 5;
     const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + NW - 1) / NW : 0;
     int jlo[NR], jhi[NR];  // keys [jlo, jhi) are seen by this lane's row
     T8 qf[NR][NS];
@@ -664,33 +666,35 @@ __global__ __launch_bounds__((64 * few_waves<HD, NR>())) void k_paged_few(const 
                     }
         }
     }
-    // the waves' states side by side: acc[u][d][e] is O[row 16 u + fq][dim 16 d + 4 fg + e]
+    // the waves' states side by side: acc[u][d][e] is O[row 16 u + fq][dim 16 d + 4 fg + e].  (4 dims
+    // at their place ^ row % 16, so that neither side meets a bank twice)
+    float* const mine = om(wv);
 #pragma unroll
     for (int u = 0; u < NR; u++) {
         l[u] += __shfl_xor(l[u], 16);
         l[u] += __shfl_xor(l[u], 32);
 #pragma unroll
-        for (int d = 0; d < ND; d++) *reinterpret_cast<f32x4*>(&Om[wv][16 * u + fq][16 * d + 4 * fg]) = acc[u][d];
-        if (fg == 0) Mm[wv][16 * u + fq] = m[u], Lm[wv][16 * u + fq] = l[u];
+        for (int d = 0; d < ND; d++) *reinterpret_cast<f32x4*>(mine + (16 * u + fq) * HD + 4 * ((4 * d + fg) ^ fq)) = acc[u][d];
+        if (fg == 0) Ms[wv * R + 16 * u + fq] = m[u], Ls[wv * R + 16 * u + fq] = l[u];
     }
     __syncthreads();
     for (int i = tid; i < nrows * (HD / 4); i += 64 * NW) {
         const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
         float mx = -INFINITY, ls = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) mx = fmaxf(mx, Mm[w][r]);
+        for (int w = 0; w < NW; w++) mx = fmaxf(mx, Ms[w * R + r]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float lw = Lm[w][r], f = lw == 0.f ? 0.f : exp2_fast(Mm[w][r] - mx);
+            const float lw = Ls[w * R + r], f = lw == 0.f ? 0.f : exp2_fast(Ms[w * R + r] - mx);
             ls += lw == 0.f ? 0.f : lw * f;
-            const f32x4 x = *reinterpret_cast<const f32x4*>(&Om[w][r][d]);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(om(w) + r * HD + (d ^ 4 * (r & 15)));
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] += lw == 0.f ? 0.f : x[e] * f;
         }
         const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G;
         const size_t row = (size_t)t * a.HQ + h;
-        if (a.ks == 1) {
+        if (a.few_ks == 1) {
             finish4<T>(o, ls, big, gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d), out + row * HD + d);
         } else {
             const size_t pr = (size_t)z * a.rows * a.HQ + row;
@@ -698,6 +702,19 @@ __global__ __launch_bounds__((64 * few_waves<HD, NR>())) void k_paged_few(const 
             if (d == 0) pml[2 * pr] = mx, pml[2 * pr + 1] = ls;
         }
     }
+}
+
+template <class T, int HD, int NR, bool ONCE>
+__global__ __launch_bounds__((64 * few_waves<HD, NR>())) void k_paged_few(const T* __restrict__ Q, const T* __restrict__ Kp,
+                                                                          const T* __restrict__ Vp, AttnArgs a,
+                                                                          const T* __restrict__ big, T* __restrict__ out,
+                                                                          float* __restrict__ pacc,
+                                                                          float* __restrict__ pml) {
+    constexpr int NW = few_waves<HD, NR>(), R = 16 * NR;
+    __shared__ __align__(16) float Om[NW][R * HD];
+    __shared__ float Ms[NW * R], Ls[NW * R];
+    few_part<T, HD, NR, ONCE, NW>(blockIdx.x, blockIdx.y, Q, Kp, Vp, a, big, out, pacc, pml, [&](int w) { return Om[w]; }, Ms,
+                                  Ls);
 }
 
 // Joins up to 64 splits of one row and writes it: 256 threads, HD / 4 of them side by side (4 dims each), their groups
@@ -719,7 +736,7 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
     const size_t row = (size_t)t * a.HQ + h, zs = (size_t)a.rows * a.HQ;
     const u32x2 gate = gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d);
     // (every wave for itself, the same)
-    const float2 ml = lane < a.ks ? *reinterpret_cast<const float2*>(pml + 2 * (lane * zs + row)) : float2{-INFINITY, 0.f};
+    const float2 ml = lane < a.few_ks ? *reinterpret_cast<const float2*>(pml + 2 * (lane * zs + row)) : float2{-INFINITY, 0.f};
     float mx = ml.x;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
@@ -731,7 +748,7 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
     __syncthreads();
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int z = tid / W; z < a.ks; z += NG) {
+    for (int z = tid / W; z < a.few_ks; z += NG) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
         const float w = wt[z];
 #pragma unroll
@@ -792,7 +809,11 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
     return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(x)};
 }
 
-template <class T, int HD>
+// FEW (2: with the non-temporal hint): the launch ends with the workgroups of the requests with few rows, which would
+// otherwise wait for the last tile while most of the chip is idle.  us in a launch of their own and in this one: a chunk
+// of 1501 tokens and 40 single ones, window 1024, 16 and 4 heads of 128 dims 42.8 and 31.1; 512 tokens among 64 single
+// ones, 32 and 8 heads 186 and 174; 1024 among 32, 8 and 2 heads of 256 dims 85.6 and 61.6.
+template <class T, int HD, int FEW>
 __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* __restrict__ Q, const T* __restrict__ Kp,
                                                        const T* __restrict__ Vp, AttnArgs a, const T* __restrict__ big,
                                                        T* __restrict__ out, float* __restrict__ pacc,
@@ -807,8 +828,18 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     __shared__ int rare;  // some value was taken as 0
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
-    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK % a.ks;
-    const Tile tl = find_tile(a, blockIdx.x / (a.HK * a.ks));
+    if constexpr (FEW != 0) {
+        const int x = (int)blockIdx.x - a.tiles * a.HK * a.rows_ks, per = a.HK * a.few_ks;
+        if (x >= 0) {  // (a wave's states fit a block's buffer)
+            few_part<T, HD, 1, FEW == 2, 4>(
+                x % per, x / per, Q, Kp, Vp, a, big, out, pacc, pml,
+                [&](int w) { return reinterpret_cast<float*>(w & 2 ? (w & 1 ? K3 : K2) : (w & 1 ? K1 : K0)); },
+                reinterpret_cast<float*>(V0), reinterpret_cast<float*>(V1));
+            return;
+        }
+    }
+    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK % a.rows_ks;
+    const Tile tl = find_tile(a, blockIdx.x / (a.HK * a.rows_ks));
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const int nrows = rq.n * a.G, r0 = tl.i * TILE_ROWS, r1 = min(nrows, r0 + TILE_ROWS);
@@ -817,7 +848,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     // keys seen by some row of the workgroup, and this split's blocks of them
     const int hi = min(rq.p0 + (r1 - 1) / a.G + 1, rq.kcap);
     const int lo = a.window ? max(0, rq.p0 + r0 / a.G - a.window + 1) : 0;
-    const int blk0 = (lo >> 5) + z * a.span, blk1 = z + 1 < a.ks ? min((hi + 31) >> 5, blk0 + a.span) : (hi + 31) >> 5;
+    const int blk0 = (lo >> 5) + z * a.rows_span, blk1 = z + 1 < a.rows_ks ? min((hi + 31) >> 5, blk0 + a.rows_span) : (hi + 31) >> 5;
     const int nb = max(blk1 - blk0, 0);
     // the lane's row (one past the last is the last again, also in the output) and the keys [jlo, jhi) that it sees
     const int r = min(w0 + c, r1 - 1), t = r / a.G, h = kh * a.G + r % a.G;
@@ -1138,7 +1169,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     // acc[d][e] is O[row c][dim 32 d + 8 (e / 4) + 4 g + e % 4]
     l += __shfl_xor(l, 32);
     const size_t row = (size_t)(rq.q0 + t) * a.HQ + h, pr = (size_t)z * a.rows * a.HQ + row;
-    if (a.ks > 1) {
+    if (a.rows_ks > 1) {
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -1189,7 +1220,7 @@ __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float
     const u32x2 gate = gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d);
 #pragma unroll
     for (int z = 0; z < MAX_ROWS_KS; z++) {
-        const size_t at = min(z, a.ks - 1) * zs + row;
+        const size_t at = min(z, a.rows_ks - 1) * zs + row;
         ml[z] = *reinterpret_cast<const float2*>(pml + 2 * at);
         x[z] = *reinterpret_cast<const f32x4*>(pacc + at * HD + d);
     }
@@ -1199,7 +1230,7 @@ __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int z = 0; z < MAX_ROWS_KS; z++) {
-        if (z >= a.ks || ml[z].y == 0.f) continue;
+        if (z >= a.rows_ks || ml[z].y == 0.f) continue;
         const float f = exp2_fast(ml[z].x - mx);
         ls += ml[z].y * f;
 #pragma unroll
@@ -1288,38 +1319,46 @@ void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
 template <class T, int HD>
 void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
     const Plan p = plan_attn(s, a.B, a.rows, a.max_new, a.max_kv, a.window);
-    AttnArgs g{a.table, a.cu, a.kv_lens, a.max_blocks, a.B, a.rows, s.HQ, s.HK, s.HQ / s.HK, log2i(s.PS), s.n_pages,
-               a.max_new, a.max_kv, a.window, p.few, 1, 1, a.stride, a.scale * LOG2E, s.pstride};
+    const AttnArgs g{a.table, a.cu, a.kv_lens, a.max_blocks, a.B, a.rows, s.HQ, s.HK, s.HQ / s.HK, log2i(s.PS), s.n_pages,
+                     a.max_new, a.max_kv, a.window, a.stride, p.few, p.few_ks, p.few_span, p.tiles, p.rows_ks, p.rows_span,
+                     a.scale * LOG2E, s.pstride};
     const T *Q = static_cast<const T*>(a.Q), *K = static_cast<const T*>(a.Kp), *V = static_cast<const T*>(a.Vp),
             *big = static_cast<const T*>(a.big);
     T* const out = static_cast<T*>(a.out);
     float* const pacc = static_cast<float*>(a.ws);
     float* const pml = pacc + p.slots * a.rows * s.HQ * HD;
-    if (p.tiles) {
-        g.ks = p.rows_ks, g.span = p.rows_span;
-        const dim3 grid((unsigned)((size_t)p.tiles * s.HK * g.ks));
-        hipLaunchKernelGGL((k_paged_rows<T, HD>), grid, dim3(256), 0, st, Q, K, V, g, big, out, pacc, pml);
+    const size_t tiles = (size_t)p.tiles * s.HK * p.rows_ks, parts = (size_t)a.B * s.HK * p.few_ks;
+    const bool both = p.tiles && p.nr == 1 && tiles + parts < (size_t(1) << 31);
+    auto launch = [&](auto kernel, dim3 grid, int threads) {
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, Q, K, V, g, big, out, pacc, pml);
         launched("paged_attention");
-        if (g.ks > 1) {
-            hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, TILE_ROWS / (1024 / HD) * s.HK), dim3(256), 0, st, g, pacc, pml,
-                               big, out);
-            launched("paged_attention");
+    };
+    if (both) {
+        if (p.once) launch(k_paged_rows<T, HD, 2>, dim3((unsigned)(tiles + parts)), 256);
+        else launch(k_paged_rows<T, HD, 1>, dim3((unsigned)(tiles + parts)), 256);
+    } else {
+        if (p.tiles) launch(k_paged_rows<T, HD, 0>, dim3((unsigned)tiles), 256);
+        const dim3 grid(s.HK * p.few_ks, a.B);
+        if (p.nr == 1) {
+            if (p.once) launch(k_paged_few<T, HD, 1, true>, grid, 64 * few_waves<HD, 1>());
+            else launch(k_paged_few<T, HD, 1, false>, grid, 64 * few_waves<HD, 1>());
         }
+        if constexpr (HD < 256)
+            if (p.nr == 2) {
+                if (p.once) launch(k_paged_few<T, HD, 2, true>, grid, 64 * few_waves<HD, 2>());
+                else launch(k_paged_few<T, HD, 2, false>, grid, 64 * few_waves<HD, 2>());
+            }
     }
-    if (p.nr) {
-        g.ks = p.few_ks, g.span = p.few_span;
-        const dim3 grid(s.HK * g.ks, a.B);
-        auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, Q, K, V, g, big, out, pacc, pml); };
-        if (p.nr == 1) p.once ? go(k_paged_few<T, HD, 1, true>, few_waves<HD, 1>()) : go(k_paged_few<T, HD, 1, false>, few_waves<HD, 1>());
-        else if constexpr (HD < 256)
-            p.once ? go(k_paged_few<T, HD, 2, true>, few_waves<HD, 2>()) : go(k_paged_few<T, HD, 2, false>, few_waves<HD, 2>());
+    if (p.rows_ks > 1) {
+        hipLaunchKernelGGL((k_paged_join_rows<T, HD>), dim3(p.tiles, TILE_ROWS / (1024 / HD) * s.HK), dim3(256), 0, st, g, pacc, pml,
+                           big, out);
         launched("paged_attention");
-        if (g.ks > 1) {
-            const int rows_max = (int)std::min((long long)p.few, (long long)std::min(a.max_new, a.rows) * g.G);
-            hipLaunchKernelGGL((k_paged_join_few<T, HD>), dim3(s.HK * rows_max, a.B), dim3(256), 0, st, g, pacc, pml, big, out,
-                               rows_max);
-            launched("paged_attention");
-        }
+    }
+    if (p.few_ks > 1) {
+        const int rows_max = (int)std::min((long long)p.few, (long long)std::min(a.max_new, a.rows) * g.G);
+        hipLaunchKernelGGL((k_paged_join_few<T, HD>), dim3(s.HK * rows_max, a.B), dim3(256), 0, st, g, pacc, pml, big, out,
+                           rows_max);
+        launched("paged_attention");
     }
 }
 
