@@ -159,135 +159,137 @@ __device__ __forceinline__ size_t block_at(int slot, int kh, int lps, size_t pst
     return (size_t)(slot >> lps) * pstride + ((size_t)kh * (1 << (lps - 5)) + ((slot & ((1 << lps) - 1)) >> 5)) * (HD * 32);
 }
 
+// The sum over each N adjacent lanes, in all of them.
+template <int N>
+__device__ __forceinline__ float head_sum(float x) {
+    auto dpp = [&](auto ctrl) {
+        x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, false));
+    };
+    dpp(std::integral_constant<int, 0xB1>());   // lane i and i ^ 1
+    dpp(std::integral_constant<int, 0x4E>());   // i ^ 2
+    dpp(std::integral_constant<int, 0x141>());  // 7 - i of each 8
+    if (N >= 16) dpp(std::integral_constant<int, 0x140>());  // 15 - i of each 16
+    if (N >= 32) x += __shfl_xor(x, 16);
+    return x;
+}
+
 constexpr int VT = 64, VD = 64;  // rows and dims of a V workgroup
 
 // Workgroups [0, nv) transpose V, 64 rows of 64 dims of a kv head each, through LDS, so that 8 consecutive slots go out as
-// 16 bytes.  In the others HD / 8 threads share a row and `hpu` of its q or k heads, 8 dims each, with one set of cosines
-// and sines (they are f32 and twice a row's bytes), NH heads in flight; every load that depends on nothing is issued
-// before the first is used.
-template <class T, int HD, int NH>
+// 16 bytes.  Each of the others does 512 / HD rows of `hpt` q (or k) heads per thread: HD / 8 threads share a row and a
+// head, 8 dims each, 4 heads side by side.  The rows' cosines and sines (f32 and gathered by axis: more work than a head)
+// come once, through LDS, while each thread's first head is on its way; the next one always is.
+template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, int stride, int q_step,
                                                     const float* __restrict__ qw, const float* __restrict__ kw,
                                                     const float* __restrict__ rope, int rope_len,
                                                     const int* __restrict__ pos, int axes,
                                                     const uint8_t* __restrict__ axis, const int* __restrict__ slots,
                                                     int rows, int HQ, int HK, int RD, int lps, int n_pages,
-                                                    size_t pstride, int hpu, int nv, T* __restrict__ Q,
+                                                    size_t pstride, int hpt, int nv, T* __restrict__ Q,
                                                     T* __restrict__ Kp, T* __restrict__ Vp) {
     typedef typename Vec8<T>::type T8;
-    constexpr int LPH = HD / 8;
+    constexpr int LPH = HD / 8, R = 512 / HD;
     const int tid = threadIdx.x;
     const int k_off = HQ * q_step, v_off = k_off + HK * HD;
     const long long n_slots = (long long)n_pages << lps;
     if ((int)blockIdx.x >= nv) {
-        const int gq = (HQ + hpu - 1) / hpu, gk = (HK + hpu - 1) / hpu, per = gq + gk;
-        const int unit = (blockIdx.x - nv) * (256 / LPH) + tid / LPH, c = tid % LPH;
-        const int t = unit / per, u = unit % per;
-        if (t >= rows) return;
+        __shared__ __align__(16) float2 turns[R][HD / 2];
+        const int tiles = (rows + R - 1) / R, u = (blockIdx.x - nv) / tiles, t0 = (blockIdx.x - nv) % tiles * R;
+        const int gq = (HQ + 4 * hpt - 1) / (4 * hpt);
         const bool isq = u < gq;
-        const int h0 = (isq ? u : u - gq) * hpu, heads = isq ? HQ : HK, h1 = min(heads, h0 + hpu);
+        const int c = tid % LPH, r = tid / (4 * LPH), t = min(t0 + r, rows - 1);
+        const int heads = isq ? HQ : HK, first = (isq ? u : u - gq) * 4 * hpt, end = min(heads, first + 4 * hpt);
+        const int h0 = first + tid / LPH % 4;  // the thread's heads: h0, h0 + 4, ...
         const T* const src = big + (size_t)t * stride + (isq ? 0 : k_off);
         const int step = isq ? q_step : HD;
+        auto load = [&](int h) { return *reinterpret_cast<const T8*>(src + (size_t)min(h, heads - 1) * step + 8 * c); };
+        T8 next = load(h0);
         const int slot = slots[t];
-        T8 x8[NH];
-        auto load = [&](int h) {  // NH heads from h on
-#pragma unroll
-            for (int i = 0; i < NH; i++) x8[i] = *reinterpret_cast<const T8*>(src + (size_t)min(h + i, heads - 1) * step + 8 * c);
-        };
-        load(h0);
         const float* const nw = isq ? qw : kw;
-        int at[4] = {0, 0, 0, 0};  // the row's positions
-        if (RD) {
-#pragma unroll
-            for (int a = 0; a < 4; a++)
-                if (a < axes) at[a] = pos[(size_t)a * rows + t];
-        }
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = nw ? nw[8 * c + e] : 1.f;
         // the pair of dim d: j = d % (RD / 2); its other dim is RD / 2 away
         const int rd2 = RD / 2;
-        const bool whole = rd2 % 8 == 0;  // a chunk's partners are one other chunk
+        const bool whole = rd2 % 8 == 0;  // a chunk's others are one chunk
+        auto other = [&](int e) { const int d = 8 * c + e; return d < rd2 ? d + rd2 : d < RD ? d - rd2 : d; };
+        float w[8], w2[8];  // the weights of the thread's dims and of their others
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = w2[e] = 1.f;
+        if (nw && whole) {
+            typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+            const F4* const a = reinterpret_cast<const F4*>(nw + 8 * c);
+            const F4* const b = reinterpret_cast<const F4*>(nw + other(0));
+            const F4 v[4] = {a[0], a[1], b[0], b[1]};
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = v[e >> 2][e & 3], w2[e] = v[2 + (e >> 2)][e & 3];
+        } else if (nw) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = nw[8 * c + e], w2[e] = nw[other(e)];
+        }
+        for (int i = tid; i < R * rd2; i += 256) {
+            const int y = i / rd2, j = i % rd2, ty = min(t0 + y, rows - 1);
+            int at[4];
+#pragma unroll
+            for (int a = 0; a < 4; a++) at[a] = a < axes ? pos[(size_t)a * rows + ty] : 0;
+            const int b = axes > 1 ? axis[j] : 0;
+            const int p = axes == 1 || b == 0 ? at[0] : min(b, axes - 1) == 1 ? at[1] : min(b, axes - 1) == 2 ? at[2] : at[3];
+            turns[y][j] = *reinterpret_cast<const float2*>(rope + ((size_t)min(max(p, 0), rope_len - 1) * rd2 + j) * 2);
+        }
+        __syncthreads();
+        // a result is (x cs + x' sn) / rms, x' its other dim, cs and sn with the weights in them
         float cs[8], sn[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) cs[e] = 1.f, sn[e] = 0.f;
+        if (whole && 8 * c < RD) {
+            const f32x4* const p = reinterpret_cast<const f32x4*>(&turns[r][8 * c < rd2 ? 8 * c : 8 * c - rd2]);
 #pragma unroll
-        for (int a = 0; a < 4; a++) at[a] = min(max(at[a], 0), rope_len - 1);
-        auto turn = [&](int e, float2 v) {
-            cs[e] = v.x;
-            sn[e] = 8 * c + e < rd2 ? -v.y : v.y;
-        };
-        if (8 * c < RD && whole) {
-            const int j = 8 * c < rd2 ? 8 * c : 8 * c - rd2;
-            if (axes == 1) {
-                typedef float F4 __attribute__((ext_vector_type(4), aligned(8)));
-                const F4* const p = reinterpret_cast<const F4*>(rope + ((size_t)at[0] * rd2 + j) * 2);
-                F4 v[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = p[e];
-#pragma unroll
-                for (int e = 0; e < 4; e++) turn(2 * e, float2{v[e][0], v[e][1]}), turn(2 * e + 1, float2{v[e][2], v[e][3]});
-            } else {
-                uint64_t ax;
-                __builtin_memcpy(&ax, axis + j, 8);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int b = min((int)(ax >> (8 * e) & 255), axes - 1);
-                    const int p = b == 0 ? at[0] : b == 1 ? at[1] : b == 2 ? at[2] : at[3];
-                    turn(e, *reinterpret_cast<const float2*>(rope + ((size_t)p * rd2 + j + e) * 2));
-                }
+            for (int e = 0; e < 4; e++) {
+                const f32x4 v = p[e];
+                cs[2 * e] = v[0], sn[2 * e] = v[1], cs[2 * e + 1] = v[2], sn[2 * e + 1] = v[3];
             }
-        } else if (8 * c < RD) {
+        } else if (!whole) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int d = min(8 * c + e, RD - 1), j = d < rd2 ? d : d - rd2, b = axes > 1 ? min((int)axis[j], axes - 1) : 0;
-                const int p = b == 0 ? at[0] : b == 1 ? at[1] : b == 2 ? at[2] : at[3];
-                turn(e, *reinterpret_cast<const float2*>(rope + ((size_t)p * rd2 + j) * 2));
+                const int d = 8 * c + e;
+                if (d < RD) cs[e] = turns[r][d < rd2 ? d : d - rd2].x, sn[e] = turns[r][d < rd2 ? d : d - rd2].y;
             }
         }
-        if (slot < 0 || slot >= n_slots) return;
-        for (int hb = h0; hb < h1; hb += NH) {
-        T8 now[NH];
 #pragma unroll
-        for (int i = 0; i < NH; i++) now[i] = x8[i];
-        if (hb + NH < h1) load(hb + NH);
-#pragma unroll
-        for (int i = 0; i < NH; i++) {
-            const int h = hb + i;
-            float x[8], ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = (float)now[i][e], ss += x[e] * x[e];
-            float inv = 1.f;
-            if (nw) {
-#pragma unroll
-                for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o);
-                inv = 1.0f / sqrtf(ss / (float)HD + 1e-6f);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = x[e] * inv * w[e];
-            T8 y8;
+        for (int e = 0; e < 8; e++) {
+            cs[e] *= w[e];
+            sn[e] *= 8 * c + e < rd2 ? -w2[e] : w2[e];
+        }
+        if (t0 + r >= rows || slot < 0 || slot >= n_slots) return;
+        for (int h = h0; h < end; h += 4) {
+            const T8 x8 = next;
+            if (h + 4 < end) next = load(h + 4);
+            T8 o8;
             if (whole) {
                 const int s = rd2 / 8, from = c < s ? c + s : c - s;
+                const u32x4 v = __builtin_bit_cast(u32x4, x8);
+                u32x4 o;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float o = __shfl(x[e], from, LPH);
-                    y8[e] = (T)(8 * c + e < RD ? x[e] * cs[e] + o * sn[e] : x[e]);
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t y = __shfl(v[e], from, LPH);
+                    o[e] = 8 * c < RD ? y : 0;
                 }
+                o8 = __builtin_bit_cast(T8, o);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int d = 8 * c + e, o = d < rd2 ? d + rd2 : d - rd2;
-                    float r = x[e];
-                    if (d < RD) r = x[e] * cs[e] + (float)src[(size_t)min(h, heads - 1) * step + o] * inv * (nw ? nw[o] : 1.f) * sn[e];
-                    y8[e] = (T)r;
-                }
+                for (int e = 0; e < 8; e++) o8[e] = 8 * c + e < RD ? src[(size_t)h * step + other(e)] : (T)0.f;
             }
-            if (h >= h1) break;
+            float inv = 1.f;
+            if (nw) {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) ss += (float)x8[e] * (float)x8[e];
+                inv = __builtin_amdgcn_rsqf(head_sum<LPH>(ss) * (1.0f / HD) + 1e-6f);
+            }
+            T8 y8;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y8[e] = (T)(((float)x8[e] * cs[e] + (float)o8[e] * sn[e]) * inv);
             if (isq) *reinterpret_cast<T8*>(Q + ((size_t)t * HQ + h) * HD + 8 * c) = y8;
             else
-                *reinterpret_cast<T8*>(Kp + block_at<HD>(slot, h, lps, pstride) + (c / 4) * 1024 + (slot & 31) * 32 +
-                                       8 * (c % 4)) = y8;
-        }
+                *reinterpret_cast<T8*>(Kp + block_at<HD>(slot, h, lps, pstride) + (c / 4) * 1024 + (slot & 31) * 32 + 8 * (c % 4)) = y8;
         }
         return;
     }
@@ -295,15 +297,23 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
     __shared__ int sl[VT];
     __shared__ int first, whole8[VT / 8 + 1];
     const int v = blockIdx.x, d0 = v % (HD / VD) * VD, kh = v / (HD / VD) % HK, t0 = v / (HD / VD) / HK * VT, nt = min(VT, rows - t0);
+    T8 y8[VT * VD / 8 / 256];
+#pragma unroll
+    for (int i = 0; i < VT * VD / 8 / 256; i++) {
+        const int x = tid + 256 * i;
+        y8[i] = *reinterpret_cast<const T8*>(big + (size_t)(t0 + min(x / (VD / 8), nt - 1)) * stride + v_off + kh * HD + d0 + 8 * (x % (VD / 8)));
+    }
     if (tid < VT) {
         const int s = tid < nt ? slots[t0 + tid] : -1;
         sl[tid] = s >= 0 && s < n_slots ? s : -1;
         const unsigned long long any = __ballot(sl[tid] >= 0);
         if (tid == 0) first = any ? __ffsll((long long)any) - 1 : 0;
     }
-    for (int i = tid; i < nt * (VD / 8); i += 256)
-        *reinterpret_cast<T8*>(&tile[i / (VD / 8)][8 * (i % (VD / 8))]) =
-            *reinterpret_cast<const T8*>(big + (size_t)(t0 + i / (VD / 8)) * stride + v_off + kh * HD + d0 + 8 * (i % (VD / 8)));
+#pragma unroll
+    for (int i = 0; i < VT * VD / 8 / 256; i++) {
+        const int x = tid + 256 * i;
+        *reinterpret_cast<T8*>(&tile[x / (VD / 8)][8 * (x % (VD / 8))]) = y8[i];
+    }
     __syncthreads();
     // octets of rows cut where the slots of the first request here are multiples of 8
     const int s0 = sl[first], cut = s0 < 0 ? 0 : ((first - s0) & 7) - 8;
@@ -1296,23 +1306,18 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
 
 template <class T, int HD>
 void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
-    constexpr int PER = 256 / (HD / 8);  // (row, heads) units of a workgroup
-    auto groups = [&](int hpu) { return ((size_t)a.rows * ((s.HQ + hpu - 1) / hpu + (s.HK + hpu - 1) / hpu) + PER - 1) / PER; };
-    // heads per thread: as many as leave a workgroup per CU (us at 1, 2, 4, 8: 32 and 8 heads of 128, three axes, 256 rows
-    // 8.4 7.1 7.0 9.3, 1024 rows 21.4 15.0 13.4 12.9, 4099 rows 71 45 36 31; the engine's heads, 2048 rows 18.0 13.4 13.0 12.4)
-    int hpu = 8;
-    while (hpu > 1 && groups(hpu) < 300) hpu /= 2;
-    const int nh = std::min(hpu, 4);
-    const size_t nv = (size_t)((a.rows + VT - 1) / VT) * s.HK * (HD / VD);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(nv + groups(hpu))), dim3(256), 0, st, static_cast<const T*>(a.big), a.stride,
-                           a.gated ? 2 * HD : HD, a.qw, a.kw, a.rope, a.rope_len, a.pos, a.axes, a.axis, a.slots, a.rows, s.HQ,
-                           s.HK, a.RD, log2i(s.PS), s.n_pages, s.pstride, hpu, (int)nv, static_cast<T*>(a.Q),
-                           static_cast<T*>(a.Kp), static_cast<T*>(a.Vp));
+    auto groups = [&](int hpt) {
+        return ((size_t)a.rows * HD + 511) / 512 * ((s.HQ + 4 * hpt - 1) / (4 * hpt) + (s.HK + 4 * hpt - 1) / (4 * hpt));
     };
-    if (nh == 4) go(k_paged_prep<T, HD, 4>);
-    else if (nh == 2) go(k_paged_prep<T, HD, 2>);
-    else go(k_paged_prep<T, HD, 1>);
+    // heads per thread: as many as leave nearly three workgroups per CU (us at 1, 2, 4, 8: 32 and 8 heads of 128, three
+    // axes, 256 rows 6.4 7.5 7.1 7.5, 1024 rows 10.4 8.6 7.7 8.7, 4099 rows 30.9 22.4 20.7 20.1)
+    int hpt = 8;
+    while (hpt > 1 && groups(hpt) < 700) hpt /= 2;
+    const size_t nv = (size_t)((a.rows + VT - 1) / VT) * s.HK * (HD / VD);
+    hipLaunchKernelGGL((k_paged_prep<T, HD>), dim3((unsigned)(nv + groups(hpt))), dim3(256), 0, st,
+                       static_cast<const T*>(a.big), a.stride, a.gated ? 2 * HD : HD, a.qw, a.kw, a.rope, a.rope_len, a.pos,
+                       a.axes, a.axis, a.slots, a.rows, s.HQ, s.HK, a.RD, log2i(s.PS), s.n_pages, s.pstride, hpt, (int)nv,
+                       static_cast<T*>(a.Q), static_cast<T*>(a.Kp), static_cast<T*>(a.Vp));
     launched("paged_prep");
 }
 
