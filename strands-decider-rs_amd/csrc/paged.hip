@@ -1276,16 +1276,17 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
     };
     if (p.nr) {
         const int nb = blocks(std::max(1, p.few / G));
-        // Two workgroups per CU want keys to read, but the parts cost a join: no split of few elements, and none where the
-        // unsplit workgroups draw most of the bandwidth already. us unsplit and split, at n keys of each request:
-        // 16 workgroups, dims 64: 1000 7.0 7.8, 2000 10.5 7.9; 128: 500 7.6 9.1, 1000 11.1 9.2; 256: 500 11.6 11.1
+        // One workgroup per CU wants keys to read, at least 2 blocks each (8 and 2 heads of 256 dims, 700 keys: 8.8 us, at
+        // least 4 9.3, 8 10.6); but the parts cost a join: no split of few elements, and none where the unsplit workgroups
+        // draw most of the bandwidth already.  us unsplit and split, at n keys of each request:
+        // 8 workgroups, dims 64: 1000 6.9 7.8, 2000 10.5 7.5; 128: 700 9.1 7.8; 256: 200 7.8 7.9, 400 10.3 8.3
         // 128 workgroups, dims 64: 8000 39 44; 128: 4000 40 46, 8000 90 81; 256: 2000 41 46, 4000 93 82
         const int wgs = B * s.HK;
         const double elems = 32.0 * nb * s.HD;
-        const int want = elems < (wgs < 128 ? 100e3 : 768e3) ? 1 : std::min(MAX_KS, std::max(1, 256 / wgs));
-        p.few_span = std::max(8, ((nb + want - 1) / want + 3) / 4 * 4);
+        const int want = elems < (wgs < 128 ? 75e3 : 768e3) ? 1 : std::min(MAX_KS, std::max(1, 256 / wgs));
+        p.few_span = ((nb + want - 1) / want + 1) / 2 * 2;
         p.few_ks = (nb + p.few_span - 1) / p.few_span;
-        p.slots = std::min(want, (nb + 7) / 8);
+        p.slots = std::min(want, (nb + 1) / 2);
         // beyond the 256 MB that stay in the last-level cache a layer's keys are gone before they are read again (64
         // requests of 1000 to 8191 rows 159 -> 142 us with the hint, two of 90 and 131 thousand 89 -> 78; 85 MB, read again
         // and again, 22 -> 24)
