@@ -277,7 +277,8 @@ int sd_op_attention(const void* big, int stride, const void* qw, const void* kw,
  * These calls allocate nothing, wait for nothing and keep nothing: they may be captured, and calls on
  * several streams or threads run at once where they share no output and no workspace.  All counts, tables
  * and lengths are device arrays of i32, read when the kernels run; what they hold cannot make a kernel
- * leave the given buffers.  The buffers belong to the calling thread's current device. ---- */
+ * leave the given buffers.  The buffers belong to the calling thread's current device.  A launch of more
+ * than 2^24 workgroups (millions of rows) is refused. ---- */
 
 /* Types of the rows and caches below. */
 enum { SD_F16 = 0, SD_BF16 = 1 };
@@ -306,7 +307,8 @@ int sd_op_page_plan(const void* lens, const void* news, int B, int T, int page_s
  * j's axis a = pair_axis[j] (u8; null with one axis), pos [axes][T] (1 to 4 axes: time, height and width of
  * an image's patches, say).  Positions outside the table take its nearest row, axes past the last the last.
  * All in f32, rounded once: q to Q [T][HQ][HD], k and v to their rows' slots.  A row whose slot is outside
- * [0, n_pages * page_size) is passed over (Q too); two rows of one slot give either's values. */
+ * [0, n_pages * page_size) is passed over (Q too); two rows of one slot give either's values.  Q may not
+ * overlap big. */
 int sd_op_paged_prep(const void* big, int stride, int gated, const void* qw, const void* kw, const void* rope, int rope_len,
                      const void* pos, int axes, const void* pair_axis, const void* slots, int T, int HQ, int HK, int HD,
                      int RD, int page_size, int n_pages, size_t page_stride, void* Q, void* Kp, void* Vp, int type,
@@ -324,7 +326,8 @@ int sd_op_paged_attention_ws(int B, int T, int max_new, int max_kv, int HQ, int 
  * infinities among them, change nothing.  Rows of out outside every request are left as they are.
  * max_new and max_kv are upper bounds of n and kv_lens that the launch is made for (rows and keys past them
  * are left out).  ws holds what sd_op_paged_attention_ws says, 16-byte aligned, and is free again when the
- * call's kernels have run: calls that may overlap, captured graphs among them, need one each. */
+ * call's kernels have run: calls that may overlap, captured graphs among them, need one each.  out, ws and
+ * the inputs may not overlap. */
 int sd_op_paged_attention(const void* Q, const void* big, int stride, const void* Kp, const void* Vp, const void* table,
                           int max_blocks, const void* cu, const void* kv_lens, int B, int T, int max_new, int max_kv, int HQ,
                           int HK, int HD, int page_size, int n_pages, size_t page_stride, int window, float scale, void* out,

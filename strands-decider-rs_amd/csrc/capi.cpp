@@ -682,6 +682,7 @@ int sd_op_paged_prep(const void* big, int stride, int gated, const void* qw, con
             throw sd::Error(who + ": big, Q and the caches must be aligned to 16 bytes");
         if (!aligned(rope, 8) || !aligned(qw, 4) || !aligned(kw, 4) || !aligned(pos, 4) || !aligned(slots, 4))
             throw sd::Error(who + ": the table must be aligned to 8 bytes, weights, positions and slots to 4");
+        if (overlap(Q, (size_t)T * HQ * HD * 2, big, ((size_t)(T - 1) * stride + width) * 2)) throw sd::Error(who + ": Q overlaps big");
         sd::paged_prep(s, {big, stride, gated != 0, static_cast<const float*>(qw), static_cast<const float*>(kw),
                            static_cast<const float*>(rope), rope_len, static_cast<const int*>(pos), axes,
                            static_cast<const uint8_t*>(pair_axis), static_cast<const int*>(slots), T, RD, Q, Kp, Vp},
@@ -727,6 +728,7 @@ int sd_op_paged_attention(const void* Q, const void* big, int stride, const void
         if (need && (!ws || ws_bytes < need))
             throw sd::Error(who + ": needs a workspace of " + std::to_string(need) + " bytes, got " +
                             std::to_string(ws ? ws_bytes : 0));
+        if (need && (overlap(ws, need, out, rows) || overlap(ws, need, Q, rows))) throw sd::Error(who + ": the workspace overlaps Q or out");
         sd::paged_attn(s, {Q, big, stride, Kp, Vp, static_cast<const int*>(table), max_blocks, static_cast<const int*>(cu),
                            static_cast<const int*>(kv_lens), B, T, max_new, max_kv, window, scale, out, ws},
                        static_cast<hipStream_t>(stream));

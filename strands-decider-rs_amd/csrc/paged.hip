@@ -459,6 +459,8 @@ struct AttnArgs {
     int tiles, rows_ks, rows_span;   // of k_paged_rows
     float c;  // scale log2(e)
     size_t pstride;
+    // the first key that a row at position p sees (one before position 0 sees none, whatever this says)
+    __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
 
 // Output of 4 dims of a row: unnormalised o over the sum l, times the sigmoid of its gates where it has some, rounded once.
@@ -511,7 +513,7 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
     const int nrows = rq.n * a.G;
     if (nrows == 0 || nrows > a.few) return;
     // keys [lo, hi) are seen by some row; this workgroup's blocks of them
-    const int hi = min(rq.p0 + rq.n, rq.kcap), lo = a.window ? max(0, rq.p0 - a.window + 1) : 0;
+    const int hi = min(rq.p0 + rq.n, rq.kcap), lo = max(0, a.from(rq.p0));
     const int blk0 = (lo >> 5) + z * a.few_span;
     const int blk1 = z + 1 < a.few_ks ? min((hi + 31) >> 5, blk0 + a.few_span) : (hi + 31) >> 5;
     const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + NW - 1) / NW : 0;
@@ -521,14 +523,14 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
     for (int u = 0; u < NR; u++) {
         const int r = min(16 * u + fq, nrows - 1), t = r / a.G, h = kh * a.G + r % a.G;
         const int p = rq.p0 + t;
-        jlo[u] = a.window ? p - a.window + 1 : 0;
+        jlo[u] = a.from(p);
         jhi[u] = min(p + 1, hi);
         const T* q = Q + ((size_t)(rq.q0 + t) * a.HQ + h) * HD + 8 * fg;
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[u][s] = *reinterpret_cast<const T8*>(q + 32 * s);
     }
     // blocks in [open0, open1) are seen whole by every row
-    const int open0 = a.window ? rq.p0 + rq.n - a.window : 0, open1 = min(rq.p0 + 1, hi);
+    const int open0 = a.from(rq.p0 + rq.n - 1), open1 = min(rq.p0 + 1, hi);
 
     const int lbpp = a.lps - 5;
     const int* const tb = a.table + (size_t)b * a.max_blocks;
@@ -798,7 +800,8 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
         return n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
     };
     int own = 0;
-    for (int i = 0; i < per; i++) own += tiles(lane * per + i);
+    // (cut at 2^24 per lane, which row starts that do not ascend could pass: the sums stay in range)
+    for (int i = 0; i < per; i++) own = min(own + tiles(lane * per + i), 1 << 24);
     int to = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -857,15 +860,15 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     const bool live = w0 < r1;
     // keys seen by some row of the workgroup, and this split's blocks of them
     const int hi = min(rq.p0 + (r1 - 1) / a.G + 1, rq.kcap);
-    const int lo = a.window ? max(0, rq.p0 + r0 / a.G - a.window + 1) : 0;
+    const int lo = max(0, a.from(rq.p0 + r0 / a.G));
     const int blk0 = (lo >> 5) + z * a.rows_span, blk1 = z + 1 < a.rows_ks ? min((hi + 31) >> 5, blk0 + a.rows_span) : (hi + 31) >> 5;
     const int nb = max(blk1 - blk0, 0);
     // the lane's row (one past the last is the last again, also in the output) and the keys [jlo, jhi) that it sees
     const int r = min(w0 + c, r1 - 1), t = r / a.G, h = kh * a.G + r % a.G;
-    const int jlo = a.window ? rq.p0 + t - a.window + 1 : 0, jhi = min(rq.p0 + t + 1, hi);
+    const int jlo = a.from(rq.p0 + t), jhi = min(rq.p0 + t + 1, hi);
     // the keys that every row of the wave, and of the workgroup, sees
-    const int all0 = a.window ? rq.p0 + (w1 - 1) / a.G - a.window + 1 : 0, all1 = min(rq.p0 + w0 / a.G + 1, hi);
-    const int wg0 = a.window ? rq.p0 + (r1 - 1) / a.G - a.window + 1 : 0, wg1 = min(rq.p0 + r0 / a.G + 1, hi);
+    const int all0 = a.from(rq.p0 + (w1 - 1) / a.G), all1 = min(rq.p0 + w0 / a.G + 1, hi);
+    const int wg0 = a.from(rq.p0 + (r1 - 1) / a.G), wg1 = min(rq.p0 + r0 / a.G + 1, hi);
     if (tid == 0) rare = 0;
 
     const int lbpp = a.lps - 5;
@@ -1267,8 +1270,13 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
     const long long most = (long long)std::min(max_new, rows) * G;
     Plan p;
     const int fits = s.HD == 256 ? 16 : 32;  // (a second group's outputs and queries do not fit the registers at 256)
+    // Among chunks, requests with few rows are k_paged_few's where most are such, and where some may have long caches,
+    // which no tile of one row should walk: a prompt of 512 tokens and one token on 30000 keys, 32 and 8 heads of 128
+    // dims, 260 us with both in tiles, 38 so.  Where all are chunks after all, the parts that exit and their join cost
+    // 1 to 3 us.
     if (most <= fits) p.nr = most <= 16 ? 1 : 2, p.few = 16 * p.nr;
-    else if (B > 1 && (long long)rows * 2 < (long long)max_new * B && G <= fits) p.nr = G <= 16 ? 1 : 2, p.few = 16 * p.nr;
+    else if (G <= fits && rows < (long long)max_new * B && (2ll * rows < (long long)max_new * B || max_kv >= 2048))
+        p.nr = G <= 16 ? 1 : 2, p.few = 16 * p.nr;
     auto blocks = [&](long long n) {  // of 32 keys that n adjacent rows may see
         long long k = max_kv;
         if (window) k = std::min(k, (long long)window + n + 31);
@@ -1315,6 +1323,7 @@ void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
     int hpt = 8;
     while (hpt > 1 && groups(hpt) < 700) hpt /= 2;
     const size_t nv = (size_t)((a.rows + VT - 1) / VT) * s.HK * (HD / VD);
+    if (nv + groups(hpt) >= size_t(1) << 24) throw Error("sd_op_paged_prep: too many rows for one launch");
     hipLaunchKernelGGL((k_paged_prep<T, HD>), dim3((unsigned)(nv + groups(hpt))), dim3(256), 0, st,
                        static_cast<const T*>(a.big), a.stride, a.gated ? 2 * HD : HD, a.qw, a.kw, a.rope, a.rope_len, a.pos,
                        a.axes, a.axis, a.slots, a.rows, s.HQ, s.HK, a.RD, log2i(s.PS), s.n_pages, s.pstride, hpt, (int)nv,
@@ -1334,7 +1343,8 @@ void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
     float* const pacc = static_cast<float*>(a.ws);
     float* const pml = pacc + p.slots * a.rows * s.HQ * HD;
     const size_t tiles = (size_t)p.tiles * s.HK * p.rows_ks, parts = (size_t)a.B * s.HK * p.few_ks;
-    const bool both = p.tiles && p.nr == 1 && tiles + parts < (size_t(1) << 31);
+    const bool both = p.tiles && p.nr == 1;
+    if (tiles + parts >= size_t(1) << 24) throw Error("sd_op_paged_attention: too many rows and requests for one launch");
     auto launch = [&](auto kernel, dim3 grid, int threads) {
         hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, Q, K, V, g, big, out, pacc, pml);
         launched("paged_attention");

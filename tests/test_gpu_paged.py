@@ -200,6 +200,27 @@ def test_prep_keeps_what_is_not_finite_to_its_row_and_pair(sdamd):
     check_prep(sdamd, "bf16", 2, 1, 128, 24, np.arange(40), 32, 4, norm=False, poke=poke)
 
 
+def test_prep_of_weights_and_tables_at_the_alignment_that_is_asked(sdamd):
+    """Norm weights 4 bytes, the table 8 bytes past a 16-byte boundary: the same results."""
+    for hq, hk, hd, rd in [(4, 2, 128, 64), (2, 1, 64, 24)]:
+        T, g = 70, torch.Generator("cuda").manual_seed(hd)
+        big = torch.randn(T, (hq + 2 * hk) * hd, generator=g, device="cuda").half()
+        w = [1 + 0.2 * torch.randn(hd, generator=g, device="cuda") for _ in range(2)]
+        rope, pos, slots = rope_table(rd, 100), dev(np.arange(T)), dev(np.arange(T) + 9)
+        got = []
+        for off in (0, 1):
+            ww = [torch.cat([torch.zeros(off, device="cuda"), x]) for x in w]
+            rr = torch.cat([torch.zeros(2 * off, device="cuda"), rope.flatten()])
+            c = Cache("f16", hk, hd, 32, 4)
+            Q = torch.zeros(T, hq, hd, dtype=torch.float16, device="cuda")
+            sdamd.op_paged_prep(big.data_ptr(), big.shape[1], False, ww[0].data_ptr() + 4 * off, ww[1].data_ptr() + 4 * off,
+                                rr.data_ptr() + 8 * off, 100, pos.data_ptr(), 1, None, slots.data_ptr(), T, hq, hk, hd, rd, 32,
+                                4, Q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), sdamd.F16, 0, stream())
+            torch.cuda.synchronize()
+            got.append([x.view(torch.int16) for x in (Q, c.k, c.v)])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 # ---- attention ------------------------------------------------------------------------------------
 
 def attn_case(sdamd, kind, hq, hk, hd, ps, reqs, window=0, gated=False, scale=None, seed=0, gain=1.0, pstride=0, more_new=0,
@@ -351,6 +372,50 @@ def test_small_weights_count(sdamd):
         tol = want * (22 * math.log(2) + 3) * half_step(kind)
         got = d["out"][0].double()
         assert ((got - want).abs() <= tol).all(), (kind, float(got.min()), float(got.max()), want)
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(20, 1, 64), (20, 1, 128), (40, 2, 256), (8, 2, 128)])
+def test_attention_of_a_prompt_among_longer_caches(sdamd, hq, hk, hd):
+    """A fresh prompt and single tokens or drafts on much longer caches, up to 20 heads per kv head."""
+    for i, reqs in enumerate([[(300, 300), (5000, 1)], [(2300, 1), (150, 150), (0, 0), (2050, 1)], [(2048, 200), (900, 150)]]):
+        check_attn(sdamd, "bf16", hq, hk, hd, 64, reqs, seed=20 + i)
+        check_attn(sdamd, "f16", hq, hk, hd, 32, reqs, gated=True, window=700, seed=30 + i)
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (6, 2, 128), (24, 8, 64)])
+def test_a_window_past_every_key_is_none(sdamd, hq, hk, hd):
+    """The largest windows there are, rows before position 0 among the requests': bit for bit the call without one."""
+    for reqs in ([(3, 7), (60, 1), (500, 90), (0, 2)], [(5, 6), (200, 1)], [(3000, 1)]):
+        d = attn_case(sdamd, "bf16", hq, hk, hd, 32, reqs, seed=21)
+        outs = []
+        for w in (0, 2 ** 31 - 1, 2 ** 30):
+            d["window"] = w
+            d["out"].fill_(7.0)
+            call(sdamd, d)
+            torch.cuda.synchronize()
+            outs.append(d["out"].clone())
+        d["window"] = 0
+        compare(d, fast=False)
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_scores_that_are_not_finite(sdamd, kind):
+    """Infinities and NaN in seen keys and in queries give what the definition gives, to their rows alone."""
+    def poke(b, k, v):
+        if b < 2:
+            k[20, 0, 3], k[45, -1, 7] = math.inf, math.nan
+
+    for hq, hk, hd in [(8, 2, 256), (4, 2, 128), (3, 1, 64)]:
+        d = attn_case(sdamd, kind, hq, hk, hd, 32, [(90, 80), (70, 1), (100, 1), (2500, 2), (64, 40)], poke=poke, seed=22)
+        at = d["at"]
+        d["q"][at[0] + 5, 0, 2] = math.nan
+        d["q"][at[2], -1, 0] = math.inf
+        d["q"][at[3] + 1, 0, 9] = -math.inf
+        d["q"][at[4] + 33, :, 1] = math.inf
+        call(sdamd, d)
+        torch.cuda.synchronize()
+        compare(d, fast=False)
 
 
 def test_rows_that_see_nothing(sdamd):
@@ -580,6 +645,41 @@ def test_serving_steps_replayed_from_a_graph(sdamd):
     with torch.cuda.graph(graph):
         sv.step()
     serve(sv, STEPS, graph.replay)
+
+
+def test_two_graphs_with_a_workspace_each(sdamd):
+    """Two captured calls whose work is split, replayed at once on two streams, eager calls between: bit for bit the
+    eager results, every time."""
+    reqs = [(6000, 1), (300, 1), (900, 120)]
+    ds = [attn_case(sdamd, "f16", 8, 2, 256, 64, reqs, gated=True, seed=40 + i) for i in range(2)]
+    assert all(d["ws"].numel() > 1 for d in ds)
+    first, graphs, ss = [], [], [torch.cuda.Stream() for _ in ds]
+    for d in ds:
+        call(sdamd, d)
+        torch.cuda.synchronize()
+        compare(d)
+        first.append(d["out"].clone())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(sdamd, d)
+        graphs.append(graph)
+    for i in range(4):
+        for d in ds:
+            d["out"].fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, s in zip(graphs, ss):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for d, f in zip(ds, first):
+            assert torch.equal(d["out"].view(torch.int16), f.view(torch.int16))
+            d["out"].fill_(7.0)
+        torch.cuda.synchronize()
+        for d, f in zip(ds, first):
+            call(sdamd, d)
+            torch.cuda.synchronize()
+            assert torch.equal(d["out"].view(torch.int16), f.view(torch.int16))
 
 
 def test_one_sequence_is_the_contiguous_attention(sdamd):

@@ -51,7 +51,8 @@ def test_plan_refuses(sdamd, kw, message):
     (dict(axes=5, pair_axis=A), "axes"), (dict(axes=3), "each pair's axis"), (dict(stride=767), "row stride"),
     (dict(stride=760), "row stride"), (dict(gated=True), "row stride"), (dict(big=A + 8), "16 bytes"), (dict(Vp=A + 2), "16 bytes"),
     (dict(rope=A + 4), "8 bytes"), (dict(page_stride=4088), "page stride"), (dict(page_stride=4100), "page stride"),
-    (dict(page_size=8), "power of two"), (dict(n_pages=-1), "at least one page"),
+    (dict(page_size=8), "power of two"), (dict(n_pages=-1), "at least one page"), (dict(Q=A + 6128), "Q overlaps big"),
+    (dict(T=1 << 28, HQ=1, HD=64, stride=192, Q=1 << 50), "too many rows"),
 ])
 def test_prep_refuses(sdamd, kw, message):
     with pytest.raises(sdamd.EngineError, match="sd_op_paged_prep: .*" + message):
@@ -69,6 +70,9 @@ def test_prep_refuses(sdamd, kw, message):
     (dict(out=A + 4080), "out overlaps Q"), (dict(big=A + 65536 - 4096, stride=1024), "out overlaps the gates"),
     (dict(HD=80), "head_dim"), (dict(HQ=5, HK=2), "multiple of kv heads"), (dict(type=3), "type"), (dict(page_size=33), "power of two"),
     (dict(page_stride=8), "page stride"),
+    (dict(B=1, T=1, max_new=1, max_blocks=4000, max_kv=100000, ws=A + 65536), "workspace overlaps"),
+    (dict(B=1, T=1, max_new=1, max_blocks=4000, max_kv=100000, ws=A), "workspace overlaps"),
+    (dict(B=8192, T=1 << 19, max_new=1 << 19, HQ=1024, HK=1024, HD=64, out=1 << 50), "too many rows"),
 ])
 def test_attention_refuses(sdamd, kw, message):
     with pytest.raises(sdamd.EngineError, match="sd_op_paged_attention: .*" + message):
