@@ -68,6 +68,7 @@ __device__ __forceinline__ void scan2(long long& a, long long& b, long long (*ws
 // had are read and only entries behind them written.
 // First come, first admitted: requests 0 .. bad - 1 get their rows and pages, where `bad` is the first one that does
 // not fit (rows, free pages, table width) or whose counts are negative.
+// Bound by its launch and four barriers: 4.3 us for 8 requests, 5.4 for 384 with 13000 rows.
 __global__ __launch_bounds__(PLAN_T) void k_page_plan(const int* __restrict__ lens, const int* __restrict__ news, int B,
                                                       int T, int lps, int n_pages, const int* __restrict__ free_pages,
                                                       const int* __restrict__ n_free, int* table, int max_blocks,
@@ -179,6 +180,9 @@ constexpr int VT = 64, VD = 64;  // rows and dims of a V workgroup
 // 16 bytes.  Each of the others does 512 / HD rows of `hpt` q (or k) heads per thread: HD / 8 threads share a row and a
 // head, 8 dims each, 4 heads side by side.  The rows' cosines and sines (f32 and gathered by axis: more work than a head)
 // come once, through LDS, while each thread's first head is on its way; the next one always is.
+// Bound by bytes: 4099 rows of 32 and 8 heads of 128 dims on three axes, 103 MB, 22.7 us, 4.5 TB/s, where a copy makes
+// 4.8.  (33.5 us with scalar loads of the weights and the angles gathered by every thread; several heads of a thread in
+// flight at a time cost more registers than they hid: 30.)
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, int stride, int q_step,
                                                     const float* __restrict__ qw, const float* __restrict__ kw,
@@ -485,8 +489,11 @@ __device__ __forceinline__ u32x2 gate4(const T* big, size_t at) {
 // ---- few rows: up to 16 NR rows per (request, kv head), one new token's heads or a short draft's ----
 //
 // Bound by the cache's bytes: each is read once and used for a handful of rows.  The keys are split over workgroups
-// (span blocks of 32 each) and inside one over its NW waves, block by block; a wave loads a block's K and V straight
-// into registers in MFMA operand order, one block ahead of the one it works on.
+// (span blocks of 32 each) and inside one over its NW waves, block by block; a wave loads K and V straight into registers
+// in MFMA operand order, 16 rows on v_mfma_f32_16x16x32, the next block while it works on one (LDS would be a second trip
+// for bytes that one wave alone uses).  64 requests of 1000 to 8191 keys, 32 and 8 heads of 128 dims, 776 MB: 143 us, 5.4
+// TB/s; two of 90 and 131 thousand, 8 and 2 heads of 256 dims: 79 us, 6.2 TB/s.  A CU alone draws 60 GB/s, so short
+// caches are split as far as a join lets them: 700 keys of those heads 9.0 us, launches and two trips to memory.
 // 16 bytes per lane; ONCE: of data that nothing reads again before it has left the caches (the non-temporal hint).
 template <bool ONCE>
 __device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t voff, uint32_t soff) {
@@ -497,7 +504,7 @@ __device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t voff, uint32_t soff) {
 }
 
 template <int HD, int NR>
-constexpr int few_waves() { return HD * NR <= 128 ? 8 : 4; }  // 8 where two fit a SIMD's registers
+constexpr int few_waves() { return HD * NR <= 128 ? 8 : 4; }  // 8 where two fit a SIMD's registers (157 -> 143)
 // Workgroup x of request b, of NW waves: om(w) gives LDS of R x HD floats for each wave, Ms and Ls are R of them per wave.
 template <class T, int HD, int NR, bool ONCE, int NW, class Om>
 __device__ __forceinline__ void few_part(const int x, const int b, const T* __restrict__ Q, const T* __restrict__ Kp,
@@ -779,7 +786,12 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
 // ---- many rows: 128 rows of a kv head per workgroup ----
 //
 // Bound by MFMA and the softmax beside it: each wave has 32 rows on v_mfma_f32_32x32x16, its queries and outputs in
-// registers, and all 4 share tiles of keys that arrive by LDS DMA, one tile ahead.
+// registers, and all 4 share blocks of 32 keys that arrive by LDS DMA, three ahead.  A block's probabilities run between
+// the products of the next one's scores and of its own output.  A prompt of 8192 tokens, 8 and 2 heads of 256 dims: 291
+// us, 945 TFLOP/s; four chunks of 2048 on 2048 to 8192 old keys, 32 and 8 heads of 128 dims: 515 us, 1020 TFLOP/s, where
+// a library product of 8192^3 makes 1200.  MFMA is busy half of the cycles (2.0 GHz under this load), the softmax's
+// vector instructions the other half (16 exponentials of 16 cycles per block are half of those); which probabilities run
+// where, and wave priorities, change 1 %.
 // Workgroup x of the launch is kv head x % HK (with 8 heads, one per XCD's L2), split and tile; the tiles of all
 // requests with more than `few` rows are numbered through, and taken from the last on: a causal chunk's late tiles are
 // the long ones.
@@ -1036,8 +1048,9 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
         for (int e = 0; e < 16; e++) s[e] = 0.f;
     };
     auto none = [](int) {};
-    // Block i (scores s): its probabilities and output, beside the scores s2 of the next, whose keys are in K.  The first EARLY keys' probabilities run beside the scores' products, the others beside the first half of the
-    // output's, the new scores' maximum beside the second half.  The stage NB - 1 further on goes into (Kx, Vx).
+    // Block i (scores s): its probabilities and output, beside the scores s2 of the next, whose keys are in K.  The first
+    // EARLY keys' probabilities run beside the scores' products, the others beside the first half of the output's, the new
+    // scores' maximum beside the second half.  The stage NB - 1 further on goes into (Kx, Vx).
     // (the pins keep the compiler from sinking work behind the products that it runs beside)
     constexpr int EARLY = 12;
     At nk{0, 0}, nv{0, 0};  // the blocks that the next step fetches: found in the shadow of this one's products
