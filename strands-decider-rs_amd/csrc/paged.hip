@@ -1228,8 +1228,8 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
                        o + 32 * d + 8 * i);
 }
 
-// Joins the splits of k_paged_rows: HD / 4 threads per row, 4 dims each, every load issued before the first is used.
-constexpr int MAX_ROWS_KS = 8;
+// Joins the splits of k_paged_rows: HD / 4 threads per row, 4 dims each, 8 splits at a time; the next 8 are on their way
+// meanwhile (what goes past the last split is the last again).
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float* __restrict__ pacc,
                                                          const float* __restrict__ pml, const T* __restrict__ big,
@@ -1242,26 +1242,43 @@ __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float
     if (r >= rq.n * a.G) return;
     const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G, d = 4 * (threadIdx.x % W);
     const size_t row = (size_t)t * a.HQ + h, zs = (size_t)a.rows * a.HQ;
-    float2 ml[MAX_ROWS_KS];
-    f32x4 x[MAX_ROWS_KS];
+    constexpr int N = 8;
+    struct Set {
+        float2 ml[N];
+        f32x4 x[N];
+    };
+    auto load = [&](int z0, Set& v) INL {
+#pragma unroll
+        for (int z = 0; z < N; z++) {
+            const size_t at = min(z0 + z, a.rows_ks - 1) * zs + row;
+            v.ml[z] = *reinterpret_cast<const float2*>(pml + 2 * at);
+            v.x[z] = *reinterpret_cast<const f32x4*>(pacc + at * HD + d);
+        }
+    };
+    Set v;
+    load(0, v);
     const u32x2 gate = gate4(big, (size_t)t * a.stride + h * 2 * HD + HD + d);
-#pragma unroll
-    for (int z = 0; z < MAX_ROWS_KS; z++) {
-        const size_t at = min(z, a.rows_ks - 1) * zs + row;
-        ml[z] = *reinterpret_cast<const float2*>(pml + 2 * at);
-        x[z] = *reinterpret_cast<const f32x4*>(pacc + at * HD + d);
-    }
     float mx = -INFINITY, ls = 0.f;
-#pragma unroll
-    for (int z = 0; z < MAX_ROWS_KS; z++) mx = fmaxf(mx, ml[z].x);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int z0 = 0; z0 < a.rows_ks; z0 += N) {
+        const Set now = v;
+        if (z0 + N < a.rows_ks) load(z0 + N, v);
+        float mn = mx;
 #pragma unroll
-    for (int z = 0; z < MAX_ROWS_KS; z++) {
-        if (z >= a.rows_ks || ml[z].y == 0.f) continue;
-        const float f = exp2_fast(ml[z].x - mx);
-        ls += ml[z].y * f;
+        for (int z = 0; z < N; z++) mn = fmaxf(mn, now.ml[z].x);
+        const float f0 = ls == 0.f ? 0.f : exp2_fast(mx - mn);
+        mx = mn;
+        ls *= f0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] += x[z][e] * f;
+        for (int e = 0; e < 4; e++) o[e] *= f0;
+#pragma unroll
+        for (int z = 0; z < N; z++) {
+            if (z0 + z >= a.rows_ks || now.ml[z].y == 0.f) continue;
+            const float f = exp2_fast(now.ml[z].x - mx);
+            ls += now.ml[z].y * f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] += now.x[z][e] * f;
+        }
     }
     finish4<T>(o, ls, big, gate, out + row * HD + d);
 }
@@ -1318,7 +1335,11 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
         const long long all = (long long)rows * G;
         p.tiles = (int)(all / TILE_ROWS) + B;
         const int nb = blocks(TILE_ROWS / G + 2);
-        const int want = (int)std::min((long long)MAX_ROWS_KS, std::max(1ll, 256ll / std::max(1ll, all / TILE_ROWS * s.HK)));
+        // One workgroup per CU: tiles as many as there will be, if every request has one (a request's 64 heads of 128 dims on
+        // 8000 and 30000 keys 25 and 71 us in at most 8 splits, 15 and 23 in 64; 32 of them 33 and 101 us in 16, 31 and 93
+        // in 8)
+        const long long tiles = std::max({1ll, all / TILE_ROWS, p.nr ? 1ll : std::min(B, rows)});
+        const int want = (int)std::min((long long)MAX_KS, std::max(1ll, 256 / (tiles * s.HK)));
         p.rows_span = std::max(8, ((nb + want - 1) / want + 1) / 2 * 2);
         p.rows_ks = (nb + p.rows_span - 1) / p.rows_span;
         p.slots = std::max(p.slots, (size_t)std::min(want, (nb + 7) / 8));
