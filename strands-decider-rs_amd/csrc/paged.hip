@@ -299,7 +299,7 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
     }
     __shared__ __align__(16) T tile[VT][VD + 8];
     __shared__ int sl[VT];
-    __shared__ int first, whole8[VT / 8 + 1];
+    __shared__ int cut, whole8[VT / 8 + 1];
     const int v = blockIdx.x, d0 = v % (HD / VD) * VD, kh = v / (HD / VD) % HK, t0 = v / (HD / VD) / HK * VT, nt = min(VT, rows - t0);
     T8 y8[VT * VD / 8 / 256];
 #pragma unroll
@@ -307,25 +307,23 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
         const int x = tid + 256 * i;
         y8[i] = *reinterpret_cast<const T8*>(big + (size_t)(t0 + min(x / (VD / 8), nt - 1)) * stride + v_off + kh * HD + d0 + 8 * (x % (VD / 8)));
     }
-    if (tid < VT) {
-        const int s = tid < nt ? slots[t0 + tid] : -1;
-        sl[tid] = s >= 0 && s < n_slots ? s : -1;
-        const unsigned long long any = __ballot(sl[tid] >= 0);
-        if (tid == 0) first = any ? __ffsll((long long)any) - 1 : 0;
+    if (tid < VT) {  // (the first wave)
+        const int s = tid < nt ? slots[t0 + tid] : -1, mine = s >= 0 && s < n_slots ? s : -1;
+        sl[tid] = mine;
+        // octets of rows cut where the slots of the first request here are multiples of 8: which of them are 8 slots on end
+        const unsigned long long any = __ballot(mine >= 0);
+        const int first = any ? __ffsll((long long)any) - 1 : 0, s0 = __shfl(mine, first);
+        const int c = s0 < 0 ? 0 : ((first - s0) & 7) - 8, before = __shfl_up(mine, 1);
+        const unsigned long long next = __ballot(tid > 0 && mine == before + 1);
+        const int r0 = c + 8 * tid, at = __shfl(mine, min(max(r0, 0), VT - 1));
+        if (tid < VT / 8 + 1)
+            whole8[tid] = r0 >= 0 && r0 + 7 < VT && at >= 0 && at % 8 == 0 && (next >> (r0 + 1) & 127) == 127;
+        if (tid == 0) cut = c;
     }
 #pragma unroll
     for (int i = 0; i < VT * VD / 8 / 256; i++) {
         const int x = tid + 256 * i;
         *reinterpret_cast<T8*>(&tile[x / (VD / 8)][8 * (x % (VD / 8))]) = y8[i];
-    }
-    __syncthreads();
-    // octets of rows cut where the slots of the first request here are multiples of 8
-    const int s0 = sl[first], cut = s0 < 0 ? 0 : ((first - s0) & 7) - 8;
-    if (tid < VT / 8 + 1) {
-        const int r0 = cut + 8 * tid;
-        bool ok = r0 >= 0 && r0 + 7 < VT && sl[max(r0, 0)] >= 0 && sl[max(r0, 0)] % 8 == 0;
-        for (int i = 1; ok && i < 8; i++) ok = sl[r0 + i] == sl[r0] + i;
-        whole8[tid] = ok;
     }
     __syncthreads();
     for (int i = tid; i < VD * (VT / 8 + 1); i += 256) {
