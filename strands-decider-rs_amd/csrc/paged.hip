@@ -180,7 +180,7 @@ constexpr int VT = 64, VD = 64;  // rows and dims of a V workgroup
 // 16 bytes.  Each of the others does 512 / HD rows of `hpt` q (or k) heads per thread: HD / 8 threads share a row and a
 // head, 8 dims each, 4 heads side by side.  The rows' cosines and sines (f32 and gathered by axis: more work than a head)
 // come once, through LDS, while each thread's first head is on its way; the next one always is.
-// Bound by bytes: 4099 rows of 32 and 8 heads of 128 dims on three axes, 103 MB, 22.7 us, 4.5 TB/s, where a copy makes
+// Bound by bytes: 4099 rows of 32 and 8 heads of 128 dims on three axes, 103 MB, 22.4 us, 4.6 TB/s, where a copy makes
 // 4.8.  (33.5 us with scalar loads of the weights and the angles gathered by every thread; several heads of a thread in
 // flight at a time cost more registers than they hid: 30.)
 template <class T, int HD>
