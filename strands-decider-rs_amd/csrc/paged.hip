@@ -806,31 +806,37 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
         return {x < total ? 0 : -1, total - 1 - x};
     }
     auto tiles = [&](int b) {
-        if (b >= a.B) return 0;
-        const int n = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap).n * a.G;
-        return n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
+        const int n = request(a.cu, a.kv_lens, min(b, a.B - 1), a.rows, a.max_new, a.kcap).n * a.G;
+        return b < a.B && n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
     };
-    int own = 0;
-    // (cut at 2^24 per lane, which row starts that do not ascend could pass: the sums stay in range)
-    for (int i = 0; i < per; i++) own = min(own + tiles(lane * per + i), 1 << 24);
-    int to = own;
+    auto upto = [&](int v) {  // the sum of lanes 0 to the own
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(to, o);
-        if (lane >= o) to += y;
-    }
-    const int total = __builtin_amdgcn_readlane(to, 63);
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(v, o);
+            if (lane >= o) v += y;
+        }
+        return v;
+    };
+    // lane l counts requests l, l + 64, ..., the tiles are numbered lane by lane
+    // (cut at 2^24 per lane, which row starts that do not ascend could pass: the sums stay in range)
+    int own = 0;
+#pragma unroll 8
+    for (int i = 0; i < per; i++) own = min(own + tiles(64 * i + lane), 1 << 24);
+    const int to = upto(own), total = __builtin_amdgcn_readlane(to, 63);
     if (x >= total) return {-1, 0};
     x = total - 1 - x;
     const int at = __ffsll((long long)__ballot(to > x)) - 1;
     x -= __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(own, at);
-    int b = at * per;
-    for (int i = 0; i < per - 1; i++, b++) {
-        const int n = tiles(b);
-        if (x < n) break;
-        x -= n;
+    if (per == 1) return {at, x};
+    for (int i = 0; i < per; i += 64) {  // lane l: request 64 (i + l) + at
+        const int n = i + lane < per ? tiles(64 * (i + lane) + at) : 0, t = upto(n), sum = __builtin_amdgcn_readlane(t, 63);
+        if (x < sum) {
+            const int l = __ffsll((long long)__ballot(t > x)) - 1;
+            return {64 * (i + l) + at, x - (__builtin_amdgcn_readlane(t, l) - __builtin_amdgcn_readlane(n, l))};
+        }
+        x -= sum;
     }
-    return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(x)};
+    return {-1, 0};
 }
 
 // FEW (2: with the non-temporal hint): the launch ends with the workgroups of the requests with few rows, which would
@@ -1331,7 +1337,7 @@ Plan plan_attn(const PagedShape& s, int B, int rows, int max_new, int max_kv, in
     }
     if (most > p.few) {
         const long long all = (long long)rows * G;
-        p.tiles = (int)(all / TILE_ROWS) + B;
+        p.tiles = (int)(all / TILE_ROWS + std::min((long long)B, all / (p.few + 1)));
         const int nb = blocks(TILE_ROWS / G + 2);
         // One workgroup per CU: tiles as many as there will be, if every request has one (a request's 64 heads of 128 dims on
         // 8000 and 30000 keys 25 and 71 us in at most 8 splits, 15 and 23 in 64; 32 of them 33 and 101 us in 16, 31 and 93
