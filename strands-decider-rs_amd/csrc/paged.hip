@@ -807,7 +807,7 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
     }
     auto tiles = [&](int b) {
         const int n = request(a.cu, a.kv_lens, min(b, a.B - 1), a.rows, a.max_new, a.kcap).n * a.G;
-        return b < a.B && n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
+        return ((b < a.B) & (n > a.few)) ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;  // (no branch: several loads in flight)
     };
     auto upto = [&](int v) {  // the sum of lanes 0 to the own
 #pragma unroll
