@@ -382,6 +382,22 @@ def test_attention_of_a_prompt_among_longer_caches(sdamd, hq, hk, hd):
         check_attn(sdamd, "f16", hq, hk, hd, 32, reqs, gated=True, window=700, seed=30 + i)
 
 
+@pytest.mark.parametrize("B", [65, 150, 5000, 8192])
+def test_attention_of_many_requests(sdamd, B):
+    """Chunks, drafts and single tokens anywhere among many requests, most of them idle; and all of them in tiles."""
+    rng = np.random.default_rng(B)
+    busy = set(rng.permutation(B)[:60].tolist()) | {0, 63, 64, B - 1}
+    for hq, hk, hd, hi, most in [(8, 2, 64, 900, 70), (3, 1, 128, 60, 40), (8, 1, 256, 300, 9)]:
+        reqs = [(0, 0)] * B
+        for i, b in enumerate(sorted(busy)):
+            new = 1 if i % 3 == 0 else int(rng.integers(1, most))
+            reqs[b] = (int(rng.integers(0, hi)) + new, new)
+        check_attn(sdamd, "bf16", hq, hk, hd, 32, reqs, seed=B)
+        check_attn(sdamd, "f16", hq, hk, hd, 32, reqs, seed=B, more_kv=1500, window=100)
+    if B == 150:
+        check_attn(sdamd, "f16", 4, 1, 64, 32, [(40 + b % 7, 5 + b % 3) for b in range(B)], seed=3)
+
+
 @pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (6, 2, 128), (24, 8, 64)])
 def test_a_window_past_every_key_is_none(sdamd, hq, hk, hd):
     """The largest windows there are, rows before position 0 among the requests': bit for bit the call without one."""
