@@ -465,6 +465,11 @@ struct AttnArgs {
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
 
+// Weight of a part of a row's keys (a wave's, a split's) whose running maximum is m, where the largest is mx.  A part that
+// saw no score above -inf has 0, and its zeros, or its NaN (0 times a value that is not finite), are multiplied like any
+// other's: what is seen stays seen, whatever the split.
+__device__ __forceinline__ float part_weight(float m, float mx) { return m == -INFINITY ? 0.f : exp2_fast(m - mx); }
+
 // Output of 4 dims of a row: unnormalised o over the sum l, times the sigmoid of its gates where it has some, rounded once.
 template <class T>
 __device__ __forceinline__ void finish4(f32x4 o, float l, bool gated, u32x2 gate, T* out) {
@@ -703,11 +708,11 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float lw = Ls[w * R + r], f = lw == 0.f ? 0.f : exp2_fast(Ms[w * R + r] - mx);
-            ls += lw == 0.f ? 0.f : lw * f;
+            const float f = part_weight(Ms[w * R + r], mx);
+            ls += Ls[w * R + r] * f;
             const f32x4 x = *reinterpret_cast<const f32x4*>(om(w) + r * HD + (d ^ 4 * (r & 15)));
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] += lw == 0.f ? 0.f : x[e] * f;
+            for (int e = 0; e < 4; e++) o[e] += x[e] * f;
         }
         const int t = rq.q0 + r / a.G, h = kh * a.G + r % a.G;
         const size_t row = (size_t)t * a.HQ + h;
@@ -735,7 +740,7 @@ __global__ __launch_bounds__((64 * few_waves<HD, NR>())) void k_paged_few(const 
 }
 
 // Joins up to 64 splits of one row and writes it: 256 threads, HD / 4 of them side by side (4 dims each), their groups
-// each every so many splits.  Every split of a row has written its maximum and sum, 0 where it had no key.
+// each every so many splits.  Every split of a row has written its maximum, sum and output, zeros where it saw no key.
 constexpr int MAX_KS = 64;
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float* __restrict__ pacc,
@@ -757,8 +762,8 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
     float mx = ml.x;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - mx);
-    float ls = ml.y == 0.f ? 0.f : ml.y * f;
+    const float f = part_weight(ml.x, mx);
+    float ls = ml.y * f;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) ls += __shfl_xor(ls, o);
     if (tid < 64) wt[lane] = f;
@@ -769,7 +774,7 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
         const f32x4 x = *reinterpret_cast<const f32x4*>(pacc + (z * zs + row) * HD + d);
         const float w = wt[z];
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] += w == 0.f ? 0.f : x[e] * w;
+        for (int e = 0; e < 4; e++) o[e] += x[e] * w;
     }
     part[tid / W][tid % W] = o;
     __syncthreads();
@@ -1270,15 +1275,15 @@ __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float
         float mn = mx;
 #pragma unroll
         for (int z = 0; z < N; z++) mn = fmaxf(mn, now.ml[z].x);
-        const float f0 = ls == 0.f ? 0.f : exp2_fast(mx - mn);
+        const float f0 = part_weight(mx, mn);
         mx = mn;
         ls *= f0;
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] *= f0;
 #pragma unroll
         for (int z = 0; z < N; z++) {
-            if (z0 + z >= a.rows_ks || now.ml[z].y == 0.f) continue;
-            const float f = exp2_fast(now.ml[z].x - mx);
+            if (z0 + z >= a.rows_ks) continue;
+            const float f = part_weight(now.ml[z].x, mx);
             ls += now.ml[z].y * f;
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] += now.x[z][e] * f;

@@ -1,0 +1,58 @@
+"""Paged attention on the GPU with values and scores at the ends of their ranges."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+import paged_ref as ref  # noqa: E402
+from test_gpu_paged import attn_case, call  # noqa: E402
+
+
+def results(d):
+    """(request, want, tolerance, got) of every request that has rows."""
+    got = d["out"].view(d["T"], d["hq"], d["hd"])
+    for b, (kv, n) in enumerate(zip(d["kv"], d["new"])):
+        if n:
+            a = int(d["at"][b])
+            want, mag, top = ref.attend_fast(d["q"][a:a + n].double(), d["ks"][b].double(), d["vs"][b].double(), kv, d["scale"])
+            yield b, want, ref.attend_bound(d["kind"], want, mag, top, d["hd"], kv), got[a:a + n].double()
+
+
+# ---- values that are seen with a weight of next to nothing, or of nothing ----
+
+# one request whose keys are split, with a single token and with a chunk; the same unsplit
+SPLIT = [("one token, split", 4, 2, 64, [(5000, 1)]), ("chunk, split", 8, 2, 128, [(5000, 40)]),
+         ("one token, unsplit", 4, 2, 64, [(5000, 1)] + [(1, 1)] * 99), ("chunk, unsplit", 16, 4, 64, [(1200, 1100)])]
+
+
+@pytest.mark.parametrize("far", [True, False])
+@pytest.mark.parametrize("name,hq,hk,hd,reqs", SPLIT)
+def test_a_seen_value_that_is_not_finite_is_never_lost(sdamd, name, hq, hk, hd, reqs, far):
+    """The first keys' scores are 300 below the others' or -inf: their weights vanish in f32, in whole splits, but their
+    infinities and NaN are seen, so these dims are not finite, however the keys are split.  The other dims are as ever."""
+    low = 1000 if reqs[0][0] == 5000 else 64
+
+    def poke(b, k, v):
+        if b == 0:
+            k[:] = 0
+            k[:low, :, 0] = -300.0 if far else -math.inf
+            v[7, :, 3], v[low // 2, :, 5], v[9, :, 9], v[low - 1, :, 11] = math.inf, math.nan, -math.inf, math.nan
+
+    for kind in ("f16", "bf16"):
+        d = attn_case(sdamd, kind, hq, hk, hd, 32, reqs, scale=1.0, poke=poke, seed=1)
+        d["q"][:, :, 0] = 1.0
+        call(sdamd, d)
+        torch.cuda.synchronize()
+        for b, want, tol, g in results(d):
+            dims = torch.zeros(hd, dtype=torch.bool, device="cuda")
+            if b == 0:
+                dims[[3, 5, 9, 11]] = True
+                # rows that see a key of a finite score (a row of -inf alone gives zeros)
+                rows = torch.arange(len(g), device="cuda") + d["kv"][0] - len(g) >= low
+                g, want, tol = g[rows], want[rows], tol[rows]
+                assert int(g[..., dims].isfinite().sum()) == 0, (kind, "a seen value was lost")
+                assert int((~g[..., [5, 11]].isnan()).sum()) == 0, (kind, "a seen NaN was lost")
+            bad = ~((g - want).abs() <= tol)[..., ~dims]
+            assert int(bad.sum()) == 0, (kind, b)
