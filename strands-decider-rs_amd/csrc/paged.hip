@@ -351,7 +351,9 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 // rounded to the rows' type before the second product (f32 sums; the row sum takes the unrounded values): half a step
 // of the type relative to each weight, as the result's own rounding.  The 8 puts f16's normal range at weights down to
 // 2^-22 of the largest (30000 keys of 2^-22 each are 0.7 % of a result); m is raised, and O and the sum rescaled, only
-// when a block's maximum exceeds it by more than 6, so p stays below 2^14 and most blocks rescale nothing.
+// when a block's maximum exceeds it by more than 6, so p stays below 2^15 and most blocks rescale nothing.  From FAR on,
+// where f32 has no fractions left, m and c s in the exponent's one rounding would be apart by more than p's range: there
+// c s is rounded as m was, and the difference taken first (a wave whose m are all nearer, as good as ever, skips it).
 //
 // A masked product is 0 times the value, which is NaN where that is not finite.  Blocks that some row does not see
 // whole (the diagonal, a window's edge, the last block) look at their values first; where one is not finite, the
@@ -366,9 +368,16 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 #define PIN_V(x) (void)(x)
 #endif
 
-constexpr float P_UP = 8.0f, RAISE = 6.0f;
+constexpr float P_UP = 8.0f, RAISE = 6.0f, FAR = 8388608.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A score as it is before c turns it into c s - m, c s rounded.
+__device__ __forceinline__ float less_max(float s, float c, float m) {
+#pragma clang fp contract(off)
+    const float x = s * c;
+    return (x - m) * __builtin_amdgcn_rcpf(c);
+}
 
 // The largest of a value and the one 32 lanes away, and of the four 16 lanes apart.  (The swap of a register with itself
 // leaves one half's values in both halves of each result.)
@@ -605,7 +614,7 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
 #pragma unroll
             for (int e = 1; e < 8; e++) tmax[u] = fmaxf(tmax[u], s2[u][e >> 2][e & 3]);
             tmax[u] = max_quarters(tmax[u]) * a.c;
-            up |= tmax[u] > m[u] + RAISE;
+            up |= tmax[u] - m[u] > RAISE;
         }
         if (__any(up)) {
 #pragma unroll
@@ -619,13 +628,25 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
                     for (int e = 0; e < 4; e++) acc[u][d][e] *= f;
             }
         }
+        float nm[NR];
+        bool far = false;
+#pragma unroll
+        for (int u = 0; u < NR; u++) nm[u] = m[u] == -INFINITY ? 0.f : P_UP - m[u], far |= fabsf(nm[u]) >= FAR;
+        if (__builtin_expect(__any(far), 0)) {
+#pragma unroll
+            for (int u = 0; u < NR; u++)
+                if (fabsf(nm[u]) >= FAR) {
+                    nm[u] = P_UP;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) s2[u][e >> 2][e & 3] = less_max(s2[u][e >> 2][e & 3], a.c, m[u]);
+                }
+        }
         T8 pf[NR];
 #pragma unroll
         for (int u = 0; u < NR; u++) {
-            const float nm = m[u] == -INFINITY ? 0.f : P_UP - m[u];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float p = exp2_fast(__builtin_fmaf(s2[u][e >> 2][e & 3], a.c, nm));
+                const float p = exp2_fast(__builtin_fmaf(s2[u][e >> 2][e & 3], a.c, nm[u]));
                 l[u] += p;
                 pf[u][e] = (T)p;
             }
@@ -963,6 +984,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
     float m = -INFINITY, l = 0.f, nm = 0.f, tmax = -INFINITY;
+    bool far = false;  // m is
     T8 pf[2];
     auto prob = [&](const f32x16& s, int e) INL {
         const float p = exp2_fast(__builtin_fmaf(s[e], a.c, nm));
@@ -1041,8 +1063,8 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
             s[e] = keep ? s[e] : -INFINITY;
         }
     };
-    auto raise = [&]() INL {
-        if (__any(tmax > m + RAISE)) {
+    auto raise = [&](f32x16& s) INL {  // (s: the scores whose maximum is tmax)
+        if (__any(tmax - m > RAISE)) {
             const float mn = fmaxf(m, tmax), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);
             m = mn;
             l *= f;
@@ -1050,8 +1072,16 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[d][e] *= f;
+            nm = m == -INFINITY ? 0.f : P_UP - m;
+            far = fabsf(nm) >= FAR;
+            if (far) nm = P_UP;
         }
-        nm = m == -INFINITY ? 0.f : P_UP - m;
+        if (__builtin_expect(__any(far), 0)) {
+            if (far) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = less_max(s[e], a.c, m);
+            }
+        }
     };
     auto zero = [](f32x16& s) INL {
 #pragma unroll
@@ -1069,7 +1099,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
 #pragma unroll
         for (int n = 0; n < AHEAD; n++) read(n, K, V);
         __builtin_amdgcn_sched_barrier(0);
-        raise();
+        raise(s);
         zero(s2);
         const Rsrc rk = block(nk, Kp), rv = block(nv, Vp);
 #pragma unroll
@@ -1111,7 +1141,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     };
     // the wave's last block
     auto last = [&](f32x16& s, const uint8_t* V) INL {
-        raise();
+        raise(s);
 #pragma unroll
         for (int x = 0; x < 16; x++) prob(s, x);
 #pragma unroll

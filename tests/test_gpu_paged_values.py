@@ -56,3 +56,37 @@ def test_a_seen_value_that_is_not_finite_is_never_lost(sdamd, name, hq, hk, hd, 
                 assert int((~g[..., [5, 11]].isnan()).sum()) == 0, (kind, "a seen NaN was lost")
             bad = ~((g - want).abs() <= tol)[..., ~dims]
             assert int(bad.sum()) == 0, (kind, b)
+
+
+# ---- scores past the f32 integers ----
+
+@pytest.mark.parametrize("kind,sizes", [("f16", [2.0 ** 6, 2.0 ** 11, 2.0 ** 12, 2.0 ** 13, 2.0 ** 14, 2.0 ** 15]),
+                                        ("bf16", [2.0 ** 6, 2.0 ** 13, 2.0 ** 15, 2.0 ** 20, 2.0 ** 40, 2.0 ** 54])])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_of_any_size(sdamd, kind, sizes, sign):
+    """Queries of `size`, keys of +-size times 1 or 5/4 and scores size^2 hd / sqrt(hd) and 5/4 of it, exact in f32: at
+    this distance the lesser weights are 0, and a row's result is the mean of the values at its equal largest scores."""
+    for hq, hk, hd, reqs in [(8, 2, 256, [(5000, 1)]), (4, 2, 64, [(900, 1), (300, 1)]), (8, 2, 128, [(700, 150), (65, 65)]),
+                             (4, 1, 256, [(3000, 40), (90, 1)])]:
+        for size in sizes:
+            def poke(b, k, v):
+                k[:] = sign * size
+                k[-1, :, :] *= 1.25 if sign < 0 else 1.0
+                k[5::29] = sign * size * (1.25 if sign > 0 else 1.0)
+                k[:5] *= 1.25 if sign < 0 else 1.0
+            d = attn_case(sdamd, kind, hq, hk, hd, 32, reqs, poke=poke, seed=3)
+            d["q"].fill_(size)
+            call(sdamd, d)
+            torch.cuda.synchronize()
+            got, u, e = d["out"].view(d["T"], hq, hd), ref.half_step(kind), 2.0 ** -24
+            for b, (kv, n) in enumerate(zip(d["kv"], d["new"])):
+                a, j = int(d["at"][b]), torch.arange(kv, device="cuda")
+                s = d["ks"][b][:, 0, 0].double()
+                for i in {0, n // 2, n - 1}:
+                    seen = j <= kv - n + i
+                    top = seen & (s == s[seen].max())
+                    v = d["vs"][b][top].double().repeat_interleave(hq // hk, 1)
+                    # the equal weights and the result are rounded to the type, sums are in f32 (as in attend_bound)
+                    tol = u * v.mean(0).abs() + (u + (2 * kv + 16) * e) * v.abs().mean(0) * (1 + u) + 2.0 ** -25
+                    bad = ~((got[a + i].double() - v.mean(0)).abs() <= tol)
+                    assert int(bad.sum()) == 0, (kind, hd, reqs, size, b, i, int(bad.sum()))
