@@ -347,13 +347,15 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 // rows) on MFMA with the keys of a 32-row block ordered so that S^T's accumulator layout is the B operand's of O^T +=
 // V^T P^T: probabilities never move between lanes, and both operands come out of the cache's blocks 16 bytes at a time.
 //
-// The online softmax is in base 2 and f32: p = 2^(c s - m + 8), c = scale log2(e), m the running maximum of c s.  P is
+// The online softmax is in base 2 and f32: p = 2^(c s - m + UP), c = scale log2(e), m the running maximum of c s.  P is
 // rounded to the rows' type before the second product (f32 sums; the row sum takes the unrounded values): half a step
-// of the type relative to each weight, as the result's own rounding.  The 8 puts f16's normal range at weights down to
-// 2^-22 of the largest (30000 keys of 2^-22 each are 0.7 % of a result); m is raised, and O and the sum rescaled, only
-// when a block's maximum exceeds it by more than 6, so p stays below 2^15 and most blocks rescale nothing.  From FAR on,
-// where f32 has no fractions left, m and c s in the exponent's one rounding would be apart by more than p's range: there
-// c s is rounded as m was, and the difference taken first (a wave whose m are all nearer, as good as ever, skips it).
+// of the type relative to each weight, as the result's own rounding.  m is raised, and O and the sum rescaled, only
+// when a block's maximum exceeds it by more than 6, so p stays below 2^(UP + 7) and most blocks rescale nothing.  f16's
+// UP is 8: its normal range then is at weights down to 2^-22 of the largest (30000 keys of 2^-22 each are 0.7 % of a
+// result), and p within it.  bf16, whose range is f32's, has -16: sums of a thousand of the type's largest values stay in
+// range, and weights down to 2^-110.  From FAR on, where f32 has no fractions left, m and c s in the exponent's one rounding
+// would be apart by more than p's range: there c s is rounded as m was, and the difference taken first (a wave whose m
+// are all nearer, as good as ever, skips it).
 //
 // A masked product is 0 times the value, which is NaN where that is not finite.  Blocks that some row does not see
 // whole (the diagonal, a window's edge, the last block) look at their values first; where one is not finite, the
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 #define PIN_V(x) (void)(x)
 #endif
 
-constexpr float P_UP = 8.0f, RAISE = 6.0f, FAR = 8388608.f;
+constexpr float RAISE = 6.0f, FAR = 8388608.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -405,6 +407,7 @@ struct Num;
 template <>
 struct Num<f16> {
     static constexpr uint32_t EXP = 0x7C00;
+    static constexpr float UP = 8.0f;
     static __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -415,6 +418,7 @@ struct Num<f16> {
 template <>
 struct Num<bf16> {
     static constexpr uint32_t EXP = 0x7F80;
+    static constexpr float UP = -16.0f;
     typedef Vec8<bf16>::type B8;
     static __device__ __forceinline__ f32x4 mfma16(B8 a, B8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -631,12 +635,12 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
         float nm[NR];
         bool far = false;
 #pragma unroll
-        for (int u = 0; u < NR; u++) nm[u] = m[u] == -INFINITY ? 0.f : P_UP - m[u], far |= fabsf(nm[u]) >= FAR;
+        for (int u = 0; u < NR; u++) nm[u] = m[u] == -INFINITY ? 0.f : Num<T>::UP - m[u], far |= fabsf(nm[u]) >= FAR;
         if (__builtin_expect(__any(far), 0)) {
 #pragma unroll
             for (int u = 0; u < NR; u++)
                 if (fabsf(nm[u]) >= FAR) {
-                    nm[u] = P_UP;
+                    nm[u] = Num<T>::UP;
 #pragma unroll
                     for (int e = 0; e < 8; e++) s2[u][e >> 2][e & 3] = less_max(s2[u][e >> 2][e & 3], a.c, m[u]);
                 }
@@ -1072,9 +1076,9 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[d][e] *= f;
-            nm = m == -INFINITY ? 0.f : P_UP - m;
+            nm = m == -INFINITY ? 0.f : Num<T>::UP - m;
             far = fabsf(nm) >= FAR;
-            if (far) nm = P_UP;
+            if (far) nm = Num<T>::UP;
         }
         if (__builtin_expect(__any(far), 0)) {
             if (far) {

@@ -90,3 +90,33 @@ def test_scores_of_any_size(sdamd, kind, sizes, sign):
                     tol = u * v.mean(0).abs() + (u + (2 * kv + 16) * e) * v.abs().mean(0) * (1 + u) + 2.0 ** -25
                     bad = ~((got[a + i].double() - v.mean(0)).abs() <= tol)
                     assert int(bad.sum()) == 0, (kind, hd, reqs, size, b, i, int(bad.sum()))
+
+
+# ---- values up to the type's largest ----
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (4, 2, 64), (8, 2, 128)])
+def test_values_up_to_the_largest(sdamd, hq, hk, hd):
+    """Values of +-3e38 in bf16 and 65504 in f16 at keys whose weight is 1 (the others' are at most e^-20 in all, of
+    values of the same size): the result is the value, not an infinity."""
+    for kind, most in (("bf16", 3e38), ("f16", 65504.0)):
+        for reqs in ([(4000, 1)], [(400, 1), (33, 1)], [(900, 200), (3, 1)], [(5000, 40)]):
+            for at in (0, 1, -1):  # the key that counts: the first of all, the second, or the last of all
+                def poke(b, k, v):
+                    k[:] = 0
+                    k[at, :, 0] = 32.0
+                    v[:] = v.sign() * most
+                d = attn_case(sdamd, kind, hq, hk, hd, 32, reqs, scale=1.0, poke=poke, seed=4)
+                d["q"].zero_()
+                d["q"][:, :, 0] = 1.0
+                call(sdamd, d)
+                torch.cuda.synchronize()
+                got, u = d["out"].view(d["T"], hq, hd).double(), ref.half_step(kind)
+                for b, (kv, n) in enumerate(zip(d["kv"], d["new"])):
+                    a = int(d["at"][b])
+                    # (a single row's own key is its last; the first row of a chunk sees the first keys)
+                    g = got[a + n - 1] if at < 0 else got[a:a + n][torch.arange(n) + kv - n >= at]
+                    want = d["vs"][b][at].double().repeat_interleave(hq // hk, 0)
+                    # the weight and the result are rounded to the type; 5000 weights of e^-32, each value once more
+                    tol = (2.02 * u + 2 * 5000 * math.exp(-32)) * want.abs()
+                    bad = ~((g - want).abs() <= tol)
+                    assert int(bad.sum()) == 0, (kind, hd, reqs, at, b, int(bad.sum()))
