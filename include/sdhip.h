@@ -321,10 +321,10 @@ int sd_op_paged_attention_ws(int B, int T, int max_new, int max_kv, int HQ, int 
 /* Causal attention of every request's new rows over its pages: row t = cu[b] + i of request b with n =
  * cu[b + 1] - cu[b] rows has position p = kv_lens[b] - n + i and sees the cache rows j <= p, with a window
  * (> 0) those above p - window, holes left out.  out [T][HQ*HD] = softmax(scale q . k) v over the seen rows
- * of kv head h / (HQ/HK), in f32, times sigmoid(gate) when big (rows as in sd_op_paged_prep, gated) is
- * given; zeros where no row is seen or every seen score is -inf.  Values in rows that are not seen, NaN and
- * infinities among them, change nothing; a seen infinity gives one, or NaN where its weight rounds to 0.  Rows
- * of out outside every request are left as they are.
+ * of kv head h / (HQ/HK), zeros where no row is seen or every seen score is -inf, times sigmoid(gate) when
+ * big (rows as in sd_op_paged_prep, gated) is given; in f32, scale from its smallest up to 2.3e38.  Values in
+ * rows that are not seen, NaN and infinities among them, change nothing; a seen infinity gives one, or NaN
+ * where its weight rounds to 0, a seen NaN NaN.  Rows of out outside every request are left as they are.
  * max_new and max_kv are upper bounds of n and kv_lens that the launch is made for (rows and keys past them
  * are left out).  ws holds what sd_op_paged_attention_ws says, 16-byte aligned, and is free again when the
  * call's kernels have run: calls that may overlap, captured graphs among them, need one each.  out, ws and

@@ -714,7 +714,8 @@ int sd_op_paged_attention(const void* Q, const void* big, int stride, const void
             throw sd::Error(who + ": a table row must hold at least one page and fewer than 2^31 cache rows");
         if (max_kv > (long long)max_blocks * page_size) throw sd::Error(who + ": max_kv is more than a table row's pages hold");
         if (window < 0) throw sd::Error(who + ": the window must be at least 1, or 0 for none");
-        if (!(scale > 0.f) || !std::isfinite(scale)) throw sd::Error(who + ": the scale must be positive and finite");
+        if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950f))  // (the kernels' exponentials are in base 2)
+            throw sd::Error(who + ": the scale must be positive and at most 2.3e38");
         if (big && (stride < 2ll * HQ * HD || stride % 8))
             throw sd::Error(who + ": the gates' row stride must be a multiple of 8 and at least 2 * q heads * head_dim");
         for (const void* p : {Q, big, Kp, Vp, static_cast<const void*>(out), static_cast<const void*>(ws)})

@@ -120,3 +120,16 @@ def test_values_up_to_the_largest(sdamd, hq, hk, hd):
                     tol = (2.02 * u + 2 * 5000 * math.exp(-32)) * want.abs()
                     bad = ~((g - want).abs() <= tol)
                     assert int(bad.sum()) == 0, (kind, hd, reqs, at, b, int(bad.sum()))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [1e-45, 1e-39, 1e-20])
+def test_scales_that_make_all_weights_equal(sdamd, kind, scale):
+    """The smallest scales (subnormal ones among them): a row's result is the mean of the values that it sees."""
+    for hq, hk, hd, reqs in [(8, 2, 256, [(700, 1), (60, 50)]), (4, 2, 64, [(900, 1), (31, 1)]), (8, 2, 128, [(5000, 40)])]:
+        d = attn_case(sdamd, kind, hq, hk, hd, 32, reqs, scale=scale, seed=5)
+        call(sdamd, d)
+        torch.cuda.synchronize()
+        for b, want, tol, g in results(d):
+            bad = ~((g - want).abs() <= tol)
+            assert int(bad.sum()) == 0, (kind, hd, b, int(bad.sum()))

@@ -96,3 +96,10 @@ def test_attention_refuses_a_small_workspace(sdamd):
         for ws, n in ((A, need - 1), (None, need), (A, 0)):
             with pytest.raises(sdamd.EngineError, match="workspace"):
                 attn(sdamd, B=1, T=1, max_new=1, max_blocks=4000, max_kv=100000, HQ=8, HK=2, HD=256, ws=ws, ws_bytes=n)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_attention_refuses_a_scale_past_its_range(sdamd, scale):
+    """A scale that is finite, but not in base 2 (times log2 e): 0 times it would not be 0."""
+    with pytest.raises(sdamd.EngineError, match="sd_op_paged_attention: .*scale"):
+        attn(sdamd, scale=scale)
