@@ -1,0 +1,314 @@
+"""Paged attention on the GPU where its work is cut: every key counted once at the edges of splits, waves, blocks and
+pages, holes and values that are not finite among split keys, and nothing written but the documented rows."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+import paged_ref as ref  # noqa: E402
+from paged_ref import slots_of  # noqa: E402
+from test_gpu_paged import attn_case, call, check_attn, compare  # noqa: E402
+
+E = 2.0 ** -24  # half a step of f32
+
+
+def table_of(d):
+    return d["table"].cpu().numpy().astype(np.int64)
+
+
+def zero(b, k, v):
+    k.zero_()
+    v.zero_()
+
+
+# ---- every key once ----
+
+def seen_keys(d, b):
+    """[n][kv] whether a row sees a key."""
+    kv, n = d["kv"][b], d["new"][b]
+    j, p = torch.arange(kv, device="cuda"), torch.arange(kv - n, kv, device="cuda")[:, None]
+    see = j <= p
+    if d["window"]:
+        see = see & (j > p - d["window"])
+    for bb, blk in d["holes"]:
+        if bb == b:
+            see[:, blk * d["ps"]:(blk + 1) * d["ps"]] = False
+    return see
+
+
+def count_keys(sdamd, kind, hq, hk, hd, ps, reqs, **kw):
+    """Queries of zeros weigh all seen keys alike, and a value is 1 in one dim of one call: the dim's result is the share
+    of the seen keys that are its own, at most 32, so that a key lost or taken twice is 3 % of it.  The weights are equal
+    powers of two and their sums whole numbers: a result is a quotient rounded in f32 (4 e) and to the type."""
+    d = attn_case(sdamd, kind, hq, hk, hd, ps, reqs, poke=zero, **kw)
+    d["q"].zero_()
+    table, u, rounds = table_of(d), ref.half_step(kind), -(-max(d["kv"]) // (32 * hd))
+    for r in range(rounds):
+        dims = {}
+        for b, kv in enumerate(d["kv"]):
+            # key j's dim is another one for each request and head, and -1 in all calls but one
+            j, h = torch.arange(kv, device="cuda")[:, None], torch.arange(hk, device="cuda")
+            dim = (j + 17 * b + 5 * h) % (rounds * hd) - r * hd
+            dims[b] = torch.where((dim >= 0) & (dim < hd), dim, -1)
+            v = torch.zeros(kv, hk, hd + 1, dtype=ref.DT[kind], device="cuda")
+            v.scatter_(2, torch.where(dims[b] < 0, hd, dims[b])[..., None], 1.0)
+            slots = slots_of(table, b, ps, 0, kv)
+            keep = np.nonzero((slots >= 0) & (slots < d["n_pages"] * ps))[0]  # (not those of holes)
+            s = torch.as_tensor(slots[keep], device="cuda")
+            d["c"].views()[1][s // ps, :, s % ps // 32, :, s % 32] = v[torch.as_tensor(keep, device="cuda"), :, :hd]
+        d["out"].fill_(7.0)
+        call(sdamd, d)
+        torch.cuda.synchronize()
+        got = d["out"].view(d["T"], hk, hq // hk, hd).double()
+        for b, n in enumerate(d["new"]):
+            if not n:
+                continue
+            see = seen_keys(d, b).float()
+            total = see.sum(1).clamp(min=1)[:, None].double()
+            a = int(d["at"][b])
+            for h in range(hk):
+                mine = torch.zeros(d["kv"][b], hd + 1, device="cuda")
+                mine.scatter_(1, torch.where(dims[b][:, h] < 0, hd, dims[b][:, h])[:, None], 1.0)
+                want = ((see @ mine)[:, :hd].double() / total)[:, None]
+                bad = ~((got[a:a + n, h] - want).abs() <= (u + 4 * E) * want + 2.0 ** -25)
+                assert int(bad.sum()) == 0, (kind, reqs, f"call {r}, request {b}, head {h}: {int(bad.sum())} shares off")
+    return d
+
+
+HEADS = [(8, 2, 256), (32, 8, 128), (24, 8, 64)]
+
+
+@pytest.mark.parametrize("hq,hk,hd", HEADS)
+def test_every_key_counts_once_in_long_caches(sdamd, hq, hk, hd):
+    count_keys(sdamd, "bf16", hq, hk, hd, 64, [(20001, 1)], seed=1)
+    count_keys(sdamd, "f16", hq, hk, hd, 64, [(9000, 1), (130, 1), (16000, 1)], seed=2)
+    count_keys(sdamd, "bf16", hq, hk, hd, 128, [(4097, 2), (8191, 1)], seed=3, more_kv=50000)
+    count_keys(sdamd, "f16", hq, hk, hd, 32, [(6000, 1), (3001, 1)], seed=4, window=2500)
+
+
+@pytest.mark.parametrize("hq,hk,hd", HEADS)
+def test_every_key_counts_once_for_chunks(sdamd, hq, hk, hd):
+    count_keys(sdamd, "bf16", hq, hk, hd, 32, [(7000, 40)], seed=1)
+    count_keys(sdamd, "f16", hq, hk, hd, 32, [(7000, 200), (6000, 1), (300, 2)], seed=2)
+    count_keys(sdamd, "bf16", hq, hk, hd, 64, [(700, 700), (1000, 301), (33, 33)], seed=3)
+    count_keys(sdamd, "f16", hq, hk, hd, 256, [(5000, 90), (2000, 1)], seed=4, window=1000)
+
+
+@pytest.mark.parametrize("hq,hk,hd", HEADS)
+def test_every_key_counts_once_in_batches(sdamd, hq, hk, hd):
+    """Enough requests that nothing is split; drafts; chunks among single tokens."""
+    count_keys(sdamd, "bf16", hq, hk, hd, 32, [(37 + 61 * i, 1) for i in range(128 // hk)], seed=1)
+    count_keys(sdamd, "f16", hq, hk, hd, 64, [(300 + 97 * i, 6) for i in range(16)], seed=2)
+    count_keys(sdamd, "bf16", hq, hk, hd, 32, [(2500, 130)] + [(100 + 153 * i, 1) for i in range(20)] + [(50, 0)], seed=3)
+
+
+@pytest.mark.parametrize("hq,hk,hd,B,kv", [(64, 64, 64, 4, 40000), (320, 16, 128, 16, 9500), (32, 32, 256, 8, 18500)])
+def test_every_key_counts_once_in_long_caches_without_a_split(sdamd, hq, hk, hd, B, kv):
+    """256 workgroups: each reads a whole cache, and a wave more than 64 table entries (some more than 128), in windows."""
+    reqs = [(kv - 129 * b, 1) for b in range(B)]
+    count_keys(sdamd, "bf16", hq, hk, hd, 32, reqs, seed=1)
+
+
+def one_key(sdamd, kind, hq, hk, hd, ps, reqs, keys, seed=0, **kw):
+    """A key that outweighs all others by e^40, in turn each of `keys` (another one for each head): the result of the
+    rows that see it is its value."""
+    d = attn_case(sdamd, kind, hq, hk, hd, ps, reqs, scale=1.0, poke=lambda b, k, v: k.zero_(), seed=seed, **kw)
+    d["q"].zero_()
+    d["q"][:, :, 5] = 1.0
+    table, u = table_of(d), ref.half_step(kind)
+    K = d["c"].views()[0]
+    h = torch.arange(hk, device="cuda")
+    for key in keys:
+        spots, at = [], {}
+        for b, kv in enumerate(d["kv"]):
+            j = (np.arange(hk) * 224 + key + 32 * b) % kv
+            s = torch.as_tensor(table[b, j // ps] * ps + j % ps, device="cuda")
+            spots.append((s // ps, h, s % ps // 32, torch.zeros_like(s), s % 32, torch.full_like(s, 5)))
+            at[b] = torch.as_tensor(j, device="cuda")
+            K[spots[-1]] = 40.0
+        call(sdamd, d)
+        torch.cuda.synchronize()
+        got = d["out"].view(d["T"], hk, hq // hk, hd).double()
+        for b, (kv, n) in enumerate(zip(d["kv"], d["new"])):
+            a, p = int(d["at"][b]), torch.arange(kv - n, kv, device="cuda")[:, None]
+            v = d["vs"][b].double()
+            want = v[at[b], h][None, :, None]
+            # the weight and the result rounded to the type; the other weights are e^-40 each, of values up to 6
+            tol = (2.02 * u) * want.abs() + 12 * kv * math.exp(-40) + 2.0 ** -24
+            bad = ~((got[a:a + n] - want).abs() <= tol) & (p >= at[b])[:, :, None, None]
+            assert int(bad.sum()) == 0, (kind, reqs, f"key {key}, request {b}: {int(bad.sum())} off")
+        for s in spots:
+            K[s] = 0.0
+
+
+def edges(kv):
+    return [j for i in range(0, kv, 32) for j in (i, i + 31) if j < kv]
+
+
+@pytest.mark.parametrize("hq,hk,hd", HEADS)
+def test_the_first_and_last_key_of_every_block(sdamd, hq, hk, hd):
+    one_key(sdamd, "bf16", hq, hk, hd, 64, [(5003, 1)], edges(5003))
+    one_key(sdamd, "f16", hq, hk, hd, 32, [(2100, 40)], edges(2100))
+    one_key(sdamd, "f16", hq, hk, hd, 32, [(900, 6), (1300, 6), (40, 3)], edges(1300))
+    one_key(sdamd, "bf16", hq, hk, hd, 32, [(600, 600), (1000, 1)], edges(1000))
+
+
+def test_single_keys_of_long_caches_without_a_split(sdamd):
+    one_key(sdamd, "bf16", 64, 64, 64, 32, [(40000 - 129 * b, 1) for b in range(4)],
+            [0, 31, 16383, 16384, 16385, 16384 + 255, 32767, 32768, 39000, 39600])
+
+
+# ---- holes and what is not finite, among split keys ----
+
+SPLIT = [[(6000, 1)], [(3000, 2), (9000, 1), (500, 3)], [(5000, 40)], [(4000, 70), (3000, 1)]]
+
+
+@pytest.mark.parametrize("reqs", SPLIT)
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (8, 2, 128), (3, 1, 64)])
+def test_holes_among_split_keys(sdamd, hq, hk, hd, reqs):
+    """Whole splits of holes, holes at their edges, the first and last pages."""
+    ps = 64
+    blocks = [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 11, 17, 30, 31, 32, 33, 34, 35, 36, (reqs[0][0] - 1) // ps]
+    holes = [(0, x) for x in blocks if x * ps < reqs[0][0]] + [(len(reqs) - 1, 3)]
+    check_attn(sdamd, "bf16", hq, hk, hd, ps, reqs, holes=holes, fast=False, seed=3)
+    check_attn(sdamd, "f16", hq, hk, hd, ps, reqs, holes=holes, window=2000, fast=False, gated=True, seed=4)
+    count_keys(sdamd, "f16", hq, hk, hd, ps, reqs, holes=holes, seed=5)
+    # nothing but holes
+    every = [(0, x) for x in range(-(-reqs[0][0] // ps))]
+    d = check_attn(sdamd, "f16", hq, hk, hd, ps, reqs, holes=every, fast=False, seed=6)
+    assert int((d["out"][:reqs[0][1]] != 0).sum()) == 0
+
+
+@pytest.mark.parametrize("reqs", SPLIT)
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (8, 2, 128), (3, 1, 64)])
+def test_values_that_are_not_finite_among_split_keys(sdamd, hq, hk, hd, reqs):
+    """Seen by all rows, by the later rows only, by none; beside a window's edge; in splits of their own."""
+    def poke(b, k, v):
+        n = len(v)
+        v[40, 0, 3], v[n // 2, -1, 9], v[n - 2, 0, 7], v[n - 1, 0, 8] = math.inf, math.nan, -math.inf, math.inf
+        v[n - 1, 0, 3], v[max(n - 2010, 0), -1, 12], v[max(n - 1995, 0), -1, 13] = -math.inf, math.nan, math.inf
+
+    for kind in ("f16", "bf16"):
+        check_attn(sdamd, kind, hq, hk, hd, 64, reqs, poke=poke, fast=False, seed=6)
+        check_attn(sdamd, kind, hq, hk, hd, 64, reqs, poke=poke, fast=False, window=2000, gated=True, seed=7)
+
+
+def test_holes_after_a_call_that_leaves_nan_on_chip(sdamd):
+    """Blocks that are not there give zeros, not what an earlier workgroup left where they would have been."""
+    for hq, hk, hd in [(8, 2, 256), (8, 2, 128), (3, 1, 64)]:
+        nan = attn_case(sdamd, "bf16", hq, hk, hd, 32, [(600, 200)] * 12 + [(500, 1)] * 12,
+                        poke=lambda b, k, v: (k.fill_(math.nan), v.fill_(math.nan)), seed=1)
+        for reqs in ([(200, 60)], [(130, 130), (90, 1)], [(700, 1)]):
+            holes = [(0, x) for x in (0, 1, 2, 3, 5) if 32 * x < reqs[0][0]]
+            d = attn_case(sdamd, "bf16", hq, hk, hd, 32, reqs, holes=holes, seed=2)
+            for _ in range(3):
+                call(sdamd, nan)
+                call(sdamd, d)
+                torch.cuda.synchronize()
+                compare(d, fast=False)
+
+
+# ---- what a call may write, and its bounds ----
+
+def guarded(d, n=4096):
+    """out and ws between guards, and the bits of everything else."""
+    def slab(t):
+        x = torch.empty(t.numel() * t.element_size() + 2 * n, dtype=torch.uint8, device="cuda").fill_(0x5A)
+        body = x[n:n + t.numel() * t.element_size()]
+        body.copy_(t.view(-1).view(torch.uint8))
+        return x, body.view(t.dtype).view(t.shape)
+    og, d["out"] = slab(d["out"])
+    wg, d["ws"] = slab(d["ws"])
+    inputs = [t for t in (d["q"], d["big"], d["c"].k, d["c"].v, d["table"], d["cu"], d["kvl"]) if t is not None]
+    bits = [t.view(torch.uint8).clone() if t.dim() else t for t in inputs]
+
+    def check():
+        torch.cuda.synchronize()
+        for x in (og, wg):
+            assert int((x[:n] != 0x5A).sum()) == 0 and int((x[-n:] != 0x5A).sum()) == 0, "written outside a buffer"
+        for t, b in zip(inputs, bits):
+            assert torch.equal(t.view(torch.uint8), b), "an input was written"
+    return check
+
+
+GUARD = [[(100, 1), (100, 30), (64, 2)], [(5000, 1)], [(7000, 40), (900, 1)], [(300, 300), (0, 0), (2500, 1)], [(6000, 3), (40, 7)]]
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (20, 1, 128), (3, 1, 64)])
+@pytest.mark.parametrize("reqs", GUARD)
+def test_only_out_and_the_workspace_are_written(sdamd, hq, hk, hd, reqs):
+    """The workspace is as large as is asked for, out and it lie between guards; results as ever.  Then row starts and
+    lengths that do not fit: they are cut, whatever they are."""
+    for kind, window, gated in (("bf16", 0, True), ("f16", 500, False)):
+        d = attn_case(sdamd, kind, hq, hk, hd, 32, reqs, window=window, gated=gated, seed=15)
+        check = guarded(d)
+        call(sdamd, d)
+        check()
+        compare(d)
+        for cu, kv in [([0, 2 ** 31 - 1, 31, 2 ** 31 - 1], [2 ** 31 - 1, 100, -64]), ([-5, 40, -7, 33], [-2 ** 31, 2 ** 31 - 1, 0])]:
+            cu, kv = (cu * 2)[:len(reqs) + 1], (kv * 2)[:len(reqs)]
+            d["cu"].copy_(torch.tensor(cu, dtype=torch.int32))
+            d["kvl"].copy_(torch.tensor(kv, dtype=torch.int32))
+            check = guarded(d)
+            call(sdamd, d)
+            check()
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (8, 2, 128), (3, 1, 64)])
+@pytest.mark.parametrize("max_new", [1, 4, 20])
+def test_rows_past_max_new_are_left_out(sdamd, hq, hk, hd, max_new):
+    for reqs in ([(100, 30), (64, 2), (300, 21)], [(5000, 25)]):
+        d = attn_case(sdamd, "bf16", hq, hk, hd, 32, reqs, seed=16)
+        d["max_new"] = max_new
+        d["ws"] = torch.full((max(sdamd.paged_attention_ws(len(reqs), d["T"], max_new, d["max_kv"], hq, hk, hd), 16),), 255,
+                             dtype=torch.uint8, device="cuda")
+        check = guarded(d)
+        call(sdamd, d)
+        check()
+        got = d["out"].view(d["T"], hq, hd)
+        for b, (kv, n) in enumerate(reqs):
+            a, m = int(d["at"][b]), min(n, max_new)
+            want, mag, top = ref.attend_fast(d["q"][a:a + n].double(), d["ks"][b].double(), d["vs"][b].double(), kv, d["scale"])
+            tol = ref.attend_bound("bf16", want, mag, top, hd, kv)
+            bad = ~((got[a:a + m].double() - want[:m]).abs() <= tol[:m])
+            assert int(bad.sum()) == 0, (reqs, b)
+            assert int((got[a + m:a + n] != 7.0).sum()) == 0, (reqs, b, "a row past max_new was written")
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 2, 256), (8, 2, 128), (3, 1, 64)])
+def test_keys_past_max_kv_are_left_out(sdamd, hq, hk, hd):
+    """Also where a row, or a row in its window, is past them all."""
+    for reqs in ([(100, 1), (80, 7), (300, 21)], [(5000, 1)], [(5000, 25)]):
+        for cut in (1, 33, 64, 290, 4001):
+            for window in (0, 40):
+                if cut >= reqs[-1][0]:
+                    continue
+                d = attn_case(sdamd, "f16", hq, hk, hd, 32, reqs, window=window, seed=17)
+                d["max_kv"] = cut
+                d["ws"] = torch.full((max(sdamd.paged_attention_ws(len(reqs), d["T"], d["max_new"], cut, hq, hk, hd), 16),), 255,
+                                     dtype=torch.uint8, device="cuda")
+                check = guarded(d)
+                call(sdamd, d)
+                check()
+                d["ks"], d["vs"] = [k[:cut] for k in d["ks"]], [v[:cut] for v in d["vs"]]
+                compare(d, fast=False)
+
+
+def test_keys_and_values_of_a_page_side_by_side(sdamd):
+    """One buffer with each page's keys and then its values: the page stride is two pages."""
+    for hq, hk, hd, ps in [(8, 2, 256, 32), (4, 4, 64, 64)]:
+        page = hk * ps * hd
+        d = attn_case(sdamd, "bf16", hq, hk, hd, ps, [(100, 1), (200, 100), (3000, 1)], pstride=2 * page, seed=12)
+        c = d["c"]
+        both = torch.zeros((c.n_pages + 1) * 2 * page, dtype=torch.bfloat16, device="cuda")
+        for p in range(c.n_pages):
+            both[2 * p * page:(2 * p + 1) * page] = c.k[2 * p * page:(2 * p + 1) * page]
+            both[(2 * p + 1) * page:(2 * p + 2) * page] = c.v[2 * p * page:(2 * p + 1) * page]
+        c.k, c.v = both[:c.n_pages * 2 * page], both[page:page + c.n_pages * 2 * page]
+        check = guarded(d)
+        call(sdamd, d)
+        check()
+        compare(d)
