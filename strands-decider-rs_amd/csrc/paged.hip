@@ -359,7 +359,9 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 //
 // A masked product is 0 times the value, which is NaN where that is not finite.  Blocks that some row does not see
 // whole (the diagonal, a window's edge, the last block) look at their values first; where one is not finite, the
-// products take it as 0, and at the end the rows that see it add it, element by element (add_seen).
+// products take it as 0, and where some row sees it, the rows that do add it at the end, element by element, in those
+// blocks alone (add_seen).  (Cache rows behind a request's last that were never written may be NaN: 64 requests of 1000
+// to 8191 keys take 143 us with them and without; with a look at every block at the end 697.)
 
 // (left to itself the compiler keeps the larger lambdas as calls, and with them their captures in memory)
 #define INL __attribute__((always_inline))
@@ -444,6 +446,16 @@ __device__ __forceinline__ u32x4 finite8(u32x4 v) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = v[i] & ~(((((v[i] & M) + A) & 0x80008000u) >> 15) * 0xFFFFu);
+    return r;
+}
+
+// Whether one of the values of keys j to j + 7 that is not finite is a key's in [lo, hi).
+template <class T>
+__device__ __forceinline__ bool odd_within(u32x4 v, int j, int lo, int hi) {
+    constexpr uint32_t M = Num<T>::EXP;
+    bool r = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) r |= (v[i >> 1] >> (16 * (i & 1)) & M) == M && j + i >= lo && j + i < hi;
     return r;
 }
 
@@ -570,7 +582,7 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
 #pragma unroll
         for (int d = 0; d < ND; d++) acc[u][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    bool rare = false;  // some value was taken as 0
+    bool rare = false;  // some value that is seen was taken as 0
     struct Blk {
         u32x4 k[2][NS], v[ND];
         bool there;
@@ -660,9 +672,13 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
 #pragma unroll
             for (int d = 0; d < ND; d++) odd |= not_finite<T>(x.v[d]);
             if (__builtin_expect(__any(odd != 0), 0)) {
-                rare = true;
+                bool seen = false;
 #pragma unroll
-                for (int d = 0; d < ND; d++) x.v[d] = finite8<T>(x.v[d]);
+                for (int d = 0; d < ND; d++) {
+                    seen |= odd_within<T>(x.v[d], j0 + 8 * fg, lo, hi);
+                    x.v[d] = finite8<T>(x.v[d]);
+                }
+                rare |= __any(seen) != 0;
             }
         }
 #pragma unroll
@@ -694,9 +710,8 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
     if (__builtin_expect(rare, 0)) {  // add_seen: see above
 #pragma unroll 1
         for (int i = 0; i < cnt; i++) {
-            // (every block: a second time what a product gave already changes neither an infinity nor a NaN)
             const int blk = first + NW * i, page = tb[blk >> lbpp], j0 = 32 * blk;
-            if ((unsigned)page >= (unsigned)a.n_pages) continue;
+            if ((unsigned)page >= (unsigned)a.n_pages || (j0 >= open0 && j0 + 32 <= open1)) continue;
             const T* const v = Vp + (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32);
 #pragma unroll 1
             for (int j = j0; j < j0 + 32; j++)
@@ -885,7 +900,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     constexpr int IW = PART / 1024;  // in so many DMAs
     // (an array per buffer: the compiler then sees that the DMAs into one never alias the reads of another)
     __shared__ __align__(1024) uint8_t K0[BB], K1[BB], K2[BB], K3[BB], V0[BB], V1[BB], V2[BB], V3[BB];
-    __shared__ int rare;  // some value was taken as 0
+    __shared__ int rare;  // some value that is seen was taken as 0
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
     if constexpr (FEW != 0) {
@@ -1050,9 +1065,13 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
 #pragma unroll
         for (int u = 0; u < IW; u++) x |= not_finite<T>(v[u]);
         if (__builtin_expect(__any(x != 0), 0)) {
+            bool seen = false;
 #pragma unroll
-            for (int u = 0; u < IW; u++) *reinterpret_cast<u32x4*>(p + u * 1024) = finite8<T>(v[u]);
-            rare = 1;
+            for (int u = 0; u < IW; u++) {
+                seen |= odd_within<T>(v[u], j0 + 8 * ((lane & 3) ^ ((lane >> 4) & 3)), lo, hi);
+                *reinterpret_cast<u32x4*>(p + u * 1024) = finite8<T>(v[u]);
+            }
+            if (seen) rare = 1;
         }
     };
     // masks the scores of block j
@@ -1218,9 +1237,8 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(rare), 0)) {  // add_seen: see above
 #pragma unroll 1
         for (int blk = blk0; blk < blk1; blk++) {
-            // (every block: a second time what a product gave already changes neither an infinity nor a NaN)
             const int j0 = 32 * blk, page = tb[blk >> lbpp];
-            if ((unsigned)page >= (unsigned)a.n_pages) continue;
+            if ((unsigned)page >= (unsigned)a.n_pages || (j0 >= wg0 && j0 + 32 <= wg1)) continue;
             const T* const v = Vp + (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32);
 #pragma unroll 1
             for (int j = j0; j < j0 + 32; j++)
