@@ -181,8 +181,9 @@ constexpr int VT = 64, VD = 64;  // rows and dims of a V workgroup
 // head, 8 dims each, 4 heads side by side.  The rows' cosines and sines (f32 and gathered by axis: more work than a head)
 // come once, through LDS, while each thread's first head is on its way; the next one always is.
 // Bound by bytes: 4099 rows of 32 and 8 heads of 128 dims on three axes, 103 MB, 22.4 us, 4.6 TB/s, where a copy makes
-// 4.8.  (33.5 us with scalar loads of the weights and the angles gathered by every thread; several heads of a thread in
-// flight at a time cost more registers than they hid: 30.)
+// 4.8; 19.6 again and again on the same buffers, which the last-level cache holds in part.  (33.5 us with scalar loads of
+// the weights and the angles gathered by every thread.  Two and four heads of a thread in flight at a time cost more
+// registers than they hid: 20.2 and 21.9 where one takes 19.8.)
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, int stride, int q_step,
                                                     const float* __restrict__ qw, const float* __restrict__ kw,
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 // whole (the diagonal, a window's edge, the last block) look at their values first; where one is not finite, the
 // products take it as 0, and where some row sees it, the rows that do add it at the end, element by element, in those
 // blocks alone (add_seen).  (Cache rows behind a request's last that were never written may be NaN: 64 requests of 1000
-// to 8191 keys take 143 us with them and without; with a look at every block at the end 697.)
+// to 8191 keys take 144 us with them and without; with a look at every block at the end 697.)
 
 // (left to itself the compiler keeps the larger lambdas as calls, and with them their captures in memory)
 #define INL __attribute__((always_inline))
@@ -449,13 +450,12 @@ __device__ __forceinline__ u32x4 finite8(u32x4 v) {
     return r;
 }
 
-// Whether one of the values of keys j to j + 7 that is not finite is a key's in [lo, hi).
-template <class T>
-__device__ __forceinline__ bool odd_within(u32x4 v, int j, int lo, int hi) {
-    constexpr uint32_t M = Num<T>::EXP;
-    bool r = false;
+// All bits of the values of keys j to j + 7 that are in [lo, hi).
+__device__ __forceinline__ u32x4 keys_within(int j, int lo, int hi) {
+    u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 8; i++) r |= (v[i >> 1] >> (16 * (i & 1)) & M) == M && j + i >= lo && j + i < hi;
+    for (int i = 0; i < 4; i++)
+        r[i] = (j + 2 * i >= lo && j + 2 * i < hi ? 0xFFFFu : 0u) | (j + 2 * i + 1 >= lo && j + 2 * i + 1 < hi ? 0xFFFF0000u : 0u);
     return r;
 }
 
@@ -672,13 +672,15 @@ __device__ __forceinline__ void few_part(const int x, const int b, const T* __re
 #pragma unroll
             for (int d = 0; d < ND; d++) odd |= not_finite<T>(x.v[d]);
             if (__builtin_expect(__any(odd != 0), 0)) {
-                bool seen = false;
+                const u32x4 some = keys_within(j0 + 8 * fg, lo, hi);  // (seen by some row)
+                odd = 0;
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    seen |= odd_within<T>(x.v[d], j0 + 8 * fg, lo, hi);
-                    x.v[d] = finite8<T>(x.v[d]);
+                for (int d = 0; d < ND; d++) x.v[d] &= some, odd |= not_finite<T>(x.v[d]);
+                if (__any(odd != 0)) {
+                    rare = true;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) x.v[d] = finite8<T>(x.v[d]);
                 }
-                rare |= __any(seen) != 0;
             }
         }
 #pragma unroll
@@ -831,14 +833,16 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
 // Bound by MFMA and the softmax beside it: each wave has 32 rows on v_mfma_f32_32x32x16, its queries and outputs in
 // registers, and all 4 share blocks of 32 keys that arrive by LDS DMA, three ahead.  A block's probabilities run between
 // the products of the next one's scores and of its own output.  A prompt of 8192 tokens, 8 and 2 heads of 256 dims: 291
-// us, 945 TFLOP/s; four chunks of 2048 on 2048 to 8192 old keys, 32 and 8 heads of 128 dims: 515 us, 1020 TFLOP/s, where
+// to 303 us, up to 945 TFLOP/s; four chunks of 2048 on 2048 to 8192 old keys, 32 and 8 heads of 128 dims: 508 to 530 us,
+// up to 1040 TFLOP/s, where
 // a library product of 8192^3 makes 1200.  MFMA is busy half of the cycles, the softmax's vector instructions (half of
 // them 16 exponentials of 16 cycles per block) the other half, and the power limit sets the clock: 2.0 GHz on random data,
 // while zeros take 252 and 408 us.  Fragments read a step ahead, which probabilities run where, and wave priorities
 // change 1 %.
 // Workgroup x of the launch is kv head x % HK (with 8 heads, one per XCD's L2), split and tile; the tiles of all
 // requests with more than `few` rows are numbered through, and taken from the last on: a causal chunk's late tiles are
-// the long ones.
+// the long ones.  (Each workgroup finds its tile by itself, from all requests: 1086 us for 8192 requests of 20 new tokens
+// on 300 keys, 8 and 2 heads of 128 dims, whose keys and values alone are 455.)
 constexpr int TILE_ROWS = 128;
 struct Tile {
     int b, i;  // request and tile in it; b < 0: none
@@ -1065,13 +1069,14 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_rows(const T* _
 #pragma unroll
         for (int u = 0; u < IW; u++) x |= not_finite<T>(v[u]);
         if (__builtin_expect(__any(x != 0), 0)) {
-            bool seen = false;
+            const u32x4 some = keys_within(j0 + 8 * ((lane & 3) ^ ((lane >> 4) & 3)), lo, hi);  // (seen by some row)
+            x = 0;
 #pragma unroll
             for (int u = 0; u < IW; u++) {
-                seen |= odd_within<T>(v[u], j0 + 8 * ((lane & 3) ^ ((lane >> 4) & 3)), lo, hi);
+                v[u] &= some, x |= not_finite<T>(v[u]);
                 *reinterpret_cast<u32x4*>(p + u * 1024) = finite8<T>(v[u]);
             }
-            if (seen) rare = 1;
+            if (x != 0) rare = 1;
         }
     };
     // masks the scores of block j
@@ -1414,8 +1419,8 @@ void prep_as(const PagedShape& s, const PagedPrep& a, hipStream_t st) {
     auto groups = [&](int hpt) {
         return ((size_t)a.rows * HD + 511) / 512 * ((s.HQ + 4 * hpt - 1) / (4 * hpt) + (s.HK + 4 * hpt - 1) / (4 * hpt));
     };
-    // heads per thread: as many as leave nearly three workgroups per CU (us at 1, 2, 4, 8: 32 and 8 heads of 128, three
-    // axes, 256 rows 6.4 7.5 7.1 7.5, 1024 rows 10.4 8.6 7.7 8.7, 4099 rows 30.9 22.4 20.7 20.1)
+    // heads per thread: as many as leave nearly three workgroups per CU (us at 1, 2, 4, 8, on the same buffers again and
+    // again: 32 and 8 heads of 128, three axes, 256 rows 6.4 7.5 7.1 7.5, 1024 rows 10.4 8.6 7.7 8.7, 4099 rows 30.9 22.4 20.7 20.1)
     int hpt = 8;
     while (hpt > 1 && groups(hpt) < 700) hpt /= 2;
     const size_t nv = (size_t)((a.rows + VT - 1) / VT) * s.HK * (HD / VD);
