@@ -308,7 +308,7 @@ int sd_op_page_plan(const void* lens, const void* news, int B, int T, int page_s
  * an image's patches, say).  Positions outside the table take its nearest row, axes past the last the last.
  * All in f32, rounded once: q to Q [T][HQ][HD], k and v to their rows' slots.  A row whose slot is outside
  * [0, n_pages * page_size) is passed over (Q too); two rows of one slot give either's values.  Q may not
- * overlap big. */
+ * overlap big, nor Q and the pages each other or an input (K and V pages may lie in turn in one buffer). */
 int sd_op_paged_prep(const void* big, int stride, int gated, const void* qw, const void* kw, const void* rope, int rope_len,
                      const void* pos, int axes, const void* pair_axis, const void* slots, int T, int HQ, int HK, int HD,
                      int RD, int page_size, int n_pages, size_t page_stride, void* Q, void* Kp, void* Vp, int type,
@@ -326,7 +326,8 @@ int sd_op_paged_attention_ws(int B, int T, int max_new, int max_kv, int HQ, int 
  * rows that are not seen, NaN and infinities among them, change nothing; a seen infinity gives one, or NaN
  * where its weight rounds to 0, a seen NaN NaN.  Rows of out outside every request are left as they are.
  * max_new and max_kv are upper bounds of n and kv_lens that the launch is made for (rows and keys past them
- * are left out).  ws holds what sd_op_paged_attention_ws says, 16-byte aligned, and is free again when the
+ * are left out): max_new chooses the kernels and max_kv the split of the keys, so bounds near the sizes are
+ * the fastest.  ws holds what sd_op_paged_attention_ws says, 16-byte aligned, and is free again when the
  * call's kernels have run: calls that may overlap, captured graphs among them, need one each.  out, ws and
  * the inputs may not overlap. */
 int sd_op_paged_attention(const void* Q, const void* big, int stride, const void* Kp, const void* Vp, const void* table,
