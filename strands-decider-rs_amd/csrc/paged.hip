@@ -5,45 +5,14 @@
 // has: K [HK][PS / 32][HD / 32][32 rows][32 dims], V transposed [HK][PS / 32][HD][32 rows].  Page p starts `pstride`
 // elements after page p - 1.  Row j of a request lies in page table[j / PS] at row j % PS; a table entry outside
 // [0, n_pages) is a hole, whose rows nothing reads or writes.
-#include <algorithm>
-#include <climits>
-#include <cmath>
-#include <type_traits>
-
-#include "common.h"
-#include "device.h"
+#include "paged.h"
 
 namespace sd {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-
-typedef __bf16 bf16;
-template <class T>
-struct Vec8;
-template <>
-struct Vec8<f16> {
-    typedef f16x8 type;
-};
-template <>
-struct Vec8<bf16> {
-    typedef __bf16 type __attribute__((ext_vector_type(8)));
-};
-
 // ---- the page plan --------------------------------------------------------------------------------------------------
 
 constexpr int PLAN_T = 1024;  // threads of a plan workgroup
-
-// The last index b of [0, B) with to[b] <= x, for to[0] = 0 <= x < to[B] ascending (empty ranges are passed over).
-__device__ __forceinline__ int find_range(const int* to, int B, int x) {
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (to[mid] <= x) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
 
 // Two sums side by side over the workgroup: exclusive prefixes of (a, b) in thread order.
 __device__ __forceinline__ void scan2(long long& a, long long& b, long long (*ws)[2]) {
@@ -153,12 +122,6 @@ __global__ __launch_bounds__(PLAN_T) void k_page_plan(const int* __restrict__ le
 }
 
 // ---- norm, rotation and cache write ---------------------------------------------------------------------------------
-
-// Element offset of (slot, kv head) in a cache whose rows' 32-row blocks hold HD x 32 elements.
-template <int HD>
-__device__ __forceinline__ size_t block_at(int slot, int kh, int lps, size_t pstride) {
-    return (size_t)(slot >> lps) * pstride + ((size_t)kh * (1 << (lps - 5)) + ((slot & ((1 << lps) - 1)) >> 5)) * (HD * 32);
-}
 
 // The sum over each N adjacent lanes, in all of them.
 template <int N>
@@ -364,72 +327,7 @@ __global__ __launch_bounds__(256) void k_paged_prep(const T* __restrict__ big, i
 // blocks alone (add_seen).  (Cache rows behind a request's last that were never written may be NaN: 64 requests of 1000
 // to 8191 keys take 144 us with them and without; with a look at every block at the end 697.)
 
-// (left to itself the compiler keeps the larger lambdas as calls, and with them their captures in memory)
-#define INL __attribute__((always_inline))
-// (and it moves work that the products are to cover out from between them: a volatile asm keeps its place)
-#if defined(__HIP_DEVICE_COMPILE__)
-#define PIN_V(x) asm volatile("" : "+v"(x))
-#else
-#define PIN_V(x) (void)(x)
-#endif
-
-constexpr float RAISE = 6.0f, FAR = 8388608.f;
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// A score as it is before c turns it into c s - m, c s rounded.
-__device__ __forceinline__ float less_max(float s, float c, float m) {
-#pragma clang fp contract(off)
-    const float x = s * c;
-    return (x - m) * __builtin_amdgcn_rcpf(c);
-}
-
-// The largest of a value and the one 32 lanes away, and of the four 16 lanes apart.  (The swap of a register with itself
-// leaves one half's values in both halves of each result.)
-__device__ __forceinline__ float max_halves(float x) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-    const uint32_t lo = sw[0], hi = sw[1];
-    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
-#else
-    return x;
-#endif
-}
-__device__ __forceinline__ float max_quarters(float x) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const auto sw = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-    const uint32_t lo = sw[0], hi = sw[1];
-    return max_halves(fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)));
-#else
-    return x;
-#endif
-}
-
-template <class T>
-struct Num;
-template <>
-struct Num<f16> {
-    static constexpr uint32_t EXP = 0x7C00;
-    static constexpr float UP = 8.0f;
-    static __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Num<bf16> {
-    static constexpr uint32_t EXP = 0x7F80;
-    static constexpr float UP = -16.0f;
-    typedef Vec8<bf16>::type B8;
-    static __device__ __forceinline__ f32x4 mfma16(B8 a, B8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ f32x16 mfma32(B8 a, B8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    }
-};
+constexpr float RAISE = 6.0f;
 
 // Nonzero where one of 8 values is not finite (its exponent's bits all set: one more carries into the sign's place).
 template <class T>
@@ -459,25 +357,6 @@ __device__ __forceinline__ u32x4 keys_within(int j, int lo, int hi) {
     return r;
 }
 
-// One request's part in a launch, cut to the bounds that the launch is made for.
-struct Req {
-    int q0;        // its first row
-    int n;         // rows to do
-    int p0;        // position of its first row
-    int kcap;      // keys that may be read
-};
-__device__ __forceinline__ Req request(const int* __restrict__ cu, const int* __restrict__ kv_lens, int b, int rows,
-                                       int max_new, int kcap) {
-    const int a = cu[b], e = cu[b + 1], kv = max(kv_lens[b], -(1 << 30));
-    Req r;
-    r.q0 = min(max(a, 0), rows);
-    const int n = min(max(e, r.q0), rows) - r.q0;
-    r.n = min(n, max_new);
-    r.p0 = kv - n;
-    r.kcap = min(kcap, max(kv, 0));
-    return r;
-}
-
 // The launch's arguments that all attention kernels share.
 struct AttnArgs {
     const int *table, *cu, *kv_lens;
@@ -489,11 +368,6 @@ struct AttnArgs {
     // the first key that a row at position p sees (one before position 0 sees none, whatever this says)
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
-
-// Weight of a part of a row's keys (a wave's, a split's) whose running maximum is m, where the largest is mx.  A part that
-// saw no score above -inf has 0, and its zeros, or its NaN (0 times a value that is not finite), are multiplied like any
-// other's: what is seen stays seen, whatever the split.
-__device__ __forceinline__ float part_weight(float m, float mx) { return m == -INFINITY ? 0.f : exp2_fast(m - mx); }
 
 // Output of 4 dims of a row: unnormalised o over the sum l, times the sigmoid of its gates where it has some, rounded once.
 template <class T>
@@ -522,15 +396,6 @@ __device__ __forceinline__ u32x2 gate4(const T* big, size_t at) {
 // for bytes that one wave alone uses).  64 requests of 1000 to 8191 keys, 32 and 8 heads of 128 dims, 776 MB: 143 us, 5.4
 // TB/s; two of 90 and 131 thousand, 8 and 2 heads of 256 dims: 79 us, 6.2 TB/s.  A CU alone draws 60 GB/s, so short
 // caches are split as far as a join lets them: 700 keys of those heads 9.0 us, launches and two trips to memory.
-// 16 bytes per lane; ONCE: of data that nothing reads again before it has left the caches (the non-temporal hint).
-template <bool ONCE>
-__device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t voff, uint32_t soff) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    if constexpr (ONCE) return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 2));
-#endif
-    return buf_b128(r, voff, soff);
-}
-
 template <int HD, int NR>
 constexpr int few_waves() { return HD * NR <= 128 ? 8 : 4; }  // 8 where two fit a SIMD's registers (157 -> 143)
 // Workgroup x of request b, of NW waves: om(w) gives LDS of R x HD floats for each wave, Ms and Ls are R of them per wave.
@@ -1349,8 +1214,6 @@ __global__ __launch_bounds__(256) void k_paged_join_rows(AttnArgs a, const float
     finish4<T>(o, ls, big, gate, out + row * HD + d);
 }
 
-int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
-
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
 struct Plan {
     int nr = 0;                      // 16-row groups of k_paged_few, 0: not launched
@@ -1477,18 +1340,6 @@ void attn_as(const PagedShape& s, const PagedAttn& a, hipStream_t st) {
                            rows_max);
         launched("paged_attention");
     }
-}
-
-// f(type tag, head_dim constant)
-template <class F>
-void by_type(const PagedShape& s, F&& f) {
-    auto dims = [&](auto t) {
-        if (s.HD == 64) f(t, std::integral_constant<int, 64>());
-        else if (s.HD == 128) f(t, std::integral_constant<int, 128>());
-        else f(t, std::integral_constant<int, 256>());
-    };
-    if (s.bf16) dims(bf16());
-    else dims(f16());
 }
 
 }  // namespace
