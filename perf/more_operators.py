@@ -315,23 +315,24 @@ def run(st):
     return {"rope": _plain_rope, "angles": _plain_angles, "weights": _plain_weights, "evict": _plain_evict, "move": _plain_move}[st["op"]](st)
 
 
-def _own_params(st):
-    """The parameters as the package takes them, made once for a state as a program makes them once for a model."""
-    if "rope" not in st:
-        sd, p = _pkg(), dict(st["params"])
+def _own_freqs(st):
+    """The pairs' frequencies on the device, made once for a state as a program makes them once for a model."""
+    if "freqs" not in st:
+        sd, p = _pkg(), st["params"]
         kinds = {"plain": sd.ROPE_PLAIN, "linear": sd.ROPE_LINEAR, "base": sd.ROPE_BASE, "parts": sd.ROPE_PARTS}
-        st["rope"] = sd.rope_params(p.pop("rotary_dim"), p.pop("theta"), kinds[p.pop("scaling")], **p)
-    return st["rope"]
+        f = sd.rope_freqs(p["rotary_dim"], p["theta"], kinds[p["scaling"]], p["factor"], p["length"], p["low"], p["high"])
+        st["freqs"] = torch.from_numpy(f).cuda()
+    return st["freqs"].data_ptr()
 
 
 def _own_rope(st):
     sd = _pkg()
     big, hq, hk, hd = st["big"], st["hq"], st["hk"], st["hd"]
     step = hd * (2 if st["gated"] else 1)
-    sd.op_rope(_own_params(st), sd.ROPE_HALF if st["layout"] == "half" else sd.ROPE_PAIRS, st["pos"].data_ptr(), st["t"],
-               hd, big.data_ptr(), big.shape[1], step, hq, big.data_ptr() + hq * step * big.element_size(), big.shape[1],
-               hd, hk, {"f16": sd.F16, "bf16": sd.BF16, "f32": sd.F32}[st["type"]], inverse=st["inverse"],
-               Qo=st["q"].data_ptr(), Ko=st["k"].data_ptr())
+    sd.op_rope(_own_freqs(st), st["rd"], sd.ROPE_HALF if st["layout"] == "half" else sd.ROPE_PAIRS, st["pos"].data_ptr(),
+               st["t"], hd, big.data_ptr(), big.shape[1], step, hq, big.data_ptr() + hq * step * big.element_size(),
+               big.shape[1], hd, hk, {"f16": sd.F16, "bf16": sd.BF16, "f32": sd.F32}[st["type"]],
+               magnitude=st["params"]["magnitude"], inverse=st["inverse"], Qo=st["q"].data_ptr(), Ko=st["k"].data_ptr())
     return {"q": st["q"], "k": st["k"]}
 
 
@@ -339,7 +340,8 @@ def _own_angles(st):
     sd = _pkg()
     sd.op_page_positions(st["cu"].data_ptr(), st["dropped"].data_ptr(), st["b"], st["t"], st["at"].data_ptr(),
                          st["pos"].data_ptr())
-    sd.op_rope_table(_own_params(st), st["pos"].data_ptr(), st["t"], st["table"].data_ptr())
+    sd.op_rope_table(_own_freqs(st), st["rd"] // 2, st["pos"].data_ptr(), st["t"], st["table"].data_ptr(),
+                     magnitude=st["params"]["magnitude"])
     return {"pos": st["pos"], "table": st["table"]}
 
 
