@@ -335,6 +335,118 @@ int sd_op_paged_attention(const void* Q, const void* big, int stride, const void
                           int HK, int HD, int page_size, int n_pages, size_t page_stride, int window, float scale, void* out,
                           void* ws, size_t ws_bytes, int type, void* stream, char* err, size_t errlen);
 
+/* ---- rotary positions apart from the paged cache's own (no counterpart in the reference, whose positions are the
+ * cache's rows): angles scaled for contexts longer than the trained one, at any position, as a table of a step's rows for
+ * sd_op_paged_prep or applied to rows, for pairs in either layout.  A request that has dropped cached rows (below) counts
+ * its positions apart from them: sd_op_page_positions, then sd_op_rope_table once per step, then sd_op_paged_prep with the
+ * row's own number in the place of its position.  These calls allocate nothing, wait for nothing and keep nothing. ---- */
+
+/* float32 rows, of sd_op_rope alone. */
+enum { SD_F32 = 2 };
+/* Pair j of a head's RD rotated dims: dims j and j + RD/2 (sd_op_paged_prep's layout), or dims 2j and 2j + 1. */
+enum { SD_ROPE_HALF = 0, SD_ROPE_PAIRS = 1 };
+/* How the frequencies f_j = theta^(-2j/RD) are scaled by factor s: not at all; f_j / s; theta s^(RD/(RD-2)) in the place
+ * of theta; or f_j (k + (1 - k) / s) with k = (length f_j / (2 pi) - low) / (high - low) within [0, 1]: pairs that make
+ * fewer than `low` turns over the trained length are slowed down, those that make more than `high` are left. */
+enum { SD_ROPE_PLAIN = 0, SD_ROPE_LINEAR = 1, SD_ROPE_BASE = 2, SD_ROPE_PARTS = 3 };
+
+/* freqs [RD/2] f64, on the host: the pairs' frequencies in radians per position.  RD even, 2 to 256 (4 for SD_ROPE_BASE),
+ * theta and s at least 1; length, low and high of SD_ROPE_PARTS alone: length > 0, 0 <= low < high.  The calls below take
+ * such an array on the device, or any other frequencies. */
+int sd_rope_freqs(int RD, double theta, int scaling, double factor, double length, double low, double high, double* freqs,
+                  char* err, size_t errlen);
+
+/* table [n][pairs][2] f32: magnitude times the cosine and the sine of pos[i] freqs[j] (pos i32 [n], any value; null: i),
+ * computed in f64 and rounded once.  freqs [pairs] f64 on the device, 1 to 128 pairs; n * pairs below 2^31.  It is
+ * sd_op_paged_prep's table: with the positions of a step's T rows (axes times T, axis by axis, where there are several) and
+ * rope_len = n, row t's position there is t (a T + t on axis a). */
+int sd_op_rope_table(const void* freqs, int pairs, double magnitude, const void* pos, int n, void* table, void* stream,
+                     char* err, size_t errlen);
+
+/* Rotation of T rows of HQ heads Q and HK heads K (K null: none) of HD dims (a multiple of 8 to 1024), rows q_stride and
+ * heads q_step elements apart (multiples of 8, no two heads overlapping, in any order): (x, y) of pair j of the first RD
+ * dims becomes magnitude (x cos a - y sin a, y cos a + x sin a), a = pos[t] freqs[j] (pos i32 [T], any value; null: t;
+ * freqs [RD/2] f64 on the device), RD even, 2 to 256; `inverse` turns back (-a: with magnitude 1 the inverse, with any the
+ * gradient).  Angles in f64, products in f32, rounded once; other dims are copied as they are.  type SD_F16, SD_BF16 or
+ * SD_F32.  Qo null: in place, and K in place too; else Qo (and Ko) receive the heads at their own strides and may overlap
+ * neither the inputs nor each other.  All aligned to 16 bytes. */
+int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inverse, const void* pos, int T, int HD, void* Q,
+               size_t q_stride, size_t q_step, int HQ, void* K, size_t k_stride, size_t k_step, int HK, void* Qo,
+               size_t qo_stride, size_t qo_step, void* Ko, size_t ko_stride, size_t ko_step, int type, void* stream, char* err,
+               size_t errlen);
+
+/* Positions of a step's rows: out[t] = pos[t] + dropped[b] for row t of request b (cu[b] <= t < cu[b + 1]; pos as
+ * sd_op_page_plan writes it, dropped i32 [B] as sd_op_page_release counts it), pos[t] in no request's rows.  out may be pos
+ * (then once per plan); it overlaps no other input.  B at most 8192. */
+int sd_op_page_positions(const void* cu, const void* dropped, int B, int T, const void* pos, void* out, void* stream,
+                         char* err, size_t errlen);
+
+/* ---- rows that leave the paged cache, so that a request holds no more than its budget.  Per layer and step, after
+ * sd_op_paged_attention: sd_op_paged_weights adds up the attention weight that every cached key receives.  Every few steps
+ * (or once behind a prompt), per layer: sd_op_page_evict picks, for each request and kv head by itself, the rows that stay,
+ * and sd_op_paged_move puts those of them that lie behind the budget into the places of those that go.  Then, once,
+ * sd_op_page_release pushes the pages behind the budget onto sd_op_page_plan's free stack.
+ *
+ * Rows keep the angles of the positions that they were written with, and their order is lost: a window of
+ * sd_op_paged_attention goes by row and is not for requests that have dropped some (`recent` below keeps the latest).
+ * Scores (f32) and positions (kpos, i32) of cached rows are arrays [n_pages][HK][page_size] of each layer, addressed by the
+ * same table.  The pages of a request that drops rows are its own: in a page that two requests share, moves would change
+ * the other's rows.  As above: nothing is allocated, waited for or kept; counts, tables and lengths are device arrays of
+ * i32, and what they hold cannot make a kernel leave the given buffers; calls on several streams run at once where they
+ * share no output and no workspace. ---- */
+
+/* Workspace of an sd_op_paged_weights call with these sizes, in bytes. */
+int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int observers, size_t* bytes,
+                           char* err, size_t errlen);
+
+/* Attention weight of every cached key: with w = softmax(scale q . k) over the rows that sd_op_paged_attention's row t lets
+ * query head g see (the same position, window and holes; arguments as there), every row j of a request that has new rows
+ * receives, for each kv head h,
+ *   out[j] = decay scores[j] (rows that were there before this step; decay 0: nothing is read, scores may be null)
+ *          + the sum of w[t][g][j] over the request's last `observers` new rows t (0: all) and the heads g of h,
+ * and its new rows kpos[j] = pos[t] (pos i32 [T]; both null: none).  All in f32; a row t that sees no key, or -inf alone,
+ * adds nothing; where its scores hold NaN or +inf, all keys that it sees become NaN.  Sums have one order: equal calls
+ * give equal bits.  out may be scores; other rows of both are left as they are.  max_new, max_kv and ws as in
+ * sd_op_paged_attention, sized by sd_op_paged_weights_ws. */
+int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int max_blocks, const void* cu, const void* kv_lens,
+                        const void* pos, int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int page_size,
+                        int n_pages, size_t page_stride, int window, float scale, int observers, float decay,
+                        const void* scores, void* out, void* kpos, void* ws, size_t ws_bytes, int type, void* stream,
+                        char* err, size_t errlen);
+
+/* Workspace of an sd_op_page_evict call with these sizes, in bytes (0: none). */
+int sd_op_page_evict_ws(int B, int max_kv, int HK, size_t* bytes, char* err, size_t errlen);
+
+/* Which rows go.  Request b with n = kv_lens[b] rows and budget m = budgets[b] (i32 [B]; below 0: no limit) keeps, where
+ * m < n <= max_kv, m rows of each kv head: first those whose position is below `sink` or among the latest `recent` (above
+ * the head's largest less `recent`), then those of the largest scores; equal ones in row order; NaN, and rows in a hole,
+ * come last.  kpos null: positions are row numbers (nothing dropped yet).
+ *   new_lens [B]: m where rows go, kv_lens[b] elsewhere
+ *   counts   [B][HK], moves [B][HK][max(max_kv / 2, 1)][2]: the head's moves, pairs (place, row): the places below m whose
+ *            rows go, ascending, and the rows from m on that stay, ascending; entries behind the count are left as they are
+ * ws holds what sd_op_page_evict_ws says, 16-byte aligned.  No output overlaps an input or another output. */
+int sd_op_page_evict(const void* scores, const void* kpos, const void* table, int max_blocks, const void* kv_lens,
+                     const void* budgets, int B, int max_kv, int HK, int page_size, int n_pages, int sink, int recent,
+                     void* new_lens, void* moves, void* counts, void* ws, size_t ws_bytes, void* stream, char* err,
+                     size_t errlen);
+
+/* The moves: row moves[..][1] of K, V, scores and kpos (null: not moved) becomes row moves[..][0], for the first counts
+ * moves of every request and kv head, at most max(max_kv / 2, 1).  Places ascend and every row that is read lies behind all
+ * places, as sd_op_page_evict makes them (else what is read is either value).  Moves whose place or row lies in a hole or
+ * outside the table are passed over. */
+int sd_op_paged_move(const void* moves, const void* counts, const void* table, int max_blocks, int B, int max_kv, int HK,
+                     int HD, int page_size, int n_pages, size_t page_stride, void* Kp, void* Vp, void* scores, void* kpos,
+                     int type, void* stream, char* err, size_t errlen);
+
+/* The pages that hold rows new_lens[b] .. kv_lens[b] - 1 of request b alone go onto the free stack: free_pages [n_pages]
+ * holds n_free[0] of them; the others' numbers are written behind, request by request, by table order (holes left out, none
+ * past n_pages), and n_free_out[0] is how many there are now; dropped_out[b] = dropped[b] + kv_lens[b] - new_lens[b].  The
+ * table's entries stay; new_lens are the next step's lens.  A new length that is negative or not below the old one releases
+ * nothing (new_lens 0: a request that has ended).  No output overlaps an input or another output (free_pages is both). */
+int sd_op_page_release(const void* kv_lens, const void* new_lens, const void* dropped, const void* table, int max_blocks,
+                       int B, int page_size, int n_pages, void* free_pages, const void* n_free, void* dropped_out,
+                       void* n_free_out, void* stream, char* err, size_t errlen);
+
 /* No counterpart in the reference (a test hook for per-layer parity): the forward of ids from cache
  * (nullable) run step by step; after every residual add + RMSNorm of the layers (each layer's
  * in_norm, then its post_norm) the residual x (f32) and the normalized h (f16 bits) of rows[0..n_rows)

@@ -31,7 +31,9 @@ SYMBOLS = [
     "sd_op_repack_w4", "sd_decode_scale_codes", "sd_op_matmul_fmt", "sd_op_matmul_split", "sd_op_gate_up_silu",
     "sd_op_embed", "sd_op_add_norm", "sd_op_silu_mul", "sd_op_add_bias", "sd_op_conv", "sd_op_gnorm",
     "sd_op_attention", "sd_engine_trace", "sd_op_matmul_noalloc", "sd_op_page_plan", "sd_op_paged_prep",
-    "sd_op_paged_attention_ws", "sd_op_paged_attention",
+    "sd_op_paged_attention_ws", "sd_op_paged_attention", "sd_rope_freqs", "sd_op_rope_table", "sd_op_rope",
+    "sd_op_page_positions", "sd_op_paged_weights_ws", "sd_op_paged_weights", "sd_op_page_evict_ws", "sd_op_page_evict",
+    "sd_op_paged_move", "sd_op_page_release",
 ]
 VOID_SYMBOLS = ("sd_engine_free", "sd_snapshot_free", "sd_head_free", "sd_engine_hidden_size", "sd_engine_adapter",
                 "sd_snapshot_len")
@@ -122,6 +124,19 @@ def lib():
         L.sd_op_paged_attention_ws.argtypes = [i32, i32, i32, i32, i32, i32, i32, C.POINTER(sz), err, sz]
         L.sd_op_paged_attention.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32,
                                             sz, i32, C.c_float, vp, vp, sz, i32, vp, err, sz]
+        f64 = C.c_double
+        L.sd_rope_freqs.argtypes = [i32, f64, i32, f64, f64, f64, f64, vp, err, sz]
+        L.sd_op_rope_table.argtypes = [vp, i32, f64, vp, i32, vp, vp, err, sz]
+        L.sd_op_rope.argtypes = [vp, i32, f64, i32, i32, vp, i32, i32, vp, sz, sz, i32, vp, sz, sz, i32, vp, sz, sz, vp, sz, sz,
+                                 i32, vp, err, sz]
+        L.sd_op_page_positions.argtypes = [vp, vp, i32, i32, vp, vp, vp, err, sz]
+        L.sd_op_paged_weights_ws.argtypes = [i32, i32, i32, i32, i32, i32, i32, i32, C.POINTER(sz), err, sz]
+        L.sd_op_paged_weights.argtypes = [vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, sz, i32,
+                                          C.c_float, i32, C.c_float, vp, vp, vp, vp, sz, i32, vp, err, sz]
+        L.sd_op_page_evict_ws.argtypes = [i32, i32, i32, C.POINTER(sz), err, sz]
+        L.sd_op_page_evict.argtypes = [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp, err, sz]
+        L.sd_op_paged_move.argtypes = [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, sz, vp, vp, vp, vp, i32, vp, err, sz]
+        L.sd_op_page_release.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, err, sz]
         for name in SYMBOLS:
             if name not in VOID_SYMBOLS:
                 getattr(L, name).restype = i32
@@ -488,7 +503,7 @@ def op_matmul_noalloc(A, Wq, Sc, Y, M, N, K, exact=False, stream=None):
 
 # ---- a K/V cache in pages, shared by many requests ------------------------------------------------
 
-F16, BF16 = 0, 1  # the rows' and caches' type
+F16, BF16, F32 = 0, 1, 2  # the rows' and caches' type (F32: op_rope's rows alone)
 
 
 def op_page_plan(lens, news, B, T, page_size, n_pages, free_pages, n_free, table, max_blocks, cu, kv_lens, slots, pos,
@@ -519,6 +534,84 @@ def op_paged_attention(Q, big, stride, Kp, Vp, table, max_blocks, cu, kv_lens, B
     _call(lib().sd_op_paged_attention, Q, big, stride, Kp, Vp, table, max_blocks, cu, kv_lens, B, T, max_new, max_kv, HQ,
           HK, HD, page_size, n_pages, page_stride, window, HD ** -0.5 if scale is None else scale, out, ws, ws_bytes, type,
           stream)
+
+
+# ---- rotary positions at any distance, and rows that leave the paged cache -------------------------
+
+ROPE_HALF, ROPE_PAIRS = 0, 1  # pair j: dims j and j + RD/2, or 2j and 2j + 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3  # how the frequencies are scaled
+
+
+def rope_freqs(RD, theta, scaling=ROPE_PLAIN, factor=1.0, length=0.0, low=0.0, high=0.0) -> np.ndarray:
+    """sd_rope_freqs: the pairs' frequencies [RD/2] f64 in radians per position; the calls below take them on the device."""
+    if not 2 <= RD <= 256:
+        raise EngineError("sd_rope_freqs: rotary_dim must be even, 2 to 256")
+    out = np.empty(RD // 2, np.float64)
+    _call(lib().sd_rope_freqs, RD, theta, scaling, factor, length, low, high, _ptr(out))
+    return out
+
+
+def op_rope_table(freqs, pairs, pos, n, table, magnitude=1.0, stream=None):
+    """sd_op_rope_table: cosines and sines of n positions (pos None: 0 to n - 1)."""
+    _call(lib().sd_op_rope_table, freqs, pairs, magnitude, pos, n, table, stream)
+
+
+def op_rope(freqs, RD, layout, pos, T, HD, Q, q_stride, q_step, HQ, K, k_stride, k_step, HK, type, magnitude=1.0, inverse=False,
+            Qo=None, Ko=None, qo_stride=None, qo_step=None, ko_stride=None, ko_step=None, stream=None):
+    """sd_op_rope: q's and k's rows turned by their positions' angles, in place (Qo None), or into Qo and Ko (strides None:
+    [T][heads][HD])."""
+    _call(lib().sd_op_rope, freqs, RD, magnitude, layout, int(inverse), pos, T, HD, Q, q_stride, q_step, HQ, K, k_stride,
+          k_step, HK, Qo, HQ * HD if qo_stride is None else qo_stride, HD if qo_step is None else qo_step, Ko,
+          HK * HD if ko_stride is None else ko_stride, HD if ko_step is None else ko_step, type, stream)
+
+
+def op_page_positions(cu, dropped, B, T, pos, out, stream=None):
+    """sd_op_page_positions: the rows' positions, with what their requests have dropped from the cache."""
+    _call(lib().sd_op_page_positions, cu, dropped, B, T, pos, out, stream)
+
+
+def paged_weights_ws(B, T, max_new, max_kv, HQ, HK, HD, observers=0) -> int:
+    """sd_op_paged_weights_ws: bytes of the workspace of an op_paged_weights call with these sizes."""
+    n = C.c_size_t()
+    _call(lib().sd_op_paged_weights_ws, B, T, max_new, max_kv, HQ, HK, HD, observers, C.byref(n))
+    return n.value
+
+
+def op_paged_weights(Q, Kp, table, max_blocks, cu, kv_lens, B, T, max_new, max_kv, HQ, HK, HD, page_size, n_pages, scores, out,
+                     ws, ws_bytes, type, decay=1.0, observers=0, window=0, scale=None, pos=None, kpos=None, page_stride=0,
+                     stream=None):
+    """sd_op_paged_weights: the attention weight that every cached key receives (scale None: 1/sqrt(HD))."""
+    _call(lib().sd_op_paged_weights, Q, Kp, table, max_blocks, cu, kv_lens, pos, B, T, max_new, max_kv, HQ, HK, HD, page_size,
+          n_pages, page_stride, window, HD ** -0.5 if scale is None else scale, observers, decay, scores, out, kpos, ws,
+          ws_bytes, type, stream)
+
+
+def page_evict_ws(B, max_kv, HK) -> int:
+    """sd_op_page_evict_ws: bytes of the workspace of an op_page_evict call with these sizes."""
+    n = C.c_size_t()
+    _call(lib().sd_op_page_evict_ws, B, max_kv, HK, C.byref(n))
+    return n.value
+
+
+def op_page_evict(scores, kpos, table, max_blocks, kv_lens, budgets, B, max_kv, HK, page_size, n_pages, sink, recent, new_lens,
+                  moves, counts, ws, ws_bytes, stream=None):
+    """sd_op_page_evict: the moves that bring every request within its budget (moves [B][HK][max(max_kv // 2, 1)][2])."""
+    _call(lib().sd_op_page_evict, scores, kpos, table, max_blocks, kv_lens, budgets, B, max_kv, HK, page_size, n_pages, sink,
+          recent, new_lens, moves, counts, ws, ws_bytes, stream)
+
+
+def op_paged_move(moves, counts, table, max_blocks, B, max_kv, HK, HD, page_size, n_pages, Kp, Vp, scores, kpos, type,
+                  page_stride=0, stream=None):
+    """sd_op_paged_move: rows of K, V, scores and positions into the places of those that go."""
+    _call(lib().sd_op_paged_move, moves, counts, table, max_blocks, B, max_kv, HK, HD, page_size, n_pages, page_stride, Kp, Vp,
+          scores, kpos, type, stream)
+
+
+def op_page_release(kv_lens, new_lens, dropped, table, max_blocks, B, page_size, n_pages, free_pages, n_free, dropped_out,
+                    n_free_out, stream=None):
+    """sd_op_page_release: the pages behind the requests' new lengths, onto the free stack."""
+    _call(lib().sd_op_page_release, kv_lens, new_lens, dropped, table, max_blocks, B, page_size, n_pages, free_pages, n_free,
+          dropped_out, n_free_out, stream)
 
 
 # ---- achievable-peak microbenchmarks (libsdpeak.so, include/sdpeak.h; used by bench.py) ----------

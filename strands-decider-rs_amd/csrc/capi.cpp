@@ -1,8 +1,10 @@
 // extern "C" entry points declared in include/sdhip.h.  Every call catches C++ exceptions and
 // reports them through (err, errlen), the C form of the reference's `crate::Error(String)`.
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 
@@ -733,6 +735,267 @@ int sd_op_paged_attention(const void* Q, const void* big, int stride, const void
         sd::paged_attn(s, {Q, big, stride, Kp, Vp, static_cast<const int*>(table), max_blocks, static_cast<const int*>(cu),
                            static_cast<const int*>(kv_lens), B, T, max_new, max_kv, window, scale, out, ws},
                        static_cast<hipStream_t>(stream));
+    });
+}
+
+namespace {
+
+using Span = std::pair<const void*, size_t>;
+
+// The spans of a call: what is read and what is written.  Nothing that is written may overlap what is read or written.
+void apart(const std::string& who, std::initializer_list<Span> in, std::initializer_list<Span> out) {
+    for (auto o = out.begin(); o != out.end(); ++o) {
+        if (!o->first) continue;
+        for (const auto& i : in)
+            if (i.first && overlap(i.first, i.second, o->first, o->second)) throw sd::Error(who + ": an output overlaps an input");
+        for (auto q = out.begin(); q != o; ++q)
+            if (q->first && overlap(q->first, q->second, o->first, o->second)) throw sd::Error(who + ": two outputs overlap");
+    }
+}
+
+void words(const std::string& who, std::initializer_list<const void*> p) {
+    for (const void* x : p)
+        if (!aligned(x, 4)) throw sd::Error(who + ": the arrays must be aligned to 4 bytes");
+}
+
+void requests(const std::string& who, int B) {
+    if (B < 1 || B > sd::PAGE_PLAN_MAX_B) throw sd::Error(who + ": 1 to " + std::to_string(sd::PAGE_PLAN_MAX_B) + " requests");
+}
+
+void table_row(const std::string& who, int max_blocks, int page_size, int max_kv) {
+    if (max_blocks < 1 || (long long)max_blocks * page_size > INT32_MAX)
+        throw sd::Error(who + ": a table row must hold at least one page and fewer than 2^31 cache rows");
+    if (max_kv < 1) throw sd::Error(who + ": max_kv must be at least 1");
+    if (max_kv > (long long)max_blocks * page_size) throw sd::Error(who + ": max_kv is more than a table row's pages hold");
+}
+
+int moves_width(int max_kv) { return max_kv / 2 < 1 ? 1 : max_kv / 2; }
+
+}  // namespace
+
+int sd_rope_freqs(int RD, double theta, int scaling, double factor, double length, double low, double high, double* freqs,
+                  char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_rope_freqs";
+        if (!freqs) throw sd::Error(who + ": null argument");
+        if (scaling < SD_ROPE_PLAIN || scaling > SD_ROPE_PARTS) throw sd::Error(who + ": no such scaling");
+        if (RD < (scaling == SD_ROPE_BASE ? 4 : 2) || RD > 256 || RD % 2)
+            throw sd::Error(who + ": rotary_dim must be even, 2 to 256 (from 4 where the base is scaled)");
+        if (!(theta >= 1) || !std::isfinite(theta) || !(factor >= 1) || !std::isfinite(factor))
+            throw sd::Error(who + ": theta and the factor must be finite and at least 1");
+        if (scaling == SD_ROPE_PARTS && (!(length > 0) || !std::isfinite(length) || !(low >= 0) || !(high > low) || !std::isfinite(high)))
+            throw sd::Error(who + ": scaling in parts needs a length above 0 and 0 <= low < high");
+        if (scaling == SD_ROPE_BASE) theta *= std::pow(factor, RD / (RD - 2.0));
+        for (int j = 0; j < RD / 2; j++) {
+            double f = std::pow(theta, -2.0 * j / RD);
+            if (scaling == SD_ROPE_LINEAR) f /= factor;
+            if (scaling == SD_ROPE_PARTS) {
+                const double turns = length * f / 6.28318530717958647693, k = std::min(1.0, std::max(0.0, (turns - low) / (high - low)));
+                f = f * k + f / factor * (1 - k);
+            }
+            freqs[j] = f;
+        }
+    });
+}
+
+int sd_op_rope_table(const void* freqs, int pairs, double magnitude, const void* pos, int n, void* table, void* stream,
+                     char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_rope_table";
+        if (!freqs || !table) throw sd::Error(who + ": null argument");
+        if (pairs < 1 || pairs > 128) throw sd::Error(who + ": 1 to 128 pairs");
+        if (n < 1 || (long long)n * pairs > INT32_MAX) throw sd::Error(who + ": need at least one row, and rows * pairs below 2^31");
+        if (!std::isfinite(magnitude)) throw sd::Error(who + ": the magnitude must be finite");
+        if (!aligned(freqs, 8) || !aligned(table, 8) || !aligned(pos, 4))
+            throw sd::Error(who + ": the frequencies and the table must be aligned to 8 bytes, the positions to 4");
+        apart(who, {{freqs, (size_t)pairs * 8}, {pos, (size_t)n * 4}}, {{table, (size_t)n * pairs * 8}});
+        sd::rope_table(static_cast<const double*>(freqs), pairs, magnitude, static_cast<const int*>(pos), n,
+                       static_cast<float*>(table), static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inverse, const void* pos, int T, int HD, void* Q,
+               size_t q_stride, size_t q_step, int HQ, void* K, size_t k_stride, size_t k_step, int HK, void* Qo,
+               size_t qo_stride, size_t qo_step, void* Ko, size_t ko_stride, size_t ko_step, int type, void* stream, char* err,
+               size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_rope";
+        if (!freqs || !Q) throw sd::Error(who + ": null argument");
+        if (!K) HK = 0;
+        if (T < 1) throw sd::Error(who + ": need at least one row");
+        if (HQ < 1 || HQ > 1024 || HK < 0 || HK > 1024 || (K && !HK)) throw sd::Error(who + ": 1 to 1024 q heads, and as many k heads");
+        if (HD < 8 || HD > 1024 || HD % 8) throw sd::Error(who + ": head_dim must be a multiple of 8, 8 to 1024");
+        if (RD < 2 || RD % 2 || RD > HD || RD > 256) throw sd::Error(who + ": rotary_dim must be even, 2 to 256, and at most head_dim");
+        if (layout != SD_ROPE_HALF && layout != SD_ROPE_PAIRS) throw sd::Error(who + ": the layout must be SD_ROPE_HALF or SD_ROPE_PAIRS");
+        if (type != SD_F16 && type != SD_BF16 && type != SD_F32) throw sd::Error(who + ": the type must be SD_F16, SD_BF16 or SD_F32");
+        if (!std::isfinite(magnitude)) throw sd::Error(who + ": the magnitude must be finite");
+        if ((Ko && !Qo) || (K && Qo && !Ko) || (Ko && !K)) throw sd::Error(who + ": outputs for both q and k, or for neither");
+        if (!Qo) Qo = Q, qo_stride = q_stride, qo_step = q_step, Ko = K, ko_stride = k_stride, ko_step = k_step;
+        const size_t size = type == SD_F32 ? 4 : 2;
+        auto span = [&](const void* p, size_t stride, size_t step, int heads) {  // and its checks
+            if (stride % 8 || step % 8 || stride > (size_t(1) << 40) || step > (size_t(1) << 40))
+                throw sd::Error(who + ": strides must be multiples of 8, at most 2^40");
+            const size_t wide = (heads - 1) * step + HD, tall = (T - 1) * stride + HD;
+            if ((heads > 1 && step < (size_t)HD) || (T > 1 && stride < (size_t)HD) || (heads > 1 && T > 1 && stride < wide && step < tall))
+                throw sd::Error(who + ": two heads overlap");
+            if (!aligned(p, 16)) throw sd::Error(who + ": the rows must be aligned to 16 bytes");
+            return Span{p, ((T - 1) * stride + (heads - 1) * step + HD) * size};
+        };
+        const Span q = span(Q, q_stride, q_step, HQ), k = K ? span(K, k_stride, k_step, HK) : Span{nullptr, 0};
+        const Span qo = span(Qo, qo_stride, qo_step, HQ), ko = K ? span(Ko, ko_stride, ko_step, HK) : Span{nullptr, 0};
+        if (!aligned(freqs, 8) || !aligned(pos, 4)) throw sd::Error(who + ": the frequencies must be aligned to 8 bytes, the positions to 4");
+        const Span f{freqs, (size_t)RD * 4}, p{pos, (size_t)T * 4};
+        if (Qo != Q) apart(who, {q, k, f, p}, {qo}), apart(who, {q, k, f, p}, {ko});  // (q's and k's rows may lie in turn in one buffer)
+        else apart(who, {f, p}, {qo}), apart(who, {f, p}, {ko});
+        sd::rope({static_cast<const double*>(freqs), RD, magnitude, layout == SD_ROPE_PAIRS, inverse != 0, static_cast<const int*>(pos),
+                  T, HD, {Q, Qo, q_stride, q_step, qo_stride, qo_step}, {K, Ko, k_stride, k_step, ko_stride, ko_step}, HQ, HK, type},
+                 static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_page_positions(const void* cu, const void* dropped, int B, int T, const void* pos, void* out, void* stream,
+                         char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_page_positions";
+        if (!cu || !dropped || !pos || !out) throw sd::Error(who + ": null argument");
+        requests(who, B);
+        if (T < 1 || T > (1 << 30)) throw sd::Error(who + ": 1 to 2^30 rows");
+        words(who, {cu, dropped, pos, out});
+        apart(who, {{cu, (size_t)(B + 1) * 4}, {dropped, (size_t)B * 4}, {pos == out ? nullptr : pos, (size_t)T * 4}},
+              {{out, (size_t)T * 4}});
+        sd::page_positions(static_cast<const int*>(cu), static_cast<const int*>(dropped), B, T, static_cast<const int*>(pos),
+                           static_cast<int*>(out), static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int observers, size_t* bytes,
+                           char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_paged_weights_ws";
+        if (!bytes) throw sd::Error(who + ": null argument");
+        const sd::PagedShape s = paged_shape(who, HQ, HK, HD, 32, 1, 0, SD_F16);
+        paged_attn_sizes(who, B, T, max_new, max_kv, HQ);
+        if (observers < 0) throw sd::Error(who + ": the observers must be at least 1, or 0 for all");
+        *bytes = sd::paged_weights_ws(s, B, T, max_new, max_kv, observers);
+    });
+}
+
+int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int max_blocks, const void* cu, const void* kv_lens,
+                        const void* pos, int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int page_size,
+                        int n_pages, size_t page_stride, int window, float scale, int observers, float decay,
+                        const void* scores, void* out, void* kpos, void* ws, size_t ws_bytes, int type, void* stream,
+                        char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_paged_weights";
+        if (!Q || !Kp || !table || !cu || !kv_lens || !out) throw sd::Error(who + ": null argument");
+        if (!pos != !kpos) throw sd::Error(who + ": positions of both the rows and the cached keys, or of neither");
+        if (!std::isfinite(decay)) throw sd::Error(who + ": the decay must be finite");
+        if (decay != 0.f && !scores) throw sd::Error(who + ": a decay needs the scores so far");
+        const sd::PagedShape s = paged_shape(who, HQ, HK, HD, page_size, n_pages, page_stride, type);
+        paged_attn_sizes(who, B, T, max_new, max_kv, HQ);
+        table_row(who, max_blocks, page_size, max_kv);
+        if (window < 0) throw sd::Error(who + ": the window must be at least 1, or 0 for none");
+        if (observers < 0) throw sd::Error(who + ": the observers must be at least 1, or 0 for all");
+        if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950f))  // (the kernels' exponentials are in base 2)
+            throw sd::Error(who + ": the scale must be positive and at most 2.3e38");
+        if (!aligned(Q, 16) || !aligned(Kp, 16) || !aligned(ws, 16)) throw sd::Error(who + ": Q, the keys and ws must be aligned to 16 bytes");
+        words(who, {table, cu, kv_lens, pos, scores, out, kpos});
+        const size_t marks = (size_t)n_pages * HK * page_size * 4, need = sd::paged_weights_ws(s, B, T, max_new, max_kv, observers);
+        if (need && (!ws || ws_bytes < need))
+            throw sd::Error(who + ": needs a workspace of " + std::to_string(need) + " bytes, got " +
+                            std::to_string(ws ? ws_bytes : 0));
+        apart(who,
+              {{Q, (size_t)T * HQ * HD * 2}, {Kp, ((size_t)(n_pages - 1) * s.pstride + (size_t)HK * page_size * HD) * 2},
+               {table, (size_t)B * max_blocks * 4}, {cu, (size_t)(B + 1) * 4}, {kv_lens, (size_t)B * 4}, {pos, (size_t)T * 4},
+               {scores == out || decay == 0.f ? nullptr : scores, marks}},
+              {{out, marks}, {kpos, marks}, {need ? ws : nullptr, need}});
+        if (need && decay != 0.f && overlap(ws, need, scores, marks)) throw sd::Error(who + ": the workspace overlaps the scores");
+        sd::paged_weights(s, {Q, Kp, static_cast<const int*>(table), max_blocks, static_cast<const int*>(cu),
+                              static_cast<const int*>(kv_lens), static_cast<const int*>(pos), B, T, max_new, max_kv, window,
+                              observers, scale, decay, static_cast<const float*>(scores), static_cast<float*>(out),
+                              static_cast<int*>(kpos), ws},
+                          static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_page_evict_ws(int B, int max_kv, int HK, size_t* bytes, char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_page_evict_ws";
+        if (!bytes) throw sd::Error(who + ": null argument");
+        requests(who, B);
+        if (max_kv < 1) throw sd::Error(who + ": max_kv must be at least 1");
+        paged_shape(who, HK, HK, 64, 32, 1, 0, SD_F16);
+        *bytes = sd::page_evict_ws(B, max_kv, HK);
+    });
+}
+
+int sd_op_page_evict(const void* scores, const void* kpos, const void* table, int max_blocks, const void* kv_lens,
+                     const void* budgets, int B, int max_kv, int HK, int page_size, int n_pages, int sink, int recent,
+                     void* new_lens, void* moves, void* counts, void* ws, size_t ws_bytes, void* stream, char* err,
+                     size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_page_evict";
+        if (!scores || !table || !kv_lens || !budgets || !new_lens || !moves || !counts) throw sd::Error(who + ": null argument");
+        paged_shape(who, HK, HK, 64, page_size, n_pages, 0, SD_F16);
+        requests(who, B);
+        table_row(who, max_blocks, page_size, max_kv);
+        if (sink < 0 || recent < 0) throw sd::Error(who + ": sink and recent must be at least 0");
+        words(who, {scores, kpos, table, kv_lens, budgets, new_lens, moves, counts});
+        if (!aligned(ws, 16)) throw sd::Error(who + ": ws must be aligned to 16 bytes");
+        const size_t marks = (size_t)n_pages * HK * page_size * 4, need = sd::page_evict_ws(B, max_kv, HK);
+        if (need && (!ws || ws_bytes < need))
+            throw sd::Error(who + ": needs a workspace of " + std::to_string(need) + " bytes, got " +
+                            std::to_string(ws ? ws_bytes : 0));
+        apart(who, {{scores, marks}, {kpos, marks}, {table, (size_t)B * max_blocks * 4}, {kv_lens, (size_t)B * 4}, {budgets, (size_t)B * 4}},
+              {{new_lens, (size_t)B * 4}, {moves, (size_t)B * HK * moves_width(max_kv) * 8}, {counts, (size_t)B * HK * 4},
+               {need ? ws : nullptr, need}});
+        sd::page_evict({static_cast<const float*>(scores), static_cast<const int*>(kpos), static_cast<const int*>(table), max_blocks,
+                        static_cast<const int*>(kv_lens), static_cast<const int*>(budgets), B, max_kv, HK, page_size, n_pages, sink,
+                        recent, static_cast<int*>(new_lens), static_cast<int*>(moves), static_cast<int*>(counts), ws},
+                       static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_paged_move(const void* moves, const void* counts, const void* table, int max_blocks, int B, int max_kv, int HK,
+                     int HD, int page_size, int n_pages, size_t page_stride, void* Kp, void* Vp, void* scores, void* kpos,
+                     int type, void* stream, char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_paged_move";
+        if (!moves || !counts || !table || !Kp || !Vp) throw sd::Error(who + ": null argument");
+        const sd::PagedShape s = paged_shape(who, HK, HK, HD, page_size, n_pages, page_stride, type);
+        requests(who, B);
+        table_row(who, max_blocks, page_size, max_kv);
+        if (!aligned(Kp, 16) || !aligned(Vp, 16)) throw sd::Error(who + ": the caches must be aligned to 16 bytes");
+        words(who, {moves, counts, table, scores, kpos});
+        const size_t marks = (size_t)n_pages * HK * page_size * 4;
+        const size_t cache = ((size_t)(n_pages - 1) * s.pstride + (size_t)HK * page_size * HD) * 2;
+        const Span mv{moves, (size_t)B * HK * moves_width(max_kv) * 8}, ct{counts, (size_t)B * HK * 4}, tb{table, (size_t)B * max_blocks * 4};
+        apart(who, {mv, ct, tb, {Kp, cache}}, {{scores, marks}, {kpos, marks}});
+        apart(who, {mv, ct, tb, {scores, marks}, {kpos, marks}}, {{Vp, cache}});  // (K and V pages may lie in turn in one buffer)
+        apart(who, {mv, ct, tb}, {{Kp, cache}});
+        sd::paged_move(s, {static_cast<const int*>(moves), static_cast<const int*>(counts), static_cast<const int*>(table), max_blocks,
+                           B, max_kv, Kp, Vp, static_cast<float*>(scores), static_cast<int*>(kpos)},
+                       static_cast<hipStream_t>(stream));
+    });
+}
+
+int sd_op_page_release(const void* kv_lens, const void* new_lens, const void* dropped, const void* table, int max_blocks,
+                       int B, int page_size, int n_pages, void* free_pages, const void* n_free, void* dropped_out,
+                       void* n_free_out, void* stream, char* err, size_t errlen) {
+    return guarded(err, errlen, [&] {
+        const std::string who = "sd_op_page_release";
+        if (!kv_lens || !new_lens || !dropped || !table || !free_pages || !n_free || !dropped_out || !n_free_out)
+            throw sd::Error(who + ": null argument");
+        paged_shape(who, 1, 1, 64, page_size, n_pages, 0, SD_F16);
+        requests(who, B);
+        table_row(who, max_blocks, page_size, 1);
+        words(who, {kv_lens, new_lens, dropped, table, free_pages, n_free, dropped_out, n_free_out});
+        apart(who, {{kv_lens, (size_t)B * 4}, {new_lens, (size_t)B * 4}, {dropped, (size_t)B * 4}, {table, (size_t)B * max_blocks * 4}, {n_free, 4}},
+              {{free_pages, (size_t)n_pages * 4}, {dropped_out, (size_t)B * 4}, {n_free_out, 4}});
+        sd::page_release({static_cast<const int*>(kv_lens), static_cast<const int*>(new_lens), static_cast<const int*>(dropped),
+                          static_cast<const int*>(table), max_blocks, B, page_size, n_pages, static_cast<int*>(free_pages),
+                          static_cast<const int*>(n_free), static_cast<int*>(dropped_out), static_cast<int*>(n_free_out)},
+                         static_cast<hipStream_t>(stream));
     });
 }
 

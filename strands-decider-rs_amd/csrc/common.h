@@ -306,4 +306,68 @@ struct PagedAttn {
 size_t paged_attn_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv);
 void paged_attn(const PagedShape& s, const PagedAttn& a, hipStream_t st);
 
+// ---- rotary positions (rope.hip) --------------------------------------------------------------
+struct RopeHeads {
+    const void* in;
+    void* out;  // may be in
+    size_t stride, step, ostride, ostep;  // elements from a row, and from a head, to the next
+};
+struct RopeRows {
+    const double* freqs;  // [RD / 2], radians per position
+    int RD;
+    double magnitude;
+    bool pairs, inverse;
+    const int* pos;
+    int rows, HD;
+    RopeHeads q, k;
+    int HQ, HK;  // HK may be 0
+    int type;
+};
+void rope(const RopeRows& a, hipStream_t st);
+void rope_table(const double* freqs, int pairs, double magnitude, const int* pos, int n, float* table, hipStream_t st);
+void page_positions(const int* cu, const int* dropped, int B, int T, const int* pos, int* out, hipStream_t st);
+
+// ---- rows that leave the paged cache (evict.hip) ------------------------------------------------
+struct PagedWeights {
+    const void *Q, *Kp;
+    const int* table;
+    int max_blocks;
+    const int *cu, *kv_lens, *pos;
+    int B, rows, max_new, max_kv, window, observers;
+    float scale, decay;
+    const float* scores;  // null: none
+    float* out;
+    int* kpos;  // null: none
+    void* ws;
+};
+size_t paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers);
+void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st);
+struct PageEvict {
+    const float* scores;
+    const int *kpos, *table;
+    int max_blocks;
+    const int *kv_lens, *budgets;
+    int B, max_kv, HK, PS, n_pages, sink, recent;
+    int *new_lens, *moves, *counts;
+    void* ws;
+};
+size_t page_evict_ws(int B, int max_kv, int HK);
+void page_evict(const PageEvict& a, hipStream_t st);
+struct PageRelease {
+    const int *kv_lens, *new_lens, *dropped, *table;
+    int max_blocks, B, PS, n_pages;
+    int* free_pages;
+    const int* n_free;
+    int *dropped_out, *n_free_out;
+};
+void page_release(const PageRelease& a, hipStream_t st);
+struct PagedMove {
+    const int *moves, *counts, *table;
+    int max_blocks, B, max_kv;
+    void *Kp, *Vp;
+    float* scores;  // null: none
+    int* kpos;      // null: none
+};
+void paged_move(const PagedShape& s, const PagedMove& a, hipStream_t st);
+
 }  // namespace sd

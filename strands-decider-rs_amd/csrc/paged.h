@@ -149,7 +149,7 @@ __device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t voff, uint32_t soff) {
     return buf_b128(r, voff, soff);
 }
 
-int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
+inline int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 // f(type tag, head_dim constant)
 template <class F>
