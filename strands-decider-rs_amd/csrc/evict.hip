@@ -14,91 +14,652 @@ __device__ __forceinline__ size_t mark_at(int page, int HK, int h, int j, int lp
 }
 
 // ---- the weight that every cached key receives ----------------------------------------------------------------------
+//
+// A key's weight is the sum over rows of exp(s - m) / l, and a row's maximum m and sum l are known only when all of its
+// keys have been read: two passes over the scores.  A kv head's rows are its request's (token, query head) pairs as in the
+// attention kernels.
+//
+// Few rows (one new token's heads, or up to 32): bound by the keys' bytes, so they are read once: the first pass leaves
+// its scores, rows x 4 bytes a key where a key has 2 HD.  Many rows: bound by the products and the exponentials, and rows x
+// 4 bytes a key would be the more: both passes compute the scores, with the roles swapped: the first keeps 32 rows of
+// queries in a wave's registers and lets keys pass, the second keeps 32 keys and lets rows pass, so each sums in registers
+// over what passes and neither needs another lane's values until its end.
+//
+// Scores are S^T = K Q^T (keys x rows) on MFMA, in f32, and so is all behind them; exponentials are in base 2.  A row's
+// maximum is c s rounded (c = scale log2 e).  c s - m is one fma, or, from FAR on, where m has no fractions, the difference
+// of two rounded products.
+// Sums have one order: over a lane's own keys or rows, then lanes, waves, and parts by their number.
+
+constexpr int ROW_TILE = 128, KEY_TILE = 128;  // of a workgroup of the kernels for many rows
 
 struct WeightArgs {
     const int *table, *cu, *kv_lens, *pos;
     int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, observers;
+    int few, few_ks, few_span, rw, kvp;        // rows of a request that the few rows' kernels do; their splits, blocks of 32
+                                               // keys in each; rows and keys of a request's scores
+    int tiles, ks, span, part, parts, units;   // many rows: tiles of rows, their splits, blocks in each; rows of a part,
+                                               // parts of a request at most, (key tile, part)s at most
+    uint32_t magic;  // 2^32 / G and 1 more: x / G is the upper half of a product for x below 2^16
     float c, decay;  // c: scale log2(e)
     size_t pstride;
     const float* scores;
     float* out;
     int* kpos;
+    float* S;         // [B][HK][rw][kvp]: c s of the few rows
+    float2* few_ml;   // [B][HK][few_ks][rw]: their maxima and sums
+    float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
+    float2* stat;     // [rows][HQ]: of a row's whole, the sum's reciprocal
+    float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
     // the first key that a row at position p sees
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
 
-// The rows of a request that are counted: its last `observers`.
-__device__ __forceinline__ int first_observer(const Req& r, int observers) { return observers ? max(0, r.n - observers) : 0; }
-
-template <class T, int HD>
-__device__ __forceinline__ const T* key_row(const T* Kp, const WeightArgs& a, int page, int h, int j) {
-    return Kp + (size_t)page * a.pstride + ((size_t)(h << (a.lps - 5)) + ((j & ((1 << a.lps) - 1)) >> 5)) * (HD * 32) + (j & 31) * 32;
+// The rows of a request that are counted: its last `observers` tokens, from `t0` on, n of them.
+struct Seen {
+    int t0, n;
+};
+__device__ __forceinline__ Seen observed(const Req& r, int observers) {
+    const int n = observers ? min(r.n, observers) : r.n;
+    return {r.n - n, n};
 }
-// c s, rounded: what a row's maximum is one of.  (In one fma with the maximum taken off, scores from 2^23 on, whose maximum
-// has no fractions, would be off by more than an exponential's range.)
+
+// c s, rounded: what a row's maximum is one of.
 __device__ __forceinline__ float scaled(float s, float c) {
 #pragma clang fp contract(off)
     return s * c;
 }
-template <class T, int HD>
-__device__ __forceinline__ float dot(const T* q, const T* k) {
-    float s = 0.f;
-    for (int d = 0; d < HD; d++) s = __builtin_fmaf((float)q[d], (float)k[d / 32 * 1024 + d % 32], s);
-    return s;
-}
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= FAR; }
 
-// A row's maximum and sum: one wave per (row, query head).
-template <class T, int HD>
-__global__ __launch_bounds__(64) void k_weights_stats(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a,
-                                                      float2* __restrict__ ml) {
-    const int b = blockIdx.y, lane = threadIdx.x, h = blockIdx.x % a.HQ;
-    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
-    const int* const tb = a.table + (size_t)b * a.max_blocks;
-    for (int i = first_observer(rq, a.observers) + blockIdx.x / a.HQ; i < rq.n; i += gridDim.x / a.HQ) {
-        const int p = rq.p0 + i, lo = max(0, a.from(p)), hi = min(p + 1, rq.kcap);
-        const T* const q = Q + ((size_t)(rq.q0 + i) * a.HQ + h) * HD;
-        float m = -INFINITY, l = 0.f;
-        for (int pass = 0; pass < 2; pass++)
-            for (int j0 = lo; j0 < hi; j0 += 64) {
-                const int j = j0 + lane, page = tb[min(j >> a.lps, a.max_blocks - 1)];
-                if (j >= hi || (unsigned)page >= (unsigned)a.n_pages) continue;
-                const float x = scaled(dot<T, HD>(q, key_row<T, HD>(Kp, a, page, h / a.G, j)), a.c);
-                if (pass == 0) m = fmaxf(m, x);
-                else l += m == -INFINITY && x == -INFINITY ? 0.f : exp2_fast(x - m);
-            }
-        float mx = m;  // (m is the lane's own)
-        for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        l *= part_weight(m, mx);
-        for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
-        if (lane == 0) ml[(size_t)(rq.q0 + i) * a.HQ + h] = make_float2(mx, l);
-    }
-}
+// A row's part: maximum and sum, and their turn to a row's whole.
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }  // (its sum is 0, or NaN)
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
-// A key's weight from all rows: one thread per (key, kv head).
-template <class T, int HD>
-__global__ __launch_bounds__(256) void k_weights_sum(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a,
-                                                     const float2* __restrict__ ml) {
-    const int b = blockIdx.z, kh = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
-    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
-    if (rq.n == 0 || j >= rq.kcap) return;
-    const int page = a.table[(size_t)b * a.max_blocks + (j >> a.lps)];
-    if ((unsigned)page >= (unsigned)a.n_pages) return;
-    const T* const k = key_row<T, HD>(Kp, a, page, kh, j);
-    float w = 0.f;
-    for (int i = first_observer(rq, a.observers); i < rq.n; i++) {
-        const int p = rq.p0 + i;
-        if (j > p || j < a.from(p)) continue;
-        for (int g = 0; g < a.G; g++) {
-            const size_t row = (size_t)(rq.q0 + i) * a.HQ + kh * a.G + g;
-            const float2 s = ml[row];
-            if (s.y == 0.f) continue;
-            w += exp2_fast(scaled(dot<T, HD>(Q + row * HD, k), a.c) - s.x) / s.y;
-        }
-    }
-    const size_t at = mark_at(page, a.HK, kh, j, a.lps);
+// Key j's weight w of a request's rows, into the scores of kv head h.
+__device__ __forceinline__ void put_weight(const WeightArgs& a, const Req& rq, size_t at, int j, float w) {
     const bool old = j < rq.p0;
     a.out[at] = old && a.decay != 0.f ? __builtin_fmaf(a.decay, a.scores[at], w) : w;
     if (!old && a.kpos) a.kpos[at] = a.pos[rq.q0 + j - rq.p0];
+}
+
+// ---- few rows ----
+
+constexpr int FEW_W = 4;  // waves of a workgroup
+
+// Scores of up to 16 NR rows of a (request, kv head) over this workgroup's blocks of keys, and the rows' maxima and sums
+// over them.  A wave loads K straight into registers in MFMA operand order, D blocks of 32 keys in flight.
+template <class T, int HD, int NR, bool ONCE>
+__global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    typedef typename Vec8<T>::type T8;
+    constexpr int NS = HD / 32, R = 16 * NR, D = HD == 64 ? 4 : HD == 128 ? 3 : 2;
+    __shared__ float Ms[FEW_W * R], Ls[FEW_W * R];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int fq = lane & 15, fg = lane >> 4;
+    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
+    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    const Seen ob = observed(rq, a.observers);
+    const int nrows = ob.n * a.G;
+    if (nrows == 0 || nrows > a.few) return;
+    const int p0 = rq.p0 + ob.t0;  // position of the first row
+    const int hi = min(p0 + ob.n, rq.kcap), lo = max(0, a.from(p0));
+    const int blk0 = (lo >> 5) + z * a.few_span;
+    const int blk1 = z + 1 < a.few_ks ? min((hi + 31) >> 5, blk0 + a.few_span) : (hi + 31) >> 5;
+    const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + FEW_W - 1) / FEW_W : 0;
+    int jlo[NR], jhi[NR];  // keys [jlo, jhi) are seen by this lane's row
+    T8 qf[NR][NS];
+#pragma unroll
+    for (int u = 0; u < NR; u++) {
+        const int r = min(16 * u + fq, nrows - 1), t = ob.t0 + r / a.G, h = kh * a.G + r % a.G;
+        jlo[u] = a.from(rq.p0 + t);
+        jhi[u] = min(rq.p0 + t + 1, hi);
+        const T* q = Q + ((size_t)(rq.q0 + t) * a.HQ + h) * HD + 8 * fg;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[u][s] = *reinterpret_cast<const T8*>(q + 32 * s);
+    }
+    const int open0 = a.from(p0 + ob.n - 1), open1 = min(p0 + 1, hi);  // keys in [open0, open1) are seen by every row
+    const int lbpp = a.lps - 5;
+    const int* const tb = a.table + (size_t)b * a.max_blocks;
+    auto entries = [&](int i) {  // lane l: the table entry of the wave's block i + l
+        return tb[min((first + FEW_W * (i + lane)) >> lbpp, a.max_blocks - 1)];
+    };
+    int ids = cnt ? entries(0) : 0, ids2 = cnt > 64 ? entries(64) : 0;
+    // rows of K in the order in which a lane's 8 scores are 8 keys on end: j0 + 8 fg + e
+    const uint32_t kofs = ((8 * (fq >> 2) + (fq & 3)) * 32 + fg * 8) * 2;
+    float m[NR], l[NR];
+#pragma unroll
+    for (int u = 0; u < NR; u++) m[u] = -INFINITY, l[u] = 0.f;
+    struct Blk {
+        u32x4 k[2][NS];
+        bool there;
+    };
+    auto load = [&](int i, Blk& x) INL {
+        const int page = __builtin_amdgcn_readlane(ids, i & 63), blk = first + FEW_W * i;
+        x.there = i < cnt && (unsigned)page < (unsigned)a.n_pages;
+        const size_t at = x.there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+        const Rsrc rk = make_rsrc(Kp + at, x.there ? HD * 64u : 0u);
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++) x.k[tt][s] = load16<ONCE>(rk, kofs + tt * 256, s * 2048);
+    };
+    float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp + 8 * fg;
+    auto work = [&](int i, Blk& x) INL {
+        const int j0 = (first + FEW_W * i) * 32;
+        const bool open = x.there && j0 >= open0 && j0 + 32 <= open1;
+        f32x4 s2[NR][2];
+#pragma unroll
+        for (int u = 0; u < NR; u++) s2[u][0] = s2[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                for (int u = 0; u < NR; u++)
+                    s2[u][tt] = Num<T>::mfma16(__builtin_bit_cast(T8, x.k[tt][s]), qf[u][s], s2[u][tt]);
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) s2[u][e >> 2][e & 3] = scaled(s2[u][e >> 2][e & 3], a.c);
+            if (!open) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int j = j0 + 8 * fg + e;
+                    const bool keep = x.there & (j >= jlo[u]) & (j < jhi[u]);
+                    s2[u][e >> 2][e & 3] = keep ? s2[u][e >> 2][e & 3] : -INFINITY;
+                }
+            }
+            if (16 * u + fq < nrows) {
+                f32x4* const to = reinterpret_cast<f32x4*>(S + (size_t)(16 * u + fq) * a.kvp + j0);
+                to[0] = s2[u][0], to[1] = s2[u][1];
+            }
+            float mn = m[u];
+#pragma unroll
+            for (int e = 0; e < 8; e++) mn = fmaxf(mn, s2[u][e >> 2][e & 3]);
+            const float base = base_of(mn);
+            float sum = l[u] * exp2_fast(m[u] - base);
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum += exp2_fast(s2[u][e >> 2][e & 3] - base);
+            m[u] = mn, l[u] = sum;
+        }
+    };
+    Blk set[D];
+    auto ahead = [&](int i) INL {  // before block i's load: its window of table entries
+        if ((i & 63) == 0 && i) {
+            ids = ids2;
+            if (i + 64 < cnt) ids2 = entries(i + 64);
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < D - 1; u++) load(u, set[u]);
+    for (int i = 0; i < cnt; i += D) {
+#pragma unroll
+        for (int u = 0; u < D; u++) {
+            if (u && i + u >= cnt) break;
+            ahead(i + u + D - 1);
+            load(i + u + D - 1, set[(u + D - 1) % D]);
+            __builtin_amdgcn_sched_barrier(0);
+            work(i + u, set[u]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < NR; u++) {
+        const float mx = max_quarters(m[u]);
+        float sum = l[u] * part_weight(m[u], mx);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (fg == 0) Ms[wv * R + 16 * u + fq] = mx, Ls[wv * R + 16 * u + fq] = sum;
+    }
+    __syncthreads();
+    if (tid < nrows) {
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_W; w++) mx = fmaxf(mx, Ms[w * R + tid]);
+#pragma unroll
+        for (int w = 0; w < FEW_W; w++) sum += Ls[w * R + tid] * part_weight(Ms[w * R + tid], mx);
+        a.few_ml[(((size_t)b * a.HK + kh) * a.few_ks + z) * a.rw + tid] = make_float2(mx, sum);
+    }
+}
+
+// The few rows' weights, from their scores: 4 keys per thread, after every workgroup has joined the rows' parts, 8 threads
+// a row.
+__global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
+    __shared__ float2 stat[32];
+    const int tid = threadIdx.x, kh = blockIdx.y, b = blockIdx.z;
+    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    const Seen ob = observed(rq, a.observers);
+    const int nrows = ob.n * a.G;
+    if (nrows == 0 || nrows > a.few || blockIdx.x * 1024 >= (unsigned)rq.kcap) return;
+    const int p0 = rq.p0 + ob.t0, hi = min(p0 + ob.n, rq.kcap), lo = max(0, a.from(p0));
+    {
+        const int r = tid >> 3, u = tid & 7;
+        const float2* const ml = a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw + min(r, nrows - 1);
+        float mx = -INFINITY, l = 0.f;
+        for (int z = u; z < a.few_ks; z += 8) {
+            const float2 v = ml[z * a.rw];
+            const float mn = fmaxf(mx, v.x);
+            l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
+            mx = mn;
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            const float m2 = __shfl_xor(mx, o), l2 = __shfl_xor(l, o), mn = fmaxf(mx, m2);
+            l = l * part_weight(mx, mn) + l2 * part_weight(m2, mn);
+            mx = mn;
+        }
+        if (u == 0) stat[r] = make_float2(base_of(mx), inverse_of(l));
+    }
+    __syncthreads();
+    for (int j0 = blockIdx.x * 1024; j0 < rq.kcap; j0 += gridDim.x * 1024) {
+        const int j = j0 + 4 * tid;
+        if (j >= rq.kcap) return;
+        const int page = a.table[(size_t)b * a.max_blocks + (j >> a.lps)];
+        if ((unsigned)page >= (unsigned)a.n_pages) continue;
+        const float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp + j;
+        f32x4 w = {0.f, 0.f, 0.f, 0.f};
+        if (j + 4 > lo && j < hi) {  // (scores outside were not written)
+            int t = 0, g = 0;
+#pragma unroll 4
+            for (int r = 0; r < nrows; r++) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp);
+                const float2 st = stat[r];
+                const int jlo = a.from(p0 + t), jhi = min(p0 + t + 1, hi);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool keep = (j + e >= jlo) & (j + e < jhi);
+                    w[e] += keep ? exp2_fast(x[e] - st.x) * st.y : 0.f;
+                }
+                if (++g == a.G) g = 0, t++;
+            }
+        }
+        const size_t at = mark_at(page, a.HK, kh, j, a.lps);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (j + e < rq.kcap) put_weight(a, rq, at + e, j + e, w[e]);
+    }
+}
+
+// ---- many rows ----
+
+__device__ __forceinline__ int many_rows(const WeightArgs& a, int b) {  // of request b, 0 where they are few
+    const int n = observed(request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap), a.observers).n * a.G;
+    return n > a.few ? n : 0;
+}
+__device__ __forceinline__ Tile row_tile(const WeightArgs& a, int x) {
+    return find_tile(a.B, x, [&](int b) { return (many_rows(a, b) + ROW_TILE - 1) / ROW_TILE; });
+}
+
+// A tile's rows, the keys that some of them see, and this split's blocks of those.
+struct RowTile {
+    Req rq;
+    Seen ob;
+    int nrows, r0, r1, lo, hi, blk0, blk1;
+};
+__device__ __forceinline__ RowTile row_tile_of(const WeightArgs& a, const Tile& tl, int z) {
+    RowTile t;
+    t.rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    t.ob = observed(t.rq, a.observers);
+    t.nrows = t.ob.n * a.G;
+    t.r0 = tl.i * ROW_TILE;
+    t.r1 = min(t.nrows, t.r0 + ROW_TILE);
+    const int p = t.rq.p0 + t.ob.t0;
+    t.hi = min(p + (t.r1 - 1) / a.G + 1, t.rq.kcap);
+    t.lo = max(0, a.from(p + t.r0 / a.G));
+    t.blk0 = (t.lo >> 5) + z * a.span;
+    t.blk1 = min((t.hi + 31) >> 5, t.blk0 + a.span);
+    return t;
+}
+
+// Blocks of 32 rows x HD of a ring in LDS: [HD / 32][32 rows][64 bytes], the 16-byte pieces of each row at p ^ (row / 4) % 4,
+// so that neither the DMAs' writes nor the fragments' reads meet a bank twice.
+template <int HD>
+struct Ring {
+    static constexpr int BYTES = HD * 64, IW = BYTES / 4096;  // of a block; its DMAs per wave
+    static __device__ __forceinline__ u32x4 read(const uint8_t* buf, int st, int c, int g) {
+        return *reinterpret_cast<const u32x4*>(buf + (st >> 1) * 2048 + c * 64 + (((2 * (st & 1) + g) ^ ((c >> 2) & 3)) << 4));
+    }
+};
+
+// Maxima and sums of 128 rows over a split of their keys: each wave has 32 rows' queries in registers, and all four share
+// blocks of 32 keys that arrive by LDS DMA, three ahead.  A lane keeps its own maximum and sum of the half of each block that
+// it has; the two halves meet at the end.
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void k_weights_rows(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    typedef typename Vec8<T>::type T8;
+    typedef Ring<HD> Rg;
+    constexpr int NS = HD / 16, NB = 4, IW = Rg::IW, PART = Rg::BYTES / 4;
+    // (an array per buffer: the compiler then sees that the DMAs into one never alias the reads of another)
+    __shared__ __align__(1024) uint8_t K0[Rg::BYTES], K1[Rg::BYTES], K2[Rg::BYTES], K3[Rg::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK % a.ks;
+    const Tile tl = row_tile(a, blockIdx.x / (a.HK * a.ks));
+    if (tl.b < 0 || tl.x >= a.tiles) return;  // (more tiles than rows make: row starts that do not ascend)
+    const RowTile t = row_tile_of(a, tl, z);
+    const int nb = t.blk1 - t.blk0;
+    if (nb <= 0) return;
+    const int w0 = t.r0 + 32 * wv;
+    const bool live = w0 < t.r1;
+    const int p0 = t.rq.p0 + t.ob.t0;
+    const int r = min(w0 + c, t.r1 - 1), tok = t.ob.t0 + r / a.G, h = kh * a.G + r % a.G;
+    const int jlo = a.from(t.rq.p0 + tok), jhi = min(t.rq.p0 + tok + 1, t.hi);
+    const int all0 = a.from(p0 + (min(w0 + 32, t.r1) - 1) / a.G), all1 = min(p0 + w0 / a.G + 1, t.hi);
+    const int lbpp = a.lps - 5;
+    const int* const tb = a.table + (size_t)tl.b * a.max_blocks;
+    auto entries = [&](int i) { return tb[min((t.blk0 + i + lane) >> lbpp, a.max_blocks - 1)]; };  // lane l: of block i + l
+    int win = 0, ids = entries(0), ids2 = entries(32);
+    auto there = [&](int i, int& page) INL {
+        page = __builtin_amdgcn_readlane(ids, i - win);
+        return i < nb && (unsigned)page < (unsigned)a.n_pages;
+    };
+    const uint32_t dlane = (uint32_t)((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
+    auto fetch = [&](int i, uint8_t* buf) INL {  // (the same number of DMAs always: of what is not there, of zeros)
+        int page;
+        const bool ok = there(i, page);
+        const int blk = t.blk0 + i;
+        const size_t at = ok ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+        const Rsrc rs = make_rsrc(Kp + at, ok ? Rg::BYTES : 0);
+#pragma unroll
+        for (int u = 0; u < IW; u++) buf_lds16(rs, dlane, wv * PART + u * 1024, buf + wv * PART + u * 1024);
+    };
+    T8 qf[NS];
+    {
+        const T* p = Q + ((size_t)(t.rq.q0 + tok) * a.HQ + h) * HD + 8 * g;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const T8*>(p + 16 * s);
+    }
+    float m = -INFINITY, l = 0.f;
+    fetch(0, K0);
+    fetch(1, K1);
+    fetch(2, K2);
+    auto turn = [&](int i, const uint8_t* K, uint8_t* Kx) INL {
+        wait_loads<vmcnt_imm((NB - 2) * IW)>();
+        lds_barrier();  // block i is there for every wave, the one before is done with
+        if (i >= win + 32) win += 32, ids = ids2, ids2 = entries(win + 32);
+        fetch(i + NB - 1, Kx);
+        if (!live) return;
+        f32x16 s;
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < NS; st++) s = Num<T>::mfma32(__builtin_bit_cast(T8, Rg::read(K, st, c, g)), qf[st], s);
+        const int j0 = (t.blk0 + i) * 32;
+        int page;
+        const bool ok = there(i, page);
+        if (!(ok && j0 >= all0 && j0 + 32 <= all1)) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int j = j0 + 8 * (e >> 2) + 4 * g + (e & 3);
+                const bool keep = ok & (j >= jlo) & (j < jhi);
+                s[e] = keep ? s[e] : -INFINITY;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+        const float mn = fmaxf(m, scaled(top, a.c)), base = base_of(mn);
+        float sum = l * exp2_fast(m - base);
+        if (__builtin_expect(__any(is_far(base)), 0)) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) sum += exp2_fast(scaled(s[e], a.c) - base);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) sum += exp2_fast(__builtin_fmaf(s[e], a.c, -base));
+        }
+        m = mn, l = sum;
+    };
+    for (int i = 0;;) {
+        turn(i, K0, K3);
+        if (++i >= nb) break;
+        turn(i, K1, K0);
+        if (++i >= nb) break;
+        turn(i, K2, K1);
+        if (++i >= nb) break;
+        turn(i, K3, K2);
+        if (++i >= nb) break;
+    }
+    wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
+    const float mx = max_halves(m);
+    float sum = l * part_weight(m, mx);
+    sum += __shfl_xor(sum, 32);
+    if (!live || g || w0 + c >= t.r1) return;
+    if (a.ks == 1) a.stat[(size_t)(t.rq.q0 + tok) * a.HQ + h] = make_float2(base_of(mx), inverse_of(sum));
+    else a.ml[(((size_t)z * a.tiles + tl.x) * a.HK + kh) * ROW_TILE + 32 * wv + c] = make_float2(mx, sum);
+}
+
+// Joins the splits of the rows: one thread per row.
+__global__ __launch_bounds__(ROW_TILE) void k_weights_join(WeightArgs a) {
+    const int kh = blockIdx.x % a.HK;
+    const Tile tl = row_tile(a, blockIdx.x / a.HK);
+    if (tl.b < 0 || tl.x >= a.tiles) return;
+    const RowTile t = row_tile_of(a, tl, 0);
+    const int r = t.r0 + threadIdx.x;
+    if (r >= t.r1) return;
+    const int n = min(a.ks, (((t.hi + 31) >> 5) - t.blk0 + a.span - 1) / a.span);
+    const float2* const ml = a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + threadIdx.x;
+    const size_t step = (size_t)a.tiles * a.HK * ROW_TILE;
+    float mx = -INFINITY, l = 0.f;
+#pragma unroll 8
+    for (int z = 0; z < n; z++) {
+        const float2 v = ml[z * step];
+        const float mn = fmaxf(mx, v.x);
+        l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
+        mx = mn;
+    }
+    a.stat[(size_t)(t.rq.q0 + t.ob.t0 + r / a.G) * a.HQ + kh * a.G + r % a.G] = make_float2(base_of(mx), inverse_of(l));
+}
+
+// (key tile, part of the rows) x of the requests', numbered through.
+__device__ __forceinline__ int key_tiles(const Req& rq) { return (rq.kcap + KEY_TILE - 1) / KEY_TILE; }
+__device__ __forceinline__ int key_parts(const WeightArgs& a, int b) {
+    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    const int n = observed(rq, a.observers).n * a.G;
+    return n > a.few ? (n + a.part - 1) / a.part * key_tiles(rq) : 0;
+}
+__device__ __forceinline__ Tile key_tile(const WeightArgs& a, int x) {
+    return find_tile(a.B, x, [&](int b) { return key_parts(a, b); });
+}
+// The number of request b's first one, in find_tile's order: lane by lane, lane l's requests l, l + 64, ...
+__device__ __forceinline__ int first_key_tile(const WeightArgs& a, int b) {
+    if (a.B == 1) return 0;
+    const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
+    int own = 0, before = 0;
+#pragma unroll 8
+    for (int i = 0; i < per; i++) {
+        const int r = 64 * i + lane, n = key_parts(a, min(r, a.B - 1));
+        before += r < b ? n : 0;
+        own = min(own + (r < a.B ? n : 0), 1 << 24);
+    }
+    int to = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(to, o);
+        if (lane >= o) to += y;
+    }
+    return __shfl(to - own + before, b & 63);
+}
+// The rows [lo, hi) of a request that see some key of [j0, j1).
+__device__ __forceinline__ void rows_of(const WeightArgs& a, const Req& rq, const Seen& ob, int j0, int j1, int& lo, int& hi) {
+    const int p0 = rq.p0 + ob.t0;
+    const int last = a.window ? (int)min((long long)ob.n, (long long)j1 - 1 + a.window - p0) : ob.n;  // tokens
+    lo = max(0, j0 - p0) * a.G;
+    hi = max(0, last) * a.G;
+    if (j0 - p0 >= ob.n) lo = hi = 0;
+}
+
+// Weights of 128 keys from a part of the rows: each wave has 32 keys in registers, and all four share blocks of 32 rows of
+// queries that arrive by LDS DMA, three ahead, in the ring's layout.  A lane adds its row's weight to its 16 keys' sums, in
+// registers; the 32 lanes meet at the end.
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void k_weights_keys(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    typedef typename Vec8<T>::type T8;
+    typedef Ring<HD> Rg;
+    constexpr int NS = HD / 16, NB = 4, IW = Rg::IW;
+    __shared__ __align__(1024) uint8_t Q0[Rg::BYTES], Q1[Rg::BYTES], Q2[Rg::BYTES], Q3[Rg::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    const int kh = blockIdx.x % a.HK;
+    const Tile tl = key_tile(a, blockIdx.x / a.HK);
+    if (tl.b < 0 || tl.x >= a.units) return;  // (as above)
+    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    const Seen ob = observed(rq, a.observers);
+    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part;
+    const int z = tl.i % parts, j0 = tl.i / parts * KEY_TILE;
+    int lo, hi;
+    rows_of(a, rq, ob, j0, j0 + KEY_TILE, lo, hi);
+    const int r0 = max(lo, z * a.part) & ~31, r1 = min(hi, (z + 1) * a.part), nb = (r1 - r0 + 31) >> 5;  // (parts are multiples of 32)
+    const bool sole = a.parts == 1;  // this workgroup's sums are the keys' weights
+    if (r1 <= r0 && !sole) return;
+    const int jw = j0 + 32 * wv, lbpp = a.lps - 5, blk = jw >> 5;
+    const int page = a.table[(size_t)tl.b * a.max_blocks + min(blk >> lbpp, a.max_blocks - 1)];
+    const bool there = jw < rq.kcap && (unsigned)page < (unsigned)a.n_pages;
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    if (r1 > r0) {
+        u32x4 kf[NS];
+        {
+            const size_t at = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+            const Rsrc rk = make_rsrc(Kp + at, there ? HD * 64u : 0u);
+#pragma unroll
+            for (int st = 0; st < NS; st++) kf[st] = buf_b128(rk, c * 64 + (2 * (st & 1) + g) * 16, (st >> 1) * 2048);
+        }
+        const int p0 = rq.p0 + ob.t0;
+        // row r0 + 32 i + x is token t + (g0 + x) / G, head (g0 + x) % G
+        auto split = [&](int x, int& t, int& h) INL {
+            t = a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.magic);
+            h = x - t * a.G;
+        };
+        const int dt = 32 / a.G, dg = 32 % a.G;
+        int tf = r0 / a.G, gf = r0 % a.G;  // of the block that is fetched next
+        const size_t row = (size_t)a.HQ * HD;
+        const uint32_t piece = (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+        auto fetch = [&](int i, uint8_t* buf) INL {
+            const int left = nrows - (r0 + 32 * i);  // (rows past the last are the last again, blocks past it too)
+            const size_t t0 = (size_t)rq.q0 + ob.t0 + min(tf, ob.n - 1);
+            const T* const base = Q + t0 * row + (size_t)kh * a.G * HD;
+            const Rsrc rs = make_rsrc(base, (uint32_t)min((size_t)0x7FFFFFFF, (((size_t)a.rows - t0) * row - (size_t)kh * a.G * HD) * 2));
+            uint32_t off[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                int t, h;
+                split(gf + min(16 * u + (lane >> 2), max(left, 1) - 1), t, h);
+                off[u] = left > 0 ? (uint32_t)(t * (int)row + h * HD) * 2 + piece : piece;
+            }
+#pragma unroll
+            for (int u = 0; u < IW; u++) {
+                const int x = wv * IW + u;  // half x % 2 of dims 32 (x / 2) ..
+                const bool odd = IW == 1 ? wv & 1 : u & 1;
+                buf_lds16(rs, odd ? off[1] : off[0], (x >> 1) * 64, buf + x * 1024);
+            }
+            tf += dt, gf += dg;
+            if (gf >= a.G) gf -= a.G, tf++;
+        };
+        int ts = r0 / a.G, gs = r0 % a.G;  // of the block whose rows' statistics are loaded next
+        float2 st;
+        int pr;  // the lane's row's position
+        bool valid;
+        auto next_stat = [&]() INL {
+            int t, h;
+            split(gs + c, t, h);
+            const int tok = ts + t;
+            valid = tok < ob.n;
+            const int tc = min(tok, ob.n - 1);
+            st = a.stat[((size_t)rq.q0 + ob.t0 + tc) * a.HQ + kh * a.G + h];
+            pr = p0 + tc;
+            ts += dt, gs += dg;
+            if (gs >= a.G) gs -= a.G, ts++;
+        };
+        next_stat();
+        fetch(0, Q0);
+        fetch(1, Q1);
+        fetch(2, Q2);
+        auto turn = [&](int i, const uint8_t* buf, uint8_t* bufx) INL {
+            wait_loads<vmcnt_imm((NB - 2) * IW)>();
+            lds_barrier();
+            const float2 now = st;
+            const int p = pr;
+            const bool ok = valid;
+            next_stat();
+            fetch(i + NB - 1, bufx);
+            // every row of the block sees every key of the wave
+            const int ra = r0 + 32 * i, first = __builtin_amdgcn_readlane(p, 0), last = __builtin_amdgcn_readlane(p, 31);
+            const bool open = there && ra + 32 <= r1 && first >= jw + 31 && a.from(last) <= jw && jw + 32 <= rq.kcap;
+            f32x16 s;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+            for (int x = 0; x < NS; x++) s = Num<T>::mfma32(__builtin_bit_cast(T8, kf[x]), __builtin_bit_cast(T8, Rg::read(buf, x, c, g)), s);
+            if (__builtin_expect(__any(is_far(now.x)), 0)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = exp2_fast(scaled(s[e], a.c) - now.x) * now.y;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = exp2_fast(__builtin_fmaf(s[e], a.c, -now.x)) * now.y;
+            }
+            if (!open) {
+                const int from = a.from(p);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int j = jw + 8 * (e >> 2) + 4 * g + (e & 3);
+                    const bool keep = there & ok & (ra + c < r1) & (j <= p) & (j >= from);
+                    s[e] = keep ? s[e] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[e] += s[e];
+        };
+        for (int i = 0;;) {
+            turn(i, Q0, Q3);
+            if (++i >= nb) break;
+            turn(i, Q1, Q0);
+            if (++i >= nb) break;
+            turn(i, Q2, Q1);
+            if (++i >= nb) break;
+            turn(i, Q3, Q2);
+            if (++i >= nb) break;
+        }
+        wait_loads<vmcnt_imm(0)>();
+    }
+    // the sum over the 32 rows' lanes, halving the registers at each step: lane c has key e = c / 2
+#pragma unroll
+    for (int o = 16, n = 8; n; o >>= 1, n >>= 1) {
+#pragma unroll
+        for (int e = 0; e < n; e++) {
+            const bool up = c & o;
+            const float keep = up ? acc[e + n] : acc[e], send = up ? acc[e] : acc[e + n];
+            acc[e] = keep + __shfl_xor(send, o);
+        }
+    }
+    const float w = acc[0] + __shfl_xor(acc[0], 1);
+    const int e = c >> 1, x = 8 * (e >> 2) + 4 * g + (e & 3), j = jw + x;
+    if (c & 1) return;
+    if (!sole) a.col[((size_t)tl.x * a.HK + kh) * KEY_TILE + 32 * wv + x] = w;
+    else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
+}
+
+// Adds up the parts of 128 keys, in their order.
+__global__ __launch_bounds__(KEY_TILE) void k_weights_sum(WeightArgs a) {
+    const int kh = blockIdx.x % a.HK;
+    const Tile tl = find_tile(a.B, blockIdx.x / a.HK, [&](int b) {
+        return many_rows(a, b) ? key_tiles(request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
+    });
+    if (tl.b < 0) return;
+    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    const Seen ob = observed(rq, a.observers);
+    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part, j0 = tl.i * KEY_TILE, j = j0 + threadIdx.x;
+    const int first = first_key_tile(a, tl.b) + tl.i * parts;
+    if (j >= rq.kcap || first < 0 || first + parts > a.units) return;
+    const int page = a.table[(size_t)tl.b * a.max_blocks + (j >> a.lps)];
+    if ((unsigned)page >= (unsigned)a.n_pages) return;
+    int lo, hi;
+    rows_of(a, rq, ob, j0, j0 + KEY_TILE, lo, hi);
+    float w = 0.f;
+    const float* const col = a.col + ((size_t)first * a.HK + kh) * KEY_TILE + threadIdx.x;
+    if (hi > lo) {
+#pragma unroll 8
+        for (int z = lo / a.part; z <= (hi - 1) / a.part; z++) w += col[(size_t)z * a.HK * KEY_TILE];
+    }
+    put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
 
 // ---- the rows that go -----------------------------------------------------------------------------------------------
@@ -305,23 +866,104 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
     }
 }
 
+// How a call runs, from its sizes alone (the lengths themselves are on the device).
+struct WeightPlan {
+    int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
+    int tiles = 0, ks = 1, span = 1, part = 32, parts = 1, units = 0;  // tiles 0: no many rows
+    bool once = false;
+    size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0;  // floats of the workspace
+};
+
+WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
+    const int G = s.HQ / s.HK;
+    const int tokens = std::min({max_new, rows, observers ? observers : INT_MAX});
+    const long long most = (long long)tokens * G;
+    WeightPlan p;
+    const int nb = (int)(((long long)max_kv + 31) / 32);
+    if (most <= 32) p.few = (int)most;
+    else if (G <= 32 && rows < (long long)max_new * B) p.few = G;
+    if (p.few) {
+        p.nr = p.few <= 16 ? 1 : 2;
+        p.kvp = (int)std::min<long long>((long long)nb * 32, INT_MAX);
+        const int want = std::max(1, std::min(64, 1024 / (B * s.HK)));
+        p.few_span = std::max(FEW_W, (nb + want - 1) / want);
+        p.few_ks = (nb + p.few_span - 1) / p.few_span;
+        p.S = (size_t)B * s.HK * p.few * p.kvp;
+        p.few_ml = (size_t)B * s.HK * p.few_ks * p.few * 2;
+        p.once = (size_t)B * nb * s.HK * s.HD * 64 > (size_t(256) << 20);
+        if ((long long)B * s.HK * p.few_ks >= 1 << 24)
+            throw Error("sd_op_paged_weights: too many requests and keys for one launch");
+    }
+    if (most > p.few) {
+        const long long all = std::min((long long)rows, (long long)B * tokens) * G;  // rows that are counted
+        const long long reqs = std::min((long long)B, all / (p.few + 1));
+        p.tiles = (int)(all / ROW_TILE + reqs);
+        const int want = (int)std::min(128ll, std::max(1ll, 1024 / (std::max(1ll, all / ROW_TILE) * s.HK)));
+        p.span = std::max(16, (nb + want - 1) / want);
+        p.ks = (nb + p.span - 1) / p.span;
+        const int nkb = (int)(((long long)max_kv + KEY_TILE - 1) / KEY_TILE);
+        const long long wanted = std::max(1ll, 2048ll / ((long long)nkb * s.HK));
+        p.part = (int)std::max(128ll, ((all + wanted - 1) / wanted + 31) / 32 * 32);
+        p.parts = (int)((most + p.part - 1) / p.part);
+        const long long units = (long long)nkb * std::min(reqs * p.parts, all / p.part + reqs);
+        if (units * s.HK >= 1 << 24 || (long long)p.tiles * s.HK * p.ks >= 1 << 24)
+            throw Error("sd_op_paged_weights: too many rows and keys for one launch");
+        p.units = (int)units;
+        p.ml = p.ks > 1 ? (size_t)p.ks * p.tiles * s.HK * ROW_TILE * 2 : 0;
+        p.stat = (size_t)rows * s.HQ * 2;
+        p.col = p.parts > 1 ? (size_t)p.units * s.HK * KEY_TILE : 0;
+    }
+    for (size_t* x : {&p.S, &p.few_ml, &p.ml, &p.stat, &p.col}) *x = (*x + 3) & ~size_t(3);
+    return p;
+}
+
 template <class T, int HD>
 void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
-    const WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, s.HQ / s.HK, log2i(s.PS),
-                       s.n_pages, a.max_new, a.max_kv, a.window, a.observers, a.scale * LOG2E, a.decay, s.pstride, a.scores,
-                       a.out, a.kpos};
+    const WeightPlan p = plan_weights(s, a.B, a.rows, a.max_new, a.max_kv, a.observers);
+    const int G = s.HQ / s.HK;
+    float* const ws = static_cast<float*>(a.ws);
+    WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, G, log2i(s.PS), s.n_pages, a.max_new,
+                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.part,
+                 p.parts, p.units, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
+    g.S = ws;
+    g.few_ml = reinterpret_cast<float2*>(g.S + p.S);
+    g.ml = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.few_ml) + p.few_ml);
+    g.stat = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.ml) + p.ml);
+    g.col = reinterpret_cast<float*>(g.stat) + p.stat;
     const T *Q = static_cast<const T*>(a.Q), *K = static_cast<const T*>(a.Kp);
-    float2* const ml = static_cast<float2*>(a.ws);
-    const int most = std::min({a.max_new, a.rows, a.observers ? a.observers : INT_MAX});
-    hipLaunchKernelGGL((k_weights_stats<T, HD>), dim3(s.HQ * std::min(most, 4096), a.B), dim3(64), 0, st, Q, K, g, ml);
-    launched("paged_weights");
-    hipLaunchKernelGGL((k_weights_sum<T, HD>), dim3((a.max_kv + 255) / 256, s.HK, a.B), dim3(256), 0, st, Q, K, g, ml);
-    launched("paged_weights");
+    auto launch = [&](auto kernel, dim3 grid, int threads, auto... args) {
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, args...);
+        launched("paged_weights");
+    };
+    if (p.tiles) {
+        launch(k_weights_rows<T, HD>, dim3(p.tiles * s.HK * p.ks), 256, Q, K, g);
+        if (p.ks > 1) launch(k_weights_join, dim3(p.tiles * s.HK), ROW_TILE, g);
+        launch(k_weights_keys<T, HD>, dim3(p.units * s.HK), 256, Q, K, g);
+        if (p.parts > 1) {
+            const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
+            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), KEY_TILE, g);
+        }
+    }
+    if (p.nr) {
+        const dim3 grid(s.HK * p.few_ks, a.B);
+        if (p.nr == 1) {
+            if (p.once) launch(k_weights_few<T, HD, 1, true>, grid, 64 * FEW_W, Q, K, g);
+            else launch(k_weights_few<T, HD, 1, false>, grid, 64 * FEW_W, Q, K, g);
+        } else {
+            if (p.once) launch(k_weights_few<T, HD, 2, true>, grid, 64 * FEW_W, Q, K, g);
+            else launch(k_weights_few<T, HD, 2, false>, grid, 64 * FEW_W, Q, K, g);
+        }
+        const long long chunks = ((long long)a.max_kv + 1023) / 1024;  // of 1024 keys; at most so many workgroups that each has some
+        launch(k_weights_few_sum, dim3((unsigned)std::min(chunks, std::max(1ll, 16384ll / (s.HK * a.B))), s.HK, a.B), 256, g);
+    }
 }
 
 }  // namespace
 
-size_t paged_weights_ws(const PagedShape& s, int, int rows, int, int, int) { return (size_t)rows * s.HQ * 8; }
+size_t paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
+    const WeightPlan p = plan_weights(s, B, rows, max_new, max_kv, observers);
+    return (p.S + p.few_ml + p.ml + p.stat + p.col) * 4;
+}
 
 void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     by_type(s, [&](auto t, auto hd) { weights_as<decltype(t), decltype(hd)::value>(s, a, st); });

@@ -135,6 +135,52 @@ __device__ __forceinline__ Req request(const int* __restrict__ cu, const int* __
     return r;
 }
 
+struct Tile {
+    int b, i;  // request and tile in it; b < 0: none
+    int x;     // its number
+};
+// Tile x of the requests' tiles numbered through (tiles(b) of request b, at most 2^24), the last one first.
+template <class F>
+__device__ __forceinline__ Tile find_tile(int B, int x, F&& of) {
+    const int lane = threadIdx.x & 63, per = (B + 63) >> 6;
+    if (B == 1) {
+        const int total = of(0);
+        return {x < total ? 0 : -1, total - 1 - x, total - 1 - x};
+    }
+    auto tiles = [&](int b) {
+        const int n = of(min(b, B - 1));
+        return b < B ? n : 0;  // (no branch: several loads in flight)
+    };
+    auto upto = [&](int v) {  // the sum of lanes 0 to the own
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(v, o);
+            if (lane >= o) v += y;
+        }
+        return v;
+    };
+    // lane l counts requests l, l + 64, ..., the tiles are numbered lane by lane
+    // (cut at 2^24 per lane, which row starts that do not ascend could pass: the sums stay in range)
+    int own = 0;
+#pragma unroll 8
+    for (int i = 0; i < per; i++) own = min(own + tiles(64 * i + lane), 1 << 24);
+    const int to = upto(own), total = __builtin_amdgcn_readlane(to, 63);
+    if (x >= total) return {-1, 0, 0};
+    const int number = x = total - 1 - x;
+    const int at = __ffsll((long long)__ballot(to > x)) - 1;
+    x -= __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(own, at);
+    if (per == 1) return {at, x, number};
+    for (int i = 0; i < per; i += 64) {  // lane l: request 64 (i + l) + at
+        const int n = i + lane < per ? tiles(64 * (i + lane) + at) : 0, t = upto(n), sum = __builtin_amdgcn_readlane(t, 63);
+        if (x < sum) {
+            const int l = __ffsll((long long)__ballot(t > x)) - 1;
+            return {64 * (i + l) + at, x - (__builtin_amdgcn_readlane(t, l) - __builtin_amdgcn_readlane(n, l)), number};
+        }
+        x -= sum;
+    }
+    return {-1, 0, 0};
+}
+
 // Weight of a part of a row's keys (a wave's, a split's) whose running maximum is m, where the largest is mx.  A part that
 // saw no score above -inf has 0, and its zeros, or its NaN (0 times a value that is not finite), are multiplied like any
 // other's: what is seen stays seen, whatever the split.

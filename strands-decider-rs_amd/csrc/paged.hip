@@ -709,48 +709,11 @@ __global__ __launch_bounds__(256) void k_paged_join_few(AttnArgs a, const float*
 // the long ones.  (Each workgroup finds its tile by itself, from all requests: 1086 us for 8192 requests of 20 new tokens
 // on 300 keys, 8 and 2 heads of 128 dims, whose keys and values alone are 455.)
 constexpr int TILE_ROWS = 128;
-struct Tile {
-    int b, i;  // request and tile in it; b < 0: none
-};
 __device__ __forceinline__ Tile find_tile(const AttnArgs& a, int x) {
-    const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
-    if (a.B == 1) {
-        const int n = request(a.cu, a.kv_lens, 0, a.rows, a.max_new, a.kcap).n * a.G;
-        const int total = n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
-        return {x < total ? 0 : -1, total - 1 - x};
-    }
-    auto tiles = [&](int b) {
-        const int n = request(a.cu, a.kv_lens, min(b, a.B - 1), a.rows, a.max_new, a.kcap).n * a.G;
-        return ((b < a.B) & (n > a.few)) ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;  // (no branch: several loads in flight)
-    };
-    auto upto = [&](int v) {  // the sum of lanes 0 to the own
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(v, o);
-            if (lane >= o) v += y;
-        }
-        return v;
-    };
-    // lane l counts requests l, l + 64, ..., the tiles are numbered lane by lane
-    // (cut at 2^24 per lane, which row starts that do not ascend could pass: the sums stay in range)
-    int own = 0;
-#pragma unroll 8
-    for (int i = 0; i < per; i++) own = min(own + tiles(64 * i + lane), 1 << 24);
-    const int to = upto(own), total = __builtin_amdgcn_readlane(to, 63);
-    if (x >= total) return {-1, 0};
-    x = total - 1 - x;
-    const int at = __ffsll((long long)__ballot(to > x)) - 1;
-    x -= __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(own, at);
-    if (per == 1) return {at, x};
-    for (int i = 0; i < per; i += 64) {  // lane l: request 64 (i + l) + at
-        const int n = i + lane < per ? tiles(64 * (i + lane) + at) : 0, t = upto(n), sum = __builtin_amdgcn_readlane(t, 63);
-        if (x < sum) {
-            const int l = __ffsll((long long)__ballot(t > x)) - 1;
-            return {64 * (i + l) + at, x - (__builtin_amdgcn_readlane(t, l) - __builtin_amdgcn_readlane(n, l))};
-        }
-        x -= sum;
-    }
-    return {-1, 0};
+    return find_tile(a.B, x, [&](int b) {
+        const int n = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap).n * a.G;
+        return n > a.few ? (n + TILE_ROWS - 1) / TILE_ROWS : 0;
+    });
 }
 
 // FEW (2: with the non-temporal hint): the launch ends with the workgroups of the requests with few rows, which would
