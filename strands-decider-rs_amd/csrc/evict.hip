@@ -74,6 +74,26 @@ __device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= FAR; }
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }  // (its sum is 0, or NaN)
 __device__ __forceinline__ float inverse_of(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
+// A row's whole, from its n parts, `step` apart: 8 lanes on end share it.
+__device__ __forceinline__ float2 join_parts(const float2* ml, size_t step, int n) {
+    const int u = threadIdx.x & 7;
+    float mx = -INFINITY, l = 0.f;
+#pragma unroll 4
+    for (int z = u; z < n; z += 8) {
+        const float2 v = ml[z * step];
+        const float mn = fmaxf(mx, v.x);
+        l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
+        mx = mn;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const float m2 = __shfl_xor(mx, o), l2 = __shfl_xor(l, o), mn = fmaxf(mx, m2);
+        l = l * part_weight(mx, mn) + l2 * part_weight(m2, mn);
+        mx = mn;
+    }
+    return make_float2(base_of(mx), inverse_of(l));
+}
+
 // Key j's weight w of a request's rows, into the scores of kv head h.
 __device__ __forceinline__ void put_weight(const WeightArgs& a, const Req& rq, size_t at, int j, float w) {
     const bool old = j < rq.p0;
@@ -231,22 +251,9 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     if (nrows == 0 || nrows > a.few || blockIdx.x * 1024 >= (unsigned)rq.kcap) return;
     const int p0 = rq.p0 + ob.t0, hi = min(p0 + ob.n, rq.kcap), lo = max(0, a.from(p0));
     {
-        const int r = tid >> 3, u = tid & 7;
-        const float2* const ml = a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw + min(r, nrows - 1);
-        float mx = -INFINITY, l = 0.f;
-        for (int z = u; z < a.few_ks; z += 8) {
-            const float2 v = ml[z * a.rw];
-            const float mn = fmaxf(mx, v.x);
-            l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
-            mx = mn;
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            const float m2 = __shfl_xor(mx, o), l2 = __shfl_xor(l, o), mn = fmaxf(mx, m2);
-            l = l * part_weight(mx, mn) + l2 * part_weight(m2, mn);
-            mx = mn;
-        }
-        if (u == 0) stat[r] = make_float2(base_of(mx), inverse_of(l));
+        const int r = tid >> 3;
+        const float2 st = join_parts(a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw + min(r, nrows - 1), a.rw, a.few_ks);
+        if ((tid & 7) == 0) stat[r] = st;
     }
     __syncthreads();
     for (int j0 = blockIdx.x * 1024; j0 < rq.kcap; j0 += gridDim.x * 1024) {
@@ -426,26 +433,18 @@ __global__ __launch_bounds__(256, 2) void k_weights_rows(const T* __restrict__ Q
     else a.ml[(((size_t)z * a.tiles + tl.x) * a.HK + kh) * ROW_TILE + 32 * wv + c] = make_float2(mx, sum);
 }
 
-// Joins the splits of the rows: one thread per row.
-__global__ __launch_bounds__(ROW_TILE) void k_weights_join(WeightArgs a) {
-    const int kh = blockIdx.x % a.HK;
-    const Tile tl = row_tile(a, blockIdx.x / a.HK);
+// Joins the splits of the rows: 8 threads per row, 32 rows a workgroup.
+__global__ __launch_bounds__(256) void k_weights_join(WeightArgs a) {
+    constexpr int PER = ROW_TILE / 32;
+    const int kh = blockIdx.x / PER % a.HK;
+    const Tile tl = row_tile(a, blockIdx.x / (PER * a.HK));
     if (tl.b < 0 || tl.x >= a.tiles) return;
     const RowTile t = row_tile_of(a, tl, 0);
-    const int r = t.r0 + threadIdx.x;
+    const int i = blockIdx.x % PER * 32 + threadIdx.x / 8, r = t.r0 + i;
     if (r >= t.r1) return;
     const int n = min(a.ks, (((t.hi + 31) >> 5) - t.blk0 + a.span - 1) / a.span);
-    const float2* const ml = a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + threadIdx.x;
-    const size_t step = (size_t)a.tiles * a.HK * ROW_TILE;
-    float mx = -INFINITY, l = 0.f;
-#pragma unroll 8
-    for (int z = 0; z < n; z++) {
-        const float2 v = ml[z * step];
-        const float mn = fmaxf(mx, v.x);
-        l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
-        mx = mn;
-    }
-    a.stat[(size_t)(t.rq.q0 + t.ob.t0 + r / a.G) * a.HQ + kh * a.G + r % a.G] = make_float2(base_of(mx), inverse_of(l));
+    const float2 st = join_parts(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n);
+    if ((threadIdx.x & 7) == 0) a.stat[(size_t)(t.rq.q0 + t.ob.t0 + r / a.G) * a.HQ + kh * a.G + r % a.G] = st;
 }
 
 // (key tile, part of the rows) x of the requests', numbered through.
@@ -663,6 +662,11 @@ __global__ __launch_bounds__(KEY_TILE) void k_weights_sum(WeightArgs a) {
 }
 
 // ---- the rows that go -----------------------------------------------------------------------------------------------
+//
+// Of a (request, kv head)'s n rows the m of the highest ranks stay: a rank is 32 bits, its order the scores', protected
+// rows above all.  The m-th is found by digits of 11, 11 and 10 bits from the highest down: a histogram in LDS of the rows
+// whose digits above match, and a scan of its counts.  Rows above that rank stay, and of those that have it the first.
+// Up to 32768 rows one workgroup does it all, with every row's rank in registers, read once.
 
 // A score's place in the order, ascending: NaN, and a row in a hole, before all numbers; -0 is 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
@@ -671,7 +675,8 @@ __device__ __forceinline__ uint32_t rank_of(float s) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int EVICT_T = 1024;
+constexpr int EVICT_T = 1024, BINS = 2048;
+constexpr int EVICT_ONE = 32768;  // rows up to which one workgroup does a head
 
 // The sum over the threads before this one, and over all; `ws` holds EVICT_T / 64 counts.
 template <class I>
@@ -693,88 +698,390 @@ __device__ __forceinline__ I scan(I x, I* ws, I& total) {
     return before + v - x;
 }
 
-// One workgroup per (request, kv head): the m-th largest rank by its 8-bit digits, from the highest down (a histogram of
-// the rows whose digits above match), then one pass over the rows in order that numbers the holes below m and the rows
-// that stay behind it.
-__global__ __launch_bounds__(EVICT_T) void k_page_evict(const float* __restrict__ scores, const int* __restrict__ kpos,
-                                                        const int* __restrict__ table, int max_blocks,
-                                                        const int* __restrict__ kv_lens, const int* __restrict__ budgets,
-                                                        int max_kv, int HK, int lps, int n_pages, int sink, int recent,
-                                                        int* __restrict__ new_lens, int* __restrict__ moves,
-                                                        int* __restrict__ counts) {
-    __shared__ int hist[256], ws[EVICT_T / 64], newest, digit, above;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, W = max(max_kv / 2, 1);
-    const int n = kv_lens[b], budget = budgets[b];
-    const bool over = n <= max_kv && budget >= 0 && n > budget;
-    const int m = over ? budget : n;
-    if (h == 0 && tid == 0) new_lens[b] = m;
-    if (!over) {
-        if (tid == 0) counts[(size_t)b * HK + h] = 0;
+struct EvictArgs {
+    const float* scores;
+    const int *kpos, *table, *kv_lens, *budgets;
+    int max_blocks, B, max_kv, HK, lps, n_pages, sink, recent, W;
+    int *new_lens, *moves, *counts;
+    // heads of more than EVICT_ONE rows: chunks of CHUNK rows
+    int chunks;
+    int* newest;  // [B][HK][chunks]
+    int* hist;    // [B][HK][3][BINS]
+    int* parts;   // [B][HK][chunks][4]: rows of the m-th rank and above it, below m and from m on
+};
+
+// One head's part in a launch.  over: rows go.
+struct Head {
+    int b, h, n, m;
+    bool over;
+    const int* tb;
+    size_t bh;
+};
+__device__ __forceinline__ Head head_of(const EvictArgs& a, int h, int b) {
+    Head x;
+    x.b = b, x.h = h;
+    x.n = a.kv_lens[b];
+    const int budget = a.budgets[b];
+    x.over = x.n <= a.max_kv && budget >= 0 && x.n > budget;
+    x.m = x.over ? budget : x.n;
+    x.tb = a.table + (size_t)b * a.max_blocks;
+    x.bh = (size_t)b * a.HK + h;
+    return x;
+}
+
+typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// 4 rows from j on (a multiple of 4: they lie on end), as loaded.
+struct Four {
+    f32x4u s;
+    i32x4 p;
+    bool there;
+};
+__device__ __forceinline__ Four load4(const EvictArgs& a, const Head& x, int j) {
+    Four r;
+    const int page = j < x.n ? x.tb[j >> a.lps] : -1;
+    r.there = (unsigned)page < (unsigned)a.n_pages;
+    const size_t at = mark_at(r.there ? page : 0, a.HK, x.h, r.there ? j : 0, a.lps);
+    r.s = *reinterpret_cast<const f32x4u*>(a.scores + at);
+    if (a.kpos) r.p = *reinterpret_cast<const i32x4*>(a.kpos + at);
+    else r.p = i32x4{j, j + 1, j + 2, j + 3};
+    return r;
+}
+__device__ __forceinline__ int newest_of(const Four& v, const Head& x, int j) {
+    int most = INT_MIN;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (v.there && j + e < x.n) most = max(most, v.p[e]);
+    return most;
+}
+__device__ __forceinline__ uint32_t rank4(const EvictArgs& a, const Four& v, int e, long long keep_from) {
+    if (!v.there) return 0;
+    return v.p[e] < a.sink || v.p[e] > keep_from ? 0xFFFFFFFFu : min(rank_of(v.s[e]), 0xFFFFFFFEu);
+}
+
+__device__ __forceinline__ int max_all(int x, int* ws) {  // over the workgroup
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o));
+    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = x;
+    __syncthreads();
+    int r = ws[0];
+#pragma unroll
+    for (int w = 1; w < EVICT_T / 64; w++) r = max(r, ws[w]);
+    return r;
+}
+
+// Digit t of a rank, and the bits above it.
+constexpr int SHIFT[3] = {21, 10, 0};
+__device__ __forceinline__ int digit(uint32_t r, int shift) { return r >> shift & (shift ? BINS - 1 : 1023); }
+
+// Of a histogram's rows the `left` of the largest digits stay: the digit of the last of them, `left` less those above it,
+// and how many have it.  Two bins a thread; all threads get the answer.  (left 0: the largest digit, of which none stays)
+struct Cut {
+    int digit, left, count;
+};
+__device__ __forceinline__ Cut cut_at(const int* hist, int left, int* ws, int* found) {
+    const int tid = threadIdx.x, d1 = BINS - 1 - 2 * tid, d0 = d1 - 1;  // (from the largest digit down)
+    const int c1 = hist[d1], c0 = hist[d0];
+    int total;
+    const int before = scan(c1 + c0, ws, total);
+    if (left == 0 ? tid == 0 : before < left && left <= before + c1 + c0) {
+        const bool first = left == 0 || left <= before + c1;
+        found[0] = first ? d1 : d0;
+        found[1] = left - before - (first ? 0 : c1);
+        found[2] = first ? c1 : c0;
+    }
+    __syncthreads();
+    return {found[0], found[1], found[2]};
+}
+
+// The numbers of a chunk's holes and rows (bits 0 and 1 of what[e], 4 rows a thread) behind those of the chunks before:
+// each wave's packed counts, then a scan over the lanes.
+__device__ __forceinline__ uint32_t lanes_before(uint32_t x, uint32_t& all) {  // (packed sums over a wave)
+    const int lane = threadIdx.x & 63;
+    uint32_t v = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(v, o);
+        if (lane >= o) v += y;
+    }
+    all = __shfl(v, 63);
+    return v - x;
+}
+
+// One workgroup per (request, kv head), N times 4 rows a thread.
+template <int N>
+__global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
+    constexpr int WV = EVICT_T / 64;
+    __shared__ int hist[BINS], ws[WV], found[3];
+    __shared__ uint32_t sums[N * WV + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const Head x = head_of(a, blockIdx.x, blockIdx.y);
+    if (x.h == 0 && tid == 0) a.new_lens[x.b] = x.m;
+    if (!x.over) {
+        if (tid == 0) a.counts[x.bh] = 0;
         return;
     }
-    const int* const tb = table + (size_t)b * max_blocks;
-    auto where = [&](int j, bool& there) {
-        const int page = tb[j >> lps];
-        there = (unsigned)page < (unsigned)n_pages;
-        return mark_at(there ? page : 0, HK, h, j, lps);
-    };
-    if (tid == 0) newest = INT_MIN;
-    __syncthreads();
-    int most = INT_MIN;
-    for (int j = tid; j < n; j += EVICT_T) {
-        bool there;
-        const size_t at = where(j, there);
-        if (there) most = max(most, kpos ? kpos[at] : j);
+    uint32_t rank[4 * N];
+    {
+        Four v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = load4(a, x, (i * EVICT_T + tid) * 4);
+        for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
+        int most = INT_MIN;
+#pragma unroll
+        for (int i = 0; i < N; i++) most = max(most, newest_of(v[i], x, (i * EVICT_T + tid) * 4));
+        const long long keep_from = (long long)max_all(most, ws) - a.recent;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) rank[4 * i + e] = rank4(a, v[i], e, keep_from);
     }
-    atomicMax(&newest, most);
-    __syncthreads();
-    const long long keep_from = (long long)newest - recent;
-    auto rank = [&](int j) {
-        bool there;
-        const size_t at = where(j, there);
-        if (!there) return 0u;
-        const int p = kpos ? kpos[at] : j;
-        return p < sink || p > keep_from ? 0xFFFFFFFFu : min(rank_of(scores[at]), 0xFFFFFFFEu);
-    };
+    auto at = [&](int k) { return ((k >> 2) * EVICT_T + tid) * 4 + (k & 3); };  // the row of rank[k]
     uint32_t prefix = 0;
-    int left = m;  // of the largest ranks that begin with `prefix`, so many stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += EVICT_T) hist[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += EVICT_T) {
-            const uint32_t r = rank(j);
-            if (shift == 24 || r >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[r >> shift & 255], 1);
+    int left = x.m, count = 0;
+#pragma unroll
+    for (int t = 0; t < 3; t++) {
+        const int shift = SHIFT[t], above = t ? SHIFT[t - 1] : 0;
+        if (t) {
+            __syncthreads();
+            for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
+            __syncthreads();
         }
+#pragma unroll
+        for (int k = 0; k < 4 * N; k++)
+            if (at(k) < x.n && (t == 0 || rank[k] >> above == prefix >> above)) atomicAdd(&hist[digit(rank[k], shift)], 1);
         __syncthreads();
-        if (tid == 0) {
-            int d = 255, sum = 0;
-            while (d > 0 && sum + hist[d] < left) sum += hist[d--];
-            digit = d, above = sum;
-        }
-        __syncthreads();
-        prefix |= (uint32_t)digit << shift;
-        left -= above;
+        const Cut c = cut_at(hist, left, ws, found);
+        prefix |= (uint32_t)c.digit << shift;
+        left = c.left, count = c.count;
     }
-    // ranks above `prefix` stay, and the first `left` rows that have it
-    int ties = 0, holes = 0, rows = 0;
-    int* const mv = moves + ((size_t)b * HK + h) * W * 2;
-    for (int j0 = 0; j0 < n; j0 += EVICT_T) {
-        const int j = j0 + tid;
-        const uint32_t r = j < n ? rank(j) : 0;
-        const bool tie = j < n && r == prefix;
-        int total;
-        const int nth = ties + scan((int)tie, ws, total);
+    // Rows above `prefix` stay, and the first `left` of the `count` that have it.
+    int last = INT_MAX;  // the row of the last of those
+    if (left < count || left == 0) {
+        __syncthreads();
+        if (tid == 0) found[0] = -1;
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            int ties = 0, total;
+#pragma unroll
+            for (int e = 0; e < 4; e++) ties += at(4 * i + e) < x.n && rank[4 * i + e] == prefix;
+            int nth = before + scan(ties, ws, total);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (at(4 * i + e) < x.n && rank[4 * i + e] == prefix && ++nth == left) found[0] = at(4 * i + e);
+            before += total;
+        }
+        __syncthreads();
+        last = found[0];  // (-1: none stays)
+    }
+    auto stays = [&](int k) { return rank[k] > prefix || (rank[k] == prefix && at(k) <= last); };
+    uint32_t own[N];  // holes of the thread's 4 rows, and rows times 2^16; first numbered in their wave
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint32_t c = 0, all;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int k = 4 * i + e, j = at(k);
+            const bool s = stays(k);
+            c += j < x.m ? !s : s && j < x.n ? 0x10000u : 0u;
+        }
+        own[i] = lanes_before(c, all);
+        if (lane == 0) sums[i * WV + wv] = all;
+    }
+    __syncthreads();
+    if (wv == 0) {  // (at most 32768 of each: 2^16 holds both)
+        uint32_t carry = 0;
+        for (int i = 0; i < N * WV; i += 64) {
+            const uint32_t y = i + lane < N * WV ? sums[i + lane] : 0;
+            uint32_t all;
+            const uint32_t before = lanes_before(y, all);
+            if (i + lane < N * WV) sums[i + lane] = carry + before;
+            carry += all;
+        }
+        if (lane == 0) a.counts[x.bh] = carry >> 16;
+    }
+    __syncthreads();
+    int* const mv = a.moves + x.bh * a.W * 2;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint32_t no = sums[i * WV + wv] + own[i];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int k = 4 * i + e, j = at(k);
+            const bool s = stays(k);
+            if (j < x.m && !s) mv[2 * (no & 0xFFFF)] = j, no += 1;
+            if (j >= x.m && s && j < x.n) mv[2 * (no >> 16) + 1] = j, no += 0x10000u;
+        }
+    }
+}
+
+// ---- heads of more rows: the same in chunks, a launch for each step that needs all of them ----
+
+constexpr int CHUNK_N = 2, CHUNK = EVICT_T * 4 * CHUNK_N;
+
+// The latest position of every chunk, and the histograms cleared.
+__global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
+    __shared__ int ws[EVICT_T / 64];
+    const int tid = threadIdx.x, c = blockIdx.x;
+    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    if (c == 0 && tid == 0) {
+        if (x.h == 0) a.new_lens[x.b] = x.m;
+        if (!x.over) a.counts[x.bh] = 0;
+    }
+    if (!x.over) return;
+    for (int i = c * EVICT_T + tid; i < 3 * BINS; i += gridDim.x * EVICT_T) a.hist[x.bh * 3 * BINS + i] = 0;
+    int most = INT_MIN;
+#pragma unroll
+    for (int i = 0; i < CHUNK_N; i++) {
+        const int j = c * CHUNK + (i * EVICT_T + tid) * 4;
+        most = max(most, newest_of(load4(a, x, j), x, j));
+    }
+    most = max_all(most, ws);
+    if (tid == 0) a.newest[x.bh * a.chunks + c] = most;
+}
+
+// A chunk's ranks, and the digits of the m-th that the histograms so far give.
+struct Chunk {
+    uint32_t rank[4 * CHUNK_N], prefix;
+    int left, count;
+};
+template <int T>
+__device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int c, int* ws, int* found, Chunk& k) {
+    Four v[CHUNK_N];
+#pragma unroll
+    for (int i = 0; i < CHUNK_N; i++) v[i] = load4(a, x, c * CHUNK + (i * EVICT_T + threadIdx.x) * 4);
+    int most = INT_MIN;
+    for (int i = threadIdx.x; i < (x.n + CHUNK - 1) / CHUNK; i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
+    const long long keep_from = (long long)max_all(most, ws) - a.recent;
+#pragma unroll
+    for (int i = 0; i < CHUNK_N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) k.rank[4 * i + e] = rank4(a, v[i], e, keep_from);
+    k.prefix = 0, k.left = x.m, k.count = 0;
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        __syncthreads();
+        const Cut cut = cut_at(a.hist + (x.bh * 3 + t) * BINS, k.left, ws, found);
+        k.prefix |= (uint32_t)cut.digit << SHIFT[t];
+        k.left = cut.left, k.count = cut.count;
+    }
+}
+__device__ __forceinline__ int chunk_row(int c, int k) { return c * CHUNK + ((k >> 2) * EVICT_T + threadIdx.x) * 4 + (k & 3); }
+
+// The histogram of digit T, of all chunks.  (Whole numbers: their sum has no order.)
+template <int T>
+__global__ __launch_bounds__(EVICT_T) void k_evict_digit(EvictArgs a) {
+    __shared__ int hist[BINS], ws[EVICT_T / 64], found[3];
+    const int tid = threadIdx.x, c = blockIdx.x;
+    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    if (!x.over || (long long)c * CHUNK >= x.n) return;
+    for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
+    Chunk k;
+    chunk_of<T>(a, x, c, ws, found, k);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4 * CHUNK_N; i++)
+        if (chunk_row(c, i) < x.n && (T == 0 || k.rank[i] >> SHIFT[T ? T - 1 : 0] == k.prefix >> SHIFT[T ? T - 1 : 0]))
+            atomicAdd(&hist[digit(k.rank[i], SHIFT[T])], 1);
+    __syncthreads();
+    for (int i = tid; i < BINS; i += EVICT_T)
+        if (hist[i]) atomicAdd(&a.hist[(x.bh * 3 + T) * BINS + i], hist[i]);
+}
+
+// How many rows of each chunk have the m-th rank, and how many are above it, on either side of m.
+__global__ __launch_bounds__(EVICT_T) void k_evict_count(EvictArgs a) {
+    __shared__ int ws[EVICT_T / 64], found[3], n[4];
+    const int tid = threadIdx.x, c = blockIdx.x;
+    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    if (!x.over || (long long)c * CHUNK >= x.n) return;
+    if (tid < 4) n[tid] = 0;
+    Chunk k;
+    chunk_of<3>(a, x, c, ws, found, k);
+    uint32_t below = 0, from = 0;  // ties, and rows above times 2^16
+#pragma unroll
+    for (int i = 0; i < 4 * CHUNK_N; i++) {
+        const int j = chunk_row(c, i);
+        const uint32_t w = j >= x.n ? 0u : k.rank[i] == k.prefix ? 1u : k.rank[i] > k.prefix ? 0x10000u : 0u;
+        if (j < x.m) below += w;
+        else from += w;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) below += __shfl_xor(below, o), from += __shfl_xor(from, o);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+        atomicAdd(&n[0], (int)(below & 0xFFFF));
+        atomicAdd(&n[1], (int)(below >> 16));
+        atomicAdd(&n[2], (int)(from & 0xFFFF));
+        atomicAdd(&n[3], (int)(from >> 16));
+    }
+    __syncthreads();
+    if (tid < 4) a.parts[(x.bh * a.chunks + c) * 4 + tid] = n[tid];
+}
+
+// Each chunk's moves, numbered behind those of the chunks before it.
+__global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
+    __shared__ int ws[EVICT_T / 64], found[3];
+    __shared__ int before[3];  // ties, holes and rows of the chunks before
+    const int tid = threadIdx.x, c = blockIdx.x;
+    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    if (!x.over || (long long)c * CHUNK >= x.n) return;
+    Chunk k;
+    chunk_of<3>(a, x, c, ws, found, k);
+    if (tid < 64) {  // 64 chunks at a time: their ties from the first on stay until `left` are used up
+        int ties = 0, holes = 0, rows = 0;
+        for (int i0 = 0; i0 < c; i0 += 64) {
+            const int i = i0 + tid;
+            i32x4 n = {0, 0, 0, 0};
+            if (i < c) n = *reinterpret_cast<const i32x4*>(a.parts + (x.bh * a.chunks + i) * 4);
+            int to = n[0] + n[2];
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(to, o);
+                if (tid >= o) to += y;
+            }
+            const int first = ties + to - n[0] - n[2];
+            const int kept0 = min(max(k.left - first, 0), n[0]), kept1 = min(max(k.left - first - n[0], 0), n[2]);
+            int h = i < c ? max(0, min(CHUNK, x.m - i * CHUNK)) - n[1] - kept0 : 0, r = n[3] + kept1;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) h += __shfl_xor(h, o), r += __shfl_xor(r, o);
+            holes += h, rows += r;
+            ties += __shfl(to, 63);
+        }
+        if (tid == 0) before[0] = ties, before[1] = holes, before[2] = rows;
+    }
+    __syncthreads();
+    int ties = before[0], holes = before[1], rows = before[2];
+    int* const mv = a.moves + x.bh * a.W * 2;
+#pragma unroll
+    for (int i = 0; i < CHUNK_N; i++) {
+        int t = 0, total;
+#pragma unroll
+        for (int e = 0; e < 4; e++) t += chunk_row(c, 4 * i + e) < x.n && k.rank[4 * i + e] == k.prefix;
+        int nth = ties + scan(t, ws, total);
         ties += total;
-        const bool stays = j < n && (r > prefix || (tie && nth < left));
-        const bool hole = j < m && !stays, row = j >= m && stays;
-        const int x = holes + scan((int)hole, ws, total);
-        holes += total;
-        const int y = rows + scan((int)row, ws, total);
-        rows += total;
-        if (hole) mv[2 * x] = j;
-        if (row) mv[2 * y + 1] = j;
+        bool hole[4], row[4];
+        int mine = 0;  // holes, and rows times 2^16
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int j = chunk_row(c, 4 * i + e);
+            const uint32_t r = k.rank[4 * i + e];
+            const bool stays = j < x.n && (r > k.prefix || (r == k.prefix && nth < k.left));
+            nth += j < x.n && r == k.prefix;
+            hole[e] = j < x.m && !stays, row[e] = j >= x.m && stays;
+            mine += hole[e] + (row[e] ? 0x10000 : 0);
+        }
+        const int no = scan(mine, ws, total);
+        int h = holes + (no & 0xFFFF), r = rows + (no >> 16);
+        holes += total & 0xFFFF, rows += total >> 16;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (hole[e]) mv[2 * h++] = chunk_row(c, 4 * i + e);
+            if (row[e]) mv[2 * r++ + 1] = chunk_row(c, 4 * i + e);
+        }
     }
-    if (tid == 0) counts[(size_t)b * HK + h] = rows;
+    if (tid == 0 && (long long)(c + 1) * CHUNK >= x.n) a.counts[x.bh] = rows;
 }
 
 // ---- their pages ----------------------------------------------------------------------------------------------------
@@ -831,37 +1138,69 @@ __global__ __launch_bounds__(RELEASE_T) void k_page_release(const int* __restric
 }
 
 // ---- their moves ----------------------------------------------------------------------------------------------------
+//
+// Sources lie behind all places that are written, so moves run in any order.  Bound by bytes; K's rows are pieces of 64
+// bytes, but a row of V is one element of each of HD runs of 32 rows.  Moves ascend on both sides, so 32 of them in a row
+// touch a few blocks only: lane l takes move l % 32, and a wave's load of one dim, or its store, falls into one or two
+// runs.
+constexpr int MOVES = 32;  // that a workgroup does at a time
 
-// Sources lie behind all places that are written, so moves run in any order.  A workgroup takes every gridDim.x-th move of
-// a (request, kv head): 256 threads, HD elements of K and of V.
 template <int HD>
 __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ moves, const int* __restrict__ counts,
                                                     const int* __restrict__ table, int max_blocks, int W, int HK, int lps,
                                                     int n_pages, size_t pstride, uint16_t* Kp, uint16_t* Vp, float* scores,
                                                     int* kpos) {
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    __shared__ size_t off[2][MOVES];  // of a move's place and row: their blocks, in a cache
+    __shared__ int row[2][MOVES];     // and the rows there; -1: no move
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, l = tid % MOVES;
     const size_t bh = (size_t)b * HK + h;
     const int n = min(counts[bh], W);
     const int* const mv = moves + bh * W * 2;
     const int* const tb = table + (size_t)b * max_blocks;
     const long long rows = (long long)max_blocks << lps;
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
-        const int to = mv[2 * i], from = mv[2 * i + 1];
-        if (to < 0 || from < 0 || to >= rows || from >= rows) continue;
-        const int pt = tb[to >> lps], pf = tb[from >> lps];
-        if ((unsigned)pt >= (unsigned)n_pages || (unsigned)pf >= (unsigned)n_pages) continue;
-        auto block = [&](int page, int j) {
-            return (size_t)page * pstride + ((size_t)(h << (lps - 5)) + ((j & ((1 << lps) - 1)) >> 5)) * (HD * 32);
-        };
-        const size_t x = block(pt, to), y = block(pf, from);
-        for (int d = tid; d < HD; d += 256) {
-            Kp[x + d / 32 * 1024 + (to & 31) * 32 + d % 32] = Kp[y + d / 32 * 1024 + (from & 31) * 32 + d % 32];
-            Vp[x + d * 32 + (to & 31)] = Vp[y + d * 32 + (from & 31)];
+    for (int i0 = blockIdx.x * MOVES; i0 < n; i0 += gridDim.x * MOVES) {
+        __syncthreads();
+        if (tid < 2 * MOVES) {  // (the first wave: lane l has move l's place, lane 32 + l its row)
+            const int side = tid / MOVES, j = i0 + l < n ? mv[2 * (i0 + l) + side] : -1;
+            const bool in = j >= 0 && j < rows;
+            const int page = in ? tb[j >> lps] : -1;
+            const bool there = (unsigned)page < (unsigned)n_pages;
+            const int other = __shfl_xor((int)there, MOVES);  // (all lanes: not behind a branch)
+            const bool both = there && other;
+            off[side][l] = (size_t)(there ? page : 0) * pstride + ((size_t)(h << (lps - 5)) + ((j & ((1 << lps) - 1)) >> 5)) * (HD * 32);
+            row[side][l] = both ? j & 31 : -1;
+            const size_t at = mark_at(there ? page : 0, HK, h, j, lps);
+            const size_t to = __shfl(at, l);
+            if (side && both) {
+                if (scores) scores[to] = scores[at];
+                if (kpos) kpos[to] = kpos[at];
+            }
         }
-        if (tid == 0) {
-            const size_t u = mark_at(pt, HK, h, to, lps), v = mark_at(pf, HK, h, from, lps);
-            if (scores) scores[u] = scores[v];
-            if (kpos) kpos[u] = kpos[v];
+        __syncthreads();
+        constexpr int P = HD / 8, KN = MOVES * P / 256;  // 16-byte pieces of a row of K; those of a thread
+        u32x4 k[KN];
+#pragma unroll
+        for (int x = 0; x < KN; x++) {
+            const int i = (tid + 256 * x) / P, p = (tid + 256 * x) % P;
+            if (row[1][i] >= 0) k[x] = *reinterpret_cast<const u32x4*>(Kp + off[1][i] + (p >> 2) * 1024 + row[1][i] * 32 + (p & 3) * 8);
+        }
+        constexpr int VN = HD / 8;  // dims of a thread
+        uint16_t v[VN];
+        const bool mine = row[0][l] >= 0;
+        const uint16_t* const from = Vp + off[1][l] + row[1][l] + tid / MOVES * 32;
+        uint16_t* const to = Vp + off[0][l] + row[0][l] + tid / MOVES * 32;
+        if (mine) {
+#pragma unroll
+            for (int x = 0; x < VN; x++) v[x] = from[x * 256];
+        }
+#pragma unroll
+        for (int x = 0; x < KN; x++) {
+            const int i = (tid + 256 * x) / P, p = (tid + 256 * x) % P;
+            if (row[0][i] >= 0) *reinterpret_cast<u32x4*>(Kp + off[0][i] + (p >> 2) * 1024 + row[0][i] * 32 + (p & 3) * 8) = k[x];
+        }
+        if (mine) {
+#pragma unroll
+            for (int x = 0; x < VN; x++) to[x * 256] = v[x];
         }
     }
 }
@@ -937,7 +1276,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     };
     if (p.tiles) {
         launch(k_weights_rows<T, HD>, dim3(p.tiles * s.HK * p.ks), 256, Q, K, g);
-        if (p.ks > 1) launch(k_weights_join, dim3(p.tiles * s.HK), ROW_TILE, g);
+        if (p.ks > 1) launch(k_weights_join, dim3(p.tiles * s.HK * (ROW_TILE / 32)), 256, g);
         launch(k_weights_keys<T, HD>, dim3(p.units * s.HK), 256, Q, K, g);
         if (p.parts > 1) {
             const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
@@ -969,12 +1308,54 @@ void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     by_type(s, [&](auto t, auto hd) { weights_as<decltype(t), decltype(hd)::value>(s, a, st); });
 }
 
-size_t page_evict_ws(int, int, int) { return 0; }
+namespace {
+struct EvictWs {
+    size_t chunks = 0, newest = 0, hist = 0, parts = 0;  // ints
+};
+EvictWs evict_ws(int B, int max_kv, int HK) {
+    EvictWs w;
+    if (max_kv <= EVICT_ONE) return w;
+    const size_t heads = (size_t)B * HK;
+    w.chunks = ((size_t)max_kv + CHUNK - 1) / CHUNK;
+    w.newest = (heads * w.chunks + 3) & ~size_t(3);
+    w.hist = heads * 3 * BINS;
+    w.parts = heads * w.chunks * 4;
+    return w;
+}
+}  // namespace
+
+size_t page_evict_ws(int B, int max_kv, int HK) {
+    const EvictWs w = evict_ws(B, max_kv, HK);
+    return (w.newest + w.hist + w.parts) * 4;
+}
 
 void page_evict(const PageEvict& a, hipStream_t st) {
-    hipLaunchKernelGGL(k_page_evict, dim3(a.HK, a.B), dim3(EVICT_T), 0, st, a.scores, a.kpos, a.table, a.max_blocks, a.kv_lens,
-                       a.budgets, a.max_kv, a.HK, log2i(a.PS), a.n_pages, a.sink, a.recent, a.new_lens, a.moves, a.counts);
-    launched("page_evict");
+    const EvictWs w = evict_ws(a.B, a.max_kv, a.HK);
+    EvictArgs g{a.scores, a.kpos, a.table, a.kv_lens, a.budgets, a.max_blocks, a.B, a.max_kv, a.HK, log2i(a.PS), a.n_pages,
+                a.sink, a.recent, std::max(a.max_kv / 2, 1), a.new_lens, a.moves, a.counts, (int)w.chunks};
+    auto launch = [&](auto kernel, dim3 grid) {
+        hipLaunchKernelGGL(kernel, grid, dim3(EVICT_T), 0, st, g);
+        launched("page_evict");
+    };
+    if (!w.chunks) {
+        const dim3 grid(a.HK, a.B);
+        if (a.max_kv <= 4096) launch(k_page_evict<1>, grid);
+        else if (a.max_kv <= 8192) launch(k_page_evict<2>, grid);
+        else if (a.max_kv <= 16384) launch(k_page_evict<4>, grid);
+        else launch(k_page_evict<8>, grid);
+        return;
+    }
+    if (w.chunks * a.HK * a.B >= size_t(1) << 24) throw Error("sd_op_page_evict: too many rows for one launch");
+    g.newest = static_cast<int*>(a.ws);
+    g.hist = g.newest + w.newest;
+    g.parts = g.hist + w.hist;
+    const dim3 grid((unsigned)w.chunks, a.HK, a.B);
+    launch(k_evict_newest, grid);
+    launch(k_evict_digit<0>, grid);
+    launch(k_evict_digit<1>, grid);
+    launch(k_evict_digit<2>, grid);
+    launch(k_evict_count, grid);
+    launch(k_evict_moves, grid);
 }
 
 void page_release(const PageRelease& a, hipStream_t st) {
@@ -986,7 +1367,7 @@ void page_release(const PageRelease& a, hipStream_t st) {
 void paged_move(const PagedShape& s, const PagedMove& a, hipStream_t st) {
     const int W = std::max(a.max_kv / 2, 1);
     auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(std::min(W, std::max(1, 4096 / (s.HK * a.B))), s.HK, a.B), dim3(256), 0, st, a.moves,
+        hipLaunchKernelGGL(kernel, dim3(std::min((W + MOVES - 1) / MOVES, std::max(1, 2048 / (s.HK * a.B))), s.HK, a.B), dim3(256), 0, st, a.moves,
                            a.counts, a.table, a.max_blocks, W, s.HK, log2i(s.PS), s.n_pages, s.pstride,
                            static_cast<uint16_t*>(a.Kp), static_cast<uint16_t*>(a.Vp), a.scores, a.kpos);
     };
