@@ -678,22 +678,33 @@ __device__ __forceinline__ uint32_t rank_of(float s) {
 constexpr int EVICT_T = 1024, BINS = 2048;
 constexpr int EVICT_ONE = 32768;  // rows up to which one workgroup does a head
 
-// The sum over the threads before this one, and over all; `ws` holds EVICT_T / 64 counts.
-template <class I>
-__device__ __forceinline__ I scan(I x, I* ws, I& total) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    I v = x;
+// The sum over lanes 0 to the own, by moves between lanes: within rows of 16, then from each row's last lane on.
+__device__ __forceinline__ int lanes_upto(int x) {
+    auto add = [&](auto ctrl, auto rows) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // 1 lane up in each row
+    add(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());  // 2
+    add(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());  // 4
+    add(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());  // 8
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());  // rows 0 and 2 into 1 and 3
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());  // the lower half into the upper
+    return x;
+}
+
+// The sum over the threads before this one, and over all; `ws` holds EVICT_T / 64 sums.
+__device__ __forceinline__ int scan(int x, int* ws, int& total) {
+    const int wv = threadIdx.x >> 6, v = lanes_upto(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) ws[wv] = v;
+    __syncthreads();
+    int before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const I y = __shfl_up(v, o);
-        if (lane >= o) v += y;
+    for (int w = 0; w < EVICT_T / 64; w++) {
+        const int y = ws[w];
+        before += w < wv ? y : 0, all += y;
     }
-    __syncthreads();
-    if (lane == 63) ws[wv] = v;
-    __syncthreads();
-    I before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < EVICT_T / 64; w++) before += w < wv ? ws[w] : 0, all += ws[w];
     total = all;
     return before + v - x;
 }
@@ -707,6 +718,7 @@ struct EvictArgs {
     int chunks;
     int* newest;  // [B][HK][chunks]
     int* hist;    // [B][HK][3][BINS]
+    int* cuts;    // [B][HK][2][4]: the first two digits' cuts, as found by the launch after theirs
     int* parts;   // [B][HK][chunks][4]: rows of the m-th rank and above it, below m and from m on
 };
 
@@ -761,9 +773,17 @@ __device__ __forceinline__ uint32_t rank4(const EvictArgs& a, const Four& v, int
 }
 
 __device__ __forceinline__ int max_all(int x, int* ws) {  // over the workgroup
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o));
-    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = x;
+    auto take = [&](auto ctrl, auto rows) {
+        x = max(x, __builtin_amdgcn_update_dpp(x, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    };
+    using std::integral_constant;
+    take(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // as in lanes_upto
+    take(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());
+    take(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
+    take(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
+    take(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());
+    take(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());
+    if ((threadIdx.x & 63) == 63) ws[threadIdx.x >> 6] = x;
     __syncthreads();
     int r = ws[0];
 #pragma unroll
@@ -795,27 +815,13 @@ __device__ __forceinline__ Cut cut_at(const int* hist, int left, int* ws, int* f
     return {found[0], found[1], found[2]};
 }
 
-// The numbers of a chunk's holes and rows (bits 0 and 1 of what[e], 4 rows a thread) behind those of the chunks before:
-// each wave's packed counts, then a scan over the lanes.
-__device__ __forceinline__ uint32_t lanes_before(uint32_t x, uint32_t& all) {  // (packed sums over a wave)
-    const int lane = threadIdx.x & 63;
-    uint32_t v = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(v, o);
-        if (lane >= o) v += y;
-    }
-    all = __shfl(v, 63);
-    return v - x;
-}
-
 // One workgroup per (request, kv head), N times 4 rows a thread.
 template <int N>
 __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
     constexpr int WV = EVICT_T / 64;
     __shared__ int hist[BINS], ws[WV], found[3];
-    __shared__ uint32_t sums[N * WV + 1];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    __shared__ uint32_t sums[N * WV];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Head x = head_of(a, blockIdx.x, blockIdx.y);
     if (x.h == 0 && tid == 0) a.new_lens[x.b] = x.m;
     if (!x.over) {
@@ -838,6 +844,7 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
             for (int e = 0; e < 4; e++) rank[4 * i + e] = rank4(a, v[i], e, keep_from);
     }
     auto at = [&](int k) { return ((k >> 2) * EVICT_T + tid) * 4 + (k & 3); };  // the row of rank[k]
+    auto any = [&](int i) { return (i * EVICT_T + 64 * wv) * 4 < x.n; };        // the wave has some of rank[4 i ..]
     uint32_t prefix = 0;
     int left = x.m, count = 0;
 #pragma unroll
@@ -849,8 +856,12 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
             __syncthreads();
         }
 #pragma unroll
-        for (int k = 0; k < 4 * N; k++)
-            if (at(k) < x.n && (t == 0 || rank[k] >> above == prefix >> above)) atomicAdd(&hist[digit(rank[k], shift)], 1);
+        for (int i = 0; i < N; i++) {
+            if (!any(i)) break;
+#pragma unroll
+            for (int k = 4 * i; k < 4 * i + 4; k++)
+                if (at(k) < x.n && (t == 0 || rank[k] >> above == prefix >> above)) atomicAdd(&hist[digit(rank[k], shift)], 1);
+        }
         __syncthreads();
         const Cut c = cut_at(hist, left, ws, found);
         prefix |= (uint32_t)c.digit << shift;
@@ -880,25 +891,26 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
     uint32_t own[N];  // holes of the thread's 4 rows, and rows times 2^16; first numbered in their wave
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        uint32_t c = 0, all;
+        uint32_t c = 0;
+        if (any(i)) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int k = 4 * i + e, j = at(k);
-            const bool s = stays(k);
-            c += j < x.m ? !s : s && j < x.n ? 0x10000u : 0u;
+            for (int e = 0; e < 4; e++) {
+                const int k = 4 * i + e, j = at(k);
+                const bool s = stays(k);
+                c += j < x.m ? !s : s && j < x.n ? 0x10000u : 0u;
+            }
         }
-        own[i] = lanes_before(c, all);
-        if (lane == 0) sums[i * WV + wv] = all;
+        const uint32_t to = lanes_upto(c);
+        own[i] = to - c;
+        if (lane == 63) sums[i * WV + wv] = to;
     }
     __syncthreads();
     if (wv == 0) {  // (at most 32768 of each: 2^16 holds both)
         uint32_t carry = 0;
         for (int i = 0; i < N * WV; i += 64) {
-            const uint32_t y = i + lane < N * WV ? sums[i + lane] : 0;
-            uint32_t all;
-            const uint32_t before = lanes_before(y, all);
-            if (i + lane < N * WV) sums[i + lane] = carry + before;
-            carry += all;
+            const uint32_t y = i + lane < N * WV ? sums[i + lane] : 0, to = lanes_upto(y);
+            if (i + lane < N * WV) sums[i + lane] = carry + to - y;
+            carry += __builtin_amdgcn_readlane(to, 63);
         }
         if (lane == 0) a.counts[x.bh] = carry >> 16;
     }
@@ -906,6 +918,7 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
     int* const mv = a.moves + x.bh * a.W * 2;
 #pragma unroll
     for (int i = 0; i < N; i++) {
+        if (!any(i)) break;
         uint32_t no = sums[i * WV + wv] + own[i];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -960,10 +973,18 @@ __device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int 
 #pragma unroll
         for (int e = 0; e < 4; e++) k.rank[4 * i + e] = rank4(a, v[i], e, keep_from);
     k.prefix = 0, k.left = x.m, k.count = 0;
+    // (the cut before the last is in memory since the last launch)
 #pragma unroll
     for (int t = 0; t < T; t++) {
-        __syncthreads();
-        const Cut cut = cut_at(a.hist + (x.bh * 3 + t) * BINS, k.left, ws, found);
+        Cut cut;
+        int* const kept = a.cuts + (x.bh * 2 + t) * 4;
+        if (t + 1 < T) {
+            cut = {kept[0], kept[1], kept[2]};
+        } else {
+            __syncthreads();
+            cut = cut_at(a.hist + (x.bh * 3 + t) * BINS, k.left, ws, found);
+            if (t < 2 && c == 0 && threadIdx.x == 0) kept[0] = cut.digit, kept[1] = cut.left, kept[2] = cut.count;
+        }
         k.prefix |= (uint32_t)cut.digit << SHIFT[t];
         k.left = cut.left, k.count = cut.count;
     }
@@ -1035,12 +1056,7 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
             const int i = i0 + tid;
             i32x4 n = {0, 0, 0, 0};
             if (i < c) n = *reinterpret_cast<const i32x4*>(a.parts + (x.bh * a.chunks + i) * 4);
-            int to = n[0] + n[2];
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(to, o);
-                if (tid >= o) to += y;
-            }
+            const int to = lanes_upto(n[0] + n[2]);
             const int first = ties + to - n[0] - n[2];
             const int kept0 = min(max(k.left - first, 0), n[0]), kept1 = min(max(k.left - first - n[0], 0), n[2]);
             int h = i < c ? max(0, min(CHUNK, x.m - i * CHUNK)) - n[1] - kept0 : 0, r = n[3] + kept1;
@@ -1087,6 +1103,24 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
 // ---- their pages ----------------------------------------------------------------------------------------------------
 
 constexpr int RELEASE_T = 1024;
+
+__device__ __forceinline__ long long scan(long long x, long long* ws, long long& total) {  // as above
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    long long v = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long y = __shfl_up(v, o);
+        if (lane >= o) v += y;
+    }
+    __syncthreads();
+    if (lane == 63) ws[wv] = v;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < RELEASE_T / 64; w++) before += w < wv ? ws[w] : 0, all += ws[w];
+    total = all;
+    return before + v - x;
+}
 
 // One workgroup: the requests' pages that go numbered through by a scan over the requests, then pushed in that order, a
 // round of 1024 entries at a time, those out of range left out.
@@ -1310,7 +1344,7 @@ void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
 
 namespace {
 struct EvictWs {
-    size_t chunks = 0, newest = 0, hist = 0, parts = 0;  // ints
+    size_t chunks = 0, newest = 0, hist = 0, cuts = 0, parts = 0;  // ints
 };
 EvictWs evict_ws(int B, int max_kv, int HK) {
     EvictWs w;
@@ -1319,6 +1353,7 @@ EvictWs evict_ws(int B, int max_kv, int HK) {
     w.chunks = ((size_t)max_kv + CHUNK - 1) / CHUNK;
     w.newest = (heads * w.chunks + 3) & ~size_t(3);
     w.hist = heads * 3 * BINS;
+    w.cuts = heads * 8;
     w.parts = heads * w.chunks * 4;
     return w;
 }
@@ -1326,7 +1361,7 @@ EvictWs evict_ws(int B, int max_kv, int HK) {
 
 size_t page_evict_ws(int B, int max_kv, int HK) {
     const EvictWs w = evict_ws(B, max_kv, HK);
-    return (w.newest + w.hist + w.parts) * 4;
+    return (w.newest + w.hist + w.cuts + w.parts) * 4;
 }
 
 void page_evict(const PageEvict& a, hipStream_t st) {
@@ -1348,7 +1383,8 @@ void page_evict(const PageEvict& a, hipStream_t st) {
     if (w.chunks * a.HK * a.B >= size_t(1) << 24) throw Error("sd_op_page_evict: too many rows for one launch");
     g.newest = static_cast<int*>(a.ws);
     g.hist = g.newest + w.newest;
-    g.parts = g.hist + w.hist;
+    g.cuts = g.hist + w.hist;
+    g.parts = g.cuts + w.cuts;
     const dim3 grid((unsigned)w.chunks, a.HK, a.B);
     launch(k_evict_newest, grid);
     launch(k_evict_digit<0>, grid);
