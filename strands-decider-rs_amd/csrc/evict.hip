@@ -732,28 +732,31 @@ struct Head {
 __device__ __forceinline__ Head head_of(const EvictArgs& a, int h, int b) {
     Head x;
     x.b = b, x.h = h;
-    x.n = a.kv_lens[b];
-    const int budget = a.budgets[b];
-    x.over = x.n <= a.max_kv && budget >= 0 && x.n > budget;
-    x.m = x.over ? budget : x.n;
     x.tb = a.table + (size_t)b * a.max_blocks;
     x.bh = (size_t)b * a.HK + h;
     return x;
+}
+__device__ __forceinline__ void lengths(const EvictArgs& a, Head& x) {
+    x.n = a.kv_lens[x.b];
+    const int budget = a.budgets[x.b];
+    x.over = x.n <= a.max_kv && budget >= 0 && x.n > budget;
+    x.m = x.over ? budget : x.n;
 }
 
 typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// 4 rows from j on (a multiple of 4: they lie on end), as loaded.
+// 4 rows from j on (a multiple of 4: they lie on end), as loaded.  Their page comes first, whatever the request's length:
+// the two loads of the lengths and of the table are then on their way together.
 struct Four {
     f32x4u s;
     i32x4 p;
     bool there;
 };
-__device__ __forceinline__ Four load4(const EvictArgs& a, const Head& x, int j) {
+__device__ __forceinline__ int page_of(const EvictArgs& a, const Head& x, int j) { return x.tb[min(j >> a.lps, a.max_blocks - 1)]; }
+__device__ __forceinline__ Four load4(const EvictArgs& a, const Head& x, int j, int page) {
     Four r;
-    const int page = j < x.n ? x.tb[j >> a.lps] : -1;
-    r.there = (unsigned)page < (unsigned)a.n_pages;
+    r.there = j < x.n && (unsigned)page < (unsigned)a.n_pages;
     const size_t at = mark_at(r.there ? page : 0, a.HK, x.h, r.there ? j : 0, a.lps);
     r.s = *reinterpret_cast<const f32x4u*>(a.scores + at);
     if (a.kpos) r.p = *reinterpret_cast<const i32x4*>(a.kpos + at);
@@ -796,15 +799,21 @@ constexpr int SHIFT[3] = {21, 10, 0};
 __device__ __forceinline__ int digit(uint32_t r, int shift) { return r >> shift & (shift ? BINS - 1 : 1023); }
 
 // Of a histogram's rows the `left` of the largest digits stay: the digit of the last of them, `left` less those above it,
-// and how many have it.  Two bins a thread; all threads get the answer.  (left 0: the largest digit, of which none stays)
+// and how many have it.  Two bins a thread; all threads get the answer, behind a barrier since the histogram and since
+// ws were used.  (left 0: the largest digit, of which none stays)
 struct Cut {
     int digit, left, count;
 };
 __device__ __forceinline__ Cut cut_at(const int* hist, int left, int* ws, int* found) {
     const int tid = threadIdx.x, d1 = BINS - 1 - 2 * tid, d0 = d1 - 1;  // (from the largest digit down)
     const int c1 = hist[d1], c0 = hist[d0];
-    int total;
-    const int before = scan(c1 + c0, ws, total);
+    // (a scan as above, its first barrier done: the histogram's)
+    const int wv = tid >> 6, to = lanes_upto(c1 + c0);
+    if ((tid & 63) == 63) ws[wv] = to;
+    __syncthreads();
+    int before = to - c1 - c0;
+#pragma unroll
+    for (int w = 0; w < EVICT_T / 64; w++) before += w < wv ? ws[w] : 0;
     if (left == 0 ? tid == 0 : before < left && left <= before + c1 + c0) {
         const bool first = left == 0 || left <= before + c1;
         found[0] = first ? d1 : d0;
@@ -815,14 +824,21 @@ __device__ __forceinline__ Cut cut_at(const int* hist, int left, int* ws, int* f
     return {found[0], found[1], found[2]};
 }
 
-// One workgroup per (request, kv head), N times 4 rows a thread.
+// One workgroup per (request, kv head), N times 4 rows a thread.  Where a digit leaves up to CANDIDATES rows, each of them
+// counts those before it, and the m-th is found at once.
+constexpr int CANDIDATES = 512;
 template <int N>
-__global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
+__global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArgs a) {  // (two to a CU, where registers allow)
     constexpr int WV = EVICT_T / 64;
-    __shared__ int hist[BINS], ws[WV], found[3];
-    __shared__ uint32_t sums[N * WV];
+    __shared__ int hist[BINS], ws[WV], found[3], at_last;
+    __shared__ uint32_t sums[N * WV], rank_last;
+    __shared__ __align__(16) unsigned long long cand[CANDIDATES];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Head x = head_of(a, blockIdx.x, blockIdx.y);
+    Head x = head_of(a, blockIdx.x, blockIdx.y);
+    int page[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) page[i] = page_of(a, x, (i * EVICT_T + tid) * 4);
+    lengths(a, x);
     if (x.h == 0 && tid == 0) a.new_lens[x.b] = x.m;
     if (!x.over) {
         if (tid == 0) a.counts[x.bh] = 0;
@@ -832,7 +848,7 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
     {
         Four v[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = load4(a, x, (i * EVICT_T + tid) * 4);
+        for (int i = 0; i < N; i++) v[i] = load4(a, x, (i * EVICT_T + tid) * 4, page[i]);
         for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
         int most = INT_MIN;
 #pragma unroll
@@ -845,11 +861,14 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
     }
     auto at = [&](int k) { return ((k >> 2) * EVICT_T + tid) * 4 + (k & 3); };  // the row of rank[k]
     auto any = [&](int i) { return (i * EVICT_T + 64 * wv) * 4 < x.n; };        // the wave has some of rank[4 i ..]
+    // Rows above `prefix` stay, and those up to `last` that have it.
     uint32_t prefix = 0;
-    int left = x.m, count = 0;
+    int left = x.m, count = 0, last = INT_MAX;
+    bool done = false;
 #pragma unroll
     for (int t = 0; t < 3; t++) {
         const int shift = SHIFT[t], above = t ? SHIFT[t - 1] : 0;
+        if (done) break;
         if (t) {
             __syncthreads();
             for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
@@ -862,14 +881,37 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
             for (int k = 4 * i; k < 4 * i + 4; k++)
                 if (at(k) < x.n && (t == 0 || rank[k] >> above == prefix >> above)) atomicAdd(&hist[digit(rank[k], shift)], 1);
         }
+        if (tid == 0) at_last = 0;
         __syncthreads();
         const Cut c = cut_at(hist, left, ws, found);
         prefix |= (uint32_t)c.digit << shift;
         left = c.left, count = c.count;
+        if (left == count) {  // all of them (none where m is 0: nothing has the last digit of all)
+            done = true;
+            if (left == 0) last = -1;
+        } else if (left && count <= CANDIDATES) {
+            done = true;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (!any(i)) break;
+#pragma unroll
+                for (int k = 4 * i; k < 4 * i + 4; k++)
+                    if (at(k) < x.n && rank[k] >> shift == prefix >> shift)
+                        cand[atomicAdd(&at_last, 1)] = (unsigned long long)rank[k] << 32 | ~(uint32_t)at(k);
+            }
+            __syncthreads();
+            if (tid < count) {
+                const unsigned long long own = cand[tid];
+                int before = 0;
+#pragma unroll 8
+                for (int i = 0; i < count; i++) before += cand[i] > own;
+                if (before == left - 1) rank_last = (uint32_t)(own >> 32), found[0] = (int)~(uint32_t)own;
+            }
+            __syncthreads();
+            prefix = rank_last, last = found[0];
+        }
     }
-    // Rows above `prefix` stay, and the first `left` of the `count` that have it.
-    int last = INT_MAX;  // the row of the last of those
-    if (left < count || left == 0) {
+    if (!done) {  // the first `left` of the rows that have the m-th rank
         __syncthreads();
         if (tid == 0) found[0] = -1;
         int before = 0;
@@ -885,7 +927,7 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
             before += total;
         }
         __syncthreads();
-        last = found[0];  // (-1: none stays)
+        last = found[0];
     }
     auto stays = [&](int k) { return rank[k] > prefix || (rank[k] == prefix && at(k) <= last); };
     uint32_t own[N];  // holes of the thread's 4 rows, and rows times 2^16; first numbered in their wave
@@ -934,11 +976,19 @@ __global__ __launch_bounds__(EVICT_T) void k_page_evict(EvictArgs a) {
 
 constexpr int CHUNK_N = 2, CHUNK = EVICT_T * 4 * CHUNK_N;
 
+__device__ __forceinline__ void chunk_pages(const EvictArgs& a, const Head& x, int c, int (&page)[CHUNK_N]) {
+#pragma unroll
+    for (int i = 0; i < CHUNK_N; i++) page[i] = page_of(a, x, c * CHUNK + (i * EVICT_T + threadIdx.x) * 4);
+}
+
 // The latest position of every chunk, and the histograms cleared.
 __global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64];
     const int tid = threadIdx.x, c = blockIdx.x;
-    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    Head x = head_of(a, blockIdx.y, blockIdx.z);
+    int page[CHUNK_N];
+    chunk_pages(a, x, c, page);
+    lengths(a, x);
     if (c == 0 && tid == 0) {
         if (x.h == 0) a.new_lens[x.b] = x.m;
         if (!x.over) a.counts[x.bh] = 0;
@@ -949,7 +999,7 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
 #pragma unroll
     for (int i = 0; i < CHUNK_N; i++) {
         const int j = c * CHUNK + (i * EVICT_T + tid) * 4;
-        most = max(most, newest_of(load4(a, x, j), x, j));
+        most = max(most, newest_of(load4(a, x, j, page[i]), x, j));
     }
     most = max_all(most, ws);
     if (tid == 0) a.newest[x.bh * a.chunks + c] = most;
@@ -961,10 +1011,11 @@ struct Chunk {
     int left, count;
 };
 template <int T>
-__device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int c, int* ws, int* found, Chunk& k) {
+__device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int c, const int (&page)[CHUNK_N], int* ws, int* found,
+                                         Chunk& k) {
     Four v[CHUNK_N];
 #pragma unroll
-    for (int i = 0; i < CHUNK_N; i++) v[i] = load4(a, x, c * CHUNK + (i * EVICT_T + threadIdx.x) * 4);
+    for (int i = 0; i < CHUNK_N; i++) v[i] = load4(a, x, c * CHUNK + (i * EVICT_T + threadIdx.x) * 4, page[i]);
     int most = INT_MIN;
     for (int i = threadIdx.x; i < (x.n + CHUNK - 1) / CHUNK; i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
     const long long keep_from = (long long)max_all(most, ws) - a.recent;
@@ -996,11 +1047,14 @@ template <int T>
 __global__ __launch_bounds__(EVICT_T) void k_evict_digit(EvictArgs a) {
     __shared__ int hist[BINS], ws[EVICT_T / 64], found[3];
     const int tid = threadIdx.x, c = blockIdx.x;
-    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    Head x = head_of(a, blockIdx.y, blockIdx.z);
+    int page[CHUNK_N];
+    chunk_pages(a, x, c, page);
+    lengths(a, x);
     if (!x.over || (long long)c * CHUNK >= x.n) return;
     for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
     Chunk k;
-    chunk_of<T>(a, x, c, ws, found, k);
+    chunk_of<T>(a, x, c, page, ws, found, k);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4 * CHUNK_N; i++)
@@ -1015,11 +1069,14 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_digit(EvictArgs a) {
 __global__ __launch_bounds__(EVICT_T) void k_evict_count(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64], found[3], n[4];
     const int tid = threadIdx.x, c = blockIdx.x;
-    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    Head x = head_of(a, blockIdx.y, blockIdx.z);
+    int page[CHUNK_N];
+    chunk_pages(a, x, c, page);
+    lengths(a, x);
     if (!x.over || (long long)c * CHUNK >= x.n) return;
     if (tid < 4) n[tid] = 0;
     Chunk k;
-    chunk_of<3>(a, x, c, ws, found, k);
+    chunk_of<3>(a, x, c, page, ws, found, k);
     uint32_t below = 0, from = 0;  // ties, and rows above times 2^16
 #pragma unroll
     for (int i = 0; i < 4 * CHUNK_N; i++) {
@@ -1046,10 +1103,13 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64], found[3];
     __shared__ int before[3];  // ties, holes and rows of the chunks before
     const int tid = threadIdx.x, c = blockIdx.x;
-    const Head x = head_of(a, blockIdx.y, blockIdx.z);
+    Head x = head_of(a, blockIdx.y, blockIdx.z);
+    int page[CHUNK_N];
+    chunk_pages(a, x, c, page);
+    lengths(a, x);
     if (!x.over || (long long)c * CHUNK >= x.n) return;
     Chunk k;
-    chunk_of<3>(a, x, c, ws, found, k);
+    chunk_of<3>(a, x, c, page, ws, found, k);
     if (tid < 64) {  // 64 chunks at a time: their ties from the first on stay until `left` are used up
         int ties = 0, holes = 0, rows = 0;
         for (int i0 = 0; i0 < c; i0 += 64) {
