@@ -8,6 +8,10 @@
 namespace sd {
 namespace {
 
+// 16 bytes of arrays that are aligned to 4.
+typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
 // Index of (page, kv head, row j) in an array [n_pages][HK][PS].
 __device__ __forceinline__ size_t mark_at(int page, int HK, int h, int j, int lps) {
     return ((size_t)page * HK + h) * ((size_t)1 << lps) + (j & ((1 << lps) - 1));
@@ -30,15 +34,15 @@ __device__ __forceinline__ size_t mark_at(int page, int HK, int h, int j, int lp
 // of two rounded products.
 // Sums have one order: over a lane's own keys or rows, then lanes, waves, and parts by their number.
 
-constexpr int ROW_TILE = 128, KEY_TILE = 128;  // of a workgroup of the kernels for many rows
 
 struct WeightArgs {
     const int *table, *cu, *kv_lens, *pos;
     int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, observers;
     int few, few_ks, few_span, rw, kvp;        // rows of a request that the few rows' kernels do; their splits, blocks of 32
                                                // keys in each; rows and keys of a request's scores
-    int tiles, ks, span, part, parts, units;   // many rows: tiles of rows, their splits, blocks in each; rows of a part,
-                                               // parts of a request at most, (key tile, part)s at most
+    int tiles, ks, span;                       // many rows: tiles of rows, their splits, blocks in each;
+    int key_tile, part, parts, units;          // keys of a tile, rows of a part, parts of a request at most, (key tile,
+                                               // part)s at most
     uint32_t magic;  // 2^32 / G and 1 more: x / G is the upper half of a product for x below 2^16
     float c, decay;  // c: scale log2(e)
     size_t pstride;
@@ -48,8 +52,8 @@ struct WeightArgs {
     float* S;         // [B][HK][rw][kvp]: c s of the few rows
     float2* few_ml;   // [B][HK][few_ks][rw]: their maxima and sums
     float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
-    float2* stat;     // [rows][HQ]: of a row's whole, the sum's reciprocal
-    float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
+    float2* stat;     // [rows][HQ], a request's rows kv head by kv head: of a row's whole, the sum's reciprocal
+    float* col;       // [units][HK][key_tile]: parts of the keys' weights
     // the first key that a row at position p sees
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
@@ -74,19 +78,24 @@ __device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= FAR; }
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }  // (its sum is 0, or NaN)
 __device__ __forceinline__ float inverse_of(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
-// A row's whole, from its n parts, `step` apart: 8 lanes on end share it.
+// Where the statistics of a request's rows of kv head kh begin.
+__device__ __forceinline__ size_t stat_at(const WeightArgs& a, const Req& rq, const Seen& ob, int kh) {
+    return (size_t)(rq.q0 + ob.t0) * a.HQ + (size_t)kh * ob.n * a.G;
+}
+
+// A row's whole, from its n parts, `step` apart: N lanes on end share it.
+template <int N>
 __device__ __forceinline__ float2 join_parts(const float2* ml, size_t step, int n) {
-    const int u = threadIdx.x & 7;
     float mx = -INFINITY, l = 0.f;
 #pragma unroll 4
-    for (int z = u; z < n; z += 8) {
+    for (int z = threadIdx.x % N; z < n; z += N) {
         const float2 v = ml[z * step];
         const float mn = fmaxf(mx, v.x);
         l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
         mx = mn;
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < N; o <<= 1) {
         const float m2 = __shfl_xor(mx, o), l2 = __shfl_xor(l, o), mn = fmaxf(mx, m2);
         l = l * part_weight(mx, mn) + l2 * part_weight(m2, mn);
         mx = mn;
@@ -103,7 +112,7 @@ __device__ __forceinline__ void put_weight(const WeightArgs& a, const Req& rq, s
 
 // ---- few rows ----
 
-constexpr int FEW_W = 4;  // waves of a workgroup
+constexpr int FEW_W = 2;  // waves of a workgroup
 
 // Scores of up to 16 NR rows of a (request, kv head) over this workgroup's blocks of keys, and the rows' maxima and sums
 // over them.  A wave loads K straight into registers in MFMA operand order, D blocks of 32 keys in flight.
@@ -243,31 +252,55 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
 // The few rows' weights, from their scores: 4 keys per thread, after every workgroup has joined the rows' parts, 8 threads
 // a row.
 __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
+    constexpr int PRE = 4;
     __shared__ float2 stat[32];
-    const int tid = threadIdx.x, kh = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, kh = blockIdx.x % a.HK, b = blockIdx.y;
+    const int c0 = blockIdx.x / a.HK * 1024, step = gridDim.x / a.HK * 1024;  // (with 8 heads a head's scores stay with one XCD's L2)
     const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
     const Seen ob = observed(rq, a.observers);
     const int nrows = ob.n * a.G;
-    if (nrows == 0 || nrows > a.few || blockIdx.x * 1024 >= (unsigned)rq.kcap) return;
+    if (nrows == 0 || nrows > a.few || c0 >= rq.kcap) return;
     const int p0 = rq.p0 + ob.t0, hi = min(p0 + ob.n, rq.kcap), lo = max(0, a.from(p0));
+    const float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp;
+    const int* const tb = a.table + (size_t)b * a.max_blocks;
+    struct Keys {  // 4 keys: their place, what they have, and the scores of the first PRE rows
+        int page;
+        size_t at;
+        f32x4u old;
+        f32x4 x[PRE];
+    };
+    auto load = [&](int j) INL {
+        Keys k;
+        k.page = tb[min(j >> a.lps, a.max_blocks - 1)];
+        const bool there = j < rq.kcap && (unsigned)k.page < (unsigned)a.n_pages;
+        k.at = mark_at(there ? k.page : 0, a.HK, kh, there ? j : 0, a.lps);
+        k.old = f32x4u{0.f, 0.f, 0.f, 0.f};
+        if (there && a.decay != 0.f) k.old = *reinterpret_cast<const f32x4u*>(a.scores + k.at);
+        const bool seen = j > lo - 4 && j < hi;  // (scores outside were not written)
+#pragma unroll
+        for (int r = 0; r < PRE; r++) {
+            k.x[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (seen && r < nrows) k.x[r] = *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp + j);
+        }
+        return k;
+    };
+    Keys k = load(c0 + 4 * tid);  // (on their way while the rows are joined)
     {
-        const int r = tid >> 3;
-        const float2 st = join_parts(a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw + min(r, nrows - 1), a.rw, a.few_ks);
-        if ((tid & 7) == 0) stat[r] = st;
+        const float2* const ml = a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw;
+        if (nrows <= 4) {
+            const float2 st = join_parts<64>(ml + min(tid >> 6, nrows - 1), a.rw, a.few_ks);
+            if ((tid & 63) == 0) stat[tid >> 6] = st;
+        } else {
+            const float2 st = join_parts<8>(ml + min(tid >> 3, nrows - 1), a.rw, a.few_ks);
+            if ((tid & 7) == 0) stat[tid >> 3] = st;
+        }
     }
     __syncthreads();
-    for (int j0 = blockIdx.x * 1024; j0 < rq.kcap; j0 += gridDim.x * 1024) {
-        const int j = j0 + 4 * tid;
-        if (j >= rq.kcap) return;
-        const int page = a.table[(size_t)b * a.max_blocks + (j >> a.lps)];
-        if ((unsigned)page >= (unsigned)a.n_pages) continue;
-        const float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp + j;
+    auto put = [&](int j, const Keys& now) INL {
         f32x4 w = {0.f, 0.f, 0.f, 0.f};
-        if (j + 4 > lo && j < hi) {  // (scores outside were not written)
+        if (j > lo - 4 && j < hi) {
             int t = 0, g = 0;
-#pragma unroll 4
-            for (int r = 0; r < nrows; r++) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp);
+            auto add = [&](int r, f32x4 x) INL {
                 const float2 st = stat[r];
                 const int jlo = a.from(p0 + t), jhi = min(p0 + t + 1, hi);
 #pragma unroll
@@ -276,16 +309,37 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
                     w[e] += keep ? exp2_fast(x[e] - st.x) * st.y : 0.f;
                 }
                 if (++g == a.G) g = 0, t++;
-            }
-        }
-        const size_t at = mark_at(page, a.HK, kh, j, a.lps);
+            };
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (j + e < rq.kcap) put_weight(a, rq, at + e, j + e, w[e]);
+            for (int r = 0; r < PRE; r++)
+                if (r < nrows) add(r, now.x[r]);
+#pragma unroll 4
+            for (int r = PRE; r < nrows; r++) add(r, *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp + j));
+        }
+        if (j <= min(rq.p0, rq.kcap) - 4) {
+            f32x4u y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = a.decay != 0.f ? __builtin_fmaf(a.decay, now.old[e], w[e]) : w[e];
+            *reinterpret_cast<f32x4u*>(a.out + now.at) = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (j + e < rq.kcap) put_weight(a, rq, now.at + e, j + e, w[e]);
+        }
+    };
+    for (int j0 = c0;; j0 += step) {
+        const int j = j0 + 4 * tid;
+        const Keys now = k;
+        const bool more = step < rq.kcap - j0;
+        if (more) k = load(j + step);
+        if (j < rq.kcap && (unsigned)now.page < (unsigned)a.n_pages) put(j, now);
+        if (!more) break;
     }
 }
 
 // ---- many rows ----
+
+constexpr int ROW_TILE = 128;
 
 __device__ __forceinline__ int many_rows(const WeightArgs& a, int b) {  // of request b, 0 where they are few
     const int n = observed(request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap), a.observers).n * a.G;
@@ -316,40 +370,80 @@ __device__ __forceinline__ RowTile row_tile_of(const WeightArgs& a, const Tile& 
     return t;
 }
 
+// A ring of blocks in LDS, NB of them: block i is in buffer i % NB, and while it is worked on the NB - 1 after it are on their
+// way.  (An array per buffer: the compiler then sees that the DMAs into one never alias the reads of another.)  With 256 dims two
+// are enough, since the CU then has room for four workgroups, which cover each other's waits.
+#define RING(X)                                                                                          \
+    __shared__ __align__(1024) uint8_t X##0[Rg::BYTES], X##1[Rg::BYTES], X##2[NB > 2 ? Rg::BYTES : 16], \
+        X##3[NB > 3 ? Rg::BYTES : 16];
+// turn(i, its buffer, the buffer that block i + NB - 1 goes to) for n blocks.
+#define RING_LOOP(X, n, fetch)                                        \
+    fetch(0, X##0);                                                   \
+    if (NB > 2) fetch(1, X##1);                                       \
+    if (NB > 3) fetch(2, X##2);                                       \
+    for (int i = 0;;) {                                               \
+        turn(i, X##0, NB == 4 ? X##3 : NB == 3 ? X##2 : X##1);        \
+        if (++i >= n) break;                                          \
+        turn(i, X##1, X##0);                                          \
+        if (++i >= n) break;                                          \
+        if (NB > 2) {                                                 \
+            turn(i, X##2, X##1);                                      \
+            if (++i >= n) break;                                      \
+        }                                                             \
+        if (NB > 3) {                                                 \
+            turn(i, X##3, X##2);                                      \
+            if (++i >= n) break;                                      \
+        }                                                             \
+    }
+
 // Blocks of 32 rows x HD of a ring in LDS: [HD / 32][32 rows][64 bytes], the 16-byte pieces of each row at p ^ (row / 4) % 4,
 // so that neither the DMAs' writes nor the fragments' reads meet a bank twice.
 template <int HD>
 struct Ring {
-    static constexpr int BYTES = HD * 64, IW = BYTES / 4096;  // of a block; its DMAs per wave
+    static constexpr int BYTES = HD * 64, IW = BYTES / 4096, NB = HD == 256 ? 2 : HD == 128 ? 3 : 4;  // of a block; its DMAs per wave
     static __device__ __forceinline__ u32x4 read(const uint8_t* buf, int st, int c, int g) {
         return *reinterpret_cast<const u32x4*>(buf + (st >> 1) * 2048 + c * 64 + (((2 * (st & 1) + g) ^ ((c >> 2) & 3)) << 4));
     }
 };
 
+// The key of a block that is register e of S^T in the lanes of half g, less 4 g.
+__device__ __forceinline__ constexpr int key_of(int e) { return 8 * (e >> 2) + (e & 3); }
+
+// Keys lo to hi of a block, as a test of the constants key_of(e) that takes no register for each: one subtraction and an
+// unsigned comparison.
+struct Within {
+    uint32_t from, span;
+    __device__ __forceinline__ Within(int lo, int hi) {
+        lo = max(lo, 0);
+        from = hi < lo ? 1u << 30 : (uint32_t)lo, span = hi < lo ? 0u : (uint32_t)(hi - lo);
+    }
+    __device__ __forceinline__ bool has(int k) const { return (uint32_t)k - from <= span; }
+};
+
 // Maxima and sums of 128 rows over a split of their keys: each wave has 32 rows' queries in registers, and all four share
-// blocks of 32 keys that arrive by LDS DMA, three ahead.  A lane keeps its own maximum and sum of the half of each block that
-// it has; the two halves meet at the end.
+// blocks of 32 keys that arrive by LDS DMA, in a ring.  A lane keeps its own maximum and sum of the half of each block that it
+// has; the two halves meet at the end.
 template <class T, int HD>
-__global__ __launch_bounds__(256, 2) void k_weights_rows(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+__global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     typedef typename Vec8<T>::type T8;
     typedef Ring<HD> Rg;
-    constexpr int NS = HD / 16, NB = 4, IW = Rg::IW, PART = Rg::BYTES / 4;
-    // (an array per buffer: the compiler then sees that the DMAs into one never alias the reads of another)
-    __shared__ __align__(1024) uint8_t K0[Rg::BYTES], K1[Rg::BYTES], K2[Rg::BYTES], K3[Rg::BYTES];
+    constexpr int NS = HD / 16, NB = Rg::NB, IW = Rg::IW, PART = Rg::BYTES / 4;
+    RING(K)
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
-    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK % a.ks;
-    const Tile tl = row_tile(a, blockIdx.x / (a.HK * a.ks));
+    // The split changes slowest, and by an odd number of tiles: an XCD has every eighth workgroup, late splits have no keys for
+    // most tiles, and there are fewer tiles than their bound.
+    const int kh = blockIdx.x % a.HK, tiles = a.tiles | 1, z = blockIdx.x / (a.HK * tiles), x = blockIdx.x / a.HK % tiles;
+    if (x >= a.tiles) return;
+    const Tile tl = row_tile(a, x);
     if (tl.b < 0 || tl.x >= a.tiles) return;  // (more tiles than rows make: row starts that do not ascend)
     const RowTile t = row_tile_of(a, tl, z);
     const int nb = t.blk1 - t.blk0;
     if (nb <= 0) return;
-    const int w0 = t.r0 + 32 * wv;
+    const int w0 = t.r0 + 32 * wv, w1 = min(w0 + 32, t.r1);
     const bool live = w0 < t.r1;
     const int p0 = t.rq.p0 + t.ob.t0;
-    const int r = min(w0 + c, t.r1 - 1), tok = t.ob.t0 + r / a.G, h = kh * a.G + r % a.G;
-    const int jlo = a.from(t.rq.p0 + tok), jhi = min(t.rq.p0 + tok + 1, t.hi);
-    const int all0 = a.from(p0 + (min(w0 + 32, t.r1) - 1) / a.G), all1 = min(p0 + w0 / a.G + 1, t.hi);
+    const int all0 = a.from(p0 + (w1 - 1) / a.G), all1 = min(p0 + w0 / a.G + 1, t.hi);
     const int lbpp = a.lps - 5;
     const int* const tb = a.table + (size_t)tl.b * a.max_blocks;
     auto entries = [&](int i) { return tb[min((t.blk0 + i + lane) >> lbpp, a.max_blocks - 1)]; };  // lane l: of block i + l
@@ -369,15 +463,14 @@ __global__ __launch_bounds__(256, 2) void k_weights_rows(const T* __restrict__ Q
         for (int u = 0; u < IW; u++) buf_lds16(rs, dlane, wv * PART + u * 1024, buf + wv * PART + u * 1024);
     };
     T8 qf[NS];
+    const int r = min(w0 + c, t.r1 - 1), tok = t.ob.t0 + r / a.G;
+    const int jlo = a.from(t.rq.p0 + tok), jhi = min(t.rq.p0 + tok + 1, t.hi);
     {
-        const T* p = Q + ((size_t)(t.rq.q0 + tok) * a.HQ + h) * HD + 8 * g;
+        const T* const q = Q + ((size_t)(t.rq.q0 + tok) * a.HQ + kh * a.G + r % a.G) * HD + 8 * g;
 #pragma unroll
-        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const T8*>(p + 16 * s);
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const T8*>(q + 16 * s);
     }
     float m = -INFINITY, l = 0.f;
-    fetch(0, K0);
-    fetch(1, K1);
-    fetch(2, K2);
     auto turn = [&](int i, const uint8_t* K, uint8_t* Kx) INL {
         wait_loads<vmcnt_imm((NB - 2) * IW)>();
         lds_barrier();  // block i is there for every wave, the one before is done with
@@ -393,12 +486,9 @@ __global__ __launch_bounds__(256, 2) void k_weights_rows(const T* __restrict__ Q
         int page;
         const bool ok = there(i, page);
         if (!(ok && j0 >= all0 && j0 + 32 <= all1)) {
+            const Within keep(max(jlo, 0) - j0 - 4 * g, ok ? max(jhi, 0) - 1 - j0 - 4 * g : -1);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int j = j0 + 8 * (e >> 2) + 4 * g + (e & 3);
-                const bool keep = ok & (j >= jlo) & (j < jhi);
-                s[e] = keep ? s[e] : -INFINITY;
-            }
+            for (int e = 0; e < 16; e++) s[e] = keep.has(key_of(e)) ? s[e] : -INFINITY;
         }
         float top = s[0];
 #pragma unroll
@@ -414,22 +504,13 @@ __global__ __launch_bounds__(256, 2) void k_weights_rows(const T* __restrict__ Q
         }
         m = mn, l = sum;
     };
-    for (int i = 0;;) {
-        turn(i, K0, K3);
-        if (++i >= nb) break;
-        turn(i, K1, K0);
-        if (++i >= nb) break;
-        turn(i, K2, K1);
-        if (++i >= nb) break;
-        turn(i, K3, K2);
-        if (++i >= nb) break;
-    }
+    RING_LOOP(K, nb, fetch)
     wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
     const float mx = max_halves(m);
     float sum = l * part_weight(m, mx);
     sum += __shfl_xor(sum, 32);
     if (!live || g || w0 + c >= t.r1) return;
-    if (a.ks == 1) a.stat[(size_t)(t.rq.q0 + tok) * a.HQ + h] = make_float2(base_of(mx), inverse_of(sum));
+    if (a.ks == 1) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = make_float2(base_of(mx), inverse_of(sum));
     else a.ml[(((size_t)z * a.tiles + tl.x) * a.HK + kh) * ROW_TILE + 32 * wv + c] = make_float2(mx, sum);
 }
 
@@ -443,16 +524,16 @@ __global__ __launch_bounds__(256) void k_weights_join(WeightArgs a) {
     const int i = blockIdx.x % PER * 32 + threadIdx.x / 8, r = t.r0 + i;
     if (r >= t.r1) return;
     const int n = min(a.ks, (((t.hi + 31) >> 5) - t.blk0 + a.span - 1) / a.span);
-    const float2 st = join_parts(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n);
-    if ((threadIdx.x & 7) == 0) a.stat[(size_t)(t.rq.q0 + t.ob.t0 + r / a.G) * a.HQ + kh * a.G + r % a.G] = st;
+    const float2 st = join_parts<8>(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n);
+    if ((threadIdx.x & 7) == 0) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = st;
 }
 
 // (key tile, part of the rows) x of the requests', numbered through.
-__device__ __forceinline__ int key_tiles(const Req& rq) { return (rq.kcap + KEY_TILE - 1) / KEY_TILE; }
+__device__ __forceinline__ int key_tiles(const WeightArgs& a, const Req& rq) { return (rq.kcap + a.key_tile - 1) / a.key_tile; }
 __device__ __forceinline__ int key_parts(const WeightArgs& a, int b) {
     const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
     const int n = observed(rq, a.observers).n * a.G;
-    return n > a.few ? (n + a.part - 1) / a.part * key_tiles(rq) : 0;
+    return n > a.few ? (n + a.part - 1) / a.part * key_tiles(a, rq) : 0;
 }
 __device__ __forceinline__ Tile key_tile(const WeightArgs& a, int x) {
     return find_tile(a.B, x, [&](int b) { return key_parts(a, b); });
@@ -485,141 +566,9 @@ __device__ __forceinline__ void rows_of(const WeightArgs& a, const Req& rq, cons
     if (j0 - p0 >= ob.n) lo = hi = 0;
 }
 
-// Weights of 128 keys from a part of the rows: each wave has 32 keys in registers, and all four share blocks of 32 rows of
-// queries that arrive by LDS DMA, three ahead, in the ring's layout.  A lane adds its row's weight to its 16 keys' sums, in
-// registers; the 32 lanes meet at the end.
-template <class T, int HD>
-__global__ __launch_bounds__(256, 2) void k_weights_keys(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
-    typedef typename Vec8<T>::type T8;
-    typedef Ring<HD> Rg;
-    constexpr int NS = HD / 16, NB = 4, IW = Rg::IW;
-    __shared__ __align__(1024) uint8_t Q0[Rg::BYTES], Q1[Rg::BYTES], Q2[Rg::BYTES], Q3[Rg::BYTES];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 31, g = lane >> 5;
-    const int kh = blockIdx.x % a.HK;
-    const Tile tl = key_tile(a, blockIdx.x / a.HK);
-    if (tl.b < 0 || tl.x >= a.units) return;  // (as above)
-    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
-    const Seen ob = observed(rq, a.observers);
-    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part;
-    const int z = tl.i % parts, j0 = tl.i / parts * KEY_TILE;
-    int lo, hi;
-    rows_of(a, rq, ob, j0, j0 + KEY_TILE, lo, hi);
-    const int r0 = max(lo, z * a.part) & ~31, r1 = min(hi, (z + 1) * a.part), nb = (r1 - r0 + 31) >> 5;  // (parts are multiples of 32)
-    const bool sole = a.parts == 1;  // this workgroup's sums are the keys' weights
-    if (r1 <= r0 && !sole) return;
-    const int jw = j0 + 32 * wv, lbpp = a.lps - 5, blk = jw >> 5;
-    const int page = a.table[(size_t)tl.b * a.max_blocks + min(blk >> lbpp, a.max_blocks - 1)];
-    const bool there = jw < rq.kcap && (unsigned)page < (unsigned)a.n_pages;
-    f32x16 acc;
-#pragma unroll
-    for (int e = 0; e < 16; e++) acc[e] = 0.f;
-    if (r1 > r0) {
-        u32x4 kf[NS];
-        {
-            const size_t at = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
-            const Rsrc rk = make_rsrc(Kp + at, there ? HD * 64u : 0u);
-#pragma unroll
-            for (int st = 0; st < NS; st++) kf[st] = buf_b128(rk, c * 64 + (2 * (st & 1) + g) * 16, (st >> 1) * 2048);
-        }
-        const int p0 = rq.p0 + ob.t0;
-        // row r0 + 32 i + x is token t + (g0 + x) / G, head (g0 + x) % G
-        auto split = [&](int x, int& t, int& h) INL {
-            t = a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.magic);
-            h = x - t * a.G;
-        };
-        const int dt = 32 / a.G, dg = 32 % a.G;
-        int tf = r0 / a.G, gf = r0 % a.G;  // of the block that is fetched next
-        const size_t row = (size_t)a.HQ * HD;
-        const uint32_t piece = (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
-        auto fetch = [&](int i, uint8_t* buf) INL {
-            const int left = nrows - (r0 + 32 * i);  // (rows past the last are the last again, blocks past it too)
-            const size_t t0 = (size_t)rq.q0 + ob.t0 + min(tf, ob.n - 1);
-            const T* const base = Q + t0 * row + (size_t)kh * a.G * HD;
-            const Rsrc rs = make_rsrc(base, (uint32_t)min((size_t)0x7FFFFFFF, (((size_t)a.rows - t0) * row - (size_t)kh * a.G * HD) * 2));
-            uint32_t off[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                int t, h;
-                split(gf + min(16 * u + (lane >> 2), max(left, 1) - 1), t, h);
-                off[u] = left > 0 ? (uint32_t)(t * (int)row + h * HD) * 2 + piece : piece;
-            }
-#pragma unroll
-            for (int u = 0; u < IW; u++) {
-                const int x = wv * IW + u;  // half x % 2 of dims 32 (x / 2) ..
-                const bool odd = IW == 1 ? wv & 1 : u & 1;
-                buf_lds16(rs, odd ? off[1] : off[0], (x >> 1) * 64, buf + x * 1024);
-            }
-            tf += dt, gf += dg;
-            if (gf >= a.G) gf -= a.G, tf++;
-        };
-        int ts = r0 / a.G, gs = r0 % a.G;  // of the block whose rows' statistics are loaded next
-        float2 st;
-        int pr;  // the lane's row's position
-        bool valid;
-        auto next_stat = [&]() INL {
-            int t, h;
-            split(gs + c, t, h);
-            const int tok = ts + t;
-            valid = tok < ob.n;
-            const int tc = min(tok, ob.n - 1);
-            st = a.stat[((size_t)rq.q0 + ob.t0 + tc) * a.HQ + kh * a.G + h];
-            pr = p0 + tc;
-            ts += dt, gs += dg;
-            if (gs >= a.G) gs -= a.G, ts++;
-        };
-        next_stat();
-        fetch(0, Q0);
-        fetch(1, Q1);
-        fetch(2, Q2);
-        auto turn = [&](int i, const uint8_t* buf, uint8_t* bufx) INL {
-            wait_loads<vmcnt_imm((NB - 2) * IW)>();
-            lds_barrier();
-            const float2 now = st;
-            const int p = pr;
-            const bool ok = valid;
-            next_stat();
-            fetch(i + NB - 1, bufx);
-            // every row of the block sees every key of the wave
-            const int ra = r0 + 32 * i, first = __builtin_amdgcn_readlane(p, 0), last = __builtin_amdgcn_readlane(p, 31);
-            const bool open = there && ra + 32 <= r1 && first >= jw + 31 && a.from(last) <= jw && jw + 32 <= rq.kcap;
-            f32x16 s;
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = 0.f;
-#pragma unroll
-            for (int x = 0; x < NS; x++) s = Num<T>::mfma32(__builtin_bit_cast(T8, kf[x]), __builtin_bit_cast(T8, Rg::read(buf, x, c, g)), s);
-            if (__builtin_expect(__any(is_far(now.x)), 0)) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[e] = exp2_fast(scaled(s[e], a.c) - now.x) * now.y;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[e] = exp2_fast(__builtin_fmaf(s[e], a.c, -now.x)) * now.y;
-            }
-            if (!open) {
-                const int from = a.from(p);
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int j = jw + 8 * (e >> 2) + 4 * g + (e & 3);
-                    const bool keep = there & ok & (ra + c < r1) & (j <= p) & (j >= from);
-                    s[e] = keep ? s[e] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[e] += s[e];
-        };
-        for (int i = 0;;) {
-            turn(i, Q0, Q3);
-            if (++i >= nb) break;
-            turn(i, Q1, Q0);
-            if (++i >= nb) break;
-            turn(i, Q2, Q1);
-            if (++i >= nb) break;
-            turn(i, Q3, Q2);
-            if (++i >= nb) break;
-        }
-        wait_loads<vmcnt_imm(0)>();
-    }
-    // the sum over the 32 rows' lanes, halving the registers at each step: lane c has key e = c / 2
+// The sum of 16 keys' weights over the 32 rows' lanes, halving the registers at each step: lane c has key c / 2.
+__device__ __forceinline__ float sum_rows(f32x16& acc) {
+    const int c = threadIdx.x & 31;
 #pragma unroll
     for (int o = 16, n = 8; n; o >>= 1, n >>= 1) {
 #pragma unroll
@@ -629,34 +578,272 @@ __global__ __launch_bounds__(256, 2) void k_weights_keys(const T* __restrict__ Q
             acc[e] = keep + __shfl_xor(send, o);
         }
     }
-    const float w = acc[0] + __shfl_xor(acc[0], 1);
-    const int e = c >> 1, x = 8 * (e >> 2) + 4 * g + (e & 3), j = jw + x;
-    if (c & 1) return;
-    if (!sole) a.col[((size_t)tl.x * a.HK + kh) * KEY_TILE + 32 * wv + x] = w;
-    else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
+    return acc[0] + __shfl_xor(acc[0], 1);
+}
+// Weights of 128 KT keys from a part of the rows: each wave has 32 KT keys in registers, and all four share blocks of 32
+// rows of queries that arrive by LDS DMA, three ahead, in the ring's layout.  A lane adds its row's weights to its keys'
+// sums, in registers; the 32 lanes meet at the end.
+template <class T, int HD, int KT>
+__global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    typedef typename Vec8<T>::type T8;
+    typedef Ring<HD> Rg;
+    constexpr int NS = HD / 16, NB = Rg::NB, IW = Rg::IW;
+    RING(Q)
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    const int kh = blockIdx.x % a.HK;
+    const Tile tl = key_tile(a, blockIdx.x / a.HK);
+    if (tl.b < 0 || tl.x >= a.units) return;  // (as above)
+    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    const Seen ob = observed(rq, a.observers);
+    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part;
+    const int z = tl.i % parts, j0 = tl.i / parts * a.key_tile;
+    int lo, hi;
+    rows_of(a, rq, ob, j0, j0 + a.key_tile, lo, hi);
+    const int r0 = max(lo, z * a.part) & ~31, r1 = min(hi, (z + 1) * a.part), nb = (r1 - r0 + 31) >> 5;  // (parts are multiples of 32)
+    const bool sole = a.parts == 1;  // this workgroup's sums are the keys' weights
+    if (r1 <= r0 && !sole) return;
+    const int jw = j0 + 32 * KT * wv, lbpp = a.lps - 5;
+    int page[KT];
+    bool there[KT], whole = jw + 32 * KT <= rq.kcap;
+#pragma unroll
+    for (int v = 0; v < KT; v++) {
+        page[v] = a.table[(size_t)tl.b * a.max_blocks + min(((jw >> 5) + v) >> lbpp, a.max_blocks - 1)];
+        there[v] = jw + 32 * v < rq.kcap && (unsigned)page[v] < (unsigned)a.n_pages;
+        whole &= there[v];
+    }
+    f32x16 acc[KT];
+#pragma unroll
+    for (int v = 0; v < KT; v++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[v][e] = 0.f;
+    if (r1 > r0) {
+        u32x4 kf[KT][NS];
+#pragma unroll
+        for (int v = 0; v < KT; v++) {
+            const int blk = (jw >> 5) + v;
+            const size_t at = there[v] ? (size_t)page[v] * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+            const Rsrc rk = make_rsrc(Kp + at, there[v] ? HD * 64u : 0u);
+#pragma unroll
+            for (int st = 0; st < NS; st++) kf[v][st] = buf_b128(rk, c * 64 + (2 * (st & 1) + g) * 16, (st >> 1) * 2048);
+        }
+        const int p0 = rq.p0 + ob.t0;
+        // blocks of rows from which on every row is behind the wave's keys, and up to which it still sees them
+        const long long open0 = ((long long)jw + 32 * KT - 1 - p0) * a.G;
+        const long long open1 = a.window ? min((long long)r1, ((long long)jw + a.window - p0) * a.G) : r1;
+        // row r0 + 32 i + x is token t + (g0 + x) / G, head (g0 + x) % G, counted from the block's first: t tf, g0 gf
+        const int dt = 32 / a.G, dg = 32 % a.G;
+        int tf = r0 / a.G, gf = r0 % a.G;  // of the block that is fetched next
+        const size_t row = (size_t)a.HQ * HD;
+        const uint32_t piece = (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+        uint32_t off0, off1;  // of the lane's rows of the two halves of a block, or of the wave's one
+        auto offset = [&](int x) INL {
+            const int t = a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.magic);
+            return (uint32_t)(t * (int)row + (x - t * a.G) * HD) * 2 + piece;
+        };
+        auto offsets = [&]() INL {
+            off0 = offset(gf + (IW == 1 ? 16 * (wv & 1) : 0) + (lane >> 2));
+            if (IW > 1) off1 = offset(gf + 16 + (lane >> 2));
+        };
+        offsets();
+        auto fetch = [&](int, uint8_t* buf) INL {  // the next block (rows past the last are other rows, or zeros past Q's end: no matter)
+            const size_t t0 = (size_t)rq.q0 + ob.t0 + min(tf, ob.n - 1), left = (((size_t)a.rows - t0) * row - (size_t)kh * a.G * HD) * 2;
+            const Rsrc rs = make_rsrc(Q + t0 * row + (size_t)kh * a.G * HD, (uint32_t)min(left, (size_t)0x7FFFFFFF));
+            if (dg) offsets();
+#pragma unroll
+            for (int u = 0; u < IW; u++) {
+                const int x = wv * IW + u;  // half x % 2 of dims 32 (x / 2) ..
+                buf_lds16(rs, u & 1 ? off1 : off0, (x >> 1) * 64, buf + x * 1024);
+            }
+            tf += dt, gf += dg;
+            if (gf >= a.G) gf -= a.G, tf++;
+        };
+        const float2* const stat = a.stat + stat_at(a, rq, ob, kh);
+        float2 st = stat[min(r0 + c, nrows - 1)];
+        auto turn = [&](int i, const uint8_t* buf, uint8_t* bufx) INL {
+            wait_loads<vmcnt_imm((NB - 2) * IW)>();
+            lds_barrier();
+            const float2 now = st;
+            const int ra = r0 + 32 * i;
+            st = stat[min(ra + 32 + c, nrows - 1)];
+            fetch(i + NB - 1, bufx);
+            f32x16 s[KT];
+#pragma unroll
+            for (int v = 0; v < KT; v++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[v][e] = 0.f;
+            constexpr int F = 2;
+            u32x4 fr[2][F];  // (F fragments read while the F before them are in use)
+            auto read = [&](int n) INL {
+#pragma unroll
+                for (int x = 0; x < F; x++) fr[n & 1][x] = Rg::read(buf, F * n + x, c, g);
+            };
+            read(0);
+#pragma unroll
+            for (int n = 0; n < NS / F; n++) {
+                if (n + 1 < NS / F) read(n + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < F; x++)
+#pragma unroll
+                    for (int v = 0; v < KT; v++)
+                        s[v] = Num<T>::mfma32(__builtin_bit_cast(T8, kf[v][F * n + x]), __builtin_bit_cast(T8, fr[n & 1][x]), s[v]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const bool far = __any(is_far(now.x));
+            if (__builtin_expect(whole && ra >= open0 && ra + 32 <= open1 && !far, 1)) {  // every row sees every key
+#pragma unroll
+                for (int v = 0; v < KT; v++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        acc[v][e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[v][e], a.c, -now.x)), now.y, acc[v][e]);
+            } else {
+                const int r = ra + c, p = max(p0 + r / a.G, -1), from = max(a.from(p), 0);
+#pragma unroll
+                for (int v = 0; v < KT; v++) {
+                    const int j = jw + 32 * v + 4 * g;
+                    const Within keep(from - j, there[v] && r < r1 ? p - j : -1);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float x = far ? scaled(s[v][e], a.c) - now.x : __builtin_fmaf(s[v][e], a.c, -now.x);
+                        const float w = exp2_fast(x) * now.y;
+                        acc[v][e] += keep.has(key_of(e)) ? w : 0.f;
+                    }
+                }
+            }
+        };
+        RING_LOOP(Q, nb, fetch)
+        wait_loads<vmcnt_imm(0)>();
+    }
+#pragma unroll
+    for (int v = 0; v < KT; v++) {
+        const float w = sum_rows(acc[v]);
+        const int x = 32 * v + key_of(c >> 1) + 4 * g, j = jw + x;
+        if (c & 1) continue;
+        if (!sole) a.col[((size_t)tl.x * a.HK + kh) * a.key_tile + 32 * KT * wv + x] = w;
+        else if (there[v] && j < rq.kcap) put_weight(a, rq, mark_at(page[v], a.HK, kh, j, a.lps), j, w);
+    }
 }
 
-// Adds up the parts of 128 keys, in their order.
-__global__ __launch_bounds__(KEY_TILE) void k_weights_sum(WeightArgs a) {
+// The same for rows that fit in LDS (up to 32 SHORT of them): they come once, and every wave takes blocks of 32 keys, straight into
+// registers, the next block on its way while the rows pass by one; nothing waits for another wave.
+template <int HD>
+constexpr int short_blocks() { return HD == 256 ? 4 : 8; }
+constexpr int SHORT_KEYS = 1024;  // of a workgroup
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void k_weights_keys_short(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    typedef typename Vec8<T>::type T8;
+    typedef Ring<HD> Rg;
+    constexpr int NS = HD / 16, NB = short_blocks<HD>();
+    __shared__ __align__(1024) uint8_t rows[NB * Rg::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    const int kh = blockIdx.x % a.HK;
+    const Tile tl = key_tile(a, blockIdx.x / a.HK);
+    if (tl.b < 0) return;
+    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+    const Seen ob = observed(rq, a.observers);
+    const int nrows = min(ob.n * a.G, 32 * NB), nbr = (nrows + 31) >> 5, p0 = rq.p0 + ob.t0;
+    const int* const tb = a.table + (size_t)tl.b * a.max_blocks;
+    const int lbpp = a.lps - 5, first = tl.i * (SHORT_KEYS / 32) + wv, end = min((rq.kcap + 31) >> 5, (tl.i + 1) * (SHORT_KEYS / 32));
+    const int ids = tb[min((first + 4 * lane) >> lbpp, a.max_blocks - 1)];  // lane i: of the wave's block i
+    struct Blk {
+        u32x4 k[NS];
+        int page;
+        bool there;
+    };
+    auto load = [&](int i, Blk& x) INL {
+        const int blk = first + 4 * i;
+        x.page = __builtin_amdgcn_readlane(ids, i & 63);
+        x.there = blk < end && (unsigned)x.page < (unsigned)a.n_pages;
+        const size_t at = x.there ? (size_t)x.page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+        const Rsrc rk = make_rsrc(Kp + at, x.there ? HD * 64u : 0u);
+#pragma unroll
+        for (int st = 0; st < NS; st++) x.k[st] = buf_b128(rk, c * 64 + (2 * (st & 1) + g) * 16, (st >> 1) * 2048);
+    };
+    Blk set[2];
+    load(0, set[0]);
+    // the rows, in the ring's layout: 16 bytes a thread at a time
+    for (int i = tid; i < nbr * (HD * 4); i += 256) {
+        const int blk = i / (HD * 4), d = i % (HD * 4) / 128, x = i % 128 >> 2, piece = i & 3, r = min(32 * blk + x, nrows - 1);
+        const T* const q = Q + ((size_t)(rq.q0 + ob.t0 + r / a.G) * a.HQ + kh * a.G + r % a.G) * HD + 32 * d + 8 * piece;
+        *reinterpret_cast<T8*>(rows + blk * Rg::BYTES + d * 2048 + x * 64 + ((piece ^ ((x >> 2) & 3)) << 4)) = *reinterpret_cast<const T8*>(q);
+    }
+    float2 st[NB];
+    const float2* const stat = a.stat + stat_at(a, rq, ob, kh);
+#pragma unroll
+    for (int i = 0; i < NB; i++) st[i] = stat[min(32 * i + c, nrows - 1)];
+    __syncthreads();
+    auto work = [&](int i, const Blk& x) INL {
+        const int j0 = (first + 4 * i) * 32;
+        const bool open = x.there && p0 >= j0 + 31 && a.from(p0 + ob.n - 1) <= j0 && j0 + 32 <= rq.kcap;  // for all rows
+        f32x16 acc;
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[e] = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (b >= nbr) break;
+            f32x16 s;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+            for (int y = 0; y < NS; y++)
+                s = Num<T>::mfma32(__builtin_bit_cast(T8, x.k[y]), __builtin_bit_cast(T8, Rg::read(rows + b * Rg::BYTES, y, c, g)), s);
+            const bool far = __any(is_far(st[b].x));
+            if (__builtin_expect(open && 32 * b + 32 <= nrows && !far, 1)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    acc[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[e], a.c, -st[b].x)), st[b].y, acc[e]);
+            } else {
+                const int r = 32 * b + c, p = max(p0 + r / a.G, -1), j = j0 + 4 * g;
+                const Within keep(max(a.from(p), 0) - j, x.there && r < nrows ? p - j : -1);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float y = far ? scaled(s[e], a.c) - st[b].x : __builtin_fmaf(s[e], a.c, -st[b].x);
+                    const float w = exp2_fast(y) * st[b].y;
+                    acc[e] += keep.has(key_of(e)) ? w : 0.f;
+                }
+            }
+        }
+        const float w = sum_rows(acc);
+        const int j = j0 + key_of(c >> 1) + 4 * g;
+        if (!(c & 1) && x.there && j < rq.kcap) put_weight(a, rq, mark_at(x.page, a.HK, kh, j, a.lps), j, w);
+    };
+    const int cnt = (end - first + 3) / 4;
+    for (int i = 0; i < cnt; i += 2) {
+        load(i + 1, set[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        work(i, set[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 >= cnt) break;
+        load(i + 2, set[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        work(i + 1, set[1]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Adds up the parts of a key tile, in their order.
+__global__ __launch_bounds__(256) void k_weights_sum(WeightArgs a) {
     const int kh = blockIdx.x % a.HK;
     const Tile tl = find_tile(a.B, blockIdx.x / a.HK, [&](int b) {
-        return many_rows(a, b) ? key_tiles(request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
+        return many_rows(a, b) ? key_tiles(a, request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
     });
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const Seen ob = observed(rq, a.observers);
-    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part, j0 = tl.i * KEY_TILE, j = j0 + threadIdx.x;
+    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part, j0 = tl.i * a.key_tile, j = j0 + threadIdx.x;
     const int first = first_key_tile(a, tl.b) + tl.i * parts;
     if (j >= rq.kcap || first < 0 || first + parts > a.units) return;
     const int page = a.table[(size_t)tl.b * a.max_blocks + (j >> a.lps)];
     if ((unsigned)page >= (unsigned)a.n_pages) return;
     int lo, hi;
-    rows_of(a, rq, ob, j0, j0 + KEY_TILE, lo, hi);
+    rows_of(a, rq, ob, j0, j0 + a.key_tile, lo, hi);
     float w = 0.f;
-    const float* const col = a.col + ((size_t)first * a.HK + kh) * KEY_TILE + threadIdx.x;
+    const float* const col = a.col + ((size_t)first * a.HK + kh) * a.key_tile + threadIdx.x;
     if (hi > lo) {
 #pragma unroll 8
-        for (int z = lo / a.part; z <= (hi - 1) / a.part; z++) w += col[(size_t)z * a.HK * KEY_TILE];
+        for (int z = lo / a.part; z <= (hi - 1) / a.part; z++) w += col[(size_t)z * a.HK * a.key_tile];
     }
     put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
@@ -743,8 +930,6 @@ __device__ __forceinline__ void lengths(const EvictArgs& a, Head& x) {
     x.m = x.over ? budget : x.n;
 }
 
-typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // 4 rows from j on (a multiple of 4: they lie on end), as loaded.  Their page comes first, whatever the request's length:
 // the two loads of the lengths and of the table are then on their way together.
@@ -1302,6 +1487,7 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
 struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
+    int key_tile = 128;  // many rows: keys of a tile (more: k_weights_keys_short)
     int tiles = 0, ks = 1, span = 1, part = 32, parts = 1, units = 0;  // tiles 0: no many rows
     bool once = false;
     size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0;  // floats of the workspace
@@ -1318,7 +1504,7 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
     if (p.few) {
         p.nr = p.few <= 16 ? 1 : 2;
         p.kvp = (int)std::min<long long>((long long)nb * 32, INT_MAX);
-        const int want = std::max(1, std::min(64, 1024 / (B * s.HK)));
+        const int want = std::max(1, std::min(256, 8192 / (B * s.HK)));
         p.few_span = std::max(FEW_W, (nb + want - 1) / want);
         p.few_ks = (nb + p.few_span - 1) / p.few_span;
         p.S = (size_t)B * s.HK * p.few * p.kvp;
@@ -1330,21 +1516,22 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
     if (most > p.few) {
         const long long all = std::min((long long)rows, (long long)B * tokens) * G;  // rows that are counted
         const long long reqs = std::min((long long)B, all / (p.few + 1));
+        const int key_tile = p.key_tile = 128;
         p.tiles = (int)(all / ROW_TILE + reqs);
-        const int want = (int)std::min(128ll, std::max(1ll, 1024 / (std::max(1ll, all / ROW_TILE) * s.HK)));
-        p.span = std::max(16, (nb + want - 1) / want);
+        const int want = (int)std::min(128ll, std::max(1ll, 2048 / (std::max(1ll, all / ROW_TILE) * s.HK)));
+        p.span = std::max(8, (nb + want - 1) / want);
         p.ks = (nb + p.span - 1) / p.span;
-        const int nkb = (int)(((long long)max_kv + KEY_TILE - 1) / KEY_TILE);
+        const int nkb = (int)(((long long)max_kv + key_tile - 1) / key_tile);
         const long long wanted = std::max(1ll, 2048ll / ((long long)nkb * s.HK));
-        p.part = (int)std::max(128ll, ((all + wanted - 1) / wanted + 31) / 32 * 32);
+        p.part = (int)std::max(256ll, ((all + wanted - 1) / wanted + 31) / 32 * 32);
         p.parts = (int)((most + p.part - 1) / p.part);
         const long long units = (long long)nkb * std::min(reqs * p.parts, all / p.part + reqs);
-        if (units * s.HK >= 1 << 24 || (long long)p.tiles * s.HK * p.ks >= 1 << 24)
+        if (units * s.HK >= 1 << 24 || (long long)(p.tiles | 1) * s.HK * p.ks >= 1 << 24)
             throw Error("sd_op_paged_weights: too many rows and keys for one launch");
         p.units = (int)units;
         p.ml = p.ks > 1 ? (size_t)p.ks * p.tiles * s.HK * ROW_TILE * 2 : 0;
         p.stat = (size_t)rows * s.HQ * 2;
-        p.col = p.parts > 1 ? (size_t)p.units * s.HK * KEY_TILE : 0;
+        p.col = p.parts > 1 ? (size_t)p.units * s.HK * key_tile : 0;
     }
     for (size_t* x : {&p.S, &p.few_ml, &p.ml, &p.stat, &p.col}) *x = (*x + 3) & ~size_t(3);
     return p;
@@ -1356,7 +1543,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     const int G = s.HQ / s.HK;
     float* const ws = static_cast<float*>(a.ws);
     WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, G, log2i(s.PS), s.n_pages, a.max_new,
-                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.part,
+                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.key_tile, p.part,
                  p.parts, p.units, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
     g.S = ws;
     g.few_ml = reinterpret_cast<float2*>(g.S + p.S);
@@ -1369,12 +1556,14 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
         launched("paged_weights");
     };
     if (p.tiles) {
-        launch(k_weights_rows<T, HD>, dim3(p.tiles * s.HK * p.ks), 256, Q, K, g);
+        const dim3 rows((p.tiles | 1) * s.HK * p.ks), keys(p.units * s.HK);
+        launch(k_weights_rows<T, HD>, rows, 256, Q, K, g);
         if (p.ks > 1) launch(k_weights_join, dim3(p.tiles * s.HK * (ROW_TILE / 32)), 256, g);
-        launch(k_weights_keys<T, HD>, dim3(p.units * s.HK), 256, Q, K, g);
+        if (p.key_tile == 128) launch(k_weights_keys<T, HD, 1>, keys, 256, Q, K, g);
+        else launch(k_weights_keys_short<T, HD>, keys, 256, Q, K, g);
         if (p.parts > 1) {
-            const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
-            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), KEY_TILE, g);
+            const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + g.key_tile - 1) / g.key_tile;
+            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), g.key_tile, g);
         }
     }
     if (p.nr) {
@@ -1387,7 +1576,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
             else launch(k_weights_few<T, HD, 2, false>, grid, 64 * FEW_W, Q, K, g);
         }
         const long long chunks = ((long long)a.max_kv + 1023) / 1024;  // of 1024 keys; at most so many workgroups that each has some
-        launch(k_weights_few_sum, dim3((unsigned)std::min(chunks, std::max(1ll, 16384ll / (s.HK * a.B))), s.HK, a.B), 256, g);
+        launch(k_weights_few_sum, dim3((unsigned)std::min(chunks, std::max(1ll, 16384ll / (s.HK * a.B))) * s.HK, a.B), 256, g);
     }
 }
 
