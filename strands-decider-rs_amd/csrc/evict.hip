@@ -41,8 +41,8 @@ struct WeightArgs {
     int few, few_ks, few_span, rw, kvp;        // rows of a request that the few rows' kernels do; their splits, blocks of 32
                                                // keys in each; rows and keys of a request's scores
     int tiles, ks, span;                       // many rows: tiles of rows, their splits, blocks in each;
-    int key_tile, part, parts, units;          // keys of a tile, rows of a part, parts of a request at most, (key tile,
-                                               // part)s at most
+    int part, parts, units;                    // tokens of a part, parts of a request at most, (key tile, part)s at most
+    int dt, dg;                                // 32 rows: tokens, and heads besides
     uint32_t magic;  // 2^32 / G and 1 more: x / G is the upper half of a product for x below 2^16
     float c, decay;  // c: scale log2(e)
     size_t pstride;
@@ -53,7 +53,7 @@ struct WeightArgs {
     float2* few_ml;   // [B][HK][few_ks][rw]: their maxima and sums
     float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
     float2* stat;     // [rows][HQ], a request's rows kv head by kv head: of a row's whole, the sum's reciprocal
-    float* col;       // [units][HK][key_tile]: parts of the keys' weights
+    float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
     // the first key that a row at position p sees
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
 
 // ---- many rows ----
 
-constexpr int ROW_TILE = 128;
+constexpr int ROW_TILE = 128, KEY_TILE = 128;
 
 __device__ __forceinline__ int many_rows(const WeightArgs& a, int b) {  // of request b, 0 where they are few
     const int n = observed(request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap), a.observers).n * a.G;
@@ -377,10 +377,11 @@ __device__ __forceinline__ RowTile row_tile_of(const WeightArgs& a, const Tile& 
     __shared__ __align__(1024) uint8_t X##0[Rg::BYTES], X##1[Rg::BYTES], X##2[NB > 2 ? Rg::BYTES : 16], \
         X##3[NB > 3 ? Rg::BYTES : 16];
 // turn(i, its buffer, the buffer that block i + NB - 1 goes to) for n blocks.
-#define RING_LOOP(X, n, fetch)                                        \
-    fetch(0, X##0);                                                   \
-    if (NB > 2) fetch(1, X##1);                                       \
-    if (NB > 3) fetch(2, X##2);                                       \
+#define RING_START(X, fetch)        \
+    fetch(0, X##0);                 \
+    if (NB > 2) fetch(1, X##1);     \
+    if (NB > 3) fetch(2, X##2);
+#define RING_LOOP(X, n)                                               \
     for (int i = 0;;) {                                               \
         turn(i, X##0, NB == 4 ? X##3 : NB == 3 ? X##2 : X##1);        \
         if (++i >= n) break;                                          \
@@ -504,7 +505,8 @@ __global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q
         }
         m = mn, l = sum;
     };
-    RING_LOOP(K, nb, fetch)
+    RING_START(K, fetch)
+    RING_LOOP(K, nb)
     wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
     const float mx = max_halves(m);
     float sum = l * part_weight(m, mx);
@@ -514,26 +516,28 @@ __global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q
     else a.ml[(((size_t)z * a.tiles + tl.x) * a.HK + kh) * ROW_TILE + 32 * wv + c] = make_float2(mx, sum);
 }
 
-// Joins the splits of the rows: 8 threads per row, 32 rows a workgroup.
+// Joins the splits of the rows: N threads per row.
+template <int N>
 __global__ __launch_bounds__(256) void k_weights_join(WeightArgs a) {
-    constexpr int PER = ROW_TILE / 32;
+    constexpr int ROWS = 256 / N, PER = ROW_TILE / ROWS;
     const int kh = blockIdx.x / PER % a.HK;
     const Tile tl = row_tile(a, blockIdx.x / (PER * a.HK));
     if (tl.b < 0 || tl.x >= a.tiles) return;
     const RowTile t = row_tile_of(a, tl, 0);
-    const int i = blockIdx.x % PER * 32 + threadIdx.x / 8, r = t.r0 + i;
+    const int i = blockIdx.x % PER * ROWS + threadIdx.x / N, r = t.r0 + i;
     if (r >= t.r1) return;
     const int n = min(a.ks, (((t.hi + 31) >> 5) - t.blk0 + a.span - 1) / a.span);
-    const float2 st = join_parts<8>(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n);
-    if ((threadIdx.x & 7) == 0) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = st;
+    const float2 st = join_parts<N>(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n);
+    if (threadIdx.x % N == 0) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = st;
 }
 
 // (key tile, part of the rows) x of the requests', numbered through.
-__device__ __forceinline__ int key_tiles(const WeightArgs& a, const Req& rq) { return (rq.kcap + a.key_tile - 1) / a.key_tile; }
+__device__ __forceinline__ int key_tiles(const WeightArgs& a, const Req& rq) { return (rq.kcap + KEY_TILE - 1) / KEY_TILE; }
+__device__ __forceinline__ int parts_of(const WeightArgs& a, int tokens) { return a.parts == 1 ? 1 : (tokens + a.part - 1) / a.part; }
 __device__ __forceinline__ int key_parts(const WeightArgs& a, int b) {
     const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
-    const int n = observed(rq, a.observers).n * a.G;
-    return n > a.few ? (n + a.part - 1) / a.part * key_tiles(a, rq) : 0;
+    const int n = observed(rq, a.observers).n;
+    return n * a.G > a.few ? parts_of(a, n) * key_tiles(a, rq) : 0;
 }
 __device__ __forceinline__ Tile key_tile(const WeightArgs& a, int x) {
     return find_tile(a.B, x, [&](int b) { return key_parts(a, b); });
@@ -557,33 +561,53 @@ __device__ __forceinline__ int first_key_tile(const WeightArgs& a, int b) {
     }
     return __shfl(to - own + before, b & 63);
 }
-// The rows [lo, hi) of a request that see some key of [j0, j1).
-__device__ __forceinline__ void rows_of(const WeightArgs& a, const Req& rq, const Seen& ob, int j0, int j1, int& lo, int& hi) {
-    const int p0 = rq.p0 + ob.t0;
-    const int last = a.window ? (int)min((long long)ob.n, (long long)j1 - 1 + a.window - p0) : ob.n;  // tokens
-    lo = max(0, j0 - p0) * a.G;
-    hi = max(0, last) * a.G;
-    if (j0 - p0 >= ob.n) lo = hi = 0;
+// The tokens [lo, hi) of a request that see some key of [j0, j0 + 128).
+__device__ __forceinline__ void tokens_of(const WeightArgs& a, const Req& rq, const Seen& ob, int j0, int& lo, int& hi) {
+    const long long p0 = (long long)rq.p0 + ob.t0;
+    lo = (int)min((long long)ob.n, max(0ll, j0 - p0));
+    hi = a.window ? (int)max(0ll, min((long long)ob.n, j0 + 127ll + a.window - p0)) : ob.n;
 }
 
-// The sum of 16 keys' weights over the 32 rows' lanes, halving the registers at each step: lane c has key c / 2.
-__device__ __forceinline__ float sum_rows(f32x16& acc) {
-    const int c = threadIdx.x & 31;
-#pragma unroll
-    for (int o = 16, n = 8; n; o >>= 1, n >>= 1) {
-#pragma unroll
-        for (int e = 0; e < n; e++) {
-            const bool up = c & o;
-            const float keep = up ? acc[e + n] : acc[e], send = up ? acc[e] : acc[e + n];
-            acc[e] = keep + __shfl_xor(send, o);
-        }
-    }
-    return acc[0] + __shfl_xor(acc[0], 1);
+// The sum of 16 keys' weights over the 32 rows' lanes, halving the registers at each step: lane c has key c / 2.  The partners of
+// the first step are 16 lanes away, then 8, 4 of 7 - c, 2 and 1: each differs in the bit that says which half a lane keeps.
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false));
 }
-// Weights of 128 KT keys from a part of the rows: each wave has 32 KT keys in registers, and all four share blocks of 32
-// rows of queries that arrive by LDS DMA, three ahead, in the ring's layout.  A lane adds its row's weights to its keys'
-// sums, in registers; the 32 lanes meet at the end.
-template <class T, int HD, int KT>
+__device__ __forceinline__ float sum_rows(const f32x16& acc) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int c = threadIdx.x & 31;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {  // (one swap of two registers' halves: each lane then has what it keeps, and the other's)
+        const float x = acc[e], y = acc[e + 8];
+        const auto sw = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+        const uint32_t lo = sw[0], hi = sw[1];
+        v[e] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+    }
+    auto halve = [&](auto n, auto ctrl) INL {
+        constexpr int N = decltype(n)::value;
+        const bool up = c & 2 * N;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float x = v[e], y = v[e + N];
+            v[e] = (up ? y : x) + from_lane<decltype(ctrl)::value>(up ? x : y);
+        }
+    };
+    using std::integral_constant;
+    halve(integral_constant<int, 4>(), integral_constant<int, 0x128>());  // 8 lanes on in each row of 16
+    halve(integral_constant<int, 2>(), integral_constant<int, 0x141>());  // lane 7 - c of each 8
+    halve(integral_constant<int, 1>(), integral_constant<int, 0x4E>());   // c ^ 2
+    return v[0] + from_lane<0xB1>(v[0]);                                  // c ^ 1
+#else
+    return acc[0];
+#endif
+}
+
+// Weights of 128 keys from a part of the rows: each wave has 32 keys in registers, and all four share blocks of 32 rows of queries
+// that arrive by LDS DMA, in a ring.  A lane adds its row's weights to its 16 keys' sums, in registers; the 32 lanes meet at the
+// end.  What changes from block to block is scalar: a block's first token and head, and offsets into Q and the statistics.
+template <class T, int HD>
 __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     typedef typename Vec8<T>::type T8;
     typedef Ring<HD> Rg;
@@ -596,50 +620,41 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
     if (tl.b < 0 || tl.x >= a.units) return;  // (as above)
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const Seen ob = observed(rq, a.observers);
-    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part;
-    const int z = tl.i % parts, j0 = tl.i / parts * a.key_tile;
-    int lo, hi;
-    rows_of(a, rq, ob, j0, j0 + a.key_tile, lo, hi);
-    const int r0 = max(lo, z * a.part) & ~31, r1 = min(hi, (z + 1) * a.part), nb = (r1 - r0 + 31) >> 5;  // (parts are multiples of 32)
     const bool sole = a.parts == 1;  // this workgroup's sums are the keys' weights
-    if (r1 <= r0 && !sole) return;
-    const int jw = j0 + 32 * KT * wv, lbpp = a.lps - 5;
-    int page[KT];
-    bool there[KT], whole = jw + 32 * KT <= rq.kcap;
+    const int parts = parts_of(a, ob.n), p0 = rq.p0 + ob.t0;
+    const int z = sole ? 0 : tl.i % parts, j0 = (sole ? tl.i : tl.i / parts) * KEY_TILE;
+    int t0, t1;  // the part's tokens that see some of the keys
+    tokens_of(a, rq, ob, j0, t0, t1);
+    t0 = max(t0, z * a.part), t1 = min(t1, sole ? ob.n : (z + 1) * a.part);
+    if (t1 <= t0 && !sole) return;
+    const int nr = max(0, t1 - t0) * a.G, nb = (nr + 31) >> 5;  // rows, and blocks of them
+    const int jw = j0 + 32 * wv, lbpp = a.lps - 5, blk = jw >> 5;
+    const int page = a.table[(size_t)tl.b * a.max_blocks + min(blk >> lbpp, a.max_blocks - 1)];
+    const bool there = jw < rq.kcap && (unsigned)page < (unsigned)a.n_pages;
+    f32x16 acc;
 #pragma unroll
-    for (int v = 0; v < KT; v++) {
-        page[v] = a.table[(size_t)tl.b * a.max_blocks + min(((jw >> 5) + v) >> lbpp, a.max_blocks - 1)];
-        there[v] = jw + 32 * v < rq.kcap && (unsigned)page[v] < (unsigned)a.n_pages;
-        whole &= there[v];
-    }
-    f32x16 acc[KT];
+    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    if (nb > 0) {
+        u32x4 kf[NS];
+        {
+            const size_t at = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+            const Rsrc rk = make_rsrc(Kp + at, there ? HD * 64u : 0u);
 #pragma unroll
-    for (int v = 0; v < KT; v++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) acc[v][e] = 0.f;
-    if (r1 > r0) {
-        u32x4 kf[KT][NS];
-#pragma unroll
-        for (int v = 0; v < KT; v++) {
-            const int blk = (jw >> 5) + v;
-            const size_t at = there[v] ? (size_t)page[v] * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
-            const Rsrc rk = make_rsrc(Kp + at, there[v] ? HD * 64u : 0u);
-#pragma unroll
-            for (int st = 0; st < NS; st++) kf[v][st] = buf_b128(rk, c * 64 + (2 * (st & 1) + g) * 16, (st >> 1) * 2048);
+            for (int x = 0; x < NS; x++) kf[x] = buf_b128(rk, c * 64 + (2 * (x & 1) + g) * 16, (x >> 1) * 2048);
         }
-        const int p0 = rq.p0 + ob.t0;
-        // blocks of rows from which on every row is behind the wave's keys, and up to which it still sees them
-        const long long open0 = ((long long)jw + 32 * KT - 1 - p0) * a.G;
-        const long long open1 = a.window ? min((long long)r1, ((long long)jw + a.window - p0) * a.G) : r1;
-        // row r0 + 32 i + x is token t + (g0 + x) / G, head (g0 + x) % G, counted from the block's first: t tf, g0 gf
-        const int dt = 32 / a.G, dg = 32 % a.G;
-        int tf = r0 / a.G, gf = r0 % a.G;  // of the block that is fetched next
-        const size_t row = (size_t)a.HQ * HD;
+        // row 32 i + x of the part is token t + (g0 + x) / G, head (g0 + x) % G, counted from its first token: t tf, g0 gf
+        const uint32_t row = (uint32_t)a.HQ * HD * 2;  // bytes (a part's are fewer than 2^31)
+        const size_t q0 = (size_t)rq.q0 + ob.t0 + t0, left = (a.rows - q0) * row - (size_t)kh * a.G * HD * 2;
+        const Rsrc rs = make_rsrc(Q + (q0 * a.HQ + (size_t)kh * a.G) * HD, (uint32_t)min(left, (size_t)0x7FFFFFFF));
+        const Rsrc rst = make_rsrc(a.stat + stat_at(a, rq, ob, kh) + (size_t)t0 * a.G, (uint32_t)nr * 8);
+        int gf = 0;         // of the block that is fetched next
+        uint32_t qoff = 0;  // its token's rows, in Q
         const uint32_t piece = (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
         uint32_t off0, off1;  // of the lane's rows of the two halves of a block, or of the wave's one
+        auto token_of = [&](int x) INL { return a.G == 1 ? (uint32_t)x : __umulhi((uint32_t)x, a.magic); };
         auto offset = [&](int x) INL {
-            const int t = a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.magic);
-            return (uint32_t)(t * (int)row + (x - t * a.G) * HD) * 2 + piece;
+            const uint32_t t = token_of(x);
+            return t * row + (x - t * a.G) * (HD * 2) + piece;
         };
         auto offsets = [&]() INL {
             off0 = offset(gf + (IW == 1 ? 16 * (wv & 1) : 0) + (lane >> 2));
@@ -647,184 +662,64 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
         };
         offsets();
         auto fetch = [&](int, uint8_t* buf) INL {  // the next block (rows past the last are other rows, or zeros past Q's end: no matter)
-            const size_t t0 = (size_t)rq.q0 + ob.t0 + min(tf, ob.n - 1), left = (((size_t)a.rows - t0) * row - (size_t)kh * a.G * HD) * 2;
-            const Rsrc rs = make_rsrc(Q + t0 * row + (size_t)kh * a.G * HD, (uint32_t)min(left, (size_t)0x7FFFFFFF));
-            if (dg) offsets();
+            if (a.dg) offsets();
 #pragma unroll
             for (int u = 0; u < IW; u++) {
                 const int x = wv * IW + u;  // half x % 2 of dims 32 (x / 2) ..
-                buf_lds16(rs, u & 1 ? off1 : off0, (x >> 1) * 64, buf + x * 1024);
+                buf_lds16(rs, (u & 1 ? off1 : off0) + qoff, (x >> 1) * 64, buf + x * 1024);  // (a row in range is there whole)
             }
-            tf += dt, gf += dg;
-            if (gf >= a.G) gf -= a.G, tf++;
+            qoff += a.dt * row, gf += a.dg;
+            if (gf >= a.G) gf -= a.G, qoff += row;
+            qoff = min(qoff, 0x7FFFFFFFu - 0xFFFFu);  // (blocks past the last)
         };
-        const float2* const stat = a.stat + stat_at(a, rq, ob, kh);
-        float2 st = stat[min(r0 + c, nrows - 1)];
+        auto stat = [&](int i) INL { return __builtin_bit_cast(float2, buf_b64(rst, c * 8 + i * 256, 0)); };  // (0 past the last row)
+        float2 st = stat(0);
+        int tb = t0, gb = 0;  // the first row's of the block that is worked on
+        RING_START(Q, fetch)
         auto turn = [&](int i, const uint8_t* buf, uint8_t* bufx) INL {
             wait_loads<vmcnt_imm((NB - 2) * IW)>();
             lds_barrier();
             const float2 now = st;
-            const int ra = r0 + 32 * i;
-            st = stat[min(ra + 32 + c, nrows - 1)];
+            st = stat(i + 1);
             fetch(i + NB - 1, bufx);
-            f32x16 s[KT];
-#pragma unroll
-            for (int v = 0; v < KT; v++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[v][e] = 0.f;
-            constexpr int F = 2;
-            u32x4 fr[2][F];  // (F fragments read while the F before them are in use)
-            auto read = [&](int n) INL {
-#pragma unroll
-                for (int x = 0; x < F; x++) fr[n & 1][x] = Rg::read(buf, F * n + x, c, g);
-            };
-            read(0);
-#pragma unroll
-            for (int n = 0; n < NS / F; n++) {
-                if (n + 1 < NS / F) read(n + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int x = 0; x < F; x++)
-#pragma unroll
-                    for (int v = 0; v < KT; v++)
-                        s[v] = Num<T>::mfma32(__builtin_bit_cast(T8, kf[v][F * n + x]), __builtin_bit_cast(T8, fr[n & 1][x]), s[v]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            const bool far = __any(is_far(now.x));
-            if (__builtin_expect(whole && ra >= open0 && ra + 32 <= open1 && !far, 1)) {  // every row sees every key
-#pragma unroll
-                for (int v = 0; v < KT; v++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        acc[v][e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[v][e], a.c, -now.x)), now.y, acc[v][e]);
-            } else {
-                const int r = ra + c, p = max(p0 + r / a.G, -1), from = max(a.from(p), 0);
-#pragma unroll
-                for (int v = 0; v < KT; v++) {
-                    const int j = jw + 32 * v + 4 * g;
-                    const Within keep(from - j, there[v] && r < r1 ? p - j : -1);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float x = far ? scaled(s[v][e], a.c) - now.x : __builtin_fmaf(s[v][e], a.c, -now.x);
-                        const float w = exp2_fast(x) * now.y;
-                        acc[v][e] += keep.has(key_of(e)) ? w : 0.f;
-                    }
-                }
-            }
-        };
-        RING_LOOP(Q, nb, fetch)
-        wait_loads<vmcnt_imm(0)>();
-    }
-#pragma unroll
-    for (int v = 0; v < KT; v++) {
-        const float w = sum_rows(acc[v]);
-        const int x = 32 * v + key_of(c >> 1) + 4 * g, j = jw + x;
-        if (c & 1) continue;
-        if (!sole) a.col[((size_t)tl.x * a.HK + kh) * a.key_tile + 32 * KT * wv + x] = w;
-        else if (there[v] && j < rq.kcap) put_weight(a, rq, mark_at(page[v], a.HK, kh, j, a.lps), j, w);
-    }
-}
-
-// The same for rows that fit in LDS (up to 32 SHORT of them): they come once, and every wave takes blocks of 32 keys, straight into
-// registers, the next block on its way while the rows pass by one; nothing waits for another wave.
-template <int HD>
-constexpr int short_blocks() { return HD == 256 ? 4 : 8; }
-constexpr int SHORT_KEYS = 1024;  // of a workgroup
-template <class T, int HD>
-__global__ __launch_bounds__(256, 2) void k_weights_keys_short(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
-    typedef typename Vec8<T>::type T8;
-    typedef Ring<HD> Rg;
-    constexpr int NS = HD / 16, NB = short_blocks<HD>();
-    __shared__ __align__(1024) uint8_t rows[NB * Rg::BYTES];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 31, g = lane >> 5;
-    const int kh = blockIdx.x % a.HK;
-    const Tile tl = key_tile(a, blockIdx.x / a.HK);
-    if (tl.b < 0) return;
-    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
-    const Seen ob = observed(rq, a.observers);
-    const int nrows = min(ob.n * a.G, 32 * NB), nbr = (nrows + 31) >> 5, p0 = rq.p0 + ob.t0;
-    const int* const tb = a.table + (size_t)tl.b * a.max_blocks;
-    const int lbpp = a.lps - 5, first = tl.i * (SHORT_KEYS / 32) + wv, end = min((rq.kcap + 31) >> 5, (tl.i + 1) * (SHORT_KEYS / 32));
-    const int ids = tb[min((first + 4 * lane) >> lbpp, a.max_blocks - 1)];  // lane i: of the wave's block i
-    struct Blk {
-        u32x4 k[NS];
-        int page;
-        bool there;
-    };
-    auto load = [&](int i, Blk& x) INL {
-        const int blk = first + 4 * i;
-        x.page = __builtin_amdgcn_readlane(ids, i & 63);
-        x.there = blk < end && (unsigned)x.page < (unsigned)a.n_pages;
-        const size_t at = x.there ? (size_t)x.page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
-        const Rsrc rk = make_rsrc(Kp + at, x.there ? HD * 64u : 0u);
-#pragma unroll
-        for (int st = 0; st < NS; st++) x.k[st] = buf_b128(rk, c * 64 + (2 * (st & 1) + g) * 16, (st >> 1) * 2048);
-    };
-    Blk set[2];
-    load(0, set[0]);
-    // the rows, in the ring's layout: 16 bytes a thread at a time
-    for (int i = tid; i < nbr * (HD * 4); i += 256) {
-        const int blk = i / (HD * 4), d = i % (HD * 4) / 128, x = i % 128 >> 2, piece = i & 3, r = min(32 * blk + x, nrows - 1);
-        const T* const q = Q + ((size_t)(rq.q0 + ob.t0 + r / a.G) * a.HQ + kh * a.G + r % a.G) * HD + 32 * d + 8 * piece;
-        *reinterpret_cast<T8*>(rows + blk * Rg::BYTES + d * 2048 + x * 64 + ((piece ^ ((x >> 2) & 3)) << 4)) = *reinterpret_cast<const T8*>(q);
-    }
-    float2 st[NB];
-    const float2* const stat = a.stat + stat_at(a, rq, ob, kh);
-#pragma unroll
-    for (int i = 0; i < NB; i++) st[i] = stat[min(32 * i + c, nrows - 1)];
-    __syncthreads();
-    auto work = [&](int i, const Blk& x) INL {
-        const int j0 = (first + 4 * i) * 32;
-        const bool open = x.there && p0 >= j0 + 31 && a.from(p0 + ob.n - 1) <= j0 && j0 + 32 <= rq.kcap;  // for all rows
-        f32x16 acc;
-#pragma unroll
-        for (int e = 0; e < 16; e++) acc[e] = 0.f;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            if (b >= nbr) break;
             f32x16 s;
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = 0.f;
 #pragma unroll
-            for (int y = 0; y < NS; y++)
-                s = Num<T>::mfma32(__builtin_bit_cast(T8, x.k[y]), __builtin_bit_cast(T8, Rg::read(rows + b * Rg::BYTES, y, c, g)), s);
-            const bool far = __any(is_far(st[b].x));
-            if (__builtin_expect(open && 32 * b + 32 <= nrows && !far, 1)) {
+            for (int x = 0; x < NS; x++)
+                s = Num<T>::mfma32(__builtin_bit_cast(T8, kf[x]), __builtin_bit_cast(T8, Rg::read(buf, x, c, g)), s);
+            const bool far = __any(is_far(now.x));
+            // every row sees every key: the first token's causally, the last one's through the window
+            const bool open = there && jw + 32 <= rq.kcap && 32 * i + 32 <= nr && p0 + tb >= jw + 31 &&
+                              (!a.window || p0 + tb + a.dt + 1 - jw < a.window);
+            if (__builtin_expect(open && !far, 1)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    acc[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[e], a.c, -st[b].x)), st[b].y, acc[e]);
+                for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[e], a.c, -now.x)), now.y, acc[e]);
             } else {
-                const int r = 32 * b + c, p = max(p0 + r / a.G, -1), j = j0 + 4 * g;
-                const Within keep(max(a.from(p), 0) - j, x.there && r < nrows ? p - j : -1);
+                const int p = max(p0 + tb + (int)token_of(gb + c), -1), j = jw + 4 * g;
+                const Within keep(max(a.from(p), 0) - j, there && 32 * i + c < nr ? p - j : -1);
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const float y = far ? scaled(s[e], a.c) - st[b].x : __builtin_fmaf(s[e], a.c, -st[b].x);
-                    const float w = exp2_fast(y) * st[b].y;
+                    const float x = far ? scaled(s[e], a.c) - now.x : __builtin_fmaf(s[e], a.c, -now.x);
+                    const float w = exp2_fast(x) * now.y;
                     acc[e] += keep.has(key_of(e)) ? w : 0.f;
                 }
             }
-        }
-        const float w = sum_rows(acc);
-        const int j = j0 + key_of(c >> 1) + 4 * g;
-        if (!(c & 1) && x.there && j < rq.kcap) put_weight(a, rq, mark_at(x.page, a.HK, kh, j, a.lps), j, w);
-    };
-    const int cnt = (end - first + 3) / 4;
-    for (int i = 0; i < cnt; i += 2) {
-        load(i + 1, set[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        work(i, set[0]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 >= cnt) break;
-        load(i + 2, set[0]);
-        __builtin_amdgcn_sched_barrier(0);
-        work(i + 1, set[1]);
-        __builtin_amdgcn_sched_barrier(0);
+            tb += a.dt, gb += a.dg;
+            if (gb >= a.G) gb -= a.G, tb++;
+        };
+        RING_LOOP(Q, nb)
+        wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
     }
+    const float w = sum_rows(acc);
+    const int x = key_of(c >> 1) + 4 * g, j = jw + x;
+    if (c & 1) return;
+    if (!sole) a.col[((size_t)tl.x * a.HK + kh) * KEY_TILE + 32 * wv + x] = w;
+    else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
 
-// Adds up the parts of a key tile, in their order.
-__global__ __launch_bounds__(256) void k_weights_sum(WeightArgs a) {
+// Adds up the parts of 128 keys, in their order.
+__global__ __launch_bounds__(KEY_TILE) void k_weights_sum(WeightArgs a) {
     const int kh = blockIdx.x % a.HK;
     const Tile tl = find_tile(a.B, blockIdx.x / a.HK, [&](int b) {
         return many_rows(a, b) ? key_tiles(a, request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
@@ -832,18 +727,18 @@ __global__ __launch_bounds__(256) void k_weights_sum(WeightArgs a) {
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const Seen ob = observed(rq, a.observers);
-    const int nrows = ob.n * a.G, parts = (nrows + a.part - 1) / a.part, j0 = tl.i * a.key_tile, j = j0 + threadIdx.x;
+    const int parts = parts_of(a, ob.n), j0 = tl.i * KEY_TILE, j = j0 + threadIdx.x;
     const int first = first_key_tile(a, tl.b) + tl.i * parts;
     if (j >= rq.kcap || first < 0 || first + parts > a.units) return;
     const int page = a.table[(size_t)tl.b * a.max_blocks + (j >> a.lps)];
     if ((unsigned)page >= (unsigned)a.n_pages) return;
-    int lo, hi;
-    rows_of(a, rq, ob, j0, j0 + a.key_tile, lo, hi);
+    int t0, t1;
+    tokens_of(a, rq, ob, j0, t0, t1);
     float w = 0.f;
-    const float* const col = a.col + ((size_t)first * a.HK + kh) * a.key_tile + threadIdx.x;
-    if (hi > lo) {
+    const float* const col = a.col + ((size_t)first * a.HK + kh) * KEY_TILE + threadIdx.x;
+    if (t1 > t0) {
 #pragma unroll 8
-        for (int z = lo / a.part; z <= (hi - 1) / a.part; z++) w += col[(size_t)z * a.HK * a.key_tile];
+        for (int z = t0 / a.part; z <= (t1 - 1) / a.part; z++) w += col[(size_t)z * a.HK * KEY_TILE];
     }
     put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
@@ -1487,8 +1382,7 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
 struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
-    int key_tile = 128;  // many rows: keys of a tile (more: k_weights_keys_short)
-    int tiles = 0, ks = 1, span = 1, part = 32, parts = 1, units = 0;  // tiles 0: no many rows
+    int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0;  // tiles 0: no many rows
     bool once = false;
     size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0;  // floats of the workspace
 };
@@ -1516,22 +1410,23 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
     if (most > p.few) {
         const long long all = std::min((long long)rows, (long long)B * tokens) * G;  // rows that are counted
         const long long reqs = std::min((long long)B, all / (p.few + 1));
-        const int key_tile = p.key_tile = 128;
         p.tiles = (int)(all / ROW_TILE + reqs);
         const int want = (int)std::min(128ll, std::max(1ll, 2048 / (std::max(1ll, all / ROW_TILE) * s.HK)));
         p.span = std::max(8, (nb + want - 1) / want);
         p.ks = (nb + p.span - 1) / p.span;
-        const int nkb = (int)(((long long)max_kv + key_tile - 1) / key_tile);
+        const int nkb = (int)(((long long)max_kv + KEY_TILE - 1) / KEY_TILE);
+        // parts of at least 256 rows, so many that there are 2048 workgroups, and of fewer than 2^30 bytes of Q
         const long long wanted = std::max(1ll, 2048ll / ((long long)nkb * s.HK));
-        p.part = (int)std::max(256ll, ((all + wanted - 1) / wanted + 31) / 32 * 32);
-        p.parts = (int)((most + p.part - 1) / p.part);
-        const long long units = (long long)nkb * std::min(reqs * p.parts, all / p.part + reqs);
+        p.part = (int)(std::max(256ll, (all + wanted - 1) / wanted) + G - 1) / G;
+        p.part = (int)std::min<long long>(p.part, std::max(1ll, (1ll << 29) / ((long long)s.HQ * s.HD)));
+        p.parts = (tokens + p.part - 1) / p.part;
+        const long long units = (long long)nkb * std::min(reqs * p.parts, all / G / p.part + reqs);
         if (units * s.HK >= 1 << 24 || (long long)(p.tiles | 1) * s.HK * p.ks >= 1 << 24)
             throw Error("sd_op_paged_weights: too many rows and keys for one launch");
         p.units = (int)units;
         p.ml = p.ks > 1 ? (size_t)p.ks * p.tiles * s.HK * ROW_TILE * 2 : 0;
         p.stat = (size_t)rows * s.HQ * 2;
-        p.col = p.parts > 1 ? (size_t)p.units * s.HK * key_tile : 0;
+        p.col = p.parts > 1 ? (size_t)p.units * s.HK * KEY_TILE : 0;
     }
     for (size_t* x : {&p.S, &p.few_ml, &p.ml, &p.stat, &p.col}) *x = (*x + 3) & ~size_t(3);
     return p;
@@ -1543,8 +1438,8 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     const int G = s.HQ / s.HK;
     float* const ws = static_cast<float*>(a.ws);
     WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, G, log2i(s.PS), s.n_pages, a.max_new,
-                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.key_tile, p.part,
-                 p.parts, p.units, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
+                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.part,
+                 p.parts, p.units, 32 / G, 32 % G, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
     g.S = ws;
     g.few_ml = reinterpret_cast<float2*>(g.S + p.S);
     g.ml = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.few_ml) + p.few_ml);
@@ -1558,12 +1453,12 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     if (p.tiles) {
         const dim3 rows((p.tiles | 1) * s.HK * p.ks), keys(p.units * s.HK);
         launch(k_weights_rows<T, HD>, rows, 256, Q, K, g);
-        if (p.ks > 1) launch(k_weights_join, dim3(p.tiles * s.HK * (ROW_TILE / 32)), 256, g);
-        if (p.key_tile == 128) launch(k_weights_keys<T, HD, 1>, keys, 256, Q, K, g);
-        else launch(k_weights_keys_short<T, HD>, keys, 256, Q, K, g);
+        if (p.ks > 16) launch(k_weights_join<64>, dim3(p.tiles * s.HK * (ROW_TILE / 4)), 256, g);
+        else if (p.ks > 1) launch(k_weights_join<8>, dim3(p.tiles * s.HK * (ROW_TILE / 32)), 256, g);
+        launch(k_weights_keys<T, HD>, keys, 256, Q, K, g);
         if (p.parts > 1) {
-            const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + g.key_tile - 1) / g.key_tile;
-            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), g.key_tile, g);
+            const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
+            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), KEY_TILE, g);
         }
     }
     if (p.nr) {
