@@ -364,7 +364,7 @@ int sd_op_rope_table(const void* freqs, int pairs, double magnitude, const void*
                      char* err, size_t errlen);
 
 /* Rotation of T rows of HQ heads Q and HK heads K (K null: none) of HD dims (a multiple of 8 to 1024), rows q_stride and
- * heads q_step elements apart (multiples of 8, no two heads overlapping, in any order): (x, y) of pair j of the first RD
+ * heads q_step elements apart (multiples of 8 below 2^32, no two heads overlapping, in any order): (x, y) of pair j of the first RD
  * dims becomes magnitude (x cos a - y sin a, y cos a + x sin a), a = pos[t] freqs[j] (pos i32 [T], any value; null: t;
  * freqs [RD/2] f64 on the device), RD even, 2 to 256; `inverse` turns back (-a: with magnitude 1 the inverse, with any the
  * gradient).  Angles in f64, products in f32, rounded once; other dims are copied as they are.  type SD_F16, SD_BF16 or

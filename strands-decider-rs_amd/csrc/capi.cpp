@@ -833,8 +833,8 @@ int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inve
         if (!Qo) Qo = Q, qo_stride = q_stride, qo_step = q_step, Ko = K, ko_stride = k_stride, ko_step = k_step;
         const size_t size = type == SD_F32 ? 4 : 2;
         auto span = [&](const void* p, size_t stride, size_t step, int heads) {  // and its checks
-            if (stride % 8 || step % 8 || stride > (size_t(1) << 40) || step > (size_t(1) << 40))
-                throw sd::Error(who + ": strides must be multiples of 8, at most 2^40");
+            if (stride % 8 || step % 8 || stride > UINT32_MAX || step > UINT32_MAX)
+                throw sd::Error(who + ": strides must be multiples of 8 below 2^32");
             const size_t wide = (heads - 1) * step + HD, tall = (T - 1) * stride + HD;
             if ((heads > 1 && step < (size_t)HD) || (T > 1 && stride < (size_t)HD) || (heads > 1 && T > 1 && stride < wide && step < tall))
                 throw sd::Error(who + ": two heads overlap");

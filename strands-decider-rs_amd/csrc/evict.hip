@@ -1313,11 +1313,64 @@ __global__ __launch_bounds__(RELEASE_T) void k_page_release(const int* __restric
 
 // ---- their moves ----------------------------------------------------------------------------------------------------
 //
-// Sources lie behind all places that are written, so moves run in any order.  Bound by bytes; K's rows are pieces of 64
-// bytes, but a row of V is one element of each of HD runs of 32 rows.  Moves ascend on both sides, so 32 of them in a row
-// touch a few blocks only: lane l takes move l % 32, and a wave's load of one dim, or its store, falls into one or two
-// runs.
-constexpr int MOVES = 32;  // that a workgroup does at a time
+// Sources lie behind all places that are written, so moves run in any order.  Bound by memory: K's rows are pieces of 64
+// bytes, but a row of V is one element of each of HD runs of 32 rows.  Moves ascend on both sides, so many of them on end touch
+// few blocks: lane l takes move l % N of N, and a wave's load of a dim, or its store, falls into one or two runs.  Where a
+// head has few moves, each a block of its own, smaller N spread them over more workgroups.
+constexpr int MOVES = 32;  // that a workgroup does at a time, at most
+
+template <int HD, int N>
+__device__ __forceinline__ void move_rows(const int* mv, int n, const int* tb, size_t h, int HK, int lps, int max_blocks, int n_pages,
+                                          size_t pstride, uint16_t* Kp, uint16_t* Vp, float* scores, int* kpos,
+                                          size_t (&off)[2][MOVES], int (&row)[2][MOVES]) {
+    const int tid = threadIdx.x, l = tid % N;
+    const long long rows = (long long)max_blocks << lps;
+    for (int i0 = blockIdx.x * N; i0 < n; i0 += gridDim.x * N) {
+        __syncthreads();
+        if (tid < 2 * N) {  // (in the first wave: lane l has move l's place, lane N + l its row)
+            const int side = tid / N, j = i0 + l < n ? mv[2 * (i0 + l) + side] : -1;
+            const bool in = j >= 0 && j < rows;
+            const int page = in ? tb[j >> lps] : -1;
+            const bool there = (unsigned)page < (unsigned)n_pages;
+            const int other = __shfl_xor((int)there, N);  // (all lanes: not behind a branch)
+            const bool both = there && other;
+            off[side][l] = (size_t)(there ? page : 0) * pstride + ((h << (lps - 5)) + ((j & ((1 << lps) - 1)) >> 5)) * (HD * 32);
+            row[side][l] = both ? j & 31 : -1;
+            const size_t at = mark_at(there ? page : 0, HK, (int)h, j, lps);
+            const size_t to = __shfl(at, l);
+            if (side && both) {
+                if (scores) scores[to] = scores[at];
+                if (kpos) kpos[to] = kpos[at];
+            }
+        }
+        __syncthreads();
+        constexpr int P = HD / 8, KN = (N * P + 255) / 256;  // 16-byte pieces of a row of K; those of a thread
+        u32x4 k[KN];
+#pragma unroll
+        for (int x = 0; x < KN; x++) {
+            const int i = (tid + 256 * x) / P, p = (tid + 256 * x) % P;
+            if (i < N && row[1][i] >= 0) k[x] = *reinterpret_cast<const u32x4*>(Kp + off[1][i] + (p >> 2) * 1024 + row[1][i] * 32 + (p & 3) * 8);
+        }
+        constexpr int STEP = 256 / N, VN = (HD + STEP - 1) / STEP;  // dims side by side; dims of a thread
+        uint16_t v[VN];
+        const bool mine = row[0][l] >= 0 && tid / N < HD;
+        const uint16_t* const from = Vp + off[1][l] + row[1][l] + tid / N * 32;
+        uint16_t* const to = Vp + off[0][l] + row[0][l] + tid / N * 32;
+        if (mine) {
+#pragma unroll
+            for (int x = 0; x < VN; x++) v[x] = from[x * STEP * 32];
+        }
+#pragma unroll
+        for (int x = 0; x < KN; x++) {
+            const int i = (tid + 256 * x) / P, p = (tid + 256 * x) % P;
+            if (i < N && row[0][i] >= 0) *reinterpret_cast<u32x4*>(Kp + off[0][i] + (p >> 2) * 1024 + row[0][i] * 32 + (p & 3) * 8) = k[x];
+        }
+        if (mine) {
+#pragma unroll
+            for (int x = 0; x < VN; x++) to[x * STEP * 32] = v[x];
+        }
+    }
+}
 
 template <int HD>
 __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ moves, const int* __restrict__ counts,
@@ -1326,57 +1379,17 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
                                                     int* kpos) {
     __shared__ size_t off[2][MOVES];  // of a move's place and row: their blocks, in a cache
     __shared__ int row[2][MOVES];     // and the rows there; -1: no move
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, l = tid % MOVES;
+    const int h = blockIdx.y, b = blockIdx.z;
     const size_t bh = (size_t)b * HK + h;
-    const int n = min(counts[bh], W);
+    const int n = min(counts[bh], W), each = n / (int)gridDim.x;
     const int* const mv = moves + bh * W * 2;
     const int* const tb = table + (size_t)b * max_blocks;
-    const long long rows = (long long)max_blocks << lps;
-    for (int i0 = blockIdx.x * MOVES; i0 < n; i0 += gridDim.x * MOVES) {
-        __syncthreads();
-        if (tid < 2 * MOVES) {  // (the first wave: lane l has move l's place, lane 32 + l its row)
-            const int side = tid / MOVES, j = i0 + l < n ? mv[2 * (i0 + l) + side] : -1;
-            const bool in = j >= 0 && j < rows;
-            const int page = in ? tb[j >> lps] : -1;
-            const bool there = (unsigned)page < (unsigned)n_pages;
-            const int other = __shfl_xor((int)there, MOVES);  // (all lanes: not behind a branch)
-            const bool both = there && other;
-            off[side][l] = (size_t)(there ? page : 0) * pstride + ((size_t)(h << (lps - 5)) + ((j & ((1 << lps) - 1)) >> 5)) * (HD * 32);
-            row[side][l] = both ? j & 31 : -1;
-            const size_t at = mark_at(there ? page : 0, HK, h, j, lps);
-            const size_t to = __shfl(at, l);
-            if (side && both) {
-                if (scores) scores[to] = scores[at];
-                if (kpos) kpos[to] = kpos[at];
-            }
-        }
-        __syncthreads();
-        constexpr int P = HD / 8, KN = MOVES * P / 256;  // 16-byte pieces of a row of K; those of a thread
-        u32x4 k[KN];
-#pragma unroll
-        for (int x = 0; x < KN; x++) {
-            const int i = (tid + 256 * x) / P, p = (tid + 256 * x) % P;
-            if (row[1][i] >= 0) k[x] = *reinterpret_cast<const u32x4*>(Kp + off[1][i] + (p >> 2) * 1024 + row[1][i] * 32 + (p & 3) * 8);
-        }
-        constexpr int VN = HD / 8;  // dims of a thread
-        uint16_t v[VN];
-        const bool mine = row[0][l] >= 0;
-        const uint16_t* const from = Vp + off[1][l] + row[1][l] + tid / MOVES * 32;
-        uint16_t* const to = Vp + off[0][l] + row[0][l] + tid / MOVES * 32;
-        if (mine) {
-#pragma unroll
-            for (int x = 0; x < VN; x++) v[x] = from[x * 256];
-        }
-#pragma unroll
-        for (int x = 0; x < KN; x++) {
-            const int i = (tid + 256 * x) / P, p = (tid + 256 * x) % P;
-            if (row[0][i] >= 0) *reinterpret_cast<u32x4*>(Kp + off[0][i] + (p >> 2) * 1024 + row[0][i] * 32 + (p & 3) * 8) = k[x];
-        }
-        if (mine) {
-#pragma unroll
-            for (int x = 0; x < VN; x++) to[x * 256] = v[x];
-        }
-    }
+    auto run = [&](auto c) INL {
+        move_rows<HD, decltype(c)::value>(mv, n, tb, h, HK, lps, max_blocks, n_pages, pstride, Kp, Vp, scores, kpos, off, row);
+    };
+    if (each >= 12) run(std::integral_constant<int, 32>());
+    else if (each >= 4) run(std::integral_constant<int, 8>());
+    else run(std::integral_constant<int, 4>());
 }
 
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
@@ -1547,7 +1560,7 @@ void page_release(const PageRelease& a, hipStream_t st) {
 void paged_move(const PagedShape& s, const PagedMove& a, hipStream_t st) {
     const int W = std::max(a.max_kv / 2, 1);
     auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(std::min((W + MOVES - 1) / MOVES, std::max(1, 2048 / (s.HK * a.B))), s.HK, a.B), dim3(256), 0, st, a.moves,
+        hipLaunchKernelGGL(kernel, dim3(std::min((W + 3) / 4, std::max(1, 2048 / (s.HK * a.B))), s.HK, a.B), dim3(256), 0, st, a.moves,
                            a.counts, a.table, a.max_blocks, W, s.HK, log2i(s.PS), s.n_pages, s.pstride,
                            static_cast<uint16_t*>(a.Kp), static_cast<uint16_t*>(a.Vp), a.scores, a.kpos);
     };

@@ -54,19 +54,28 @@ template <class T>
 struct RopeSide {  // q's or k's heads
     const T* in;
     T* out;
-    size_t stride, step, ostride, ostep;
+    uint32_t stride, step, ostride, ostep;
+};
+// Division by a number that is the same for all, as one upper half of a product: exact where the dividend times it is below 2^32.
+struct Div {
+    uint32_t d, magic;
+    explicit Div(uint32_t n) : d(n), magic((uint32_t)((1ull << 32) / n + 1)) {}
+    __device__ __forceinline__ uint32_t of(uint32_t x) const { return d == 1 ? x : __umulhi(x, magic); }
 };
 template <class T, int MODE, int N>
 __global__ __launch_bounds__(256) void k_rope(const double* __restrict__ freqs, int RD, double m, float sign,
                                               const int* __restrict__ pos, int rows, int HD, RopeSide<T> q, int HQ,
-                                              RopeSide<T> k, uint32_t heads, uint32_t turning, uint32_t units, int R,
-                                              uint32_t slices) {
+                                              RopeSide<T> k, Div per, uint32_t turning, Div units, int R, uint32_t slices) {
     typedef T T8 __attribute__((ext_vector_type(8), aligned(16)));
     __shared__ Turn turns[MAX_R * 128];
     const int tid = threadIdx.x, rd2 = RD / 2;
     const uint32_t slice = slices == 1 ? 0 : blockIdx.x % slices;
     const int r0 = (slices == 1 ? blockIdx.x : blockIdx.x / slices) * R, nr = min(R, rows - r0);
-    const uint32_t per = heads * units, first = slice * (256 * N), last = min((uint32_t)nr * per, first + 256 * N);
+    const uint32_t first = slice * (256 * N), last = min((uint32_t)nr * per.d, first + 256 * N);  // (R is 1 where a row has several slices)
+    const T* const q0 = q.in + (size_t)r0 * q.stride;
+    const T* const k0 = k.in + (size_t)r0 * k.stride;
+    T* const q1 = q.out + (size_t)r0 * q.ostride;
+    T* const k1 = k.out + (size_t)r0 * k.ostride;
     T8 a[N], b[N];
     const T* src[N];
     T* dst[N];
@@ -75,15 +84,13 @@ __global__ __launch_bounds__(256) void k_rope(const double* __restrict__ freqs, 
     for (int n = 0; n < N; n++) {
         const uint32_t i = first + n * 256 + tid;
         if (i >= last) continue;
-        row[n] = i / per;
-        const uint32_t x = i - row[n] * per, h = x / units;
-        at[n] = x - h * units;
-        const size_t t = r0 + row[n];
+        row[n] = slices == 1 ? per.of(i) : 0;
+        const uint32_t x = i - row[n] * per.d, h = units.of(x);
+        at[n] = x - h * units.d;
         const bool isq = h < (uint32_t)HQ;
-        const RopeSide<T>& s = isq ? q : k;
         const uint32_t hh = isq ? h : h - HQ;
-        src[n] = s.in + t * s.stride + hh * s.step;
-        dst[n] = s.out + t * s.ostride + hh * s.ostep;
+        src[n] = (isq ? q0 : k0) + (uint64_t)row[n] * (isq ? q.stride : k.stride) + (uint64_t)hh * (isq ? q.step : k.step);
+        dst[n] = (isq ? q1 : k1) + (uint64_t)row[n] * (isq ? q.ostride : k.ostride) + (uint64_t)hh * (isq ? q.ostep : k.ostep);
         if (MODE == ODD) continue;
         if (at[n] < turning) {
             a[n] = *reinterpret_cast<const T8*>(src[n] + 8 * at[n]);
@@ -173,7 +180,8 @@ void rope_as(const RopeRows& a, hipStream_t st) {
     const uint32_t units = turning + (moved ? copied : 0), heads = a.HQ + a.HK;
     const size_t per = (size_t)heads * units, total = per * a.rows;
     auto side = [](const RopeHeads& h) {
-        return RopeSide<T>{static_cast<const T*>(h.in), static_cast<T*>(h.out), h.stride, h.step, h.ostride, h.ostep};
+        return RopeSide<T>{static_cast<const T*>(h.in), static_cast<T*>(h.out), (uint32_t)h.stride, (uint32_t)h.step,
+                           (uint32_t)h.ostride, (uint32_t)h.ostep};
     };
     auto launch = [&](auto kernel, int N) {
         const size_t wg = 256 * (size_t)N, slices = (per + wg - 1) / wg;
@@ -181,8 +189,7 @@ void rope_as(const RopeRows& a, hipStream_t st) {
         const size_t groups = (a.rows + R - 1) / R * slices;
         if (groups >= size_t(1) << 24) throw Error("sd_op_rope: too many rows for one launch");
         hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, st, a.freqs, a.RD, a.magnitude,
-                           a.inverse ? -1.f : 1.f, a.pos, a.rows, a.HD, side(a.q), a.HQ, side(a.k), heads, turning, units, R,
-                           (uint32_t)slices);
+                           a.inverse ? -1.f : 1.f, a.pos, a.rows, a.HD, side(a.q), a.HQ, side(a.k), Div((uint32_t)per), turning, Div(units), R, (uint32_t)slices);
         launched("rope");
     };
     auto sized = [&](auto mode_c) {
