@@ -406,8 +406,8 @@ int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK
  *          + the sum of w[t][g][j] over the request's last `observers` new rows t (0: all) and the heads g of h,
  * and its new rows kpos[j] = pos[t] (pos i32 [T]; both null: none).  All in f32; a row t that sees no key, or -inf alone,
  * adds nothing; where its scores hold NaN or +inf, all keys that it sees become NaN.  Sums have one order: equal calls
- * give equal bits.  out may be scores; other rows of both are left as they are.  max_new, max_kv and ws as in
- * sd_op_paged_attention, sized by sd_op_paged_weights_ws. */
+ * give equal bits.  out may be scores; other rows of both are left as they are; a row that two of the step's requests share
+ * receives either's.  max_new, max_kv and ws as in sd_op_paged_attention, sized by sd_op_paged_weights_ws. */
 int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int max_blocks, const void* cu, const void* kv_lens,
                         const void* pos, int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int page_size,
                         int n_pages, size_t page_stride, int window, float scale, int observers, float decay,
@@ -424,7 +424,8 @@ int sd_op_page_evict_ws(int B, int max_kv, int HK, size_t* bytes, char* err, siz
  *   new_lens [B]: m where rows go, kv_lens[b] elsewhere
  *   counts   [B][HK], moves [B][HK][max(max_kv / 2, 1)][2]: the head's moves, pairs (place, row): the places below m whose
  *            rows go, ascending, and the rows from m on that stay, ascending; entries behind the count are left as they are
- * ws holds what sd_op_page_evict_ws says, 16-byte aligned.  No output overlaps an input or another output. */
+ * ws holds what sd_op_page_evict_ws says, 16-byte aligned, and is free again when the call's kernels have run: calls that may
+ * overlap, captured graphs among them, need one each.  No output overlaps an input or another output. */
 int sd_op_page_evict(const void* scores, const void* kpos, const void* table, int max_blocks, const void* kv_lens,
                      const void* budgets, int B, int max_kv, int HK, int page_size, int n_pages, int sink, int recent,
                      void* new_lens, void* moves, void* counts, void* ws, size_t ws_bytes, void* stream, char* err,

@@ -1325,7 +1325,11 @@ __device__ __forceinline__ void move_rows(const int* mv, int n, const int* tb, s
                                           size_t (&off)[2][MOVES], int (&row)[2][MOVES]) {
     const int tid = threadIdx.x, l = tid % N;
     const long long rows = (long long)max_blocks << lps;
-    for (int i0 = blockIdx.x * N; i0 < n; i0 += gridDim.x * N) {
+    // Groups of N moves: an XCD (every eighth workgroup) takes adjacent ones, which share blocks in its L2.
+    const int groups = (n + N - 1) / N, X = min((int)gridDim.x, 8), per = (groups + X - 1) / X, x0 = blockIdx.x % X * per;
+    const int wgs = (gridDim.x - blockIdx.x % X + X - 1) / X;  // of this XCD
+    for (int y = blockIdx.x / X; y < per && x0 + y < groups; y += wgs) {
+        const int i0 = (x0 + y) * N;
         __syncthreads();
         if (tid < 2 * N) {  // (in the first wave: lane l has move l's place, lane N + l its row)
             const int side = tid / N, j = i0 + l < n ? mv[2 * (i0 + l) + side] : -1;
@@ -1428,13 +1432,14 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         p.span = std::max(8, (nb + want - 1) / want);
         p.ks = (nb + p.span - 1) / p.span;
         const int nkb = (int)(((long long)max_kv + KEY_TILE - 1) / KEY_TILE);
-        // parts of at least 256 rows, so many that there are 2048 workgroups, and of fewer than 2^30 bytes of Q
+        // parts of at least 256 rows, so many that there are 2048 workgroups; of at most 16384 (a lane then adds up 512 weights on
+        // end), and of fewer than 2^30 bytes of Q
         const long long wanted = std::max(1ll, 2048ll / ((long long)nkb * s.HK));
-        p.part = (int)(std::max(256ll, (all + wanted - 1) / wanted) + G - 1) / G;
+        p.part = (int)((std::min(16384ll, std::max(256ll, (all + wanted - 1) / wanted)) + G - 1) / G);
         p.part = (int)std::min<long long>(p.part, std::max(1ll, (1ll << 29) / ((long long)s.HQ * s.HD)));
         p.parts = (tokens + p.part - 1) / p.part;
         const long long units = (long long)nkb * std::min(reqs * p.parts, all / G / p.part + reqs);
-        if (units * s.HK >= 1 << 24 || (long long)(p.tiles | 1) * s.HK * p.ks >= 1 << 24)
+        if (units * s.HK >= 1 << 24 || (long long)(p.tiles | 1) * s.HK * std::max(p.ks, 32) >= 1 << 24)
             throw Error("sd_op_paged_weights: too many rows and keys for one launch");
         p.units = (int)units;
         p.ml = p.ks > 1 ? (size_t)p.ks * p.tiles * s.HK * ROW_TILE * 2 : 0;
