@@ -553,13 +553,7 @@ __device__ __forceinline__ int first_key_tile(const WeightArgs& a, int b) {
         before += r < b ? n : 0;
         own = min(own + (r < a.B ? n : 0), 1 << 24);
     }
-    int to = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(to, o);
-        if (lane >= o) to += y;
-    }
-    return __shfl(to - own + before, b & 63);
+    return __shfl(lanes_upto(own) - own + before, b & 63);
 }
 // The tokens [lo, hi) of a request that see some key of [j0, j0 + 128).
 __device__ __forceinline__ void tokens_of(const WeightArgs& a, const Req& rq, const Seen& ob, int j0, int& lo, int& hi) {
@@ -759,21 +753,6 @@ __device__ __forceinline__ uint32_t rank_of(float s) {
 
 constexpr int EVICT_T = 1024, BINS = 2048;
 constexpr int EVICT_ONE = 32768;  // rows up to which one workgroup does a head
-
-// The sum over lanes 0 to the own, by moves between lanes: within rows of 16, then from each row's last lane on.
-__device__ __forceinline__ int lanes_upto(int x) {
-    auto add = [&](auto ctrl, auto rows) {
-        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-    };
-    using std::integral_constant;
-    add(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // 1 lane up in each row
-    add(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());  // 2
-    add(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());  // 4
-    add(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());  // 8
-    add(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());  // rows 0 and 2 into 1 and 3
-    add(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());  // the lower half into the upper
-    return x;
-}
 
 // The sum over the threads before this one, and over all; `ws` holds EVICT_T / 64 sums.
 __device__ __forceinline__ int scan(int x, int* ws, int& total) {
@@ -1432,9 +1411,9 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         p.span = std::max(8, (nb + want - 1) / want);
         p.ks = (nb + p.span - 1) / p.span;
         const int nkb = (int)(((long long)max_kv + KEY_TILE - 1) / KEY_TILE);
-        // parts of at least 256 rows, so many that there are 2048 workgroups; of at most 16384 (a lane then adds up 512 weights on
+        // parts of at least 256 rows, so many that there are 4096 workgroups; of at most 16384 (a lane then adds up 512 weights on
         // end), and of fewer than 2^30 bytes of Q
-        const long long wanted = std::max(1ll, 2048ll / ((long long)nkb * s.HK));
+        const long long wanted = std::max(1ll, 4096ll / ((long long)nkb * s.HK));
         p.part = (int)((std::min(16384ll, std::max(256ll, (all + wanted - 1) / wanted)) + G - 1) / G);
         p.part = (int)std::min<long long>(p.part, std::max(1ll, (1ll << 29) / ((long long)s.HQ * s.HD)));
         p.parts = (tokens + p.part - 1) / p.part;

@@ -135,6 +135,21 @@ __device__ __forceinline__ Req request(const int* __restrict__ cu, const int* __
     return r;
 }
 
+// The sum over lanes 0 to the own, by moves between lanes: within rows of 16, then from each row's last lane on.
+__device__ __forceinline__ int lanes_upto(int x) {
+    auto add = [&](auto ctrl, auto rows) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // 1 lane up in each row
+    add(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());  // 2
+    add(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());  // 4
+    add(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());  // 8
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());  // rows 0 and 2 into 1 and 3
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());  // the lower half into the upper
+    return x;
+}
+
 struct Tile {
     int b, i;  // request and tile in it; b < 0: none
     int x;     // its number
@@ -151,27 +166,19 @@ __device__ __forceinline__ Tile find_tile(int B, int x, F&& of) {
         const int n = of(min(b, B - 1));
         return b < B ? n : 0;  // (no branch: several loads in flight)
     };
-    auto upto = [&](int v) {  // the sum of lanes 0 to the own
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(v, o);
-            if (lane >= o) v += y;
-        }
-        return v;
-    };
     // lane l counts requests l, l + 64, ..., the tiles are numbered lane by lane
     // (cut at 2^24 per lane, which row starts that do not ascend could pass: the sums stay in range)
     int own = 0;
 #pragma unroll 8
     for (int i = 0; i < per; i++) own = min(own + tiles(64 * i + lane), 1 << 24);
-    const int to = upto(own), total = __builtin_amdgcn_readlane(to, 63);
+    const int to = lanes_upto(own), total = __builtin_amdgcn_readlane(to, 63);
     if (x >= total) return {-1, 0, 0};
     const int number = x = total - 1 - x;
     const int at = __ffsll((long long)__ballot(to > x)) - 1;
     x -= __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(own, at);
     if (per == 1) return {at, x, number};
     for (int i = 0; i < per; i += 64) {  // lane l: request 64 (i + l) + at
-        const int n = i + lane < per ? tiles(64 * (i + lane) + at) : 0, t = upto(n), sum = __builtin_amdgcn_readlane(t, 63);
+        const int n = i + lane < per ? tiles(64 * (i + lane) + at) : 0, t = lanes_upto(n), sum = __builtin_amdgcn_readlane(t, 63);
         if (x < sum) {
             const int l = __ffsll((long long)__ballot(t > x)) - 1;
             return {64 * (i + l) + at, x - (__builtin_amdgcn_readlane(t, l) - __builtin_amdgcn_readlane(n, l)), number};
