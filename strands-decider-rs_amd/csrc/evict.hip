@@ -112,27 +112,37 @@ __device__ __forceinline__ void put_weight(const WeightArgs& a, const Req& rq, s
 
 // ---- few rows ----
 
-constexpr int FEW_W = 2;  // waves of a workgroup
+// What a few rows' kernel does with a request: its rows, the first one's position, and the keys [lo, hi) that some row sees.
+struct Few {
+    Req rq;
+    Seen ob;
+    int nrows, p0, lo, hi;
+};
+__device__ __forceinline__ Few few_of(const WeightArgs& a, int b) {
+    Few f;
+    f.rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    f.ob = observed(f.rq, a.observers);
+    f.nrows = f.ob.n * a.G;
+    f.p0 = f.rq.p0 + f.ob.t0;
+    f.hi = min(f.p0 + f.ob.n, f.rq.kcap);
+    f.lo = max(0, a.from(f.p0));
+    return f;
+}
 
-// Scores of up to 16 NR rows of a (request, kv head) over this workgroup's blocks of keys, and the rows' maxima and sums
-// over them.  A wave loads K straight into registers in MFMA operand order, D blocks of 32 keys in flight.
-template <class T, int HD, int NR, bool ONCE>
-__global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+// Scores of up to 16 NR rows of a (request, kv head) over blocks [blk0, blk1) of keys, by NW waves, into S (rows `stride`
+// floats apart, key j at j), and each wave's maxima and sums of the rows over them.  A wave loads K straight into registers
+// in MFMA operand order, D blocks of 32 keys in flight.
+template <class T, int HD, int NR, bool ONCE, int NW>
+__device__ __forceinline__ void few_scores(const T* __restrict__ Q, const T* __restrict__ Kp, const WeightArgs& a, const Few& f, int b,
+                                           int kh, int blk0, int blk1, float* S, int stride, float* Ms, float* Ls) {
     typedef typename Vec8<T>::type T8;
     constexpr int NS = HD / 32, R = 16 * NR, D = HD == 64 ? 4 : HD == 128 ? 3 : 2;
-    __shared__ float Ms[FEW_W * R], Ls[FEW_W * R];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fq = lane & 15, fg = lane >> 4;
-    const int kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
-    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
-    const Seen ob = observed(rq, a.observers);
-    const int nrows = ob.n * a.G;
-    if (nrows == 0 || nrows > a.few) return;
-    const int p0 = rq.p0 + ob.t0;  // position of the first row
-    const int hi = min(p0 + ob.n, rq.kcap), lo = max(0, a.from(p0));
-    const int blk0 = (lo >> 5) + z * a.few_span;
-    const int blk1 = z + 1 < a.few_ks ? min((hi + 31) >> 5, blk0 + a.few_span) : (hi + 31) >> 5;
-    const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + FEW_W - 1) / FEW_W : 0;
+    const Req& rq = f.rq;
+    const Seen& ob = f.ob;
+    const int nrows = f.nrows, p0 = f.p0, hi = f.hi;
+    const int first = blk0 + wv, cnt = first < blk1 ? (blk1 - first + NW - 1) / NW : 0;
     int jlo[NR], jhi[NR];  // keys [jlo, jhi) are seen by this lane's row
     T8 qf[NR][NS];
 #pragma unroll
@@ -148,7 +158,7 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
     const int lbpp = a.lps - 5;
     const int* const tb = a.table + (size_t)b * a.max_blocks;
     auto entries = [&](int i) {  // lane l: the table entry of the wave's block i + l
-        return tb[min((first + FEW_W * (i + lane)) >> lbpp, a.max_blocks - 1)];
+        return tb[min((first + NW * (i + lane)) >> lbpp, a.max_blocks - 1)];
     };
     int ids = cnt ? entries(0) : 0, ids2 = cnt > 64 ? entries(64) : 0;
     // rows of K in the order in which a lane's 8 scores are 8 keys on end: j0 + 8 fg + e
@@ -161,7 +171,7 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
         bool there;
     };
     auto load = [&](int i, Blk& x) INL {
-        const int page = __builtin_amdgcn_readlane(ids, i & 63), blk = first + FEW_W * i;
+        const int page = __builtin_amdgcn_readlane(ids, i & 63), blk = first + NW * i;
         x.there = i < cnt && (unsigned)page < (unsigned)a.n_pages;
         const size_t at = x.there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
         const Rsrc rk = make_rsrc(Kp + at, x.there ? HD * 64u : 0u);
@@ -170,9 +180,8 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
 #pragma unroll
             for (int tt = 0; tt < 2; tt++) x.k[tt][s] = load16<ONCE>(rk, kofs + tt * 256, s * 2048);
     };
-    float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp + 8 * fg;
     auto work = [&](int i, Blk& x) INL {
-        const int j0 = (first + FEW_W * i) * 32;
+        const int j0 = (first + NW * i) * 32;
         const bool open = x.there && j0 >= open0 && j0 + 32 <= open1;
         f32x4 s2[NR][2];
 #pragma unroll
@@ -197,7 +206,7 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
                 }
             }
             if (16 * u + fq < nrows) {
-                f32x4* const to = reinterpret_cast<f32x4*>(S + (size_t)(16 * u + fq) * a.kvp + j0);
+                f32x4* const to = reinterpret_cast<f32x4*>(S + (size_t)(16 * u + fq) * stride + j0 + 8 * fg);
                 to[0] = s2[u][0], to[1] = s2[u][1];
             }
             float mn = m[u];
@@ -238,8 +247,23 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
         sum += __shfl_xor(sum, 32);
         if (fg == 0) Ms[wv * R + 16 * u + fq] = mx, Ls[wv * R + 16 * u + fq] = sum;
     }
+}
+
+constexpr int FEW_W = 2;  // waves of a workgroup
+
+// A split of the keys per workgroup.
+template <class T, int HD, int NR, bool ONCE>
+__global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    constexpr int R = 16 * NR;
+    __shared__ float Ms[FEW_W * R], Ls[FEW_W * R];
+    const int tid = threadIdx.x, kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
+    const Few f = few_of(a, b);
+    if (f.nrows == 0 || f.nrows > a.few) return;
+    const int blk0 = (f.lo >> 5) + z * a.few_span;
+    const int blk1 = z + 1 < a.few_ks ? min((f.hi + 31) >> 5, blk0 + a.few_span) : (f.hi + 31) >> 5;
+    few_scores<T, HD, NR, ONCE, FEW_W>(Q, Kp, a, f, b, kh, blk0, blk1, a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp, a.kvp, Ms, Ls);
     __syncthreads();
-    if (tid < nrows) {
+    if (tid < f.nrows) {
         float mx = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < FEW_W; w++) mx = fmaxf(mx, Ms[w * R + tid]);
@@ -249,38 +273,79 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
     }
 }
 
-// The few rows' weights, from their scores: 4 keys per thread, after every workgroup has joined the rows' parts, 8 threads
-// a row.
+// 4 keys from j on: their place, and what they have.
+struct Keys4 {
+    int page;
+    size_t at;
+    f32x4u old;
+};
+__device__ __forceinline__ Keys4 keys4(const WeightArgs& a, const Few& f, int b, int kh, int j) {
+    Keys4 k;
+    k.page = a.table[(size_t)b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
+    const bool there = j < f.rq.kcap && (unsigned)k.page < (unsigned)a.n_pages;
+    k.at = mark_at(there ? k.page : 0, a.HK, kh, there ? j : 0, a.lps);
+    k.old = f32x4u{0.f, 0.f, 0.f, 0.f};
+    if (there && a.decay != 0.f) k.old = *reinterpret_cast<const f32x4u*>(a.scores + k.at);
+    return k;
+}
+__device__ __forceinline__ bool some_seen(const Few& f, int j) { return j > f.lo - 4 && j < f.hi; }  // (scores outside were not written)
+
+// Their weights of the rows, x(r) their scores of row r, PRE of which come from `pre`; into the cached keys' scores.
+template <int PRE, class X>
+__device__ __forceinline__ void weigh4(const WeightArgs& a, const Few& f, int j, const Keys4& k, const float2* stat, const f32x4* pre, X&& x) {
+    if (j >= f.rq.kcap || (unsigned)k.page >= (unsigned)a.n_pages) return;
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    if (some_seen(f, j)) {
+        int t = 0, g = 0;
+        auto add = [&](int r, f32x4 x) INL {
+            const float2 st = stat[r];
+            const int jlo = a.from(f.p0 + t), jhi = min(f.p0 + t + 1, f.hi);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool keep = (j + e >= jlo) & (j + e < jhi);
+                w[e] += keep ? exp2_fast(x[e] - st.x) * st.y : 0.f;
+            }
+            if (++g == a.G) g = 0, t++;
+        };
+#pragma unroll
+        for (int r = 0; r < PRE; r++)
+            if (r < f.nrows) add(r, pre[r]);
+#pragma unroll 4
+        for (int r = PRE; r < f.nrows; r++) add(r, x(r));
+    }
+    if (j <= min(f.rq.p0, f.rq.kcap) - 4) {
+        f32x4u y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = a.decay != 0.f ? __builtin_fmaf(a.decay, k.old[e], w[e]) : w[e];
+        *reinterpret_cast<f32x4u*>(a.out + k.at) = y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (j + e < f.rq.kcap) put_weight(a, f.rq, k.at + e, j + e, w[e]);
+    }
+}
+
+// The weights of the few rows' splits, from their scores: 4 keys per thread, after every workgroup has joined the rows' parts.
 __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     constexpr int PRE = 4;
     __shared__ float2 stat[32];
     const int tid = threadIdx.x, kh = blockIdx.x % a.HK, b = blockIdx.y;
     const int c0 = blockIdx.x / a.HK * 1024, step = gridDim.x / a.HK * 1024;  // (with 8 heads a head's scores stay with one XCD's L2)
-    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
-    const Seen ob = observed(rq, a.observers);
-    const int nrows = ob.n * a.G;
-    if (nrows == 0 || nrows > a.few || c0 >= rq.kcap) return;
-    const int p0 = rq.p0 + ob.t0, hi = min(p0 + ob.n, rq.kcap), lo = max(0, a.from(p0));
+    const Few f = few_of(a, b);
+    const int nrows = f.nrows;
+    if (nrows == 0 || nrows > a.few || c0 >= f.rq.kcap) return;
     const float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp;
-    const int* const tb = a.table + (size_t)b * a.max_blocks;
-    struct Keys {  // 4 keys: their place, what they have, and the scores of the first PRE rows
-        int page;
-        size_t at;
-        f32x4u old;
-        f32x4 x[PRE];
+    struct Keys {
+        Keys4 k;
+        f32x4 x[PRE];  // the scores of the first PRE rows
     };
     auto load = [&](int j) INL {
         Keys k;
-        k.page = tb[min(j >> a.lps, a.max_blocks - 1)];
-        const bool there = j < rq.kcap && (unsigned)k.page < (unsigned)a.n_pages;
-        k.at = mark_at(there ? k.page : 0, a.HK, kh, there ? j : 0, a.lps);
-        k.old = f32x4u{0.f, 0.f, 0.f, 0.f};
-        if (there && a.decay != 0.f) k.old = *reinterpret_cast<const f32x4u*>(a.scores + k.at);
-        const bool seen = j > lo - 4 && j < hi;  // (scores outside were not written)
+        k.k = keys4(a, f, b, kh, j);
 #pragma unroll
         for (int r = 0; r < PRE; r++) {
             k.x[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (seen && r < nrows) k.x[r] = *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp + j);
+            if (some_seen(f, j) && r < nrows) k.x[r] = *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp + j);
         }
         return k;
     };
@@ -296,44 +361,45 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
         }
     }
     __syncthreads();
-    auto put = [&](int j, const Keys& now) INL {
-        f32x4 w = {0.f, 0.f, 0.f, 0.f};
-        if (j > lo - 4 && j < hi) {
-            int t = 0, g = 0;
-            auto add = [&](int r, f32x4 x) INL {
-                const float2 st = stat[r];
-                const int jlo = a.from(p0 + t), jhi = min(p0 + t + 1, hi);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool keep = (j + e >= jlo) & (j + e < jhi);
-                    w[e] += keep ? exp2_fast(x[e] - st.x) * st.y : 0.f;
-                }
-                if (++g == a.G) g = 0, t++;
-            };
-#pragma unroll
-            for (int r = 0; r < PRE; r++)
-                if (r < nrows) add(r, now.x[r]);
-#pragma unroll 4
-            for (int r = PRE; r < nrows; r++) add(r, *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp + j));
-        }
-        if (j <= min(rq.p0, rq.kcap) - 4) {
-            f32x4u y;
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = a.decay != 0.f ? __builtin_fmaf(a.decay, now.old[e], w[e]) : w[e];
-            *reinterpret_cast<f32x4u*>(a.out + now.at) = y;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (j + e < rq.kcap) put_weight(a, rq, now.at + e, j + e, w[e]);
-        }
-    };
     for (int j0 = c0;; j0 += step) {
         const int j = j0 + 4 * tid;
         const Keys now = k;
-        const bool more = step < rq.kcap - j0;
+        const bool more = step < f.rq.kcap - j0;
         if (more) k = load(j + step);
-        if (j < rq.kcap && (unsigned)now.page < (unsigned)a.n_pages) put(j, now);
+        weigh4<PRE>(a, f, j, now.k, stat, now.x, [&](int r) { return *reinterpret_cast<const f32x4*>(S + (size_t)r * a.kvp + j); });
         if (!more) break;
+    }
+}
+
+// Short caches: a (request, kv head) per workgroup, its scores in LDS, in one launch.
+constexpr int ONE_W = 8, ONE_LDS = 136 << 10, ONE_KEYS = 8192;  // waves; bytes of scores, and keys, at most
+template <class T, int HD, int NR, bool ONCE>
+__global__ __launch_bounds__(64 * ONE_W) void k_weights_few_one(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+    constexpr int R = 16 * NR, KN = ONE_KEYS / (256 * ONE_W);
+    extern __shared__ __align__(16) float S[];
+    __shared__ float Ms[ONE_W * R], Ls[ONE_W * R];
+    __shared__ float2 stat[R];
+    const int tid = threadIdx.x, kh = blockIdx.x, b = blockIdx.y;
+    const Few f = few_of(a, b);
+    if (f.nrows == 0 || f.nrows > a.few) return;
+    Keys4 k[KN];  // (on their way meanwhile)
+#pragma unroll
+    for (int i = 0; i < KN; i++) k[i] = keys4(a, f, b, kh, 4 * (tid + 64 * ONE_W * i));
+    few_scores<T, HD, NR, ONCE, ONE_W>(Q, Kp, a, f, b, kh, f.lo >> 5, (f.hi + 31) >> 5, S, a.kvp, Ms, Ls);
+    __syncthreads();
+    if (tid < f.nrows) {
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < ONE_W; w++) mx = fmaxf(mx, Ms[w * R + tid]);
+#pragma unroll
+        for (int w = 0; w < ONE_W; w++) sum += Ls[w * R + tid] * part_weight(Ms[w * R + tid], mx);
+        stat[tid] = make_float2(base_of(mx), inverse_of(sum));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < KN; i++) {
+        const int j = 4 * (tid + 64 * ONE_W * i);
+        weigh4<0>(a, f, j, k[i], stat, nullptr, [&](int r) { return *reinterpret_cast<const f32x4*>(S + r * a.kvp + j); });
     }
 }
 
@@ -1379,7 +1445,7 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
 struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
     int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0;  // tiles 0: no many rows
-    bool once = false;
+    bool once = false, one = false;  // keys read past the last-level cache; k_weights_few_one
     size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0;  // floats of the workspace
 };
 
@@ -1397,8 +1463,16 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         const int want = std::max(1, std::min(256, 8192 / (B * s.HK)));
         p.few_span = std::max(FEW_W, (nb + want - 1) / want);
         p.few_ks = (nb + p.few_span - 1) / p.few_span;
-        p.S = (size_t)B * s.HK * p.few * p.kvp;
-        p.few_ml = (size_t)B * s.HK * p.few_ks * p.few * 2;
+        // One workgroup per head where there are enough of them, or few bytes of keys for each: one launch, and no scores in memory.
+        // us in splits and so, at n keys of each request:
+        // 2 heads, 256 dims: 300 8.8 7.2, 700 9.1 9.7; 8 heads, 128 dims: 700 9.2 7.4, 1200 9.1 9.3, 2000 9.3 12.0
+        // 128 heads, 256 dims: 700 14.7 11.5, 2000 27.5 23.3; 128 dims: 2000 17.0 13.5, 6000 40.9 41.4, 8100 48.3 51.9
+        // 512 heads, 128 dims: 1200 34.9 27.9, 3800 83 68, 6000 126 101, 8100 171 139; 64 dims: 1200 19.8 13.7, 8100 97 77
+        const size_t each = (size_t)nb * s.HD * 64;
+        p.one = (long long)nb * 32 <= ONE_KEYS && (size_t)p.few * p.kvp * 4 <= ONE_LDS &&
+                (B * s.HK >= 256 || each <= (size_t(B * s.HK >= 128 ? 1024 : 256) << 10));
+        p.S = p.one ? 0 : (size_t)B * s.HK * p.few * p.kvp;
+        p.few_ml = p.one ? 0 : (size_t)B * s.HK * p.few_ks * p.few * 2;
         p.once = (size_t)B * nb * s.HK * s.HD * 64 > (size_t(256) << 20);
         if ((long long)B * s.HK * p.few_ks >= 1 << 24)
             throw Error("sd_op_paged_weights: too many requests and keys for one launch");
@@ -1459,14 +1533,23 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
         }
     }
     if (p.nr) {
-        const dim3 grid(s.HK * p.few_ks, a.B);
-        if (p.nr == 1) {
-            if (p.once) launch(k_weights_few<T, HD, 1, true>, grid, 64 * FEW_W, Q, K, g);
-            else launch(k_weights_few<T, HD, 1, false>, grid, 64 * FEW_W, Q, K, g);
-        } else {
-            if (p.once) launch(k_weights_few<T, HD, 2, true>, grid, 64 * FEW_W, Q, K, g);
-            else launch(k_weights_few<T, HD, 2, false>, grid, 64 * FEW_W, Q, K, g);
-        }
+        auto few = [&](auto nr, auto once) {
+            constexpr int NR = decltype(nr)::value;
+            constexpr bool ONCE = decltype(once)::value;
+            if (p.one) {
+                hipLaunchKernelGGL((k_weights_few_one<T, HD, NR, ONCE>), dim3(s.HK, a.B), dim3(64 * ONE_W), p.few * p.kvp * 4, st, Q, K, g);
+                launched("paged_weights");
+            } else {
+                launch(k_weights_few<T, HD, NR, ONCE>, dim3(s.HK * p.few_ks, a.B), 64 * FEW_W, Q, K, g);
+            }
+        };
+        auto once = [&](auto nr) {
+            if (p.once) few(nr, std::true_type());
+            else few(nr, std::false_type());
+        };
+        if (p.nr == 1) once(std::integral_constant<int, 1>());
+        else once(std::integral_constant<int, 2>());
+        if (p.one) return;
         const long long chunks = ((long long)a.max_kv + 1023) / 1024;  // of 1024 keys; at most so many workgroups that each has some
         launch(k_weights_few_sum, dim3((unsigned)std::min(chunks, std::max(1ll, 16384ll / (s.HK * a.B))) * s.HK, a.B), 256, g);
     }
