@@ -8,6 +8,7 @@ import torch
 
 import evict_ref as er
 import paged_ref as pr
+from launches import launches
 
 pytestmark = pytest.mark.gpu
 KIND = {"f16": 0, "bf16": 1}
@@ -187,27 +188,29 @@ def test_a_request_of_holes_alone(sdamd):
 
 
 @pytest.mark.parametrize("new", [1, 5, 70])
-def test_non_finite_keys_and_queries(sdamd, new):
+@pytest.mark.parametrize("old", [200, 3001])
+def test_non_finite_keys_and_queries(sdamd, old, new):
     """A NaN or infinite score makes the rows that see it NaN, and no others."""
     for bad in (math.nan, math.inf):
-        s = Step(15, [200], [new], 8, 2, 128, 32, "f16")
-        late = 200 + new - 1  # seen by the last row alone
+        s = Step(15, [old], [new], 8, 2, 128, 32, "f16")
+        late = old + new - 1  # seen by the last row alone
         s.k[0][late, 1, 3] = bad
-        s.cache.put(pr.slots_of(s.table, 0, 32, 0, 200 + new), s.k[0], torch.zeros_like(s.k[0]))
+        s.cache.put(pr.slots_of(s.table, 0, 32, 0, old + new), s.k[0], torch.zeros_like(s.k[0]))
         s.q[:, :, 3] = s.q[:, :, 3].abs() + 0.5
         s.run(sdamd)
         s.check()
-        s = Step(16, [200], [new], 8, 2, 128, 32, "f16")
+        s = Step(16, [old], [new], 8, 2, 128, 32, "f16")
         s.q[new // 2, 6, 0] = bad
         s.run(sdamd)
         s.check()
 
 
 @pytest.mark.parametrize("new", [1, 70])
-def test_every_score_minus_infinity(sdamd, new):
-    s = Step(17, [90], [new], 4, 1, 64, 32, "bf16", window=3)
+@pytest.mark.parametrize("old,window", [(90, 3), (90, 0), (5000, 0)])
+def test_every_score_minus_infinity(sdamd, old, window, new):
+    s = Step(17, [old], [new], 4, 1, 64, 32, "bf16", window=window)
     s.k[0][:, 0, 0] = -math.inf
-    s.cache.put(pr.slots_of(s.table, 0, 32, 0, 90 + new), s.k[0], torch.zeros_like(s.k[0]))
+    s.cache.put(pr.slots_of(s.table, 0, 32, 0, old + new), s.k[0], torch.zeros_like(s.k[0]))
     s.q[:, :, 0] = 1.0
     s.run(sdamd)
     s.check()
@@ -215,28 +218,31 @@ def test_every_score_minus_infinity(sdamd, new):
 
 @pytest.mark.parametrize("loud,scale", [(0.0, None), (30.0, None), (1.5, 1e-30), (1.5, 0.5)])
 def test_ranges_of_scores(sdamd, loud, scale):
-    for new in ([1], [64]):
-        s = Step(18, [500], new, 8, 2, 128, 32, "bf16", loud=loud, scale=scale)
+    for old, new in (([500], [1]), ([500], [64]), ([3000], [1])):
+        s = Step(18, old, new, 8, 2, 128, 32, "bf16", loud=loud, scale=scale)
         s.run(sdamd)
         s.check()
 
 
-@pytest.mark.parametrize("new", [1, 70])
-def test_scores_without_fractions(sdamd, new):
+@pytest.mark.parametrize("old,new", [(100, 1), (100, 70), (3000, 1)])
+def test_scores_without_fractions(sdamd, old, new):
     """Scores of 2^30 and more: each row's largest key takes all of its weight."""
-    s = Step(19, [100], [new], 8, 2, 128, 32, "f16", loud=4.0, scale=1e9)
+    s = Step(19, [old], [new], 8, 2, 128, 32, "f16", loud=4.0, scale=1e9)
     s.run(sdamd)
     q, k = s.q.cpu().double(), s.k[0].cpu().double()
-    slots = pr.slots_of(s.table, 0, 32, 0, 100 + new)
-    got = s.out.cpu()[slots // 32, :, slots % 32].double() - s.scores.cpu()[slots // 32, :, slots % 32].double() * (torch.arange(100 + new) < 100)[:, None]
+    n = old + new
+    slots = pr.slots_of(s.table, 0, 32, 0, n)
+    got, prior = (x.cpu()[slots // 32, :, slots % 32].double() for x in (s.out, s.scores))
+    got -= prior * (torch.arange(n) < old)[:, None]
     for h in range(2):
-        want = torch.zeros(100 + new, dtype=torch.float64)
+        want = torch.zeros(n, dtype=torch.float64)
         for i in range(new):
-            x = q[i, 4 * h:4 * h + 4] @ k[:101 + i, h].T
+            x = q[i, 4 * h:4 * h + 4] @ k[:old + i + 1, h].T
             for y in x:
                 v, j = y.topk(2)
                 assert v[0] - v[1] > 1e-5 * v[0].abs()
                 want[j[0]] += 1
+        # (3 + 70 x 4 rounded twice, and what is taken off again: half a step of 2^9 each)
         assert (got[:, h] - want).abs().max() <= 1e-4
 
 
@@ -246,6 +252,40 @@ def test_same_bits_every_time(sdamd):
         a = s.run(sdamd).clone()
         for _ in range(3):
             assert torch.equal(a, s.run(sdamd))
+
+
+@pytest.mark.parametrize("hq,hk,hd,kind,most", [(16, 8, 64, "f16", 8100), (8, 8, 128, "bf16", 3000), (32, 8, 256, "f16", 700)])
+def test_many_requests(sdamd, hq, hk, hd, kind, most):
+    """A head per workgroup, its scores in LDS up to the most that it takes."""
+    rng = np.random.default_rng(hd)
+    old = [most - 1] + [int(x) for x in rng.integers(0, 400, 39)]
+    for new in ([1] * 40, [2] + [1] * 30 + [0] * 9):
+        s = Step(40, old, new, hq, hk, hd, 32, kind, window=0 if sum(new) == 40 else 300)
+        s.run(sdamd, max_new=2)
+        s.check()
+
+
+def few_launches(sdamd, B, T, max_new, max_kv, hq, hk, hd, observers=0):
+    """Workgroup sizes of a call's launches, on lengths of zero."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q, kp = torch.zeros(T * hq * hd, device="cuda").half(), torch.zeros(hk * 32 * hd, device="cuda").half()
+    table, cu, kv, out = torch.zeros(B * (max_kv // 32 + 1), **i32), torch.zeros(B + 1, **i32), torch.zeros(B, **i32), torch.zeros(hk * 32, device="cuda")
+    ws = torch.empty(sdamd.paged_weights_ws(B, T, max_new, max_kv, hq, hk, hd, observers) + 16, dtype=torch.uint8, device="cuda")
+    return [b for _, b in launches(sdamd, lambda st: sdamd.op_paged_weights(
+        q.data_ptr(), kp.data_ptr(), table.data_ptr(), max_kv // 32 + 1, cu.data_ptr(), kv.data_ptr(), B, T, max_new, max_kv, hq, hk, hd, 32, 1, None,
+        out.data_ptr(), ws.data_ptr(), ws.numel(), 0, decay=0.0, observers=observers, stream=st))]
+
+
+def test_which_kernels(sdamd):
+    """Both sides of each rule's line: a head per workgroup (512 threads), splits (128, and their sum 256), many rows (256 ...)."""
+    one, splits = [512], [128, 256]
+    assert few_launches(sdamd, 1, 1, 1, 512, 8, 2, 256) == one and few_launches(sdamd, 1, 1, 1, 513, 8, 2, 256) == splits
+    assert few_launches(sdamd, 16, 16, 1, 4096, 32, 8, 128) == one and few_launches(sdamd, 16, 16, 1, 4097, 32, 8, 128) == splits
+    assert few_launches(sdamd, 32, 32, 1, 8192, 32, 8, 128) == one and few_launches(sdamd, 32, 32, 1, 8193, 32, 8, 128) == splits
+    assert few_launches(sdamd, 32, 32, 1, 8192, 40, 8, 128) == splits  # (5 rows of 8192 scores are more than LDS takes)
+    assert few_launches(sdamd, 4, 32, 8, 300, 8, 2, 128) == one and len(few_launches(sdamd, 4, 36, 9, 300, 8, 2, 128)) >= 2
+    assert few_launches(sdamd, 4, 400, 100, 300, 8, 2, 128, observers=8) == one
+    assert few_launches(sdamd, 4, 101, 100, 300, 8, 2, 128)[-1] == 512  # (single tokens among chunks)
 
 
 def test_replayed_with_other_lengths(sdamd):
