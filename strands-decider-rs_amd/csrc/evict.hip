@@ -778,28 +778,34 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
     else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
 
-// Adds up the parts of 128 keys, in their order.
-__global__ __launch_bounds__(KEY_TILE) void k_weights_sum(WeightArgs a) {
-    const int kh = blockIdx.x % a.HK;
+// Adds up the parts of 128 keys, in their order: every fourth by a group of 128 threads, then the groups' sums.
+constexpr int SUM_G = 4;
+__global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a) {
+    __shared__ float part[SUM_G][KEY_TILE];
+    const int kh = blockIdx.x % a.HK, i = threadIdx.x % KEY_TILE, grp = threadIdx.x / KEY_TILE;
     const Tile tl = find_tile(a.B, blockIdx.x / a.HK, [&](int b) {
         return many_rows(a, b) ? key_tiles(a, request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
     });
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const Seen ob = observed(rq, a.observers);
-    const int parts = parts_of(a, ob.n), j0 = tl.i * KEY_TILE, j = j0 + threadIdx.x;
+    const int parts = parts_of(a, ob.n), j0 = tl.i * KEY_TILE, j = j0 + i;
     const int first = first_key_tile(a, tl.b) + tl.i * parts;
-    if (j >= rq.kcap || first < 0 || first + parts > a.units) return;
-    const int page = a.table[(size_t)tl.b * a.max_blocks + (j >> a.lps)];
-    if ((unsigned)page >= (unsigned)a.n_pages) return;
+    if (first < 0 || first + parts > a.units) return;
+    const int page = a.table[(size_t)tl.b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
     int t0, t1;
     tokens_of(a, rq, ob, j0, t0, t1);
     float w = 0.f;
-    const float* const col = a.col + ((size_t)first * a.HK + kh) * KEY_TILE + threadIdx.x;
+    const float* const col = a.col + ((size_t)first * a.HK + kh) * KEY_TILE + i;
     if (t1 > t0) {
 #pragma unroll 8
-        for (int z = t0 / a.part; z <= (t1 - 1) / a.part; z++) w += col[(size_t)z * a.HK * KEY_TILE];
+        for (int z = t0 / a.part + grp; z <= (t1 - 1) / a.part; z += SUM_G) w += col[(size_t)z * a.HK * KEY_TILE];
     }
+    part[grp][i] = w;
+    __syncthreads();
+    if (grp || j >= rq.kcap || (unsigned)page >= (unsigned)a.n_pages) return;
+#pragma unroll
+    for (int g = 1; g < SUM_G; g++) w += part[g][i];
     put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
 
@@ -841,7 +847,7 @@ struct EvictArgs {
     const int *kpos, *table, *kv_lens, *budgets;
     int max_blocks, B, max_kv, HK, lps, n_pages, sink, recent, W;
     int *new_lens, *moves, *counts;
-    // heads of more than EVICT_ONE rows: chunks of CHUNK rows
+    // heads of more than EVICT_ONE rows: their chunks
     int chunks;
     int* newest;  // [B][HK][chunks]
     int* hist;    // [B][HK][3][BINS]
@@ -1099,19 +1105,24 @@ __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArg
 
 // ---- heads of more rows: the same in chunks, a launch for each step that needs all of them ----
 
-constexpr int CHUNK_N = 2, CHUNK = EVICT_T * 4 * CHUNK_N;
+// (rows of a chunk: 4 CN a thread, CN 1 where few heads leave CUs idle: 4 heads of 90 to 131 thousand rows 37.9 -> 33.1 us,
+// 64 of 40 thousand 57.1 -> 62.5)
+template <int CN>
+constexpr int chunk_rows() { return EVICT_T * 4 * CN; }
 
-__device__ __forceinline__ void chunk_pages(const EvictArgs& a, const Head& x, int c, int (&page)[CHUNK_N]) {
+template <int CN>
+__device__ __forceinline__ void chunk_pages(const EvictArgs& a, const Head& x, int c, int (&page)[CN]) {
 #pragma unroll
-    for (int i = 0; i < CHUNK_N; i++) page[i] = page_of(a, x, c * CHUNK + (i * EVICT_T + threadIdx.x) * 4);
+    for (int i = 0; i < CN; i++) page[i] = page_of(a, x, c * chunk_rows<CN>() + (i * EVICT_T + threadIdx.x) * 4);
 }
 
 // The latest position of every chunk, and the histograms cleared.
+template <int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64];
     const int tid = threadIdx.x, c = blockIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
-    int page[CHUNK_N];
+    int page[CN];
     chunk_pages(a, x, c, page);
     lengths(a, x);
     if (c == 0 && tid == 0) {
@@ -1122,8 +1133,8 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
     for (int i = c * EVICT_T + tid; i < 3 * BINS; i += gridDim.x * EVICT_T) a.hist[x.bh * 3 * BINS + i] = 0;
     int most = INT_MIN;
 #pragma unroll
-    for (int i = 0; i < CHUNK_N; i++) {
-        const int j = c * CHUNK + (i * EVICT_T + tid) * 4;
+    for (int i = 0; i < CN; i++) {
+        const int j = c * chunk_rows<CN>() + (i * EVICT_T + tid) * 4;
         most = max(most, newest_of(load4(a, x, j, page[i]), x, j));
     }
     most = max_all(most, ws);
@@ -1131,21 +1142,22 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
 }
 
 // A chunk's ranks, and the digits of the m-th that the histograms so far give.
+template <int CN>
 struct Chunk {
-    uint32_t rank[4 * CHUNK_N], prefix;
+    uint32_t rank[4 * CN], prefix;
     int left, count;
 };
-template <int T>
-__device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int c, const int (&page)[CHUNK_N], int* ws, int* found,
-                                         Chunk& k) {
-    Four v[CHUNK_N];
+template <int T, int CN>
+__device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int c, const int (&page)[CN], int* ws, int* found,
+                                         Chunk<CN>& k) {
+    Four v[CN];
 #pragma unroll
-    for (int i = 0; i < CHUNK_N; i++) v[i] = load4(a, x, c * CHUNK + (i * EVICT_T + threadIdx.x) * 4, page[i]);
+    for (int i = 0; i < CN; i++) v[i] = load4(a, x, c * chunk_rows<CN>() + (i * EVICT_T + threadIdx.x) * 4, page[i]);
     int most = INT_MIN;
-    for (int i = threadIdx.x; i < (x.n + CHUNK - 1) / CHUNK; i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
+    for (int i = threadIdx.x; i < (x.n + chunk_rows<CN>() - 1) / chunk_rows<CN>(); i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
     const long long keep_from = (long long)max_all(most, ws) - a.recent;
 #pragma unroll
-    for (int i = 0; i < CHUNK_N; i++)
+    for (int i = 0; i < CN; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) k.rank[4 * i + e] = rank4(a, v[i], e, keep_from);
     k.prefix = 0, k.left = x.m, k.count = 0;
@@ -1165,25 +1177,26 @@ __device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int 
         k.left = cut.left, k.count = cut.count;
     }
 }
-__device__ __forceinline__ int chunk_row(int c, int k) { return c * CHUNK + ((k >> 2) * EVICT_T + threadIdx.x) * 4 + (k & 3); }
+template <int CN>
+__device__ __forceinline__ int chunk_row(int c, int k) { return c * chunk_rows<CN>() + ((k >> 2) * EVICT_T + threadIdx.x) * 4 + (k & 3); }
 
 // The histogram of digit T, of all chunks.  (Whole numbers: their sum has no order.)
-template <int T>
+template <int T, int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_digit(EvictArgs a) {
     __shared__ int hist[BINS], ws[EVICT_T / 64], found[3];
     const int tid = threadIdx.x, c = blockIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
-    int page[CHUNK_N];
+    int page[CN];
     chunk_pages(a, x, c, page);
     lengths(a, x);
-    if (!x.over || (long long)c * CHUNK >= x.n) return;
+    if (!x.over || (long long)c * chunk_rows<CN>() >= x.n) return;
     for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
-    Chunk k;
-    chunk_of<T>(a, x, c, page, ws, found, k);
+    Chunk<CN> k;
+    chunk_of<T, CN>(a, x, c, page, ws, found, k);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4 * CHUNK_N; i++)
-        if (chunk_row(c, i) < x.n && (T == 0 || k.rank[i] >> SHIFT[T ? T - 1 : 0] == k.prefix >> SHIFT[T ? T - 1 : 0]))
+    for (int i = 0; i < 4 * CN; i++)
+        if (chunk_row<CN>(c, i) < x.n && (T == 0 || k.rank[i] >> SHIFT[T ? T - 1 : 0] == k.prefix >> SHIFT[T ? T - 1 : 0]))
             atomicAdd(&hist[digit(k.rank[i], SHIFT[T])], 1);
     __syncthreads();
     for (int i = tid; i < BINS; i += EVICT_T)
@@ -1191,21 +1204,22 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_digit(EvictArgs a) {
 }
 
 // How many rows of each chunk have the m-th rank, and how many are above it, on either side of m.
+template <int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_count(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64], found[3], n[4];
     const int tid = threadIdx.x, c = blockIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
-    int page[CHUNK_N];
+    int page[CN];
     chunk_pages(a, x, c, page);
     lengths(a, x);
-    if (!x.over || (long long)c * CHUNK >= x.n) return;
+    if (!x.over || (long long)c * chunk_rows<CN>() >= x.n) return;
     if (tid < 4) n[tid] = 0;
-    Chunk k;
-    chunk_of<3>(a, x, c, page, ws, found, k);
+    Chunk<CN> k;
+    chunk_of<3, CN>(a, x, c, page, ws, found, k);
     uint32_t below = 0, from = 0;  // ties, and rows above times 2^16
 #pragma unroll
-    for (int i = 0; i < 4 * CHUNK_N; i++) {
-        const int j = chunk_row(c, i);
+    for (int i = 0; i < 4 * CN; i++) {
+        const int j = chunk_row<CN>(c, i);
         const uint32_t w = j >= x.n ? 0u : k.rank[i] == k.prefix ? 1u : k.rank[i] > k.prefix ? 0x10000u : 0u;
         if (j < x.m) below += w;
         else from += w;
@@ -1224,17 +1238,18 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_count(EvictArgs a) {
 }
 
 // Each chunk's moves, numbered behind those of the chunks before it.
+template <int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64], found[3];
     __shared__ int before[3];  // ties, holes and rows of the chunks before
     const int tid = threadIdx.x, c = blockIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
-    int page[CHUNK_N];
+    int page[CN];
     chunk_pages(a, x, c, page);
     lengths(a, x);
-    if (!x.over || (long long)c * CHUNK >= x.n) return;
-    Chunk k;
-    chunk_of<3>(a, x, c, page, ws, found, k);
+    if (!x.over || (long long)c * chunk_rows<CN>() >= x.n) return;
+    Chunk<CN> k;
+    chunk_of<3, CN>(a, x, c, page, ws, found, k);
     if (tid < 64) {  // 64 chunks at a time: their ties from the first on stay until `left` are used up
         int ties = 0, holes = 0, rows = 0;
         for (int i0 = 0; i0 < c; i0 += 64) {
@@ -1244,7 +1259,7 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
             const int to = lanes_upto(n[0] + n[2]);
             const int first = ties + to - n[0] - n[2];
             const int kept0 = min(max(k.left - first, 0), n[0]), kept1 = min(max(k.left - first - n[0], 0), n[2]);
-            int h = i < c ? max(0, min(CHUNK, x.m - i * CHUNK)) - n[1] - kept0 : 0, r = n[3] + kept1;
+            int h = i < c ? max(0, min(chunk_rows<CN>(), x.m - i * chunk_rows<CN>())) - n[1] - kept0 : 0, r = n[3] + kept1;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) h += __shfl_xor(h, o), r += __shfl_xor(r, o);
             holes += h, rows += r;
@@ -1256,17 +1271,17 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
     int ties = before[0], holes = before[1], rows = before[2];
     int* const mv = a.moves + x.bh * a.W * 2;
 #pragma unroll
-    for (int i = 0; i < CHUNK_N; i++) {
+    for (int i = 0; i < CN; i++) {
         int t = 0, total;
 #pragma unroll
-        for (int e = 0; e < 4; e++) t += chunk_row(c, 4 * i + e) < x.n && k.rank[4 * i + e] == k.prefix;
+        for (int e = 0; e < 4; e++) t += chunk_row<CN>(c, 4 * i + e) < x.n && k.rank[4 * i + e] == k.prefix;
         int nth = ties + scan(t, ws, total);
         ties += total;
         bool hole[4], row[4];
         int mine = 0;  // holes, and rows times 2^16
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int j = chunk_row(c, 4 * i + e);
+            const int j = chunk_row<CN>(c, 4 * i + e);
             const uint32_t r = k.rank[4 * i + e];
             const bool stays = j < x.n && (r > k.prefix || (r == k.prefix && nth < k.left));
             nth += j < x.n && r == k.prefix;
@@ -1278,11 +1293,11 @@ __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
         holes += total & 0xFFFF, rows += total >> 16;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            if (hole[e]) mv[2 * h++] = chunk_row(c, 4 * i + e);
-            if (row[e]) mv[2 * r++ + 1] = chunk_row(c, 4 * i + e);
+            if (hole[e]) mv[2 * h++] = chunk_row<CN>(c, 4 * i + e);
+            if (row[e]) mv[2 * r++ + 1] = chunk_row<CN>(c, 4 * i + e);
         }
     }
-    if (tid == 0 && (long long)(c + 1) * CHUNK >= x.n) a.counts[x.bh] = rows;
+    if (tid == 0 && (long long)(c + 1) * chunk_rows<CN>() >= x.n) a.counts[x.bh] = rows;
 }
 
 // ---- their pages ----------------------------------------------------------------------------------------------------
@@ -1529,7 +1544,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
         launch(k_weights_keys<T, HD>, keys, 256, Q, K, g);
         if (p.parts > 1) {
             const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
-            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), KEY_TILE, g);
+            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), SUM_G * KEY_TILE, g);
         }
     }
     if (p.nr) {
@@ -1568,13 +1583,16 @@ void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
 
 namespace {
 struct EvictWs {
+    int cn = 0;
     size_t chunks = 0, newest = 0, hist = 0, cuts = 0, parts = 0;  // ints
 };
 EvictWs evict_ws(int B, int max_kv, int HK) {
     EvictWs w;
     if (max_kv <= EVICT_ONE) return w;
     const size_t heads = (size_t)B * HK;
-    w.chunks = ((size_t)max_kv + CHUNK - 1) / CHUNK;
+    w.cn = heads <= 16 ? 1 : 2;
+    const size_t rows = w.cn == 1 ? chunk_rows<1>() : chunk_rows<2>();
+    w.chunks = ((size_t)max_kv + rows - 1) / rows;
     w.newest = (heads * w.chunks + 3) & ~size_t(3);
     w.hist = heads * 3 * BINS;
     w.cuts = heads * 8;
@@ -1610,12 +1628,17 @@ void page_evict(const PageEvict& a, hipStream_t st) {
     g.cuts = g.hist + w.hist;
     g.parts = g.cuts + w.cuts;
     const dim3 grid((unsigned)w.chunks, a.HK, a.B);
-    launch(k_evict_newest, grid);
-    launch(k_evict_digit<0>, grid);
-    launch(k_evict_digit<1>, grid);
-    launch(k_evict_digit<2>, grid);
-    launch(k_evict_count, grid);
-    launch(k_evict_moves, grid);
+    auto all = [&](auto cn) {
+        constexpr int CN = decltype(cn)::value;
+        launch(k_evict_newest<CN>, grid);
+        launch(k_evict_digit<0, CN>, grid);
+        launch(k_evict_digit<1, CN>, grid);
+        launch(k_evict_digit<2, CN>, grid);
+        launch(k_evict_count<CN>, grid);
+        launch(k_evict_moves<CN>, grid);
+    };
+    if (w.cn == 1) all(std::integral_constant<int, 1>());
+    else all(std::integral_constant<int, 2>());
 }
 
 void page_release(const PageRelease& a, hipStream_t st) {

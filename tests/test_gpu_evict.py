@@ -399,6 +399,11 @@ def test_evict_lengths(sdamd, n, m):
     check_evict(sdamd, n + 1, [n], [m], 1, 256, values="few", with_kpos=False)
 
 
+def test_evict_many_long(sdamd):
+    """More heads than leave CUs idle, of more rows than one workgroup takes: larger chunks."""
+    check_evict(sdamd, 9, [33001, 5, 40000, 16385, 8192, 0, 32769, 700, 24577], [100, 2, 39999, 8192, 8192, 0, 30000, 699, 0], 2, 128, 3, 500, "few")
+
+
 def test_evict_all_protected(sdamd):
     check_evict(sdamd, 3, [100, 500], [10, 20], 2, 32, sink=1 << 20)
     check_evict(sdamd, 4, [100, 500], [10, 20], 2, 32, recent=2 ** 31 - 1)
