@@ -395,7 +395,7 @@ int sd_op_page_positions(const void* cu, const void* dropped, int B, int T, cons
  * i32, and what they hold cannot make a kernel leave the given buffers; calls on several streams run at once where they
  * share no output and no workspace. ---- */
 
-/* Workspace of an sd_op_paged_weights call with these sizes, in bytes. */
+/* Workspace of an sd_op_paged_weights call with these sizes, in bytes (0: none). */
 int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int observers, size_t* bytes,
                            char* err, size_t errlen);
 
@@ -407,7 +407,8 @@ int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK
  * and its new rows kpos[j] = pos[t] (pos i32 [T]; both null: none).  All in f32; a row t that sees no key, or -inf alone,
  * adds nothing; where its scores hold NaN or +inf, all keys that it sees become NaN.  Sums have one order: equal calls
  * give equal bits.  out may be scores; other rows of both are left as they are; a row that two of the step's requests share
- * receives either's.  max_new, max_kv and ws as in sd_op_paged_attention, sized by sd_op_paged_weights_ws. */
+ * receives either's, or with out = scores both, one decayed.  max_new, max_kv and ws as in sd_op_paged_attention, sized by
+ * sd_op_paged_weights_ws. */
 int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int max_blocks, const void* cu, const void* kv_lens,
                         const void* pos, int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int page_size,
                         int n_pages, size_t page_stride, int window, float scale, int observers, float decay,

@@ -86,6 +86,7 @@ def test_positions_refuses(sdamd, kw, message):
 
 WEIGHTS = dict(Q=A, Kp=A + M, table=A + 2 * M, max_blocks=8, cu=A + 3 * M, kv_lens=A + 4 * M, B=2, T=4, max_new=2, max_kv=200, HQ=4, HK=1, HD=128,
                page_size=32, n_pages=10, scores=A + 5 * M, out=A + 6 * M, ws=A + 64 * M, ws_bytes=1 << 40, type=1, pos=A + 7 * M, kpos=A + 8 * M)
+LONG = dict(max_blocks=2048, max_kv=60000)  # (short ones need no workspace)
 
 
 @pytest.mark.parametrize("kw,message", [
@@ -96,8 +97,9 @@ WEIGHTS = dict(Q=A, Kp=A + M, table=A + 2 * M, max_blocks=8, cu=A + 3 * M, kv_le
     (dict(max_blocks=0), "table row"), (dict(max_blocks=1 << 26), "table row"), (dict(window=-1), "window"), (dict(observers=-1), "observers"), (dict(scale=0.0), "scale"),
     (dict(scale=math.nan), "scale"), (dict(scale=2.4e38), "scale"), (dict(Q=A + 8), "16 bytes"), (dict(ws=A + 64 * M + 4), "16 bytes"), (dict(out=A + 6 * M + 2), "4 bytes"),
     (dict(out=A + 5 * M + 4), "overlaps an input"), (dict(out=A + M), "overlaps an input"), (dict(kpos=A + 6 * M), "outputs overlap"), (dict(kpos=A + 5 * M), "overlaps an input"),
-    (dict(ws_bytes=0), "workspace"), (dict(ws=None), "workspace"), (dict(ws=A), "overlaps an input"), (dict(ws=A + 6 * M), "outputs overlap"),
-    (dict(ws=A + 5 * M), "overlaps"), (dict(scores=A + 5 * M, out=A + 5 * M, ws=A + 5 * M), "overlap"),
+    (dict(LONG, ws_bytes=0), "workspace"), (dict(LONG, ws=None), "workspace"), (dict(LONG, ws=A), "overlaps an input"),
+    (dict(LONG, out=A + 32 * M, ws=A + 32 * M), "outputs overlap"), (dict(LONG, ws=A + 5 * M), "overlaps"),
+    (dict(LONG, scores=A + 5 * M, out=A + 5 * M, ws=A + 5 * M), "overlap"), (dict(T=100, max_new=50, ws_bytes=1024), "workspace"),
 ])
 def test_weights_refuses(sdamd, kw, message):
     refuses(sdamd, sdamd.op_paged_weights, WEIGHTS, kw, "sd_op_paged_weights", message)
@@ -107,7 +109,9 @@ def test_weights_workspace(sdamd):
     for B, T, new, kv in [(1, 1, 1, 1), (64, 64, 1, 8192), (1, 1, 1, 2 ** 31 - 1), (8192, 8192, 1, 100), (2, 4096, 4096, 4096)]:
         for hq, hk, hd in [(8, 2, 256), (32, 8, 128), (12, 1, 64)]:
             for obs in (0, 1, 40):
-                assert 0 < sdamd.paged_weights_ws(B, T, new, kv, hq, hk, hd, obs) < 1 << 44
+                need = sdamd.paged_weights_ws(B, T, new, kv, hq, hk, hd, obs)
+                assert 0 <= need < 1 << 44 and need % 16 == 0
+                assert need or kv <= 8192  # (short caches, whose few rows' scores fit into LDS, need none)
     for bad in [(0, 1, 1, 1, 8, 2, 256), (1, 0, 1, 1, 8, 2, 256), (1, 1, 0, 1, 8, 2, 256), (1, 1, 1, 0, 8, 2, 256), (1, 1, 1, 1, 7, 2, 256),
                 (1, 1, 1, 1, 8, 2, 100), (1, 1, 1, 1, 8, 2, 64, -1)]:
         with pytest.raises(sdamd.EngineError, match="sd_op_paged_weights_ws: "):
@@ -123,6 +127,8 @@ EVICT = dict(scores=A, kpos=A + M, table=A + 2 * M, max_blocks=8, kv_lens=A + 3 
     (dict(B=8193), "requests"), (dict(HK=0), "kv heads"), (dict(HK=1025), "kv heads"), (dict(page_size=31), "power of two"), (dict(n_pages=0), "at least one page"), (dict(max_kv=0), "max_kv"),
     (dict(max_kv=257), "more than a table row"), (dict(max_blocks=0), "table row"), (dict(sink=-1), "sink"), (dict(recent=-1), "recent"), (dict(moves=A + 6 * M + 2), "4 bytes"),
     (dict(new_lens=A + 3 * M), "overlaps an input"), (dict(moves=A + M), "overlaps an input"), (dict(counts=A + 6 * M + 8), "outputs overlap"), (dict(ws=A + 8 * M + 8), "16 bytes"),
+    (dict(max_blocks=2048, max_kv=40000, ws_bytes=1024), "workspace"), (dict(max_blocks=2048, max_kv=40000, ws=None), "workspace"),
+    (dict(max_blocks=2048, max_kv=40000, ws=A), "overlaps an input"), (dict(max_blocks=2048, max_kv=40000, ws=A + 6 * M), "outputs overlap"),
 ])
 def test_evict_refuses(sdamd, kw, message):
     refuses(sdamd, sdamd.op_page_evict, EVICT, kw, "sd_op_page_evict", message)
