@@ -1154,7 +1154,7 @@ __device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int 
 #pragma unroll
     for (int i = 0; i < CN; i++) v[i] = load4(a, x, c * chunk_rows<CN>() + (i * EVICT_T + threadIdx.x) * 4, page[i]);
     int most = INT_MIN;
-    for (int i = threadIdx.x; i < (x.n + chunk_rows<CN>() - 1) / chunk_rows<CN>(); i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
+    for (int i = threadIdx.x; i <= (x.n - 1) / chunk_rows<CN>(); i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
     const long long keep_from = (long long)max_all(most, ws) - a.recent;
 #pragma unroll
     for (int i = 0; i < CN; i++)
