@@ -848,8 +848,8 @@ struct EvictArgs {
     int max_blocks, B, max_kv, HK, lps, n_pages, sink, recent, W;
     int *new_lens, *moves, *counts;
     // heads of more than EVICT_ONE rows: their chunks
-    int chunks;
-    int* newest;  // [B][HK][chunks]
+    int chunks, groups;  // at most; workgroups of a head
+    int* newest;  // [B][HK][groups]
     int* hist;    // [B][HK][3][BINS]
     int* cuts;    // [B][HK][2][4]: the first two digits' cuts, as found by the launch after theirs
     int* parts;   // [B][HK][chunks][4]: rows of the m-th rank and above it, below m and from m on
@@ -925,6 +925,17 @@ __device__ __forceinline__ int max_all(int x, int* ws) {  // over the workgroup
     return r;
 }
 
+// A histogram in LDS: COPIES counters side by side for each digit, a thread's by its number, since many rows have one digit (all
+// of them where scores are equal), and adds to one address go one by one.  (us with 1, 2, 4 and 8 of them: 512 heads of 4113
+// rows 9.0 9.1 9.0 9.9 where scores differ, 31.3 21.6 17.3 17.6 where they are equal; of 8000 rows 17.1 16.6 16.9 17.3 and
+// 52.9 32.9 23.6 21.5)
+constexpr int COPIES = 4;
+__device__ __forceinline__ void clear_bins(int* hist) {
+#pragma unroll
+    for (int i = 0; i < COPIES * BINS / (4 * EVICT_T); i++) reinterpret_cast<i32x4*>(hist)[i * EVICT_T + threadIdx.x] = i32x4{0, 0, 0, 0};
+}
+__device__ __forceinline__ void count_digit(int* hist, int d) { atomicAdd(&hist[d * COPIES + (threadIdx.x & (COPIES - 1))], 1); }
+
 // Digit t of a rank, and the bits above it.
 constexpr int SHIFT[3] = {21, 10, 0};
 __device__ __forceinline__ int digit(uint32_t r, int shift) { return r >> shift & (shift ? BINS - 1 : 1023); }
@@ -935,9 +946,12 @@ __device__ __forceinline__ int digit(uint32_t r, int shift) { return r >> shift 
 struct Cut {
     int digit, left, count;
 };
+template <int R>  // copies of the histogram
 __device__ __forceinline__ Cut cut_at(const int* hist, int left, int* ws, int* found) {
     const int tid = threadIdx.x, d1 = BINS - 1 - 2 * tid, d0 = d1 - 1;  // (from the largest digit down)
-    const int c1 = hist[d1], c0 = hist[d0];
+    int c1 = 0, c0 = 0;
+#pragma unroll
+    for (int i = 0; i < R; i++) c1 += hist[d1 * R + i], c0 += hist[d0 * R + i];
     // (a scan as above, its first barrier done: the histogram's)
     const int wv = tid >> 6, to = lanes_upto(c1 + c0);
     if ((tid & 63) == 63) ws[wv] = to;
@@ -961,7 +975,8 @@ constexpr int CANDIDATES = 512;
 template <int N>
 __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArgs a) {  // (two to a CU, where registers allow)
     constexpr int WV = EVICT_T / 64;
-    __shared__ int hist[BINS], ws[WV], found[3], at_last;
+    __shared__ __align__(16) int hist[COPIES * BINS];
+    __shared__ int ws[WV], found[3], at_last;
     __shared__ uint32_t sums[N * WV], rank_last;
     __shared__ __align__(16) unsigned long long cand[CANDIDATES];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -980,7 +995,7 @@ __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArg
         Four v[N];
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = load4(a, x, (i * EVICT_T + tid) * 4, page[i]);
-        for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
+        clear_bins(hist);
         int most = INT_MIN;
 #pragma unroll
         for (int i = 0; i < N; i++) most = max(most, newest_of(v[i], x, (i * EVICT_T + tid) * 4));
@@ -1002,7 +1017,7 @@ __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArg
         if (done) break;
         if (t) {
             __syncthreads();
-            for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
+            clear_bins(hist);
             __syncthreads();
         }
 #pragma unroll
@@ -1010,11 +1025,11 @@ __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArg
             if (!any(i)) break;
 #pragma unroll
             for (int k = 4 * i; k < 4 * i + 4; k++)
-                if (at(k) < x.n && (t == 0 || rank[k] >> above == prefix >> above)) atomicAdd(&hist[digit(rank[k], shift)], 1);
+                if (at(k) < x.n && (t == 0 || rank[k] >> above == prefix >> above)) count_digit(hist, digit(rank[k], shift));
         }
         if (tid == 0) at_last = 0;
         __syncthreads();
-        const Cut c = cut_at(hist, left, ws, found);
+        const Cut c = cut_at<COPIES>(hist, left, ws, found);
         prefix |= (uint32_t)c.digit << shift;
         left = c.left, count = c.count;
         if (left == count) {  // all of them (none where m is 0: nothing has the last digit of all)
@@ -1105,8 +1120,8 @@ __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArg
 
 // ---- heads of more rows: the same in chunks, a launch for each step that needs all of them ----
 
-// (rows of a chunk: 4 CN a thread, CN 1 where few heads leave CUs idle: 4 heads of 90 to 131 thousand rows 37.9 -> 33.1 us,
-// 64 of 40 thousand 57.1 -> 62.5)
+// (rows of a chunk: 4 CN a thread, CN 1 where few heads leave CUs idle.  us with 1 and 2: 4 heads of 131 thousand rows of which 33
+// thousand stay 30.5 33, 64 heads of 40 thousand 57 52, 512 heads of 40 thousand 204 199)
 template <int CN>
 constexpr int chunk_rows() { return EVICT_T * 4 * CN; }
 
@@ -1116,51 +1131,81 @@ __device__ __forceinline__ void chunk_pages(const EvictArgs& a, const Head& x, i
     for (int i = 0; i < CN; i++) page[i] = page_of(a, x, c * chunk_rows<CN>() + (i * EVICT_T + threadIdx.x) * 4);
 }
 
-// The latest position of every chunk, and the histograms cleared.
+// A head has gridDim.x workgroups, each of which takes every gridDim.x-th chunk: where the lengths lie far below max_kv, few
+// find none.  each(chunk, its pages) for those that there are; the first one's pages are on their way with the lengths.
+template <int CN, class F>
+__device__ __forceinline__ void chunks_of(const EvictArgs& a, const Head& x, int (&page)[CN], F&& each) {
+    const int last = (x.n - 1) / chunk_rows<CN>();
+    for (int c = blockIdx.x;;) {
+        each(c);
+        if (last - c < (int)gridDim.x) break;
+        c += gridDim.x;
+        chunk_pages(a, x, c, page);
+    }
+}
+template <int CN>
+__device__ __forceinline__ bool has_chunk(const Head& x) { return x.over && blockIdx.x <= (x.n - 1) / chunk_rows<CN>(); }
+
+// The latest position that each workgroup finds, and the histograms cleared.
 template <int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_newest(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64];
-    const int tid = threadIdx.x, c = blockIdx.x;
+    const int tid = threadIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
     int page[CN];
-    chunk_pages(a, x, c, page);
+    chunk_pages(a, x, blockIdx.x, page);
     lengths(a, x);
-    if (c == 0 && tid == 0) {
+    if (blockIdx.x == 0 && tid == 0) {
         if (x.h == 0) a.new_lens[x.b] = x.m;
         if (!x.over) a.counts[x.bh] = 0;
     }
     if (!x.over) return;
-    for (int i = c * EVICT_T + tid; i < 3 * BINS; i += gridDim.x * EVICT_T) a.hist[x.bh * 3 * BINS + i] = 0;
+    for (int i = blockIdx.x * EVICT_T + tid; i < 3 * BINS; i += gridDim.x * EVICT_T) a.hist[x.bh * 3 * BINS + i] = 0;
     int most = INT_MIN;
+    if (has_chunk<CN>(x))
+        chunks_of<CN>(a, x, page, [&](int c) INL {
 #pragma unroll
-    for (int i = 0; i < CN; i++) {
-        const int j = c * chunk_rows<CN>() + (i * EVICT_T + tid) * 4;
-        most = max(most, newest_of(load4(a, x, j, page[i]), x, j));
-    }
+            for (int i = 0; i < CN; i++) {
+                const int j = c * chunk_rows<CN>() + (i * EVICT_T + tid) * 4;
+                most = max(most, newest_of(load4(a, x, j, page[i]), x, j));
+            }
+        });
     most = max_all(most, ws);
-    if (tid == 0) a.newest[x.bh * a.chunks + c] = most;
+    if (tid == 0) a.newest[x.bh * a.groups + blockIdx.x] = most;
 }
 
-// A chunk's ranks, and the digits of the m-th that the histograms so far give.
+// A chunk's rows, as loaded, and their ranks; row 4 i + e of a thread is row e of the 4 that it loads i-th.
 template <int CN>
 struct Chunk {
-    uint32_t rank[4 * CN], prefix;
-    int left, count;
-};
-template <int T, int CN>
-__device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int c, const int (&page)[CN], int* ws, int* found,
-                                         Chunk<CN>& k) {
     Four v[CN];
+    uint32_t rank[4 * CN];
+    __device__ __forceinline__ void load(const EvictArgs& a, const Head& x, int c, const int (&page)[CN]) {
 #pragma unroll
-    for (int i = 0; i < CN; i++) v[i] = load4(a, x, c * chunk_rows<CN>() + (i * EVICT_T + threadIdx.x) * 4, page[i]);
+        for (int i = 0; i < CN; i++) v[i] = load4(a, x, c * chunk_rows<CN>() + (i * EVICT_T + threadIdx.x) * 4, page[i]);
+    }
+    __device__ __forceinline__ void ranks(const EvictArgs& a, long long keep_from) {
+#pragma unroll
+        for (int i = 0; i < CN; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) rank[4 * i + e] = rank4(a, v[i], e, keep_from);
+    }
+};
+template <int CN>
+__device__ __forceinline__ int chunk_row(int c, int k) { return c * chunk_rows<CN>() + ((k >> 2) * EVICT_T + threadIdx.x) * 4 + (k & 3); }
+
+__device__ __forceinline__ long long keep_from_of(const EvictArgs& a, const Head& x, int* ws) {
     int most = INT_MIN;
-    for (int i = threadIdx.x; i <= (x.n - 1) / chunk_rows<CN>(); i += EVICT_T) most = max(most, a.newest[x.bh * a.chunks + i]);
-    const long long keep_from = (long long)max_all(most, ws) - a.recent;
-#pragma unroll
-    for (int i = 0; i < CN; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) k.rank[4 * i + e] = rank4(a, v[i], e, keep_from);
-    k.prefix = 0, k.left = x.m, k.count = 0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += EVICT_T) most = max(most, a.newest[x.bh * a.groups + i]);
+    return (long long)max_all(most, ws) - a.recent;
+}
+// The digits of the m-th rank that the first T histograms give, and how many of those that have them stay.
+struct Prefix {
+    uint32_t rank;
+    int left;
+};
+template <int T>
+__device__ __forceinline__ Prefix prefix_of(const EvictArgs& a, const Head& x, int* ws, int* found) {
+    Prefix p{0, x.m};
     // (the cut before the last is in memory since the last launch)
 #pragma unroll
     for (int t = 0; t < T; t++) {
@@ -1170,71 +1215,87 @@ __device__ __forceinline__ void chunk_of(const EvictArgs& a, const Head& x, int 
             cut = {kept[0], kept[1], kept[2]};
         } else {
             __syncthreads();
-            cut = cut_at(a.hist + (x.bh * 3 + t) * BINS, k.left, ws, found);
-            if (t < 2 && c == 0 && threadIdx.x == 0) kept[0] = cut.digit, kept[1] = cut.left, kept[2] = cut.count;
+            cut = cut_at<1>(a.hist + (x.bh * 3 + t) * BINS, p.left, ws, found);
+            if (t < 2 && blockIdx.x == 0 && threadIdx.x == 0) kept[0] = cut.digit, kept[1] = cut.left, kept[2] = cut.count;
         }
-        k.prefix |= (uint32_t)cut.digit << SHIFT[t];
-        k.left = cut.left, k.count = cut.count;
+        p.rank |= (uint32_t)cut.digit << SHIFT[t];
+        p.left = cut.left;
     }
+    return p;
 }
-template <int CN>
-__device__ __forceinline__ int chunk_row(int c, int k) { return c * chunk_rows<CN>() + ((k >> 2) * EVICT_T + threadIdx.x) * 4 + (k & 3); }
 
 // The histogram of digit T, of all chunks.  (Whole numbers: their sum has no order.)
 template <int T, int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_digit(EvictArgs a) {
-    __shared__ int hist[BINS], ws[EVICT_T / 64], found[3];
-    const int tid = threadIdx.x, c = blockIdx.x;
+    __shared__ __align__(16) int hist[COPIES * BINS];
+    __shared__ int ws[EVICT_T / 64], found[3];
+    const int tid = threadIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
     int page[CN];
-    chunk_pages(a, x, c, page);
+    chunk_pages(a, x, blockIdx.x, page);
     lengths(a, x);
-    if (!x.over || (long long)c * chunk_rows<CN>() >= x.n) return;
-    for (int i = tid; i < BINS; i += EVICT_T) hist[i] = 0;
+    if (!has_chunk<CN>(x)) return;
     Chunk<CN> k;
-    chunk_of<T, CN>(a, x, c, page, ws, found, k);
+    k.load(a, x, blockIdx.x, page);  // (on their way meanwhile)
+    clear_bins(hist);
+    const long long keep_from = keep_from_of(a, x, ws);
+    const Prefix p = prefix_of<T>(a, x, ws, found);
     __syncthreads();
+    chunks_of<CN>(a, x, page, [&](int c) INL {
+        if (c != (int)blockIdx.x) k.load(a, x, c, page);
+        k.ranks(a, keep_from);
 #pragma unroll
-    for (int i = 0; i < 4 * CN; i++)
-        if (chunk_row<CN>(c, i) < x.n && (T == 0 || k.rank[i] >> SHIFT[T ? T - 1 : 0] == k.prefix >> SHIFT[T ? T - 1 : 0]))
-            atomicAdd(&hist[digit(k.rank[i], SHIFT[T])], 1);
+        for (int i = 0; i < 4 * CN; i++)
+            if (chunk_row<CN>(c, i) < x.n && (T == 0 || k.rank[i] >> SHIFT[T ? T - 1 : 0] == p.rank >> SHIFT[T ? T - 1 : 0]))
+                count_digit(hist, digit(k.rank[i], SHIFT[T]));
+    });
     __syncthreads();
-    for (int i = tid; i < BINS; i += EVICT_T)
-        if (hist[i]) atomicAdd(&a.hist[(x.bh * 3 + T) * BINS + i], hist[i]);
+    for (int i = tid; i < BINS; i += EVICT_T) {
+        const i32x4 n = reinterpret_cast<const i32x4*>(hist)[i];
+        const int sum = (n[0] + n[1]) + (n[2] + n[3]);
+        if (sum) atomicAdd(&a.hist[(x.bh * 3 + T) * BINS + i], sum);
+    }
 }
 
 // How many rows of each chunk have the m-th rank, and how many are above it, on either side of m.
 template <int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_count(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64], found[3], n[4];
-    const int tid = threadIdx.x, c = blockIdx.x;
+    const int tid = threadIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
     int page[CN];
-    chunk_pages(a, x, c, page);
+    chunk_pages(a, x, blockIdx.x, page);
     lengths(a, x);
-    if (!x.over || (long long)c * chunk_rows<CN>() >= x.n) return;
-    if (tid < 4) n[tid] = 0;
+    if (!has_chunk<CN>(x)) return;
     Chunk<CN> k;
-    chunk_of<3, CN>(a, x, c, page, ws, found, k);
-    uint32_t below = 0, from = 0;  // ties, and rows above times 2^16
+    k.load(a, x, blockIdx.x, page);
+    const long long keep_from = keep_from_of(a, x, ws);
+    const Prefix p = prefix_of<3>(a, x, ws, found);
+    chunks_of<CN>(a, x, page, [&](int c) INL {
+        if (c != (int)blockIdx.x) k.load(a, x, c, page);
+        k.ranks(a, keep_from);
+        uint32_t below = 0, from = 0;  // ties, and rows above times 2^16
 #pragma unroll
-    for (int i = 0; i < 4 * CN; i++) {
-        const int j = chunk_row<CN>(c, i);
-        const uint32_t w = j >= x.n ? 0u : k.rank[i] == k.prefix ? 1u : k.rank[i] > k.prefix ? 0x10000u : 0u;
-        if (j < x.m) below += w;
-        else from += w;
-    }
+        for (int i = 0; i < 4 * CN; i++) {
+            const int j = chunk_row<CN>(c, i);
+            const uint32_t w = j >= x.n ? 0u : k.rank[i] == p.rank ? 1u : k.rank[i] > p.rank ? 0x10000u : 0u;
+            if (j < x.m) below += w;
+            else from += w;
+        }
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) below += __shfl_xor(below, o), from += __shfl_xor(from, o);
-    __syncthreads();
-    if ((tid & 63) == 0) {
-        atomicAdd(&n[0], (int)(below & 0xFFFF));
-        atomicAdd(&n[1], (int)(below >> 16));
-        atomicAdd(&n[2], (int)(from & 0xFFFF));
-        atomicAdd(&n[3], (int)(from >> 16));
-    }
-    __syncthreads();
-    if (tid < 4) a.parts[(x.bh * a.chunks + c) * 4 + tid] = n[tid];
+        for (int o = 1; o < 64; o <<= 1) below += __shfl_xor(below, o), from += __shfl_xor(from, o);
+        __syncthreads();  // (the last chunk's are written)
+        if (tid < 4) n[tid] = 0;
+        __syncthreads();
+        if ((tid & 63) == 0) {
+            atomicAdd(&n[0], (int)(below & 0xFFFF));
+            atomicAdd(&n[1], (int)(below >> 16));
+            atomicAdd(&n[2], (int)(from & 0xFFFF));
+            atomicAdd(&n[3], (int)(from >> 16));
+        }
+        __syncthreads();
+        if (tid < 4) a.parts[(x.bh * a.chunks + c) * 4 + tid] = n[tid];
+    });
 }
 
 // Each chunk's moves, numbered behind those of the chunks before it.
@@ -1242,62 +1303,68 @@ template <int CN>
 __global__ __launch_bounds__(EVICT_T) void k_evict_moves(EvictArgs a) {
     __shared__ int ws[EVICT_T / 64], found[3];
     __shared__ int before[3];  // ties, holes and rows of the chunks before
-    const int tid = threadIdx.x, c = blockIdx.x;
+    const int tid = threadIdx.x;
     Head x = head_of(a, blockIdx.y, blockIdx.z);
     int page[CN];
-    chunk_pages(a, x, c, page);
+    chunk_pages(a, x, blockIdx.x, page);
     lengths(a, x);
-    if (!x.over || (long long)c * chunk_rows<CN>() >= x.n) return;
+    if (!has_chunk<CN>(x)) return;
     Chunk<CN> k;
-    chunk_of<3, CN>(a, x, c, page, ws, found, k);
-    if (tid < 64) {  // 64 chunks at a time: their ties from the first on stay until `left` are used up
-        int ties = 0, holes = 0, rows = 0;
-        for (int i0 = 0; i0 < c; i0 += 64) {
-            const int i = i0 + tid;
-            i32x4 n = {0, 0, 0, 0};
-            if (i < c) n = *reinterpret_cast<const i32x4*>(a.parts + (x.bh * a.chunks + i) * 4);
-            const int to = lanes_upto(n[0] + n[2]);
-            const int first = ties + to - n[0] - n[2];
-            const int kept0 = min(max(k.left - first, 0), n[0]), kept1 = min(max(k.left - first - n[0], 0), n[2]);
-            int h = i < c ? max(0, min(chunk_rows<CN>(), x.m - i * chunk_rows<CN>())) - n[1] - kept0 : 0, r = n[3] + kept1;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) h += __shfl_xor(h, o), r += __shfl_xor(r, o);
-            holes += h, rows += r;
-            ties += __shfl(to, 63);
-        }
-        if (tid == 0) before[0] = ties, before[1] = holes, before[2] = rows;
-    }
-    __syncthreads();
-    int ties = before[0], holes = before[1], rows = before[2];
+    k.load(a, x, blockIdx.x, page);
+    const long long keep_from = keep_from_of(a, x, ws);
+    const Prefix p = prefix_of<3>(a, x, ws, found);
     int* const mv = a.moves + x.bh * a.W * 2;
+    int upto = 0, ties0 = 0, holes0 = 0, rows0 = 0;  // (in the first wave: those of the chunks before chunk `upto`)
+    chunks_of<CN>(a, x, page, [&](int c) INL {
+        if (c != (int)blockIdx.x) k.load(a, x, c, page);
+        k.ranks(a, keep_from);
+        if (tid < 64) {  // 64 chunks at a time: their ties from the first on stay until `left` are used up
+            for (; upto < c; upto = min(c, upto + 64)) {
+                const int i = upto + tid;
+                i32x4 n = {0, 0, 0, 0};
+                if (i < c) n = *reinterpret_cast<const i32x4*>(a.parts + (x.bh * a.chunks + i) * 4);
+                const int to = lanes_upto(n[0] + n[2]);
+                const int first = ties0 + to - n[0] - n[2];
+                const int kept0 = min(max(p.left - first, 0), n[0]), kept1 = min(max(p.left - first - n[0], 0), n[2]);
+                int h = i < c ? max(0, min(chunk_rows<CN>(), x.m - i * chunk_rows<CN>())) - n[1] - kept0 : 0, r = n[3] + kept1;
 #pragma unroll
-    for (int i = 0; i < CN; i++) {
-        int t = 0, total;
-#pragma unroll
-        for (int e = 0; e < 4; e++) t += chunk_row<CN>(c, 4 * i + e) < x.n && k.rank[4 * i + e] == k.prefix;
-        int nth = ties + scan(t, ws, total);
-        ties += total;
-        bool hole[4], row[4];
-        int mine = 0;  // holes, and rows times 2^16
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int j = chunk_row<CN>(c, 4 * i + e);
-            const uint32_t r = k.rank[4 * i + e];
-            const bool stays = j < x.n && (r > k.prefix || (r == k.prefix && nth < k.left));
-            nth += j < x.n && r == k.prefix;
-            hole[e] = j < x.m && !stays, row[e] = j >= x.m && stays;
-            mine += hole[e] + (row[e] ? 0x10000 : 0);
+                for (int o = 1; o < 64; o <<= 1) h += __shfl_xor(h, o), r += __shfl_xor(r, o);
+                holes0 += h, rows0 += r;
+                ties0 += __shfl(to, 63);
+            }
+            if (tid == 0) before[0] = ties0, before[1] = holes0, before[2] = rows0;
         }
-        const int no = scan(mine, ws, total);
-        int h = holes + (no & 0xFFFF), r = rows + (no >> 16);
-        holes += total & 0xFFFF, rows += total >> 16;
+        __syncthreads();
+        int ties = before[0], holes = before[1], rows = before[2];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (hole[e]) mv[2 * h++] = chunk_row<CN>(c, 4 * i + e);
-            if (row[e]) mv[2 * r++ + 1] = chunk_row<CN>(c, 4 * i + e);
+        for (int i = 0; i < CN; i++) {
+            int t = 0, total;
+#pragma unroll
+            for (int e = 0; e < 4; e++) t += chunk_row<CN>(c, 4 * i + e) < x.n && k.rank[4 * i + e] == p.rank;
+            int nth = ties + scan(t, ws, total);
+            ties += total;
+            bool hole[4], row[4];
+            int mine = 0;  // holes, and rows times 2^16
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = chunk_row<CN>(c, 4 * i + e);
+                const uint32_t r = k.rank[4 * i + e];
+                const bool stays = j < x.n && (r > p.rank || (r == p.rank && nth < p.left));
+                nth += j < x.n && r == p.rank;
+                hole[e] = j < x.m && !stays, row[e] = j >= x.m && stays;
+                mine += hole[e] + (row[e] ? 0x10000 : 0);
+            }
+            const int no = scan(mine, ws, total);
+            int h = holes + (no & 0xFFFF), r = rows + (no >> 16);
+            holes += total & 0xFFFF, rows += total >> 16;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (hole[e]) mv[2 * h++] = chunk_row<CN>(c, 4 * i + e);
+                if (row[e]) mv[2 * r++ + 1] = chunk_row<CN>(c, 4 * i + e);
+            }
         }
-    }
-    if (tid == 0 && (long long)(c + 1) * chunk_rows<CN>() >= x.n) a.counts[x.bh] = rows;
+        if (tid == 0 && c == (x.n - 1) / chunk_rows<CN>()) a.counts[x.bh] = rows;
+    });
 }
 
 // ---- their pages ----------------------------------------------------------------------------------------------------
@@ -1583,7 +1650,7 @@ void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
 
 namespace {
 struct EvictWs {
-    int cn = 0;
+    int cn = 0, groups = 0;
     size_t chunks = 0, newest = 0, hist = 0, cuts = 0, parts = 0;  // ints
 };
 EvictWs evict_ws(int B, int max_kv, int HK) {
@@ -1593,7 +1660,10 @@ EvictWs evict_ws(int B, int max_kv, int HK) {
     w.cn = heads <= 16 ? 1 : 2;
     const size_t rows = w.cn == 1 ? chunk_rows<1>() : chunk_rows<2>();
     w.chunks = ((size_t)max_kv + rows - 1) / rows;
-    w.newest = (heads * w.chunks + 3) & ~size_t(3);
+    // (us with 512, 1024 and 2048 workgroups in all: 512 heads of 4113 rows under a bound of 131072 44 86 154, and a workgroup for
+    // each chunk of the bound 438; of 40000 rows 199 223 306; 64 heads of 100000 98 116 -)
+    w.groups = (int)std::min(w.chunks, std::max(size_t(1), 512 / heads));
+    w.newest = (heads * w.groups + 3) & ~size_t(3);
     w.hist = heads * 3 * BINS;
     w.cuts = heads * 8;
     w.parts = heads * w.chunks * 4;
@@ -1609,7 +1679,7 @@ size_t page_evict_ws(int B, int max_kv, int HK) {
 void page_evict(const PageEvict& a, hipStream_t st) {
     const EvictWs w = evict_ws(a.B, a.max_kv, a.HK);
     EvictArgs g{a.scores, a.kpos, a.table, a.kv_lens, a.budgets, a.max_blocks, a.B, a.max_kv, a.HK, log2i(a.PS), a.n_pages,
-                a.sink, a.recent, std::max(a.max_kv / 2, 1), a.new_lens, a.moves, a.counts, (int)w.chunks};
+                a.sink, a.recent, std::max(a.max_kv / 2, 1), a.new_lens, a.moves, a.counts, (int)w.chunks, w.groups};
     auto launch = [&](auto kernel, dim3 grid) {
         hipLaunchKernelGGL(kernel, grid, dim3(EVICT_T), 0, st, g);
         launched("page_evict");
@@ -1622,12 +1692,11 @@ void page_evict(const PageEvict& a, hipStream_t st) {
         else launch(k_page_evict<8>, grid);
         return;
     }
-    if (w.chunks * a.HK * a.B >= size_t(1) << 24) throw Error("sd_op_page_evict: too many rows for one launch");
     g.newest = static_cast<int*>(a.ws);
     g.hist = g.newest + w.newest;
     g.cuts = g.hist + w.hist;
     g.parts = g.cuts + w.cuts;
-    const dim3 grid((unsigned)w.chunks, a.HK, a.B);
+    const dim3 grid((unsigned)w.groups, a.HK, a.B);
     auto all = [&](auto cn) {
         constexpr int CN = decltype(cn)::value;
         launch(k_evict_newest<CN>, grid);

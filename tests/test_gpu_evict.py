@@ -404,6 +404,16 @@ def test_evict_many_long(sdamd):
     check_evict(sdamd, 9, [33001, 5, 40000, 16385, 8192, 0, 32769, 700, 24577], [100, 2, 39999, 8192, 8192, 0, 30000, 699, 0], 2, 128, 3, 500, "few")
 
 
+@pytest.mark.parametrize("requests,hk,long,bound", [(66, 2, 45001, 131072), (300, 2, 36000, 40000), (8, 2, 300001, 300001)])
+@pytest.mark.parametrize("values", ["normal", "few"])
+def test_evict_far_bound(sdamd, requests, hk, long, bound, values):
+    """Fewer workgroups for a head than chunks that a request may have."""
+    rng = np.random.default_rng(10)
+    lens = rng.integers(0, 500, requests)
+    lens[[1, requests - 2]] = long, long // 3
+    check_evict(sdamd, 11, lens.tolist(), (lens * 2 // 3).tolist(), hk, 128, 4, 20, values, max_kv=bound)
+
+
 def test_evict_all_protected(sdamd):
     check_evict(sdamd, 3, [100, 500], [10, 20], 2, 32, sink=1 << 20)
     check_evict(sdamd, 4, [100, 500], [10, 20], 2, 32, recent=2 ** 31 - 1)
