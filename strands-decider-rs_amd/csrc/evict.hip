@@ -249,9 +249,10 @@ __device__ __forceinline__ void few_scores(const T* __restrict__ Q, const T* __r
     }
 }
 
-constexpr int FEW_W = 2;  // waves of a workgroup
+constexpr int FEW_W = 2;  // waves of a workgroup (1 and 4, with as many splits: level or slower)
 
-// A split of the keys per workgroup.
+// A split of the keys per workgroup.  One token of one request, 700 keys, 2 heads of 256 dims: 4.1 us, and 4.1 for the sums
+// below: two launches whose loads (lengths, table, keys; parts, scores) come one after the other; the bytes would take 0.1.
 template <class T, int HD, int NR, bool ONCE>
 __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     constexpr int R = 16 * NR;
@@ -371,7 +372,8 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     }
 }
 
-// Short caches: a (request, kv head) per workgroup, its scores in LDS, in one launch.
+// Short caches: a (request, kv head) per workgroup, its scores in LDS, in one launch.  64 requests of 1000 to 8191 keys, 8 heads
+// of 128 dims: 83 us for 400 MB of keys, 4.8 TB/s (in splits 97); 4 waves level, 16 slower.
 constexpr int ONE_W = 8, ONE_LDS = 136 << 10, ONE_KEYS = 8192;  // waves; bytes of scores, and keys, at most
 template <class T, int HD, int NR, bool ONCE>
 __global__ __launch_bounds__(64 * ONE_W) void k_weights_few_one(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
@@ -490,6 +492,13 @@ struct Within {
 // Maxima and sums of 128 rows over a split of their keys: each wave has 32 rows' queries in registers, and all four share
 // blocks of 32 keys that arrive by LDS DMA, in a ring.  A lane keeps its own maximum and sum of the half of each block that it
 // has; the two halves meet at the end.
+//
+// A block is one chain: reads from LDS, products, maximum, exponentials.  Four workgroups on a CU cover each other's, so a wave
+// may take 128 registers.  A prompt of 4096 (8 query heads on 2, 256 dims) 51 us where the products alone would take 29: CUs are
+// busy for three quarters of it, and of those cycles products have 43 %, vector instructions 40 %.  On 32 rows of 2
+// caches of 60 to 131 thousand keys 32 us, 4.3 TB/s.  Measured and slower: 64 rows a wave with two workgroups on a CU, the
+// rows of a short question in LDS with waves by themselves, fragments read four ahead, two accumulators in turn, 256 to 1024
+// keys a workgroup less or more, tiles in the other order, the last split of each tile at the end (level).
 template <class T, int HD>
 __global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     typedef typename Vec8<T>::type T8;
@@ -667,6 +676,8 @@ __device__ __forceinline__ float sum_rows(const f32x16& acc) {
 // Weights of 128 keys from a part of the rows: each wave has 32 keys in registers, and all four share blocks of 32 rows of queries
 // that arrive by LDS DMA, in a ring.  A lane adds its row's weights to its 16 keys' sums, in registers; the 32 lanes meet at the
 // end.  What changes from block to block is scalar: a block's first token and head, and offsets into Q and the statistics.
+// As above 51 us for the prompt and 34 for the long caches; 64 keys a wave (two workgroups on a CU) took 80.  With 256 dims its
+// registers allow three workgroups on a CU.
 template <class T, int HD>
 __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     typedef typename Vec8<T>::type T8;
@@ -778,7 +789,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
     else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
 
-// Adds up the parts of 128 keys, in their order: every fourth by a group of 128 threads, then the groups' sums.
+// Adds up the parts of 128 keys, in their order: every fourth by a group of 128 threads, then the groups' sums.  (64 parts of
+// 4096 keys, 2 heads: 5.3 us; by one group 6.5)
 constexpr int SUM_G = 4;
 __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a) {
     __shared__ float part[SUM_G][KEY_TILE];
@@ -814,7 +826,8 @@ __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a) 
 // Of a (request, kv head)'s n rows the m of the highest ranks stay: a rank is 32 bits, its order the scores', protected
 // rows above all.  The m-th is found by digits of 11, 11 and 10 bits from the highest down: a histogram in LDS of the rows
 // whose digits above match, and a scan of its counts.  Rows above that rank stay, and of those that have it the first.
-// Up to 32768 rows one workgroup does it all, with every row's rank in registers, read once.
+// Up to 32768 rows one workgroup does it all, with every row's rank in registers, read once.  512 heads of 4113 rows: 11.5 us,
+// 17 MB; a chain of 16 barriers, two workgroups to a CU.
 
 // A score's place in the order, ascending: NaN, and a row in a hole, before all numbers; -0 is 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
@@ -1119,6 +1132,9 @@ __global__ __launch_bounds__(EVICT_T, N <= 2 ? 8 : 4) void k_page_evict(EvictArg
 }
 
 // ---- heads of more rows: the same in chunks, a launch for each step that needs all of them ----
+//
+// 4 heads of 90 to 131 thousand rows: 3.2, 4.1, 4.9, 4.6, 5.7 and 7.0 us, launches of 128 workgroups that are latency
+// alone (lengths, pages, rows, histogram in series); the bytes of one pass would take 1.
 
 // (rows of a chunk: 4 CN a thread, CN 1 where few heads leave CUs idle.  us with 1 and 2: 4 heads of 131 thousand rows of which 33
 // thousand stay 30.5 33, 64 heads of 40 thousand 57 52, 512 heads of 40 thousand 204 199)
@@ -1390,7 +1406,8 @@ __device__ __forceinline__ long long scan(long long x, long long* ws, long long&
 }
 
 // One workgroup: the requests' pages that go numbered through by a scan over the requests, then pushed in that order, a
-// round of 1024 entries at a time, those out of range left out.
+// round of 1024 entries at a time, those out of range left out.  64 requests, a page each: 4.3 us; 2 that drop 500 to 770 pages
+// 5.1: lengths, a scan, table and stack in series.
 __global__ __launch_bounds__(RELEASE_T) void k_page_release(const int* __restrict__ kv_lens, const int* __restrict__ new_lens,
                                                             const int* __restrict__ dropped, const int* __restrict__ table,
                                                             int max_blocks, int B, int lps, int n_pages, int* free_pages,
@@ -1444,6 +1461,10 @@ __global__ __launch_bounds__(RELEASE_T) void k_page_release(const int* __restric
 // bytes, but a row of V is one element of each of HD runs of 32 rows.  Moves ascend on both sides, so many of them on end touch
 // few blocks: lane l takes move l % N of N, and a wave's load of a dim, or its store, falls into one or two runs.  Where a
 // head has few moves, each a block of its own, smaller N spread them over more workgroups.
+//
+// 15 rows of each of 512 heads of 128 dims: 18 us, 13 of them V's stores: 983 thousand single elements, each in 64 bytes of its
+// own, which memory takes as masked writes of 32 bytes.  96 thousand rows of 256 dims: 107 us; 268 MB read and 125 written for
+// the 196 that move, 3.7 TB/s; without V 44, without its stores 77, without its loads 74.
 constexpr int MOVES = 32;  // that a workgroup does at a time, at most
 
 template <int HD, int N>

@@ -16,7 +16,8 @@ struct Turn {
 
 // m (cos, sin) of p f radians: p f in turns, less whole turns, less the nearest quarter; what is left, at most 1/8 turn,
 // goes through the first terms of the two series, up to x^11 and x^12 (the next ones are below 2^-37), in f64.  Each result
-// is rounded to f32 once.  About 30 f64 instructions; a table of 16396 rows of 64 pairs is bound by its bytes all the same.
+// is rounded to f32 once.  About 30 f64 instructions: a table of 16396 rows of 64 pairs takes 5.4 us where its bytes, 8.4 MB, would
+// take 1.8.
 __device__ __forceinline__ Turn turn_of(int p, double f, double m) {
     double t = (double)p * (f * 0.15915494309189533577);
     t -= __builtin_rint(t);
@@ -48,7 +49,9 @@ constexpr int MAX_R = 8;  // rows of a workgroup at most
 
 // Rows r0 .. r0 + R - 1 of a workgroup, or a slice of one row's units.  A unit is 8 dims of a head with the 8 that turn
 // with them (HALF), or 4 neighbouring pairs (PAIRS), or 8 dims that are only copied.  The workgroup's angles come once,
-// into LDS, for all heads, while its rows are on their way.
+// into LDS, for all heads, while its rows are on their way.  Bound by bytes: 8192 rows of 8 and 2 heads of 256 dims,
+// 64 of them rotated, written elsewhere: 18 to 20 us for 84 MB, 4.3 TB/s (four units a thread; one: 24); 64 rows 3.0 us, a launch
+// and two loads in series.
 enum { HALF, PAIRS, ODD };  // ODD: pairs half the rotated dims apart where that is no multiple of 8: element by element
 template <class T>
 struct RopeSide {  // q's or k's heads
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(256) void k_rope(const double* __restrict__ freqs, 
     }
 }
 
-// Each row's request by a search of cu in LDS.
+// Each row's request by a search of cu in LDS.  (64 requests 1.6 us, 16396 rows 2.3)
 __global__ __launch_bounds__(1024) void k_page_positions(const int* __restrict__ cu, const int* __restrict__ dropped, int B,
                                                          int T, const int* pos, int* out) {
     __shared__ int to[PAGE_PLAN_MAX_B + 1];
