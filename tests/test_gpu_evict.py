@@ -436,6 +436,52 @@ def test_evict_many_requests(sdamd):
     check_evict(sdamd, 8, lens, [int(x) for x in rng.integers(-1, 90, 700)], 2, 32, 2, 8, values="few")
 
 
+@pytest.mark.parametrize("max_kv", [512, 40000])
+def test_evict_replayed_with_other_lengths(sdamd, max_kv):
+    """Eviction, moves and release in one captured graph: lengths, budgets and scores change between the replays."""
+    B, hk, hd, ps = 3, 2, 64, 64
+    blocks = -(-max_kv // ps)
+    n_pages = B * blocks
+    rng = np.random.default_rng(21)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = pr.dev(rng.permutation(n_pages).reshape(B, blocks))
+    kv, budgets, dropped, n_free = torch.zeros(B, **i32), torch.zeros(B, **i32), pr.dev([1, 2, 3]), torch.zeros(1, **i32)
+    state = [torch.zeros(n_pages * hk * ps * hd, device="cuda").half() for _ in range(2)] + [torch.zeros(n_pages, hk, ps, device="cuda"),
+                                                                                             torch.zeros(n_pages, hk, ps, **i32)]
+    out = [torch.zeros(B, **i32), torch.zeros(B, hk, max_kv // 2, 2, **i32), torch.zeros(B, hk, **i32), torch.zeros(B, **i32), torch.zeros(1, **i32),
+           torch.zeros(n_pages, **i32)]
+    ws = torch.full((max(sdamd.page_evict_ws(B, max_kv, hk), 16),), 0xFF, dtype=torch.uint8, device="cuda")
+    p = lambda x: x.data_ptr()
+
+    def call(stream, state, out):
+        k, v, scores, kpos = state
+        new, moves, counts, gone, left, free = out
+        sdamd.op_page_evict(p(scores), p(kpos), p(table), blocks, p(kv), p(budgets), B, max_kv, hk, ps, n_pages, 2, 5, p(new), p(moves), p(counts), p(ws),
+                            ws.numel(), stream=stream)
+        sdamd.op_paged_move(p(moves), p(counts), p(table), blocks, B, max_kv, hk, hd, ps, n_pages, p(k), p(v), p(scores), p(kpos), 0, stream=stream)
+        sdamd.op_page_release(p(kv), p(new), p(dropped), p(table), blocks, B, ps, n_pages, p(free), p(n_free), p(gone), p(left), stream=stream)
+
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        call(torch.cuda.current_stream().cuda_stream, state, out)
+    for lens, keep in (([max_kv, 300, 0], [max_kv // 3, 299, 4]), ([40, max_kv - 1, 512], [41, max_kv - 70, -1]), ([max_kv, max_kv, max_kv], [0, 1, 450])):
+        kv.copy_(pr.dev(lens))
+        budgets.copy_(pr.dev(keep))
+        for t in state[:3]:
+            t.normal_()
+        state[3].random_(0, 1 << 20)
+        for t in out:
+            t.fill_(-4)
+        here, want = [t.clone() for t in state], [t.clone() for t in out]
+        call(None, here, want)
+        torch.cuda.synchronize()
+        assert want[0].tolist() == [m if 0 <= m < n else n for n, m in zip(lens, keep)] and int(want[2].sum()) > 0
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(state + out, here + want):
+            assert torch.equal(a, b)
+
+
 # ---- their moves and pages ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("hk,hd,ps,kind,pstride", [(2, 256, 32, "f16", 0), (3, 128, 64, "bf16", 3 * 64 * 128 + 40), (1, 64, 256, "f16", 0)])
