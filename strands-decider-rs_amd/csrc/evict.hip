@@ -54,6 +54,8 @@ struct WeightArgs {
     float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
     float2* stat;     // [rows][HQ], a request's rows kv head by kv head: of a row's whole, the sum's reciprocal
     float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
+    int* index;       // [3][B + 1]: the first tile of every request, and how many there are: of rows, of (key tile, part)s, of
+                      // keys.  null: each workgroup finds its own
     // the first key that a row at position p sees
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
@@ -413,8 +415,25 @@ __device__ __forceinline__ int many_rows(const WeightArgs& a, int b) {  // of re
     const int n = observed(request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap), a.observers).n * a.G;
     return n > a.few ? n : 0;
 }
+// Tile x of those that `which` says, `of(b)` of request b, as find_tile numbers them; in the index, which holds them in the
+// requests' order, by the lanes' steps through it, and by theirs through the step.
+enum { ROW_TILES, KEY_PARTS, KEY_TILES };
+template <class F>
+__device__ __forceinline__ Tile tile_of(const WeightArgs& a, int which, int x, F&& of) {
+    if (!a.index) return find_tile(a.B, x, of);
+    const int* const first = a.index + which * (a.B + 1);
+    const int lane = threadIdx.x & 63, step = (a.B + 63) >> 6;  // (128 at most)
+    const int total = first[a.B], y = first[min(lane * step, a.B)];
+    if (x >= total) return {-1, 0, 0};
+    const int n = total - 1 - x;
+    const int b0 = (__popcll(__ballot(lane * step < a.B && y <= n)) - 1) * step, b1 = min(b0 + step, a.B);
+    const int u = first[min(b0 + lane, a.B)], v = first[min(b0 + 64 + lane, a.B)];
+    const int at = __popcll(__ballot(b0 + lane < b1 && u <= n)) + __popcll(__ballot(b0 + 64 + lane < b1 && v <= n)) - 1;
+    return {b0 + at, n - (at < 64 ? __builtin_amdgcn_readlane(u, at) : __builtin_amdgcn_readlane(v, at - 64)), n};
+}
+__device__ __forceinline__ int row_tiles(const WeightArgs& a, int b) { return (many_rows(a, b) + ROW_TILE - 1) / ROW_TILE; }
 __device__ __forceinline__ Tile row_tile(const WeightArgs& a, int x) {
-    return find_tile(a.B, x, [&](int b) { return (many_rows(a, b) + ROW_TILE - 1) / ROW_TILE; });
+    return tile_of(a, ROW_TILES, x, [&](int b) { return row_tiles(a, b); });
 }
 
 // A tile's rows, the keys that some of them see, and this split's blocks of those.
@@ -615,11 +634,49 @@ __device__ __forceinline__ int key_parts(const WeightArgs& a, int b) {
     return n * a.G > a.few ? parts_of(a, n) * key_tiles(a, rq) : 0;
 }
 __device__ __forceinline__ Tile key_tile(const WeightArgs& a, int x) {
-    return find_tile(a.B, x, [&](int b) { return key_parts(a, b); });
+    return tile_of(a, KEY_PARTS, x, [&](int b) { return key_parts(a, b); });
+}
+__device__ __forceinline__ int many_key_tiles(const WeightArgs& a, int b) {
+    return many_rows(a, b) ? key_tiles(a, request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
+}
+// The index: one workgroup.  (Sums are cut at 2^24, which row starts that do not ascend could pass.)
+constexpr int INDEX_T = 1024;
+__global__ __launch_bounds__(INDEX_T) void k_weights_index(WeightArgs a) {
+    __shared__ int ws[3][INDEX_T / 64];
+    const int tid = threadIdx.x, wv = tid >> 6, per = (a.B + INDEX_T - 1) / INDEX_T, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    auto cut = [](int x) { return min(x, 1 << 24); };
+    int own[3] = {0, 0, 0}, at[3];
+    for (int b = b0; b < b1; b++) {
+        own[ROW_TILES] = cut(own[ROW_TILES] + row_tiles(a, b));
+        own[KEY_PARTS] = cut(own[KEY_PARTS] + key_parts(a, b));
+        own[KEY_TILES] = cut(own[KEY_TILES] + many_key_tiles(a, b));
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        at[k] = lanes_upto(own[k]);
+        if ((tid & 63) == 63) ws[k][wv] = cut(at[k]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < INDEX_T / 64; w++) before += w < wv ? ws[k][w] : 0, all += ws[k][w];
+        at[k] += before - own[k];
+        if (tid == 0) a.index[k * (a.B + 1) + a.B] = cut(all);
+    }
+    for (int b = b0; b < b1; b++) {
+#pragma unroll
+        for (int k = 0; k < 3; k++) a.index[k * (a.B + 1) + b] = cut(at[k]);
+        at[ROW_TILES] = cut(at[ROW_TILES] + row_tiles(a, b));
+        at[KEY_PARTS] = cut(at[KEY_PARTS] + key_parts(a, b));
+        at[KEY_TILES] = cut(at[KEY_TILES] + many_key_tiles(a, b));
+    }
 }
 // The number of request b's first one, in find_tile's order: lane by lane, lane l's requests l, l + 64, ...
 __device__ __forceinline__ int first_key_tile(const WeightArgs& a, int b) {
     if (a.B == 1) return 0;
+    if (a.index) return a.index[KEY_PARTS * (a.B + 1) + b];
     const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
     int own = 0, before = 0;
 #pragma unroll 8
@@ -795,9 +852,7 @@ constexpr int SUM_G = 4;
 __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a) {
     __shared__ float part[SUM_G][KEY_TILE];
     const int kh = blockIdx.x % a.HK, i = threadIdx.x % KEY_TILE, grp = threadIdx.x / KEY_TILE;
-    const Tile tl = find_tile(a.B, blockIdx.x / a.HK, [&](int b) {
-        return many_rows(a, b) ? key_tiles(a, request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
-    });
+    const Tile tl = tile_of(a, KEY_TILES, blockIdx.x / a.HK, [&](int b) { return many_key_tiles(a, b); });
     if (tl.b < 0) return;
     const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
     const Seen ob = observed(rq, a.observers);
@@ -1544,12 +1599,17 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
     else run(std::integral_constant<int, 4>());
 }
 
+// Requests up to which each workgroup finds its tile by itself; from there on a launch before makes an index.  (us without and with
+// it, 20 new rows on 300 keys each, 8 and 2 heads of 128 dims: 128 requests 25 27.6, 192 34.2 34.9, 256 42.7 41.5, 1024
+// 134 94, 8192 4020 768; 16 on 2000 keys, 32 and 8 heads: 128 requests 247 236, 256 522 477, 1024 2415 1790)
+constexpr int INDEX_B = 128;
+
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
 struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
     int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0;  // tiles 0: no many rows
     bool once = false, one = false;  // keys read past the last-level cache; k_weights_few_one
-    size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0;  // floats of the workspace
+    size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0, index = 0;  // floats and ints of the workspace
 };
 
 WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
@@ -1601,8 +1661,9 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         p.ml = p.ks > 1 ? (size_t)p.ks * p.tiles * s.HK * ROW_TILE * 2 : 0;
         p.stat = (size_t)rows * s.HQ * 2;
         p.col = p.parts > 1 ? (size_t)p.units * s.HK * KEY_TILE : 0;
+        p.index = B > INDEX_B ? 3 * ((size_t)B + 1) : 0;
     }
-    for (size_t* x : {&p.S, &p.few_ml, &p.ml, &p.stat, &p.col}) *x = (*x + 3) & ~size_t(3);
+    for (size_t* x : {&p.S, &p.few_ml, &p.ml, &p.stat, &p.col, &p.index}) *x = (*x + 3) & ~size_t(3);
     return p;
 }
 
@@ -1619,6 +1680,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     g.ml = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.few_ml) + p.few_ml);
     g.stat = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.ml) + p.ml);
     g.col = reinterpret_cast<float*>(g.stat) + p.stat;
+    g.index = p.index ? reinterpret_cast<int*>(g.col + p.col) : nullptr;
     const T *Q = static_cast<const T*>(a.Q), *K = static_cast<const T*>(a.Kp);
     auto launch = [&](auto kernel, dim3 grid, int threads, auto... args) {
         hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, args...);
@@ -1626,6 +1688,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     };
     if (p.tiles) {
         const dim3 rows((p.tiles | 1) * s.HK * p.ks), keys(p.units * s.HK);
+        if (p.index) launch(k_weights_index, dim3(1), INDEX_T, g);
         launch(k_weights_rows<T, HD>, rows, 256, Q, K, g);
         if (p.ks > 16) launch(k_weights_join<64>, dim3(p.tiles * s.HK * (ROW_TILE / 4)), 256, g);
         else if (p.ks > 1) launch(k_weights_join<8>, dim3(p.tiles * s.HK * (ROW_TILE / 32)), 256, g);
@@ -1662,7 +1725,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
 
 size_t paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
     const WeightPlan p = plan_weights(s, B, rows, max_new, max_kv, observers);
-    return (p.S + p.few_ml + p.ml + p.stat + p.col) * 4;
+    return (p.S + p.few_ml + p.ml + p.stat + p.col + p.index) * 4;
 }
 
 void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {

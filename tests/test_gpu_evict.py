@@ -265,6 +265,17 @@ def test_many_requests(sdamd, hq, hk, hd, kind, most):
         s.check()
 
 
+@pytest.mark.parametrize("requests,long", [(128, 2000), (129, 2000), (700, 300), (4500, 40)])
+def test_requests_with_chunks(sdamd, requests, long):
+    """Both sides of the number from which on the tiles have an index; its steps beyond 64 requests; parts and splits of some."""
+    rng = np.random.default_rng(requests)
+    old, new = rng.integers(0, long // 8, requests), rng.choice([0, 1, 1, 9, 40], requests)
+    old[[0, 70, requests - 2]], new[[0, 3, 70, requests - 1]] = (0, long, long), (0, long, 90, 33)
+    s = Step(requests, old.tolist(), new.tolist(), 8, 2, 64, 32, "f16", observers=0 if requests < 500 else 20)
+    s.run(sdamd)
+    s.check()
+
+
 def few_launches(sdamd, B, T, max_new, max_kv, hq, hk, hd, observers=0):
     """Workgroup sizes of a call's launches, on lengths of zero."""
     i32 = dict(dtype=torch.int32, device="cuda")
