@@ -134,11 +134,11 @@ __device__ __forceinline__ Few few_of(const WeightArgs& a, int b) {
 // Scores of up to 16 NR rows of a (request, kv head) over blocks [blk0, blk1) of keys, by NW waves, into S (rows `stride`
 // floats apart, key j at j), and each wave's maxima and sums of the rows over them.  A wave loads K straight into registers
 // in MFMA operand order, D blocks of 32 keys in flight.
-template <class T, int HD, int NR, bool ONCE, int NW>
+template <class T, int HD, int NR, bool ONCE, int NW, int D>
 __device__ __forceinline__ void few_scores(const T* __restrict__ Q, const T* __restrict__ Kp, const WeightArgs& a, const Few& f, int b,
                                            int kh, int blk0, int blk1, float* S, int stride, float* Ms, float* Ls) {
     typedef typename Vec8<T>::type T8;
-    constexpr int NS = HD / 32, R = 16 * NR, D = HD == 64 ? 4 : HD == 128 ? 3 : 2;
+    constexpr int NS = HD / 32, R = 16 * NR;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fq = lane & 15, fg = lane >> 4;
     const Req& rq = f.rq;
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
     if (f.nrows == 0 || f.nrows > a.few) return;
     const int blk0 = (f.lo >> 5) + z * a.few_span;
     const int blk1 = z + 1 < a.few_ks ? min((f.hi + 31) >> 5, blk0 + a.few_span) : (f.hi + 31) >> 5;
-    few_scores<T, HD, NR, ONCE, FEW_W>(Q, Kp, a, f, b, kh, blk0, blk1, a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp, a.kvp, Ms, Ls);
+    few_scores<T, HD, NR, ONCE, FEW_W, HD == 64 ? 4 : HD == 128 ? 3 : 2>(Q, Kp, a, f, b, kh, blk0, blk1, a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp, a.kvp, Ms, Ls);
     __syncthreads();
     if (tid < f.nrows) {
         float mx = -INFINITY, sum = 0.f;
@@ -282,9 +282,12 @@ struct Keys4 {
     size_t at;
     f32x4u old;
 };
-__device__ __forceinline__ Keys4 keys4(const WeightArgs& a, const Few& f, int b, int kh, int j) {
+__device__ __forceinline__ int page_of(const WeightArgs& a, int b, int j) {
+    return a.table[(size_t)b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
+}
+__device__ __forceinline__ Keys4 keys4(const WeightArgs& a, const Few& f, int kh, int j, int page) {
     Keys4 k;
-    k.page = a.table[(size_t)b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
+    k.page = page;
     const bool there = j < f.rq.kcap && (unsigned)k.page < (unsigned)a.n_pages;
     k.at = mark_at(there ? k.page : 0, a.HK, kh, there ? j : 0, a.lps);
     k.old = f32x4u{0.f, 0.f, 0.f, 0.f};
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     };
     auto load = [&](int j) INL {
         Keys k;
-        k.k = keys4(a, f, b, kh, j);
+        k.k = keys4(a, f, kh, j, page_of(a, b, j));
 #pragma unroll
         for (int r = 0; r < PRE; r++) {
             k.x[r] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -378,18 +381,27 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
 // of 128 dims: 83 us for 400 MB of keys, 4.8 TB/s (in splits 97); 4 waves level, 16 slower.
 constexpr int ONE_W = 8, ONE_LDS = 136 << 10, ONE_KEYS = 8192;  // waves; bytes of scores, and keys, at most
 template <class T, int HD, int NR, bool ONCE>
-__global__ __launch_bounds__(64 * ONE_W) void k_weights_few_one(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
+__global__ __launch_bounds__(64 * ONE_W, HD * NR <= 128 ? 4 : 2) void k_weights_few_one(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     constexpr int R = 16 * NR, KN = ONE_KEYS / (256 * ONE_W);
+    constexpr bool EARLY = HD * NR == 256;
     extern __shared__ __align__(16) float S[];
     __shared__ float Ms[ONE_W * R], Ls[ONE_W * R];
     __shared__ float2 stat[R];
     const int tid = threadIdx.x, kh = blockIdx.x, b = blockIdx.y;
     const Few f = few_of(a, b);
     if (f.nrows == 0 || f.nrows > a.few) return;
-    Keys4 k[KN];  // (on their way meanwhile)
+    int page[KN];  // (what the keys have is on its way meanwhile too, where no second workgroup fits the CU's registers anyway)
+    Keys4 k[KN];
 #pragma unroll
-    for (int i = 0; i < KN; i++) k[i] = keys4(a, f, b, kh, 4 * (tid + 64 * ONE_W * i));
-    few_scores<T, HD, NR, ONCE, ONE_W>(Q, Kp, a, f, b, kh, f.lo >> 5, (f.hi + 31) >> 5, S, a.kvp, Ms, Ls);
+    for (int i = 0; i < KN; i++) {
+        const int j = 4 * (tid + 64 * ONE_W * i);
+        page[i] = page_of(a, b, j);
+        if (EARLY) k[i] = keys4(a, f, kh, j, page[i]);
+    }
+    few_scores<T, HD, NR, ONCE, ONE_W, HD == 64 ? 3 : 2>(Q, Kp, a, f, b, kh, f.lo >> 5, (f.hi + 31) >> 5, S, a.kvp, Ms, Ls);
+#pragma unroll
+    for (int i = 0; i < KN; i++)
+        if (!EARLY) k[i] = keys4(a, f, kh, 4 * (tid + 64 * ONE_W * i), page[i]);
     __syncthreads();
     if (tid < f.nrows) {
         float mx = -INFINITY, sum = 0.f;
