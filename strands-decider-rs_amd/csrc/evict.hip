@@ -42,6 +42,7 @@ struct WeightArgs {
                                                // keys in each; rows and keys of a request's scores
     int tiles, ks, span;                       // many rows: tiles of rows, their splits, blocks in each;
     int part, parts, units;                    // tokens of a part, parts of a request at most, (key tile, part)s at most
+    int ordered;                               // requests by length, the longest first
     int dt, dg;                                // 32 rows: tokens, and heads besides
     uint32_t magic;  // 2^32 / G and 1 more: x / G is the upper half of a product for x below 2^16
     float c, decay;  // c: scale log2(e)
@@ -378,8 +379,9 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
 }
 
 // Short caches: a (request, kv head) per workgroup, its scores in LDS, in one launch.  64 requests of 1000 to 8191 keys, 8 heads
-// of 128 dims: 83 us for 400 MB of keys, 4.8 TB/s (in splits 97); 4 waves level, 16 slower.
+// of 128 dims: 70 us for 400 MB of keys, 5.7 TB/s, the longest first (as they come 83, in splits 97); 4 waves level, 16 slower.
 constexpr int ONE_W = 8, ONE_LDS = 136 << 10, ONE_KEYS = 8192;  // waves; bytes of scores, and keys, at most
+constexpr int ONE_ORDER = 64 * ONE_W;  // requests up to which they are taken by length
 template <class T, int HD, int NR, bool ONCE>
 __global__ __launch_bounds__(64 * ONE_W, HD * NR <= 128 ? 4 : 2) void k_weights_few_one(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     constexpr int R = 16 * NR, KN = ONE_KEYS / (256 * ONE_W);
@@ -387,7 +389,28 @@ __global__ __launch_bounds__(64 * ONE_W, HD * NR <= 128 ? 4 : 2) void k_weights_
     extern __shared__ __align__(16) float S[];
     __shared__ float Ms[ONE_W * R], Ls[ONE_W * R];
     __shared__ float2 stat[R];
-    const int tid = threadIdx.x, kh = blockIdx.x, b = blockIdx.y;
+    __shared__ __align__(16) uint32_t by_length[ONE_ORDER];
+    __shared__ int nth;
+    const int tid = threadIdx.x, kh = blockIdx.x;
+    int b = blockIdx.y;
+    if (a.ordered) {  // the longest first: the b-th of them
+        uint32_t own = 0;
+        if (tid < a.B) own = (uint32_t)min(max(a.kv_lens[tid], 0), ONE_KEYS) * ONE_ORDER + tid;
+        by_length[tid] = own;
+        __syncthreads();
+        if (tid < a.B) {
+            int longer = 0;
+#pragma unroll 4
+            for (int i = 0; i < a.B; i += 4) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(by_length + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) longer += x[e] > own;
+            }
+            if (longer == b) nth = tid;
+        }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(nth);
+    }
     const Few f = few_of(a, b);
     if (f.nrows == 0 || f.nrows > a.few) return;
     int page[KN];  // (what the keys have is on its way meanwhile too, where no second workgroup fits the CU's registers anyway)
@@ -1620,7 +1643,7 @@ constexpr int INDEX_B = 128;
 struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
     int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0;  // tiles 0: no many rows
-    bool once = false, one = false;  // keys read past the last-level cache; k_weights_few_one
+    bool once = false, one = false, ordered = false;  // keys read past the last-level cache; k_weights_few_one, by length
     size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0, index = 0;  // floats and ints of the workspace
 };
 
@@ -1646,6 +1669,13 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         const size_t each = (size_t)nb * s.HD * 64;
         p.one = (long long)nb * 32 <= ONE_KEYS && (size_t)p.few * p.kvp * 4 <= ONE_LDS &&
                 (B * s.HK >= 256 || each <= (size_t(B * s.HK >= 128 ? 1024 : 256) << 10));
+        // By length, the longest first, where not all run at once and a head's keys outweigh every workgroup's look at all lengths
+        // (which nothing hides where a CU has one workgroup).  us without and with it, lengths between the two (in logarithms):
+        // 8 heads, 128 dims: 64 requests of 100 to 1200 keys 15.9 15.5, of 1000 to 8100 96 79; 128 of 100 to 2000 38.0 36.2, of 500 to
+        // 8100 150 134; 200 of 100 to 2000 52.9 56.1, to 4000 92 88; 500 of 100 to 1000 76 125
+        // 64 dims: 128 of 100 to 2000 20.8 23.1, of 500 to 4000 46.9 43.5.  256 dims: 64 of 50 to 300 14.0 14.7, of 1000 to 8100 183
+        // 148, 100 of 100 to 1000 40 40, 200 of 100 to 2000 103 118
+        p.ordered = p.one && B <= ONE_ORDER && B * s.HK > 256 && each >= (size_t)B * (s.HD * p.nr > 128 ? 8192 : 4096);
         p.S = p.one ? 0 : (size_t)B * s.HK * p.few * p.kvp;
         p.few_ml = p.one ? 0 : (size_t)B * s.HK * p.few_ks * p.few * 2;
         p.once = (size_t)B * nb * s.HK * s.HD * 64 > (size_t(256) << 20);
@@ -1686,7 +1716,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     float* const ws = static_cast<float*>(a.ws);
     WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, G, log2i(s.PS), s.n_pages, a.max_new,
                  a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.part,
-                 p.parts, p.units, 32 / G, 32 % G, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
+                 p.parts, p.units, p.ordered, 32 / G, 32 % G, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
     g.S = ws;
     g.few_ml = reinterpret_cast<float2*>(g.S + p.S);
     g.ml = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.few_ml) + p.few_ml);

@@ -332,6 +332,20 @@ def test_replayed_with_other_lengths(sdamd):
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("requests,most,hk", [(64, 4000, 8), (33, 8192, 8), (300, 4900, 1)])
+def test_longest_first(sdamd, requests, most, hk):
+    """More heads than run at once, of many lengths, some of them equal, some of none: each request is done once."""
+    rng = np.random.default_rng(requests)
+    old = rng.integers(0, 300, requests)
+    old[rng.integers(0, requests, requests // 3)] = 100
+    old[[2, requests - 1]] = most - 1, most // 2
+    new = rng.choice([0, 1, 1, 1], requests)
+    new[[2, requests - 1]] = 1
+    s = Step(requests, old.tolist(), new.tolist(), 2 * hk, hk, 64 if hk == 1 else 128, 32, "bf16")
+    s.run(sdamd)
+    s.check()
+
+
 def test_two_streams(sdamd):
     """Two calls at once, a workspace each."""
     steps = [Step(30 + i, [4000, 900], [1 + 30 * i, 1], 8, 2, 128, 64, "f16") for i in range(2)]
