@@ -1663,9 +1663,10 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         p.few_ks = (nb + p.few_span - 1) / p.few_span;
         // One workgroup per head where there are enough of them, or few bytes of keys for each: one launch, and no scores in memory.
         // us in splits and so, at n keys of each request:
-        // 2 heads, 256 dims: 300 8.8 7.2, 700 9.1 9.7; 8 heads, 128 dims: 700 9.2 7.4, 1200 9.1 9.3, 2000 9.3 12.0
-        // 128 heads, 256 dims: 700 14.7 11.5, 2000 27.5 23.3; 128 dims: 2000 17.0 13.5, 6000 40.9 41.4, 8100 48.3 51.9
-        // 512 heads, 128 dims: 1200 34.9 27.9, 3800 83 68, 6000 126 101, 8100 171 139; 64 dims: 1200 19.8 13.7, 8100 97 77
+        // 2 heads, 256 dims: 300 8.5 7.6, 700 8.1 10.3; 8 heads, 128 dims: 700 8.1 7.4, 1200 8.2 9.2, 2000 8.1 11.8
+        // 128 heads, 256 dims: 700 16.4 12.4, 2000 27.8 23.4, 1000 to 8100 58 79; 128 dims: 2000 18.9 13.9, 1000 to 8100 31.2 33.4
+        // 256 heads: 128 dims, 1000 to 8100 60 52; 256 dims 101 98
+        // 512 heads, 128 dims: 1200 32.7 27.9, 3800 105 83, 8100 220 183, 1000 to 8100 113 78; 64 dims: 1200 21.8 16.3, 8100 118 92
         const size_t each = (size_t)nb * s.HD * 64;
         p.one = (long long)nb * 32 <= ONE_KEYS && (size_t)p.few * p.kvp * 4 <= ONE_LDS &&
                 (B * s.HK >= 256 || each <= (size_t(B * s.HK >= 128 ? 1024 : 256) << 10));
