@@ -34,7 +34,6 @@ __device__ __forceinline__ size_t mark_at(int page, int HK, int h, int j, int lp
 // of two rounded products.
 // Sums have one order: over a lane's own keys or rows, then lanes, waves, and parts by their number.
 
-
 struct WeightArgs {
     const int *table, *cu, *kv_lens, *pos;
     int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, observers;
@@ -53,7 +52,7 @@ struct WeightArgs {
     float* S;         // [B][HK][rw][kvp]: c s of the few rows
     float2* few_ml;   // [B][HK][few_ks][rw]: their maxima and sums
     float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
-    float2* stat;     // [rows][HQ], a request's rows kv head by kv head: of a row's whole, the sum's reciprocal
+    float2* stat;     // [rows][HQ], a request's rows kv head by kv head: the maximum, and the whole sum's reciprocal
     float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
     int* index;       // [3][B + 1]: the first tile of every request, and how many there are: of rows, of (key tile, part)s, of
                       // keys.  null: each workgroup finds its own
