@@ -29,9 +29,11 @@ __device__ __forceinline__ size_t mark_at(int page, int HK, int h, int j, int lp
 // queries in a wave's registers and lets keys pass, the second keeps 32 keys and lets rows pass, so each sums in registers
 // over what passes and neither needs another lane's values until its end.
 //
-// Scores are S^T = K Q^T (keys x rows) on MFMA, in f32, and so is all behind them; exponentials are in base 2.  A row's
-// maximum is c s rounded (c = scale log2 e).  c s - m is one fma, or, from FAR on, where m has no fractions, the difference
-// of two rounded products.
+// Scores are S^T = K Q^T (keys x rows) on MFMA, in f32, and so is all behind them; exponentials are in base 2, c = scale log2 e.
+// Few rows keep c s, rounded, and its maximum m; exponents are the differences.  Many rows keep the maximum of s, and exponents
+// are (s - m) c: a subtraction more than one fma of s, c and m, and with it sums and weights are the same function of s whatever
+// the size of the scores, of other keys' or of other rows' (a fused c s - m, m rounded, leaves the rounding's 2^x in a row's sum,
+// and has to be left from 2^23 on, where m has no fractions, at one key for the sum and at another for the weights).
 // Sums have one order: over a lane's own keys or rows, then lanes, waves, and parts by their number.
 
 struct WeightArgs {
@@ -69,12 +71,11 @@ __device__ __forceinline__ Seen observed(const Req& r, int observers) {
     return {r.n - n, n};
 }
 
-// c s, rounded: what a row's maximum is one of.
+// c s, rounded: what a few rows' maximum is one of.
 __device__ __forceinline__ float scaled(float s, float c) {
 #pragma clang fp contract(off)
     return s * c;
 }
-__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= FAR; }
 
 // A row's part: maximum and sum, and their turn to a row's whole.
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }  // (its sum is 0, or NaN)
@@ -85,21 +86,24 @@ __device__ __forceinline__ size_t stat_at(const WeightArgs& a, const Req& rq, co
     return (size_t)(rq.q0 + ob.t0) * a.HQ + (size_t)kh * ob.n * a.G;
 }
 
-// A row's whole, from its n parts, `step` apart: N lanes on end share it.
+// The weight of a part whose maximum of s is m, as part_weight.
+__device__ __forceinline__ float part_of(float m, float mx, float c) { return m == -INFINITY ? 0.f : exp2_fast((m - mx) * c); }
+
+// A row's whole, from its n parts, `step` apart: N lanes on end share it.  c: 1 where the maxima are c s.
 template <int N>
-__device__ __forceinline__ float2 join_parts(const float2* ml, size_t step, int n) {
+__device__ __forceinline__ float2 join_parts(const float2* ml, size_t step, int n, float c) {
     float mx = -INFINITY, l = 0.f;
 #pragma unroll 4
     for (int z = threadIdx.x % N; z < n; z += N) {
         const float2 v = ml[z * step];
         const float mn = fmaxf(mx, v.x);
-        l = l * part_weight(mx, mn) + v.y * part_weight(v.x, mn);
+        l = l * part_of(mx, mn, c) + v.y * part_of(v.x, mn, c);
         mx = mn;
     }
 #pragma unroll
     for (int o = 1; o < N; o <<= 1) {
         const float m2 = __shfl_xor(mx, o), l2 = __shfl_xor(l, o), mn = fmaxf(mx, m2);
-        l = l * part_weight(mx, mn) + l2 * part_weight(m2, mn);
+        l = l * part_of(mx, mn, c) + l2 * part_of(m2, mn, c);
         mx = mn;
     }
     return make_float2(base_of(mx), inverse_of(l));
@@ -359,10 +363,10 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     {
         const float2* const ml = a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw;
         if (nrows <= 4) {
-            const float2 st = join_parts<64>(ml + min(tid >> 6, nrows - 1), a.rw, a.few_ks);
+            const float2 st = join_parts<64>(ml + min(tid >> 6, nrows - 1), a.rw, a.few_ks, 1.f);
             if ((tid & 63) == 0) stat[tid >> 6] = st;
         } else {
-            const float2 st = join_parts<8>(ml + min(tid >> 3, nrows - 1), a.rw, a.few_ks);
+            const float2 st = join_parts<8>(ml + min(tid >> 3, nrows - 1), a.rw, a.few_ks, 1.f);
             if ((tid & 7) == 0) stat[tid >> 3] = st;
         }
     }
@@ -622,22 +626,17 @@ __global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q
         float top = s[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
-        const float mn = fmaxf(m, scaled(top, a.c)), base = base_of(mn);
-        float sum = l * exp2_fast(m - base);
-        if (__builtin_expect(__any(is_far(base)), 0)) {
+        const float mn = fmaxf(m, top), base = base_of(mn);
+        float sum = l * exp2_fast((m - base) * a.c);
 #pragma unroll
-            for (int e = 0; e < 16; e++) sum += exp2_fast(scaled(s[e], a.c) - base);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) sum += exp2_fast(__builtin_fmaf(s[e], a.c, -base));
-        }
+        for (int e = 0; e < 16; e++) sum += exp2_fast((s[e] - base) * a.c);
         m = mn, l = sum;
     };
     RING_START(K, fetch)
     RING_LOOP(K, nb)
     wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
     const float mx = max_halves(m);
-    float sum = l * part_weight(m, mx);
+    float sum = l * part_of(m, mx, a.c);
     sum += __shfl_xor(sum, 32);
     if (!live || g || w0 + c >= t.r1) return;
     if (a.ks == 1) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = make_float2(base_of(mx), inverse_of(sum));
@@ -655,7 +654,7 @@ __global__ __launch_bounds__(256) void k_weights_join(WeightArgs a) {
     const int i = blockIdx.x % PER * ROWS + threadIdx.x / N, r = t.r0 + i;
     if (r >= t.r1) return;
     const int n = min(a.ks, (((t.hi + 31) >> 5) - t.blk0 + a.span - 1) / a.span);
-    const float2 st = join_parts<N>(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n);
+    const float2 st = join_parts<N>(a.ml + ((size_t)tl.x * a.HK + kh) * ROW_TILE + i, (size_t)a.tiles * a.HK * ROW_TILE, n, a.c);
     if (threadIdx.x % N == 0) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = st;
 }
 
@@ -850,20 +849,18 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
 #pragma unroll
             for (int x = 0; x < NS; x++)
                 s = Num<T>::mfma32(__builtin_bit_cast(T8, kf[x]), __builtin_bit_cast(T8, Rg::read(buf, x, c, g)), s);
-            const bool far = __any(is_far(now.x));
             // every row sees every key: the first token's causally, the last one's through the window
             const bool open = there && jw + 32 <= rq.kcap && 32 * i + 32 <= nr && p0 + tb >= jw + 31 &&
                               (!a.window || p0 + tb + a.dt + 1 - jw < a.window);
-            if (__builtin_expect(open && !far, 1)) {
+            if (__builtin_expect(open, 1)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[e], a.c, -now.x)), now.y, acc[e]);
+                for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(exp2_fast((s[e] - now.x) * a.c), now.y, acc[e]);
             } else {
                 const int p = max(p0 + tb + (int)token_of(gb + c), -1), j = jw + 4 * g;
                 const Within keep(max(a.from(p), 0) - j, there && 32 * i + c < nr ? p - j : -1);
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const float x = far ? scaled(s[e], a.c) - now.x : __builtin_fmaf(s[e], a.c, -now.x);
-                    const float w = exp2_fast(x) * now.y;
+                    const float w = exp2_fast((s[e] - now.x) * a.c) * now.y;
                     acc[e] += keep.has(key_of(e)) ? w : 0.f;
                 }
             }

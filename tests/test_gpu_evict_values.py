@@ -1,0 +1,98 @@
+"""The weight that every cached key receives where scores are far from 1, sums are long, and work is cut: keys and rows are
+chosen so that every weight is known."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import evict_ref as er
+import paged_ref as pr
+from test_gpu_evict import Step
+
+pytestmark = pytest.mark.gpu
+
+
+def given(step, keys, rows):
+    """The step's keys of each request [kv][hk][hd], and its queries [T][hq][hd], in place of random ones."""
+    step.k = [k.to("cuda", pr.DT[step.kind]) for k in keys]
+    for b, k in enumerate(step.k):
+        step.cache.put(pr.slots_of(step.table, b, step.ps, 0, len(k)), k, torch.zeros_like(k))
+    step.q = rows.to("cuda", pr.DT[step.kind])
+
+
+def weights_of(step, b):
+    """[kv][hk] of request b, f64 on the CPU."""
+    s = torch.as_tensor(pr.slots_of(step.table, b, step.ps, 0, step.kv[b]))
+    return step.out.cpu()[s // step.ps, :, s % step.ps].double()
+
+
+# ---- scores of any size, rows of any neighbours ----------------------------------------------------
+
+def one_hot(rng, old, n, hq, hd, kind, window=0):
+    """64 rows, each with a dim of its own, and keys that have the 64 dims in turn: row r's scores are a_r on its keys and 0 on
+    the others, some 2^16 to 2^22.8 in base 2, so that its n keys share its weight and the others get none."""
+    s = Step(3, [old], [n], hq, 1, hd, 32, kind, decay=0.0, scale=500.0, window=window)
+    kv, g = old + n, hq
+    assert n * g == 64
+    j, r = torch.arange(kv), torch.arange(64)
+    k, q = torch.zeros(kv, 1, hd), torch.zeros(64, hd)
+    k[j, 0, j % 64] = 1.0
+    q[r, r] = torch.from_numpy(np.exp(rng.uniform(math.log(100), math.log(10000), 64))).float()
+    p = old + r // g
+    sees = (j[None] <= p[:, None]) & ((j[None] > (p - window)[:, None]) if window else True)
+    own = sees & (j[None] % 64 == r[:, None])
+    return s, k, q, sees, own
+
+
+@pytest.mark.parametrize("late", [False, True])
+@pytest.mark.parametrize("loud", [0, 17, 31, 40, 63])
+@pytest.mark.parametrize("old,n,hq,hd,kind", [(100, 64, 1, 64, "f16"), (3000, 64, 1, 128, "f16"), (100, 16, 4, 256, "bf16"), (3000, 16, 4, 64, "bf16")])
+def test_a_loud_row_leaves_the_others(sdamd, loud, old, n, hq, hd, kind, late):
+    """A row's weights are what it gives alone, whatever the size of the scores of the rows beside it."""
+    s, k, q, sees, own = one_hot(np.random.default_rng(loud), old, n, hq, hd, kind)
+    q[loud] *= 60000.0 / q[loud, loud]  # 2^25.3
+    if late:  # (its keys behind others')
+        k[:old // 2, 0, loud] = 0.0
+        own[loud] &= torch.arange(old + n) >= old // 2
+    given(s, [k], q.view(n, hq, hd))
+    s.run(sdamd)
+    want = (own / own.sum(1, keepdim=True)).double().sum(0)
+    # (equal scores: exponentials of 0, a whole number as the sum; its reciprocal within a step and a half, nothing else added)
+    assert ((weights_of(s, 0)[:, 0] - want).abs() <= 4 * er.E32 * want).all()
+
+
+@pytest.mark.parametrize("loud", [0, 8, 20, 40])
+@pytest.mark.parametrize("old,hd", [(200, 64), (1000, 256)])
+def test_an_infinite_row_leaves_the_others(sdamd, loud, old, hd):
+    """Keys that a row with infinite scores sees become NaN; the weights of all others are what they are without it."""
+    s, k, q, sees, own = one_hot(np.random.default_rng(loud), old, 64, 1, hd, "f16", window=64)
+    q[loud] = math.inf
+    given(s, [k], q.view(64, 1, hd))
+    s.run(sdamd)
+    got, want = weights_of(s, 0)[:, 0], (own / own.sum(1, keepdim=True)).double().sum(0)
+    assert torch.equal(torch.isnan(got), sees[loud])
+    assert (want > 0)[~sees[loud]].any()
+    assert ((got - want).abs() <= 4 * er.E32 * want)[~sees[loud]].all()
+
+
+@pytest.mark.parametrize("rising", [True, False])
+@pytest.mark.parametrize("old,n,hq,hd", [(200, 40, 1, 64), (700, 16, 4, 128), (2500, 64, 2, 256)])
+def test_scores_around_2_to_23(sdamd, old, n, hq, hd, rising):
+    """Scores that are whole numbers around 6 million, steps of 1.4 in base 2 around 2^23: rows on both sides of it, and rows
+    whose maximum passes it from one block of keys to the next."""
+    scale = np.float32(8388608 / 6e6 * math.log(2))
+    s = Step(4, [old], [n], hq, 1, hd, 32, "f16", decay=0.0, scale=float(scale))
+    kv = old + n
+    rng = np.random.default_rng(old)
+    t = np.sort(rng.integers(-12, 13, kv))
+    k, q = torch.zeros(kv, 1, hd), torch.zeros(n, hq, hd)
+    k[:, 0, 0], k[:, 0, 1] = 100.0, torch.from_numpy(t if rising else t[::-1].copy()).float()
+    q[..., 0], q[..., 1] = torch.from_numpy(rng.choice([59968.0, 60000.0, 60000.0, 60032.0], (n, hq))).float(), 1.0
+    given(s, [k], q)
+    s.run(sdamd)
+    want, _ = er.weights(q.double(), k.double(), kv, float(scale))
+    # scores and their differences are exact (below 2^24); up to 34 in base 2, times c of two roundings, one more, and an exponential
+    # within 2 steps, in numerator and sum; sums of kv keys and of the rows, and a few more
+    rel = 2 * (34 * 3 * math.log(2) + 2) + kv + n * hq + 16
+    assert ((weights_of(s, 0)[:, 0] - want[0]).abs() <= rel * er.E32 * want[0] + 2.0 ** -126).all()
