@@ -771,6 +771,33 @@ void table_row(const std::string& who, int max_blocks, int page_size, int max_kv
 
 int moves_width(int max_kv) { return max_kv / 2 < 1 ? 1 : max_kv / 2; }
 
+// One side's heads of HD elements: T rows `stride` apart, `heads` of them `step` apart (elements; `size` bytes each).
+struct HeadRows {
+    const void* p;
+    size_t stride, step;
+    int heads;
+    Span span(int T, int HD, size_t size) const { return {p, p ? ((T - 1) * stride + (heads - 1) * step + HD) * size : 0}; }
+    bool same(const HeadRows& o, int T) const { return p == o.p && (T == 1 || stride == o.stride) && (heads == 1 || step == o.step); }
+};
+
+// Whether a head of x overlaps one of y.  Both may lie in turn in one buffer, a row's heads behind another's, at one stride.
+bool heads_meet(const HeadRows& x, const HeadRows& y, int T, int HD, size_t size) {
+    const Span a = x.span(T, HD, size), b = y.span(T, HD, size);
+    if (!a.first || !b.first || !overlap(a.first, a.second, b.first, b.second)) return false;
+    if (T > 1 && x.stride != y.stride) return true;
+    const long long apart = (static_cast<const char*>(y.p) - static_cast<const char*>(x.p)) / (long long)size;
+    const long long s = T > 1 ? (long long)x.stride : 1, most = T - 1;
+    const long long wide = (x.heads - 1) * (long long)x.step + HD, wide2 = (y.heads - 1) * (long long)y.step + HD, at = ((apart % s) + s) % s;
+    if (T > 1 && wide <= at && at + wide2 <= s) return false;  // (rows side by side)
+    auto down = [](long long n, long long d) { return n / d - (n % d < 0); };
+    for (int i = 0; i < x.heads; i++)
+        for (int j = 0; j < y.heads; j++) {  // -HD < d + t s < HD for some t within the rows
+            const long long d = apart + j * (long long)y.step - i * (long long)x.step;
+            if (std::max(-most, -down(HD - 1 + d, s)) <= std::min(most, down(HD - 1 - d, s))) return true;
+        }
+    return false;
+}
+
 }  // namespace
 
 int sd_rope_freqs(int RD, double theta, int scaling, double factor, double length, double low, double high, double* freqs,
@@ -832,21 +859,28 @@ int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inve
         if ((Ko && !Qo) || (K && Qo && !Ko) || (Ko && !K)) throw sd::Error(who + ": outputs for both q and k, or for neither");
         if (!Qo) Qo = Q, qo_stride = q_stride, qo_step = q_step, Ko = K, ko_stride = k_stride, ko_step = k_step;
         const size_t size = type == SD_F32 ? 4 : 2;
-        auto span = [&](const void* p, size_t stride, size_t step, int heads) {  // and its checks
-            if (stride % 8 || step % 8 || stride > UINT32_MAX || step > UINT32_MAX)
+        const HeadRows q{Q, q_stride, q_step, HQ}, k{K, k_stride, k_step, HK}, qo{Qo, qo_stride, qo_step, HQ}, ko{Ko, ko_stride, ko_step, HK};
+        for (const HeadRows& x : {q, k, qo, ko}) {
+            if (!x.p) continue;
+            if (x.stride % 8 || x.step % 8 || x.stride > UINT32_MAX || x.step > UINT32_MAX)
                 throw sd::Error(who + ": strides must be multiples of 8 below 2^32");
-            const size_t wide = (heads - 1) * step + HD, tall = (T - 1) * stride + HD;
-            if ((heads > 1 && step < (size_t)HD) || (T > 1 && stride < (size_t)HD) || (heads > 1 && T > 1 && stride < wide && step < tall))
+            const size_t wide = (x.heads - 1) * x.step + HD, tall = (T - 1) * x.stride + HD;
+            if ((x.heads > 1 && x.step < (size_t)HD) || (T > 1 && x.stride < (size_t)HD) ||
+                (x.heads > 1 && T > 1 && x.stride < wide && x.step < tall))
                 throw sd::Error(who + ": two heads overlap");
-            if (!aligned(p, 16)) throw sd::Error(who + ": the rows must be aligned to 16 bytes");
-            return Span{p, ((T - 1) * stride + (heads - 1) * step + HD) * size};
-        };
-        const Span q = span(Q, q_stride, q_step, HQ), k = K ? span(K, k_stride, k_step, HK) : Span{nullptr, 0};
-        const Span qo = span(Qo, qo_stride, qo_step, HQ), ko = K ? span(Ko, ko_stride, ko_step, HK) : Span{nullptr, 0};
+            if (!aligned(x.p, 16)) throw sd::Error(who + ": the rows must be aligned to 16 bytes");
+        }
         if (!aligned(freqs, 8) || !aligned(pos, 4)) throw sd::Error(who + ": the frequencies must be aligned to 8 bytes, the positions to 4");
-        const Span f{freqs, (size_t)RD * 4}, p{pos, (size_t)T * 4};
-        if (Qo != Q) apart(who, {q, k, f, p}, {qo}), apart(who, {q, k, f, p}, {ko});  // (q's and k's rows may lie in turn in one buffer)
-        else apart(who, {f, p}, {qo}), apart(who, {f, p}, {ko});
+        const Span f{freqs, (size_t)RD * 4}, p{pos, (size_t)T * 4}, qs = q.span(T, HD, size), ks = k.span(T, HD, size);
+        // A side is in place where its output is its input; else its output lies apart from both inputs.
+        const bool q_here = qo.same(q, T), k_here = ko.same(k, T);
+        for (const auto& side : {std::make_pair(qo, q_here), std::make_pair(ko, k_here)}) {
+            const Span out = side.first.span(T, HD, size);
+            if (side.second) apart(who, {f, p}, {out});
+            else apart(who, {qs, ks, f, p}, {out});
+        }
+        if (heads_meet(qo, ko, T, HD, size) || (q_here != k_here && heads_meet(q, k, T, HD, size)))
+            throw sd::Error(who + ": a q head overlaps a k head");
         sd::rope({static_cast<const double*>(freqs), RD, magnitude, layout == SD_ROPE_PAIRS, inverse != 0, static_cast<const int*>(pos),
                   T, HD, {Q, Qo, q_stride, q_step, qo_stride, qo_step}, {K, Ko, k_stride, k_step, ko_stride, ko_step}, HQ, HK, type},
                  static_cast<hipStream_t>(stream));

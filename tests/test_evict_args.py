@@ -72,6 +72,27 @@ def test_rope_refuses(sdamd, kw, message):
     refuses(sdamd, sdamd.op_rope, ROPE, kw, "sd_op_rope", message)
 
 
+HERE = dict(Qo=A + M, qo_stride=768, qo_step=128, Ko=A + M + 1024, ko_stride=768, ko_step=128)  # ROPE's own rows
+ONLY = dict(K=None, k_stride=0, k_step=0, HK=0)
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(Qo=A + M, Ko=A + 3 * M), "overlaps an input"), (dict(ONLY, Qo=A + M), "overlaps an input"),  # dense rows over strided ones
+    (dict(HERE, qo_stride=1536), "overlaps an input"), (dict(HERE, ko_stride=1536), "overlaps an input"), (dict(HERE, qo_step=136), "overlaps an input"),
+    (dict(HERE, Ko=A + M), "overlaps an input"), (dict(HERE, Ko=A + M + 1040), "overlaps an input"), (dict(HERE, Ko=A + M + 768), "overlaps an input"),
+    (dict(HERE, Qo=A + M + 256), "overlaps an input"), (dict(OUT, Ko=A + 2 * M), "q head overlaps a k head"), (dict(OUT, Ko=A + 2 * M + 1024), "q head overlaps a k head"),
+    (dict(OUT, qo_stride=768, ko_stride=768, Ko=A + 2 * M + 768), "q head overlaps a k head"),
+    (dict(OUT, qo_stride=768, ko_stride=760, Ko=A + 2 * M + 1024), "q head overlaps a k head"),  # (row 3's: 24 dims of it)
+    (dict(OUT, qo_stride=768, ko_stride=768, Ko=A + 2 * M + 1040, HK=2), "q head overlaps a k head"),  # (in the next row's first)
+    (dict(K=A + M), "q head overlaps a k head"), (dict(K=A + M + 128 * 2), "q head overlaps a k head"), (dict(K=A + M + 1008), "q head overlaps a k head"),
+    (dict(K=A + M + 768 * 2 - 128 * 2, HK=2), "q head overlaps a k head"), (dict(T=1, K=A + M + 768), "q head overlaps a k head"),
+    (dict(HERE, K=A + M + 768, Ko=A + 3 * M), "q head overlaps a k head"),  # (q in place over k that is read)
+])
+def test_rope_refuses_rows_over_rows(sdamd, kw, message):
+    """What is written is the heads' own place, or apart from all that is read and written."""
+    refuses(sdamd, sdamd.op_rope, ROPE, kw, "sd_op_rope", message)
+
+
 POSITIONS = dict(cu=A, dropped=A + 4096, B=8, T=100, pos=A + 8192, out=A + 12288)
 
 

@@ -234,3 +234,37 @@ def test_replayed(sdamd):
         step(None)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, (pos, table, y)))
+
+
+@pytest.mark.parametrize("t,kind", [(1, "f16"), (37, "bf16"), (700, "f32")])
+@pytest.mark.parametrize("layout", ["half", "pairs"])
+def test_rows_of_one_buffer(sdamd, layout, t, kind):
+    """q's and k's heads in turn in one buffer, in place by name, and one side in place while the other goes elsewhere: the same
+    rows as into buffers of their own."""
+    hd, rd, heads = 64, 40, 3
+    f = freqs_on(er.freqs(rd, 1e5))
+    pos = pr.dev(np.arange(t) * 11 + 5)
+    size = torch.finfo(DT[kind]).bits // 8
+    for shape, strides in (((t, heads, 2, hd), lambda b: (2 * heads * hd, 2 * hd)), ((heads, 2, t, hd), lambda b: (hd, 2 * t * hd)),
+                           ((t, 2, heads, hd), lambda b: (2 * heads * hd, hd))):
+        x = torch.randn(shape, device="cuda").to(DT[kind])
+        rs, hs = strides(x)
+        second = {3: hd, 2: t * hd, 1: heads * hd}[2 if shape[0] == heads and shape[1] == 2 and shape[2] == t else 1 if shape[1] == 2 else 3]
+
+        def call(buf, **kw):
+            q, k = buf.data_ptr(), buf.data_ptr() + second * size
+            sdamd.op_rope(f.data_ptr(), rd, 0 if layout == "half" else 1, pos.data_ptr(), t, hd, q, rs, hs, heads, k, rs, hs, heads, KIND[kind], **kw)
+
+        q1, k1 = (torch.full((t, heads, hd), 3.0, device="cuda").to(DT[kind]) for _ in range(2))
+        call(x, Qo=q1.data_ptr(), Ko=k1.data_ptr())
+        here, named, half, out = x.clone(), x.clone(), x.clone(), torch.zeros_like(x)
+        call(here)
+        own = dict(qo_stride=rs, qo_step=hs, ko_stride=rs, ko_step=hs)
+        call(named, Qo=named.data_ptr(), Ko=named.data_ptr() + second * size, **own)
+        call(x, Qo=out.data_ptr(), Ko=out.data_ptr() + second * size, **own)
+        k2 = torch.zeros_like(k1)
+        call(half, **{**own, "Qo": half.data_ptr(), "Ko": k2.data_ptr(), "ko_stride": None, "ko_step": None})
+        rows = lambda b, at: torch.as_strided(b, (t, heads, hd), (rs, hs, 1), at)
+        for b in (here, named, out):
+            assert torch.equal(rows(b, 0), q1) and torch.equal(rows(b, second), k1)
+        assert torch.equal(rows(half, 0), q1) and torch.equal(k2, k1) and torch.equal(rows(half, second), rows(x, second))
