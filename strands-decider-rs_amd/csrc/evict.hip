@@ -81,6 +81,27 @@ __device__ __forceinline__ float scaled(float s, float c) {
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }  // (its sum is 0, or NaN)
 __device__ __forceinline__ float inverse_of(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
+// A row's sum over a split of its keys, block by block, and what its roundings have left out so far: the split may be the whole
+// cache, and where one key's weight stands out over thousands of equal ones each addition would be off the same way (2.4e-4 of the
+// sum after 32768 addends).  A block's exponentials are added in pairs.
+struct LongSum {
+    float sum = 0.f, rest = 0.f;
+    __device__ __forceinline__ void add(float scale, float x) {  // the sum so far times `scale`, and x
+#pragma clang fp contract(off)
+        const float l = sum * scale, y = x + rest * scale;
+        sum = l + y;
+        rest = y - (sum - l);
+    }
+};
+template <int N>
+__device__ __forceinline__ float sum_pairs(float (&x)[N]) {
+#pragma unroll
+    for (int o = N / 2; o; o >>= 1)
+#pragma unroll
+        for (int e = 0; e < o; e++) x[e] += x[e + o];
+    return x[0];
+}
+
 // Where the statistics of a request's rows of kv head kh begin.
 __device__ __forceinline__ size_t stat_at(const WeightArgs& a, const Req& rq, const Seen& ob, int kh) {
     return (size_t)(rq.q0 + ob.t0) * a.HQ + (size_t)kh * ob.n * a.G;
@@ -169,9 +190,10 @@ __device__ __forceinline__ void few_scores(const T* __restrict__ Q, const T* __r
     int ids = cnt ? entries(0) : 0, ids2 = cnt > 64 ? entries(64) : 0;
     // rows of K in the order in which a lane's 8 scores are 8 keys on end: j0 + 8 fg + e
     const uint32_t kofs = ((8 * (fq >> 2) + (fq & 3)) * 32 + fg * 8) * 2;
-    float m[NR], l[NR];
+    float m[NR];
+    LongSum l[NR];
 #pragma unroll
-    for (int u = 0; u < NR; u++) m[u] = -INFINITY, l[u] = 0.f;
+    for (int u = 0; u < NR; u++) m[u] = -INFINITY;
     struct Blk {
         u32x4 k[2][NS];
         bool there;
@@ -219,10 +241,11 @@ __device__ __forceinline__ void few_scores(const T* __restrict__ Q, const T* __r
 #pragma unroll
             for (int e = 0; e < 8; e++) mn = fmaxf(mn, s2[u][e >> 2][e & 3]);
             const float base = base_of(mn);
-            float sum = l[u] * exp2_fast(m[u] - base);
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum += exp2_fast(s2[u][e >> 2][e & 3] - base);
-            m[u] = mn, l[u] = sum;
+            for (int e = 0; e < 8; e++) x[e] = exp2_fast(s2[u][e >> 2][e & 3] - base);
+            l[u].add(exp2_fast(m[u] - base), sum_pairs(x));
+            m[u] = mn;
         }
     };
     Blk set[D];
@@ -248,7 +271,7 @@ __device__ __forceinline__ void few_scores(const T* __restrict__ Q, const T* __r
 #pragma unroll
     for (int u = 0; u < NR; u++) {
         const float mx = max_quarters(m[u]);
-        float sum = l[u] * part_weight(m[u], mx);
+        float sum = l[u].sum * part_weight(m[u], mx);
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         if (fg == 0) Ms[wv * R + 16 * u + fq] = mx, Ls[wv * R + 16 * u + fq] = sum;
@@ -603,7 +626,8 @@ __global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const T8*>(q + 16 * s);
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;
+    LongSum l;
     auto turn = [&](int i, const uint8_t* K, uint8_t* Kx) INL {
         wait_loads<vmcnt_imm((NB - 2) * IW)>();
         lds_barrier();  // block i is there for every wave, the one before is done with
@@ -627,16 +651,17 @@ __global__ __launch_bounds__(256, 4) void k_weights_rows(const T* __restrict__ Q
 #pragma unroll
         for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
         const float mn = fmaxf(m, top), base = base_of(mn);
-        float sum = l * exp2_fast((m - base) * a.c);
+        float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) sum += exp2_fast((s[e] - base) * a.c);
-        m = mn, l = sum;
+        for (int e = 0; e < 16; e++) x[e] = exp2_fast((s[e] - base) * a.c);
+        l.add(exp2_fast((m - base) * a.c), sum_pairs(x));
+        m = mn;
     };
     RING_START(K, fetch)
     RING_LOOP(K, nb)
     wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
     const float mx = max_halves(m);
-    float sum = l * part_of(m, mx, a.c);
+    float sum = l.sum * part_of(m, mx, a.c);
     sum += __shfl_xor(sum, 32);
     if (!live || g || w0 + c >= t.r1) return;
     if (a.ks == 1) a.stat[stat_at(a, t.rq, t.ob, kh) + r] = make_float2(base_of(mx), inverse_of(sum));

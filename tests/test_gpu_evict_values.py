@@ -96,3 +96,40 @@ def test_scores_around_2_to_23(sdamd, old, n, hq, hd, rising):
     # within 2 steps, in numerator and sum; sums of kv keys and of the rows, and a few more
     rel = 2 * (34 * 3 * math.log(2) + 2) + kv + n * hq + 16
     assert ((weights_of(s, 0)[:, 0] - want[0]).abs() <= rel * er.E32 * want[0] + 2.0 ** -126).all()
+
+
+# ---- long sums -------------------------------------------------------------------------------------
+
+def one_key_stands_out(sdamd, old, new, hq, hk, hd, at, depth, score, **kw):
+    """Request `at` has one key of score x and others of 0: each row's sum is 1 and e^-x for every other key that it sees."""
+    s = Step(5, old, new, hq, hk, hd, 128, "f16", decay=0.0, scale=0.125)
+    keys = [torch.zeros(kv, hk, hd) for kv in s.kv]
+    keys[at][0, :, 0] = 1.0
+    q = torch.zeros(s.T, hq, hd)
+    q[..., 0] = 8.0 * score
+    given(s, keys, q)
+    s.run(sdamd, **kw)
+    j = np.arange(s.kv[at])
+    total = np.zeros(len(j))
+    for p in range(old[at], s.kv[at]):
+        total[:p + 1] += hq // hk / (1 + p * math.exp(-score))
+    want = torch.from_numpy(np.where(j == 0, 1.0, math.exp(-score)) * total)[:, None]
+    # an exponent of 1.44 x in base 2 that has 3 roundings, an exponential within 2 steps, in a row's sum and in the weight; a block's sum
+    # in pairs (5), with what the roundings leave out carried along (3), joined (12), a reciprocal, a product; `depth` rows added in turn
+    rel = (2 * (3 * score + 2) + 5 + 3 + 12 + 3 + depth) * er.E32
+    assert ((weights_of(s, at) - want).abs() <= rel * want).all(), float(((weights_of(s, at) - want).abs() / want).max() / er.E32)
+
+
+@pytest.mark.parametrize("hd,score", [(64, 8), (128, 8), (256, 6)])
+def test_long_sums_of_many_rows(sdamd, hd, score):
+    """So many rows that no split of the keys is needed to fill the GPU: 32 thousand of a row's exponentials in one lane's sum."""
+    one_key_stands_out(sdamd, [65536], [2048], 128, 8, hd, 0, 512 + 4, score)  # (parts of 16384 rows, 32 at a time, and the parts)
+
+
+@pytest.mark.parametrize("score", [5, 6, 8, 9, 10])
+def test_long_sums_of_single_tokens(sdamd, score):
+    """So many requests that a head's keys are not split, one of them long."""
+    rng = np.random.default_rng(1)
+    old = rng.integers(0, 50, 1024)
+    old[517] = 70000
+    one_key_stands_out(sdamd, old.tolist(), [1] * 1024, 8, 8, 64, 517, 1, score)
