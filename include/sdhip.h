@@ -396,7 +396,10 @@ int sd_op_page_positions(const void* cu, const void* dropped, int B, int T, cons
  * i32, and what they hold cannot make a kernel leave the given buffers; calls on several streams run at once where they
  * share no output and no workspace. ---- */
 
-/* Workspace of an sd_op_paged_weights call with these sizes, in bytes (0: none). */
+/* Workspace of an sd_op_paged_weights call with these sizes, in bytes (0: none).  Where a request's few rows (up to 32 per kv
+ * head, or single tokens beside chunks) have their keys' scores there, it grows with the bound, whatever the lengths: B times HK
+ * times the rows per kv head times max_kv times 4 bytes, 67 MB for 16 requests, 8 kv heads, 8 rows each, under 16384.  The call
+ * takes less, down to one request's (its refusal says how much that is): such requests then go in turn, to the same bits. */
 int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int observers, size_t* bytes,
                            char* err, size_t errlen);
 

@@ -910,7 +910,7 @@ int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK
         const sd::PagedShape s = paged_shape(who, HQ, HK, HD, 32, 1, 0, SD_F16);
         paged_attn_sizes(who, B, T, max_new, max_kv, HQ);
         if (observers < 0) throw sd::Error(who + ": the observers must be at least 1, or 0 for all");
-        *bytes = sd::paged_weights_ws(s, B, T, max_new, max_kv, observers);
+        *bytes = sd::paged_weights_ws(s, B, T, max_new, max_kv, observers).whole;
     });
 }
 
@@ -934,10 +934,12 @@ int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int ma
             throw sd::Error(who + ": the scale must be positive and at most 2.3e38");
         if (!aligned(Q, 16) || !aligned(Kp, 16) || !aligned(ws, 16)) throw sd::Error(who + ": Q, the keys and ws must be aligned to 16 bytes");
         words(who, {table, cu, kv_lens, pos, scores, out, kpos});
-        const size_t marks = (size_t)n_pages * HK * page_size * 4, need = sd::paged_weights_ws(s, B, T, max_new, max_kv, observers);
-        if (need && (!ws || ws_bytes < need))
-            throw sd::Error(who + ": needs a workspace of " + std::to_string(need) + " bytes, got " +
-                            std::to_string(ws ? ws_bytes : 0));
+        const size_t marks = (size_t)n_pages * HK * page_size * 4;
+        const sd::WeightsWs sizes = sd::paged_weights_ws(s, B, T, max_new, max_kv, observers);
+        if (sizes.least && (!ws || ws_bytes < sizes.least))
+            throw sd::Error(who + ": needs a workspace of " + std::to_string(sizes.whole) + " bytes, at least " +
+                            std::to_string(sizes.least) + ", got " + std::to_string(ws ? ws_bytes : 0));
+        const size_t need = std::min(ws_bytes, sizes.whole);
         apart(who,
               {{Q, (size_t)T * HQ * HD * 2}, {Kp, ((size_t)(n_pages - 1) * s.pstride + (size_t)HK * page_size * HD) * 2},
                {table, (size_t)B * max_blocks * 4}, {cu, (size_t)(B + 1) * 4}, {kv_lens, (size_t)B * 4}, {pos, (size_t)T * 4},
@@ -947,7 +949,7 @@ int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int ma
         sd::paged_weights(s, {Q, Kp, static_cast<const int*>(table), max_blocks, static_cast<const int*>(cu),
                               static_cast<const int*>(kv_lens), static_cast<const int*>(pos), B, T, max_new, max_kv, window,
                               observers, scale, decay, static_cast<const float*>(scores), static_cast<float*>(out),
-                              static_cast<int*>(kpos), ws},
+                              static_cast<int*>(kpos), ws, need},
                           static_cast<hipStream_t>(stream));
     });
 }

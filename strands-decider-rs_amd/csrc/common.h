@@ -339,8 +339,12 @@ struct PagedWeights {
     float* out;
     int* kpos;  // null: none
     void* ws;
+    size_t ws_bytes;
 };
-size_t paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers);
+struct WeightsWs {
+    size_t whole, least;  // bytes; with less than the whole, requests of few rows go in turn
+};
+WeightsWs paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers);
 void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st);
 struct PageEvict {
     const float* scores;

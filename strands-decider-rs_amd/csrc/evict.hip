@@ -41,6 +41,7 @@ struct WeightArgs {
     int max_blocks, B, rows, HQ, HK, G, lps, n_pages, max_new, kcap, window, observers;
     int few, few_ks, few_span, rw, kvp;        // rows of a request that the few rows' kernels do; their splits, blocks of 32
                                                // keys in each; rows and keys of a request's scores
+    int first;                                 // request of a launch whose requests are some of all
     int tiles, ks, span;                       // many rows: tiles of rows, their splits, blocks in each;
     int part, parts, units;                    // tokens of a part, parts of a request at most, (key tile, part)s at most
     int ordered;                               // requests by length, the longest first
@@ -51,8 +52,8 @@ struct WeightArgs {
     const float* scores;
     float* out;
     int* kpos;
-    float* S;         // [B][HK][rw][kvp]: c s of the few rows
-    float2* few_ml;   // [B][HK][few_ks][rw]: their maxima and sums
+    float* S;         // [requests of a launch][HK][rw][kvp]: c s of the few rows
+    float2* few_ml;   // [requests of a launch][HK][few_ks][rw]: their maxima and sums
     float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
     float2* stat;     // [rows][HQ], a request's rows kv head by kv head: the maximum, and the whole sum's reciprocal
     float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
@@ -286,12 +287,13 @@ template <class T, int HD, int NR, bool ONCE>
 __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     constexpr int R = 16 * NR;
     __shared__ float Ms[FEW_W * R], Ls[FEW_W * R];
-    const int tid = threadIdx.x, kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = blockIdx.y;
+    const int tid = threadIdx.x, kh = blockIdx.x % a.HK, z = blockIdx.x / a.HK, b = a.first + blockIdx.y;
+    const size_t bh = (size_t)blockIdx.y * a.HK + kh;
     const Few f = few_of(a, b);
     if (f.nrows == 0 || f.nrows > a.few) return;
     const int blk0 = (f.lo >> 5) + z * a.few_span;
     const int blk1 = z + 1 < a.few_ks ? min((f.hi + 31) >> 5, blk0 + a.few_span) : (f.hi + 31) >> 5;
-    few_scores<T, HD, NR, ONCE, FEW_W, HD == 64 ? 4 : HD == 128 ? 3 : 2>(Q, Kp, a, f, b, kh, blk0, blk1, a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp, a.kvp, Ms, Ls);
+    few_scores<T, HD, NR, ONCE, FEW_W, HD == 64 ? 4 : HD == 128 ? 3 : 2>(Q, Kp, a, f, b, kh, blk0, blk1, a.S + bh * a.rw * a.kvp, a.kvp, Ms, Ls);
     __syncthreads();
     if (tid < f.nrows) {
         float mx = -INFINITY, sum = 0.f;
@@ -299,7 +301,7 @@ __global__ __launch_bounds__(64 * FEW_W) void k_weights_few(const T* __restrict_
         for (int w = 0; w < FEW_W; w++) mx = fmaxf(mx, Ms[w * R + tid]);
 #pragma unroll
         for (int w = 0; w < FEW_W; w++) sum += Ls[w * R + tid] * part_weight(Ms[w * R + tid], mx);
-        a.few_ml[(((size_t)b * a.HK + kh) * a.few_ks + z) * a.rw + tid] = make_float2(mx, sum);
+        a.few_ml[(bh * a.few_ks + z) * a.rw + tid] = make_float2(mx, sum);
     }
 }
 
@@ -362,12 +364,13 @@ __device__ __forceinline__ void weigh4(const WeightArgs& a, const Few& f, int j,
 __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     constexpr int PRE = 4;
     __shared__ float2 stat[32];
-    const int tid = threadIdx.x, kh = blockIdx.x % a.HK, b = blockIdx.y;
+    const int tid = threadIdx.x, kh = blockIdx.x % a.HK, b = a.first + blockIdx.y;
+    const size_t bh = (size_t)blockIdx.y * a.HK + kh;
     const int c0 = blockIdx.x / a.HK * 1024, step = gridDim.x / a.HK * 1024;  // (with 8 heads a head's scores stay with one XCD's L2)
     const Few f = few_of(a, b);
     const int nrows = f.nrows;
     if (nrows == 0 || nrows > a.few || c0 >= f.rq.kcap) return;
-    const float* const S = a.S + ((size_t)b * a.HK + kh) * a.rw * a.kvp;
+    const float* const S = a.S + bh * a.rw * a.kvp;
     struct Keys {
         Keys4 k;
         f32x4 x[PRE];  // the scores of the first PRE rows
@@ -384,7 +387,7 @@ __global__ __launch_bounds__(256) void k_weights_few_sum(WeightArgs a) {
     };
     Keys k = load(c0 + 4 * tid);  // (on their way while the rows are joined)
     {
-        const float2* const ml = a.few_ml + ((size_t)b * a.HK + kh) * a.few_ks * a.rw;
+        const float2* const ml = a.few_ml + bh * a.few_ks * a.rw;
         if (nrows <= 4) {
             const float2 st = join_parts<64>(ml + min(tid >> 6, nrows - 1), a.rw, a.few_ks, 1.f);
             if ((tid & 63) == 0) stat[tid >> 6] = st;
@@ -1665,7 +1668,13 @@ struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
     int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0;  // tiles 0: no many rows
     bool once = false, one = false, ordered = false;  // keys read past the last-level cache; k_weights_few_one, by length
-    size_t S = 0, few_ml = 0, ml = 0, stat = 0, col = 0, index = 0;  // floats and ints of the workspace
+    size_t ml = 0, stat = 0, col = 0, index = 0;  // floats and ints of the workspace
+    size_t S = 0, few_ml = 0;                     // and of each request whose few rows' splits run in one launch
+    size_t least() const { return (ml + stat + col + index + S + few_ml) * 4; }  // bytes for one such request, and for B of them
+    size_t whole(int B) const { return (ml + stat + col + index + B * (S + few_ml)) * 4; }
+    int few_at_once(int B, size_t bytes) const {
+        return S ? (int)std::min<size_t>(B, (bytes / 4 - ml - stat - col - index) / (S + few_ml)) : B;
+    }
 };
 
 WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
@@ -1679,9 +1688,6 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
     if (p.few) {
         p.nr = p.few <= 16 ? 1 : 2;
         p.kvp = (int)std::min<long long>((long long)nb * 32, INT_MAX);
-        const int want = std::max(1, std::min(256, 8192 / (B * s.HK)));
-        p.few_span = std::max(FEW_W, (nb + want - 1) / want);
-        p.few_ks = (nb + p.few_span - 1) / p.few_span;
         // One workgroup per head where there are enough of them, or few bytes of keys for each: one launch, and no scores in memory.
         // us in splits and so, at n keys of each request:
         // 2 heads, 256 dims: 300 8.5 7.6, 700 8.1 10.3; 8 heads, 128 dims: 700 8.1 7.4, 1200 8.2 9.2, 2000 8.1 11.8
@@ -1698,11 +1704,14 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         // 64 dims: 128 of 100 to 2000 20.8 23.1, of 500 to 4000 46.9 43.5.  256 dims: 64 of 50 to 300 14.0 14.7, of 1000 to 8100 183
         // 148, 100 of 100 to 1000 40 40, 200 of 100 to 2000 103 118
         p.ordered = p.one && B <= ONE_ORDER && B * s.HK > 256 && each >= (size_t)B * (s.HD * p.nr > 128 ? 8192 : 4096);
-        p.S = p.one ? 0 : (size_t)B * s.HK * p.few * p.kvp;
-        p.few_ml = p.one ? 0 : (size_t)B * s.HK * p.few_ks * p.few * 2;
         p.once = (size_t)B * nb * s.HK * s.HD * 64 > (size_t(256) << 20);
-        if ((long long)B * s.HK * p.few_ks >= 1 << 24)
-            throw Error("sd_op_paged_weights: too many requests and keys for one launch");
+        if (!p.one) {
+            const int want = std::max(1, std::min(256, 8192 / (B * s.HK)));
+            p.few_span = std::max(FEW_W, (nb + want - 1) / want);
+            p.few_ks = (nb + p.few_span - 1) / p.few_span;
+            p.S = (size_t)s.HK * p.few * p.kvp;
+            p.few_ml = (size_t)s.HK * p.few_ks * p.few * 2;
+        }
     }
     if (most > p.few) {
         const long long all = std::min((long long)rows, (long long)B * tokens) * G;  // rows that are counted
@@ -1727,7 +1736,7 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         p.col = p.parts > 1 ? (size_t)p.units * s.HK * KEY_TILE : 0;
         p.index = B > INDEX_B ? 3 * ((size_t)B + 1) : 0;
     }
-    for (size_t* x : {&p.S, &p.few_ml, &p.ml, &p.stat, &p.col, &p.index}) *x = (*x + 3) & ~size_t(3);
+    for (size_t* x : {&p.ml, &p.stat, &p.col, &p.index, &p.S, &p.few_ml}) *x = (*x + 3) & ~size_t(3);
     return p;
 }
 
@@ -1737,14 +1746,15 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     const int G = s.HQ / s.HK;
     float* const ws = static_cast<float*>(a.ws);
     WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, G, log2i(s.PS), s.n_pages, a.max_new,
-                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, p.tiles, p.ks, p.span, p.part,
+                 a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, 0, p.tiles, p.ks, p.span, p.part,
                  p.parts, p.units, p.ordered, 32 / G, 32 % G, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
-    g.S = ws;
-    g.few_ml = reinterpret_cast<float2*>(g.S + p.S);
-    g.ml = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.few_ml) + p.few_ml);
-    g.stat = reinterpret_cast<float2*>(reinterpret_cast<float*>(g.ml) + p.ml);
-    g.col = reinterpret_cast<float*>(g.stat) + p.stat;
+    g.ml = reinterpret_cast<float2*>(ws);
+    g.stat = reinterpret_cast<float2*>(ws + p.ml);
+    g.col = ws + p.ml + p.stat;
     g.index = p.index ? reinterpret_cast<int*>(g.col + p.col) : nullptr;
+    const int at_once = p.few_at_once(a.B, a.ws_bytes);
+    g.S = g.col + p.col + p.index;
+    g.few_ml = reinterpret_cast<float2*>(g.S + at_once * p.S);
     const T *Q = static_cast<const T*>(a.Q), *K = static_cast<const T*>(a.Kp);
     auto launch = [&](auto kernel, dim3 grid, int threads, auto... args) {
         hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, args...);
@@ -1769,8 +1779,13 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
             if (p.one) {
                 hipLaunchKernelGGL((k_weights_few_one<T, HD, NR, ONCE>), dim3(s.HK, a.B), dim3(64 * ONE_W), p.few * p.kvp * 4, st, Q, K, g);
                 launched("paged_weights");
-            } else {
-                launch(k_weights_few<T, HD, NR, ONCE>, dim3(s.HK * p.few_ks, a.B), 64 * FEW_W, Q, K, g);
+                return;
+            }
+            const long long chunks = ((long long)a.max_kv + 1023) / 1024;  // of 1024 keys; at most so many workgroups that each has some
+            for (g.first = 0; g.first < a.B; g.first += at_once) {  // (so many requests in turn as the workspace holds scores for)
+                const int n = std::min(at_once, a.B - g.first);
+                launch(k_weights_few<T, HD, NR, ONCE>, dim3(s.HK * p.few_ks, n), 64 * FEW_W, Q, K, g);
+                launch(k_weights_few_sum, dim3((unsigned)std::min(chunks, std::max(1ll, 16384ll / (s.HK * n))) * s.HK, n), 256, g);
             }
         };
         auto once = [&](auto nr) {
@@ -1779,17 +1794,14 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
         };
         if (p.nr == 1) once(std::integral_constant<int, 1>());
         else once(std::integral_constant<int, 2>());
-        if (p.one) return;
-        const long long chunks = ((long long)a.max_kv + 1023) / 1024;  // of 1024 keys; at most so many workgroups that each has some
-        launch(k_weights_few_sum, dim3((unsigned)std::min(chunks, std::max(1ll, 16384ll / (s.HK * a.B))) * s.HK, a.B), 256, g);
     }
 }
 
 }  // namespace
 
-size_t paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
+WeightsWs paged_weights_ws(const PagedShape& s, int B, int rows, int max_new, int max_kv, int observers) {
     const WeightPlan p = plan_weights(s, B, rows, max_new, max_kv, observers);
-    return (p.S + p.few_ml + p.ml + p.stat + p.col + p.index) * 4;
+    return {p.whole(B), p.least()};
 }
 
 void paged_weights(const PagedShape& s, const PagedWeights& a, hipStream_t st) {

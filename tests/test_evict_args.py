@@ -139,6 +139,23 @@ def test_weights_workspace(sdamd):
             sdamd.paged_weights_ws(*bad)
 
 
+def least_workspace(sdamd, **kw):
+    with pytest.raises(sdamd.EngineError, match="at least [0-9]+, got 16$") as e:
+        sdamd.op_paged_weights(**{**WEIGHTS, **kw, "ws_bytes": 16})
+    return int(str(e.value).split("at least ")[1].split(",")[0])
+
+
+@pytest.mark.parametrize("B,new,max_new", [(1024, 1, 1), (256, 16, 3841), (64, 8, 8)])
+def test_weights_least_workspace(sdamd, B, new, max_new):
+    """The scores of one request under a far bound, where all requests' would be gigabytes."""
+    T, hq, hk, hd, kv = B * new, 32, 8, 128, 131072
+    least = least_workspace(sdamd, B=B, T=T, max_new=max_new, max_kv=kv, HQ=hq, HK=hk, HD=hd, max_blocks=4096)
+    rows = min(new, 8) * 4 if max_new == new else 4
+    one = hk * rows * kv * 4
+    assert one < least < 1.3 * one + T * hq * 16 + (64 << 20)
+    assert sdamd.paged_weights_ws(B, T, max_new, kv, hq, hk, hd) >= B * one
+
+
 EVICT = dict(scores=A, kpos=A + M, table=A + 2 * M, max_blocks=8, kv_lens=A + 3 * M, budgets=A + 4 * M, B=2, max_kv=200, HK=2, page_size=32,
              n_pages=20, sink=0, recent=0, new_lens=A + 5 * M, moves=A + 6 * M, counts=A + 7 * M, ws=A + 8 * M, ws_bytes=1 << 40)
 

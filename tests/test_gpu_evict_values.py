@@ -133,3 +133,28 @@ def test_long_sums_of_single_tokens(sdamd, score):
     old = rng.integers(0, 50, 1024)
     old[517] = 70000
     one_key_stands_out(sdamd, old.tolist(), [1] * 1024, 8, 8, 64, 517, 1, score)
+
+
+# ---- work that is cut ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,max_new,max_kv", [([1] * 40, 1, 20000), ([8] * 20, 8, 9000), ([1] * 30 + [70, 0, 9], 70, 30000)])
+def test_workspaces_that_hold_some_requests(sdamd, new, max_new, max_kv):
+    """With a smaller workspace requests go in turn, to the same bits; nothing behind it is written."""
+    rng = np.random.default_rng(max_kv)
+    old = rng.integers(0, 400, len(new))
+    old[[3, len(new) - 1]] = 8500
+    s = Step(6, old.tolist(), new, 8, 2, 128, 32, "bf16", decay=0.5)
+    kw = dict(max_new=max_new, max_kv=max_kv)
+    want = s.run(sdamd, **kw).clone()
+    s.check()
+    full = s.ws.numel() - 64
+    with pytest.raises(sdamd.EngineError, match="at least") as e:
+        s.run(sdamd, ws=torch.zeros(64, dtype=torch.uint8, device="cuda"), **kw)
+    least = int(str(e.value).split("at least ")[1].split(",")[0])
+    assert 0 < least < full
+    for size in (least, least + 16, (full + least) // 2 & ~15, full - 16):
+        ws = torch.full((size + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+        assert torch.equal(s.run(sdamd, ws=ws, **kw), want)
+        assert (ws[size:] == 0xFF).all()
+    with pytest.raises(sdamd.EngineError, match="at least"):
+        s.run(sdamd, ws=torch.zeros(least + 48, dtype=torch.uint8, device="cuda"), **kw)
