@@ -412,7 +412,8 @@ int sd_op_paged_weights_ws(int B, int T, int max_new, int max_kv, int HQ, int HK
  * adds nothing; where its scores hold NaN or +inf, all keys that it sees become NaN.  Sums have one order: equal calls
  * give equal bits.  out may be scores; other rows of both are left as they are; a row that two of the step's requests share
  * receives either's, or with out = scores both, one decayed.  max_new, max_kv and ws as in sd_op_paged_attention, sized by
- * sd_op_paged_weights_ws. */
+ * sd_op_paged_weights_ws.  A call whose requests could have more than 2^24 tiles of 128 keys under max_kv is refused (with T HQ / HK
+ * up to 16384 rows per kv head: B max_kv of 2^31 and more), unless all have few rows. */
 int sd_op_paged_weights(const void* Q, const void* Kp, const void* table, int max_blocks, const void* cu, const void* kv_lens,
                         const void* pos, int B, int T, int max_new, int max_kv, int HQ, int HK, int HD, int page_size,
                         int n_pages, size_t page_stride, int window, float scale, int observers, float decay,

@@ -44,6 +44,7 @@ struct WeightArgs {
     int first;                                 // request of a launch whose requests are some of all
     int tiles, ks, span;                       // many rows: tiles of rows, their splits, blocks in each;
     int part, parts, units;                    // tokens of a part, parts of a request at most, (key tile, part)s at most
+    int slots;                                 // parts that `col` holds, of each key tile
     int ordered;                               // requests by length, the longest first
     int dt, dg;                                // 32 rows: tokens, and heads besides
     uint32_t magic;  // 2^32 / G and 1 more: x / G is the upper half of a product for x below 2^16
@@ -56,9 +57,9 @@ struct WeightArgs {
     float2* few_ml;   // [requests of a launch][HK][few_ks][rw]: their maxima and sums
     float2* ml;       // [ks][tiles][HK][ROW_TILE]: those of many rows
     float2* stat;     // [rows][HQ], a request's rows kv head by kv head: the maximum, and the whole sum's reciprocal
-    float* col;       // [units][HK][KEY_TILE]: parts of the keys' weights
+    float* col;       // [key tiles][slots][HK][KEY_TILE]: parts of the keys' weights
     int* index;       // [3][B + 1]: the first tile of every request, and how many there are: of rows, of (key tile, part)s, of
-                      // keys.  null: each workgroup finds its own
+                      // keys of requests with several parts.  null: each workgroup finds its own
     // the first key that a row at position p sees
     __device__ __forceinline__ int from(int p) const { return window ? max(p, -1) - window + 1 : 0; }
 };
@@ -697,8 +698,15 @@ __device__ __forceinline__ int key_parts(const WeightArgs& a, int b) {
 __device__ __forceinline__ Tile key_tile(const WeightArgs& a, int x) {
     return tile_of(a, KEY_PARTS, x, [&](int b) { return key_parts(a, b); });
 }
-__device__ __forceinline__ int many_key_tiles(const WeightArgs& a, int b) {
-    return many_rows(a, b) ? key_tiles(a, request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap)) : 0;
+__device__ __forceinline__ int split_key_tiles(const WeightArgs& a, int b) {  // of a request with several parts
+    const Req rq = request(a.cu, a.kv_lens, b, a.rows, a.max_new, a.kcap);
+    const int n = observed(rq, a.observers).n;
+    return n * a.G > a.few && parts_of(a, n) > 1 ? key_tiles(a, rq) : 0;
+}
+// The first of a request's parts in `col`: `parts` for each request, or, where that is more than the step's rows can need, by
+// its first row: two slots per part's tokens, since a request of r > 1 parts' tokens has ceil(r) <= floor(2 r) parts.
+__device__ __forceinline__ int slot_of(const WeightArgs& a, const Req& rq, int b) {
+    return (long long)a.B * a.parts <= a.slots ? b * a.parts : (int)(2 * (unsigned)rq.q0 / (unsigned)a.part);
 }
 // The index: one workgroup.  (Sums are cut at 2^24, which row starts that do not ascend could pass.)
 constexpr int INDEX_T = 1024;
@@ -710,7 +718,7 @@ __global__ __launch_bounds__(INDEX_T) void k_weights_index(WeightArgs a) {
     for (int b = b0; b < b1; b++) {
         own[ROW_TILES] = cut(own[ROW_TILES] + row_tiles(a, b));
         own[KEY_PARTS] = cut(own[KEY_PARTS] + key_parts(a, b));
-        own[KEY_TILES] = cut(own[KEY_TILES] + many_key_tiles(a, b));
+        own[KEY_TILES] = cut(own[KEY_TILES] + split_key_tiles(a, b));
     }
 #pragma unroll
     for (int k = 0; k < 3; k++) {
@@ -731,22 +739,8 @@ __global__ __launch_bounds__(INDEX_T) void k_weights_index(WeightArgs a) {
         for (int k = 0; k < 3; k++) a.index[k * (a.B + 1) + b] = cut(at[k]);
         at[ROW_TILES] = cut(at[ROW_TILES] + row_tiles(a, b));
         at[KEY_PARTS] = cut(at[KEY_PARTS] + key_parts(a, b));
-        at[KEY_TILES] = cut(at[KEY_TILES] + many_key_tiles(a, b));
+        at[KEY_TILES] = cut(at[KEY_TILES] + split_key_tiles(a, b));
     }
-}
-// The number of request b's first one, in find_tile's order: lane by lane, lane l's requests l, l + 64, ...
-__device__ __forceinline__ int first_key_tile(const WeightArgs& a, int b) {
-    if (a.B == 1) return 0;
-    if (a.index) return a.index[KEY_PARTS * (a.B + 1) + b];
-    const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
-    int own = 0, before = 0;
-#pragma unroll 8
-    for (int i = 0; i < per; i++) {
-        const int r = 64 * i + lane, n = key_parts(a, min(r, a.B - 1));
-        before += r < b ? n : 0;
-        own = min(own + (r < a.B ? n : 0), 1 << 24);
-    }
-    return __shfl(lanes_upto(own) - own + before, b & 63);
 }
 // The tokens [lo, hi) of a request that see some key of [j0, j0 + 128).
 __device__ __forceinline__ void tokens_of(const WeightArgs& a, const Req& rq, const Seen& ob, int j0, int& lo, int& hi) {
@@ -795,8 +789,9 @@ __device__ __forceinline__ float sum_rows(const f32x16& acc) {
 // that arrive by LDS DMA, in a ring.  A lane adds its row's weights to its 16 keys' sums, in registers; the 32 lanes meet at the
 // end.  What changes from block to block is scalar: a block's first token and head, and offsets into Q and the statistics.
 // As above 51 us for the prompt and 34 for the long caches; 64 keys a wave (two workgroups on a CU) took 80.  With 256 dims its
-// registers allow three workgroups on a CU.
-template <class T, int HD>
+// registers allow three workgroups on a CU.  LOOP: a workgroup takes several (key tile, part)s; the loop's own registers cost 8 to
+// 10 % of the times above, so calls of few workgroups go without.
+template <class T, int HD, bool LOOP>
 __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T* __restrict__ Q, const T* __restrict__ Kp, WeightArgs a) {
     typedef typename Vec8<T>::type T8;
     typedef Ring<HD> Rg;
@@ -805,134 +800,146 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
     const int kh = blockIdx.x % a.HK;
-    const Tile tl = key_tile(a, blockIdx.x / a.HK);
-    if (tl.b < 0 || tl.x >= a.units) return;  // (as above)
-    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
-    const Seen ob = observed(rq, a.observers);
-    const bool sole = a.parts == 1;  // this workgroup's sums are the keys' weights
-    const int parts = parts_of(a, ob.n), p0 = rq.p0 + ob.t0;
-    const int z = sole ? 0 : tl.i % parts, j0 = (sole ? tl.i : tl.i / parts) * KEY_TILE;
-    int t0, t1;  // the part's tokens that see some of the keys
-    tokens_of(a, rq, ob, j0, t0, t1);
-    t0 = max(t0, z * a.part), t1 = min(t1, sole ? ob.n : (z + 1) * a.part);
-    if (t1 <= t0 && !sole) return;
-    const int nr = max(0, t1 - t0) * a.G, nb = (nr + 31) >> 5;  // rows, and blocks of them
-    const int jw = j0 + 32 * wv, lbpp = a.lps - 5, blk = jw >> 5;
-    const int page = a.table[(size_t)tl.b * a.max_blocks + min(blk >> lbpp, a.max_blocks - 1)];
-    const bool there = jw < rq.kcap && (unsigned)page < (unsigned)a.n_pages;
-    f32x16 acc;
-#pragma unroll
-    for (int e = 0; e < 16; e++) acc[e] = 0.f;
-    if (nb > 0) {
-        u32x4 kf[NS];
-        {
-            const size_t at = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
-            const Rsrc rk = make_rsrc(Kp + at, there ? HD * 64u : 0u);
-#pragma unroll
-            for (int x = 0; x < NS; x++) kf[x] = buf_b128(rk, c * 64 + (2 * (x & 1) + g) * 16, (x >> 1) * 2048);
+    for (int unit = blockIdx.x / a.HK; unit < a.units; unit += gridDim.x / a.HK) {
+        if (LOOP && unit >= (int)gridDim.x / a.HK) lds_barrier();  // (the last one's blocks are done with)
+        const Tile tl = key_tile(a, unit);
+        if (tl.b < 0 || tl.x >= a.units) return;  // (as above)
+        const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+        const Seen ob = observed(rq, a.observers);
+        const int parts = parts_of(a, ob.n), p0 = rq.p0 + ob.t0;
+        const bool sole = parts == 1;  // this workgroup's sums are the keys' weights
+        const int z = sole ? 0 : tl.i % parts, tile = sole ? tl.i : tl.i / parts, j0 = tile * KEY_TILE;
+        const int slot = sole ? 0 : slot_of(a, rq, tl.b) + z;
+        int t0, t1;  // the part's tokens that see some of the keys
+        tokens_of(a, rq, ob, j0, t0, t1);
+        t0 = max(t0, z * a.part), t1 = min(t1, sole ? ob.n : (z + 1) * a.part);
+        if (!sole && (t1 <= t0 || slot >= a.slots)) {  // (slots: row starts that do not ascend)
+            if (LOOP) continue;
+            return;
         }
-        // row 32 i + x of the part is token t + (g0 + x) / G, head (g0 + x) % G, counted from its first token: t tf, g0 gf
-        const uint32_t row = (uint32_t)a.HQ * HD * 2;  // bytes (a part's are fewer than 2^31)
-        const size_t q0 = (size_t)rq.q0 + ob.t0 + t0, left = (a.rows - q0) * row - (size_t)kh * a.G * HD * 2;
-        const Rsrc rs = make_rsrc(Q + (q0 * a.HQ + (size_t)kh * a.G) * HD, (uint32_t)min(left, (size_t)0x7FFFFFFF));
-        const Rsrc rst = make_rsrc(a.stat + stat_at(a, rq, ob, kh) + (size_t)t0 * a.G, (uint32_t)nr * 8);
-        int gf = 0;         // of the block that is fetched next
-        uint32_t qoff = 0;  // its token's rows, in Q
-        const uint32_t piece = (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
-        uint32_t off0, off1;  // of the lane's rows of the two halves of a block, or of the wave's one
-        auto token_of = [&](int x) INL { return a.G == 1 ? (uint32_t)x : __umulhi((uint32_t)x, a.magic); };
-        auto offset = [&](int x) INL {
-            const uint32_t t = token_of(x);
-            return t * row + (x - t * a.G) * (HD * 2) + piece;
-        };
-        auto offsets = [&]() INL {
-            off0 = offset(gf + (IW == 1 ? 16 * (wv & 1) : 0) + (lane >> 2));
-            if (IW > 1) off1 = offset(gf + 16 + (lane >> 2));
-        };
-        offsets();
-        auto fetch = [&](int, uint8_t* buf) INL {  // the next block (rows past the last are other rows, or zeros past Q's end: no matter)
-            if (a.dg) offsets();
+        const int nr = max(0, t1 - t0) * a.G, nb = (nr + 31) >> 5;  // rows, and blocks of them
+        const int jw = j0 + 32 * wv, lbpp = a.lps - 5, blk = jw >> 5;
+        const int page = a.table[(size_t)tl.b * a.max_blocks + min(blk >> lbpp, a.max_blocks - 1)];
+        const bool there = jw < rq.kcap && (unsigned)page < (unsigned)a.n_pages;
+        f32x16 acc;
 #pragma unroll
-            for (int u = 0; u < IW; u++) {
-                const int x = wv * IW + u;  // half x % 2 of dims 32 (x / 2) ..
-                buf_lds16(rs, (u & 1 ? off1 : off0) + qoff, (x >> 1) * 64, buf + x * 1024);  // (a row in range is there whole)
+        for (int e = 0; e < 16; e++) acc[e] = 0.f;
+        if (nb > 0) {
+            u32x4 kf[NS];
+            {
+                const size_t at = there ? (size_t)page * a.pstride + ((size_t)(kh << lbpp) + (blk & ((1 << lbpp) - 1))) * (HD * 32) : 0;
+                const Rsrc rk = make_rsrc(Kp + at, there ? HD * 64u : 0u);
+#pragma unroll
+                for (int x = 0; x < NS; x++) kf[x] = buf_b128(rk, c * 64 + (2 * (x & 1) + g) * 16, (x >> 1) * 2048);
             }
-            qoff += a.dt * row, gf += a.dg;
-            if (gf >= a.G) gf -= a.G, qoff += row;
-            qoff = min(qoff, 0x7FFFFFFFu - 0xFFFFu);  // (blocks past the last)
-        };
-        auto stat = [&](int i) INL { return __builtin_bit_cast(float2, buf_b64(rst, c * 8 + i * 256, 0)); };  // (0 past the last row)
-        float2 st = stat(0);
-        int tb = t0, gb = 0;  // the first row's of the block that is worked on
-        RING_START(Q, fetch)
-        auto turn = [&](int i, const uint8_t* buf, uint8_t* bufx) INL {
-            wait_loads<vmcnt_imm((NB - 2) * IW)>();
-            lds_barrier();
-            const float2 now = st;
-            st = stat(i + 1);
-            fetch(i + NB - 1, bufx);
-            f32x16 s;
+            // row 32 i + x of the part is token t + (g0 + x) / G, head (g0 + x) % G, counted from its first token: t tf, g0 gf
+            const uint32_t row = (uint32_t)a.HQ * HD * 2;  // bytes (a part's are fewer than 2^31)
+            const size_t q0 = (size_t)rq.q0 + ob.t0 + t0, left = (a.rows - q0) * row - (size_t)kh * a.G * HD * 2;
+            const Rsrc rs = make_rsrc(Q + (q0 * a.HQ + (size_t)kh * a.G) * HD, (uint32_t)min(left, (size_t)0x7FFFFFFF));
+            const Rsrc rst = make_rsrc(a.stat + stat_at(a, rq, ob, kh) + (size_t)t0 * a.G, (uint32_t)nr * 8);
+            int gf = 0;         // of the block that is fetched next
+            uint32_t qoff = 0;  // its token's rows, in Q
+            const uint32_t piece = (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+            uint32_t off0, off1;  // of the lane's rows of the two halves of a block, or of the wave's one
+            auto token_of = [&](int x) INL { return a.G == 1 ? (uint32_t)x : __umulhi((uint32_t)x, a.magic); };
+            auto offset = [&](int x) INL {
+                const uint32_t t = token_of(x);
+                return t * row + (x - t * a.G) * (HD * 2) + piece;
+            };
+            auto offsets = [&]() INL {
+                off0 = offset(gf + (IW == 1 ? 16 * (wv & 1) : 0) + (lane >> 2));
+                if (IW > 1) off1 = offset(gf + 16 + (lane >> 2));
+            };
+            offsets();
+            auto fetch = [&](int, uint8_t* buf) INL {  // the next block (rows past the last are other rows, or zeros past Q's end: no matter)
+                if (a.dg) offsets();
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = 0.f;
-#pragma unroll
-            for (int x = 0; x < NS; x++)
-                s = Num<T>::mfma32(__builtin_bit_cast(T8, kf[x]), __builtin_bit_cast(T8, Rg::read(buf, x, c, g)), s);
-            // every row sees every key: the first token's causally, the last one's through the window
-            const bool open = there && jw + 32 <= rq.kcap && 32 * i + 32 <= nr && p0 + tb >= jw + 31 &&
-                              (!a.window || p0 + tb + a.dt + 1 - jw < a.window);
-            if (__builtin_expect(open, 1)) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(exp2_fast((s[e] - now.x) * a.c), now.y, acc[e]);
-            } else {
-                const int p = max(p0 + tb + (int)token_of(gb + c), -1), j = jw + 4 * g;
-                const Within keep(max(a.from(p), 0) - j, there && 32 * i + c < nr ? p - j : -1);
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float w = exp2_fast((s[e] - now.x) * a.c) * now.y;
-                    acc[e] += keep.has(key_of(e)) ? w : 0.f;
+                for (int u = 0; u < IW; u++) {
+                    const int x = wv * IW + u;  // half x % 2 of dims 32 (x / 2) ..
+                    buf_lds16(rs, (u & 1 ? off1 : off0) + qoff, (x >> 1) * 64, buf + x * 1024);  // (a row in range is there whole)
                 }
-            }
-            tb += a.dt, gb += a.dg;
-            if (gb >= a.G) gb -= a.G, tb++;
-        };
-        RING_LOOP(Q, nb)
-        wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
+                qoff += a.dt * row, gf += a.dg;
+                if (gf >= a.G) gf -= a.G, qoff += row;
+                qoff = min(qoff, 0x7FFFFFFFu - 0xFFFFu);  // (blocks past the last)
+            };
+            auto stat = [&](int i) INL { return __builtin_bit_cast(float2, buf_b64(rst, c * 8 + i * 256, 0)); };  // (0 past the last row)
+            float2 st = stat(0);
+            int tb = t0, gb = 0;  // the first row's of the block that is worked on
+            RING_START(Q, fetch)
+            auto turn = [&](int i, const uint8_t* buf, uint8_t* bufx) INL {
+                wait_loads<vmcnt_imm((NB - 2) * IW)>();
+                lds_barrier();
+                const float2 now = st;
+                st = stat(i + 1);
+                fetch(i + NB - 1, bufx);
+                f32x16 s;
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+                for (int x = 0; x < NS; x++)
+                    s = Num<T>::mfma32(__builtin_bit_cast(T8, kf[x]), __builtin_bit_cast(T8, Rg::read(buf, x, c, g)), s);
+                // every row sees every key: the first token's causally, the last one's through the window
+                const bool open = there && jw + 32 <= rq.kcap && 32 * i + 32 <= nr && p0 + tb >= jw + 31 &&
+                                  (!a.window || p0 + tb + a.dt + 1 - jw < a.window);
+                if (__builtin_expect(open, 1)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(exp2_fast((s[e] - now.x) * a.c), now.y, acc[e]);
+                } else {
+                    const int p = max(p0 + tb + (int)token_of(gb + c), -1), j = jw + 4 * g;
+                    const Within keep(max(a.from(p), 0) - j, there && 32 * i + c < nr ? p - j : -1);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float w = exp2_fast((s[e] - now.x) * a.c) * now.y;
+                        acc[e] += keep.has(key_of(e)) ? w : 0.f;
+                    }
+                }
+                tb += a.dt, gb += a.dg;
+                if (gb >= a.G) gb -= a.G, tb++;
+            };
+            RING_LOOP(Q, nb)
+            wait_loads<vmcnt_imm(0)>();  // (no DMA outlives the workgroup whose LDS it writes)
+        }
+        const float w = sum_rows(acc);
+        const int x = key_of(c >> 1) + 4 * g, j = jw + x;
+        if (!(c & 1)) {
+            if (!sole) a.col[(((size_t)tile * a.slots + slot) * a.HK + kh) * KEY_TILE + 32 * wv + x] = w;
+            else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
+        }
+        if (!LOOP) return;
     }
-    const float w = sum_rows(acc);
-    const int x = key_of(c >> 1) + 4 * g, j = jw + x;
-    if (c & 1) return;
-    if (!sole) a.col[((size_t)tl.x * a.HK + kh) * KEY_TILE + 32 * wv + x] = w;
-    else if (there && j < rq.kcap) put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
 }
 
 // Adds up the parts of 128 keys, in their order: every fourth by a group of 128 threads, then the groups' sums.  (64 parts of
 // 4096 keys, 2 heads: 5.3 us; by one group 6.5)
 constexpr int SUM_G = 4;
-__global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a) {
+__global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a, int units) {
     __shared__ float part[SUM_G][KEY_TILE];
     const int kh = blockIdx.x % a.HK, i = threadIdx.x % KEY_TILE, grp = threadIdx.x / KEY_TILE;
-    const Tile tl = tile_of(a, KEY_TILES, blockIdx.x / a.HK, [&](int b) { return many_key_tiles(a, b); });
-    if (tl.b < 0) return;
-    const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
-    const Seen ob = observed(rq, a.observers);
-    const int parts = parts_of(a, ob.n), j0 = tl.i * KEY_TILE, j = j0 + i;
-    const int first = first_key_tile(a, tl.b) + tl.i * parts;
-    if (first < 0 || first + parts > a.units) return;
-    const int page = a.table[(size_t)tl.b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
-    int t0, t1;
-    tokens_of(a, rq, ob, j0, t0, t1);
-    float w = 0.f;
-    const float* const col = a.col + ((size_t)first * a.HK + kh) * KEY_TILE + i;
-    if (t1 > t0) {
+    for (int unit = blockIdx.x / a.HK; unit < units; unit += gridDim.x / a.HK) {
+        const Tile tl = tile_of(a, KEY_TILES, unit, [&](int b) { return split_key_tiles(a, b); });
+        if (tl.b < 0) return;
+        const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
+        const Seen ob = observed(rq, a.observers);
+        const int parts = parts_of(a, ob.n), j0 = tl.i * KEY_TILE, j = j0 + i, slot = slot_of(a, rq, tl.b);
+        if (slot + parts > a.slots) continue;  // (row starts that do not ascend)
+        const int page = a.table[(size_t)tl.b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
+        int t0, t1;
+        tokens_of(a, rq, ob, j0, t0, t1);
+        float w = 0.f;
+        const float* const col = a.col + (((size_t)tl.i * a.slots + slot) * a.HK + kh) * KEY_TILE + i;
+        if (t1 > t0) {
 #pragma unroll 8
-        for (int z = t0 / a.part + grp; z <= (t1 - 1) / a.part; z += SUM_G) w += col[(size_t)z * a.HK * KEY_TILE];
-    }
-    part[grp][i] = w;
-    __syncthreads();
-    if (grp || j >= rq.kcap || (unsigned)page >= (unsigned)a.n_pages) return;
+            for (int z = t0 / a.part + grp; z <= (t1 - 1) / a.part; z += SUM_G) w += col[(size_t)z * a.HK * KEY_TILE];
+        }
+        part[grp][i] = w;
+        __syncthreads();
+        if (!grp && j < rq.kcap && (unsigned)page < (unsigned)a.n_pages) {
 #pragma unroll
-    for (int g = 1; g < SUM_G; g++) w += part[g][i];
-    put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
+            for (int g = 1; g < SUM_G; g++) w += part[g][i];
+            put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
+        }
+        __syncthreads();
+    }
 }
 
 // ---- the rows that go -----------------------------------------------------------------------------------------------
@@ -1663,10 +1670,16 @@ __global__ __launch_bounds__(256) void k_paged_move(const int* __restrict__ move
 // 134 94, 8192 4020 768; 16 on 2000 keys, 32 and 8 heads: 128 requests 247 236, 256 522 477, 1024 2415 1790)
 constexpr int INDEX_B = 128;
 
+// Workgroups of a pass over keys from which on 8192 take several (key tile, part)s each, so that bounds far above the lengths cost
+// little.  (us so, and with a workgroup for each, 8 heads of 128 dims: 64 requests of 20 new rows on 300 keys under 32768 45 104;
+// 200, one of them 600 rows on 20000 keys, under 131072 486 897; 256, one of 3841 rows 2468 2890; where nearly all have work, 100
+// requests of 20 rows on 16000 keys, 1650 1615)
+constexpr int LOOP_FROM = 131072, LOOP_WGS = 8192;
+
 // How a call runs, from its sizes alone (the lengths themselves are on the device).
 struct WeightPlan {
     int nr = 0, few = 0, few_ks = 1, few_span = 1, kvp = 0;  // nr: 16-row groups of k_weights_few, 0: not launched
-    int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0;  // tiles 0: no many rows
+    int tiles = 0, ks = 1, span = 1, part = 1, parts = 1, units = 0, slots = 0;  // tiles 0: no many rows
     bool once = false, one = false, ordered = false;  // keys read past the last-level cache; k_weights_few_one, by length
     size_t ml = 0, stat = 0, col = 0, index = 0;  // floats and ints of the workspace
     size_t S = 0, few_ml = 0;                     // and of each request whose few rows' splits run in one launch
@@ -1728,12 +1741,13 @@ WeightPlan plan_weights(const PagedShape& s, int B, int rows, int max_new, int m
         p.part = (int)std::min<long long>(p.part, std::max(1ll, (1ll << 29) / ((long long)s.HQ * s.HD)));
         p.parts = (tokens + p.part - 1) / p.part;
         const long long units = (long long)nkb * std::min(reqs * p.parts, all / G / p.part + reqs);
-        if (units * s.HK >= 1 << 24 || (long long)(p.tiles | 1) * s.HK * std::max(p.ks, 32) >= 1 << 24)
+        if (units >= 1 << 24 || (long long)(p.tiles | 1) * s.HK * (p.ks > 1 ? std::max(p.ks, 32) : 1) >= 1 << 24)
             throw Error("sd_op_paged_weights: too many rows and keys for one launch");
         p.units = (int)units;
+        p.slots = p.parts == 1 ? 0 : (int)std::min((long long)B * p.parts, B == 1 ? p.parts : 2ll * rows / p.part);
         p.ml = p.ks > 1 ? (size_t)p.ks * p.tiles * s.HK * ROW_TILE * 2 : 0;
         p.stat = (size_t)rows * s.HQ * 2;
-        p.col = p.parts > 1 ? (size_t)p.units * s.HK * KEY_TILE : 0;
+        p.col = (size_t)p.slots * nkb * s.HK * KEY_TILE;
         p.index = B > INDEX_B ? 3 * ((size_t)B + 1) : 0;
     }
     for (size_t* x : {&p.ml, &p.stat, &p.col, &p.index, &p.S, &p.few_ml}) *x = (*x + 3) & ~size_t(3);
@@ -1747,7 +1761,7 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
     float* const ws = static_cast<float*>(a.ws);
     WeightArgs g{a.table, a.cu, a.kv_lens, a.pos, a.max_blocks, a.B, a.rows, s.HQ, s.HK, G, log2i(s.PS), s.n_pages, a.max_new,
                  a.max_kv, a.window, a.observers, p.few, p.few_ks, p.few_span, p.few, p.kvp, 0, p.tiles, p.ks, p.span, p.part,
-                 p.parts, p.units, p.ordered, 32 / G, 32 % G, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
+                 p.parts, p.units, p.slots, p.ordered, 32 / G, 32 % G, (uint32_t)((1ull << 32) / G + 1), a.scale * LOG2E, a.decay, s.pstride, a.scores, a.out, a.kpos};
     g.ml = reinterpret_cast<float2*>(ws);
     g.stat = reinterpret_cast<float2*>(ws + p.ml);
     g.col = ws + p.ml + p.stat;
@@ -1761,15 +1775,19 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
         launched("paged_weights");
     };
     if (p.tiles) {
-        const dim3 rows((p.tiles | 1) * s.HK * p.ks), keys(p.units * s.HK);
+        const int looping = std::max(1, LOOP_WGS / s.HK);  // workgroups of a head
+        const bool loop = (long long)p.units * s.HK >= LOOP_FROM;
+        const dim3 rows((p.tiles | 1) * s.HK * p.ks), keys((loop ? looping : p.units) * s.HK);
         if (p.index) launch(k_weights_index, dim3(1), INDEX_T, g);
         launch(k_weights_rows<T, HD>, rows, 256, Q, K, g);
         if (p.ks > 16) launch(k_weights_join<64>, dim3(p.tiles * s.HK * (ROW_TILE / 4)), 256, g);
         else if (p.ks > 1) launch(k_weights_join<8>, dim3(p.tiles * s.HK * (ROW_TILE / 32)), 256, g);
-        launch(k_weights_keys<T, HD>, keys, 256, Q, K, g);
+        if (loop) launch(k_weights_keys<T, HD, true>, keys, 256, Q, K, g);
+        else launch(k_weights_keys<T, HD, false>, keys, 256, Q, K, g);
         if (p.parts > 1) {
-            const long long reqs = std::min<long long>(a.B, p.tiles), nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
-            launch(k_weights_sum, dim3((unsigned)std::min<long long>(reqs * nkb, p.units) * s.HK), SUM_G * KEY_TILE, g);
+            const long long nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
+            const int tiles = (int)std::min<long long>(std::min(a.B, p.slots) * nkb, p.units);
+            launch(k_weights_sum, dim3(std::min(tiles, 2 * looping) * s.HK), SUM_G * KEY_TILE, g, tiles);
         }
     }
     if (p.nr) {

@@ -156,6 +156,25 @@ def test_weights_least_workspace(sdamd, B, new, max_new):
     assert sdamd.paged_weights_ws(B, T, max_new, kv, hq, hk, hd) >= B * one
 
 
+def test_weights_workspace_of_parts(sdamd):
+    """A chunk in several parts beside single tokens: slots for its parts alone, whatever the requests."""
+    sizes = dict(T=8447, max_new=8192, max_kv=131072, HQ=32, HK=8, HD=128, max_blocks=4096)
+    few = [least_workspace(sdamd, B=b, **sizes) for b in (2, 256, 1024)]
+    assert max(few) < min(few) + (8 << 20) and max(few) < 120 << 20
+
+
+@pytest.mark.parametrize("B,T,max_new,max_kv,ok", [(2048, 8192, 4096, 131072, True), (8192, 16000, 100, 262016, True), (8192, 16000, 100, 262144, False), (8192, 16000, 100, 1 << 20, False),
+                                                   (8192, 8192, 1, 1 << 20, True), (1, 4096, 4096, (1 << 31) - 128, True), (2, 4096, 4096, (1 << 31) - 1, False)])
+def test_weights_largest(sdamd, B, T, max_new, max_kv, ok):
+    """Requests times tiles of keys that a call takes: below 2^24."""
+    call = lambda: sdamd.paged_weights_ws(B, T, max_new, max_kv, 32, 8, 128)
+    if ok:
+        assert call() > 0
+    else:
+        with pytest.raises(sdamd.EngineError, match="too many rows and keys"):
+            call()
+
+
 EVICT = dict(scores=A, kpos=A + M, table=A + 2 * M, max_blocks=8, kv_lens=A + 3 * M, budgets=A + 4 * M, B=2, max_kv=200, HK=2, page_size=32,
              n_pages=20, sink=0, recent=0, new_lens=A + 5 * M, moves=A + 6 * M, counts=A + 7 * M, ws=A + 8 * M, ws_bytes=1 << 40)
 

@@ -158,3 +158,62 @@ def test_workspaces_that_hold_some_requests(sdamd, new, max_new, max_kv):
         assert (ws[size:] == 0xFF).all()
     with pytest.raises(sdamd.EngineError, match="at least"):
         s.run(sdamd, ws=torch.zeros(least + 48, dtype=torch.uint8, device="cuda"), **kw)
+
+
+def spotted(sdamd, old, new, hq, hk, hd, depth, ps=128, **kw):
+    """Keys of scores 0 to 3, each head's its own: every weight follows from running sums, and a key that is left out, counted twice or
+    taken for another moves all of a row's."""
+    s = Step(8, old, new, hq, hk, hd, ps, "f16", decay=0.0, scale=0.125)
+    rng = np.random.default_rng(len(old) + sum(new))
+    levels = [rng.integers(0, 4, (kv, hk)) for kv in s.kv]
+    keys = []
+    for x in levels:
+        k = torch.zeros(len(x), hk, hd)
+        k[:, :, 0] = torch.from_numpy(x)
+        keys.append(k)
+    q = torch.zeros(max(s.T, 1), hq, hd)
+    q[..., 0] = 8.0
+    given(s, keys, q)
+    s.run(sdamd, **kw)
+    # as above: exponents of 4.3 at most
+    rel = (2 * (3 * 3 + 2) + 5 + 3 + 12 + 3 + depth) * er.E32
+    for b, (o, n, x) in enumerate(zip(old, new, levels)):
+        if n == 0:
+            continue
+        e = np.exp(x.astype(np.float64))
+        each = hq / hk / np.cumsum(e, 0)[o:]  # of the rows, one by one
+        rest = np.cumsum(each[::-1], 0)[::-1]
+        want = torch.from_numpy(e * np.concatenate([np.broadcast_to(rest[:1], (o, hk)), rest]))
+        got = weights_of(s, b)
+        assert ((got - want).abs() <= rel * want).all(), (b, float(((got - want).abs() / want).max() / er.E32), rel / er.E32)
+    return s
+
+
+@pytest.mark.parametrize("old,new,hq,hk,hd,depth", [
+    ([30011, 9000], [1, 1], 8, 2, 128, 4),  # splits
+    ([8000, 5000, 1, 0] * 10, [1] * 40, 16, 8, 64, 2),  # scores in LDS
+    ([30011, 9000], [40, 1], 8, 2, 256, 8),  # tiles of rows in splits, beside a single token
+    ([70000] + [40] * 1023, [1] * 1024, 8, 8, 64, 1),  # more than 64 blocks of a wave
+    ([65536], [2048], 128, 8, 64, 516),  # more than 32 blocks of a tile's split
+    ([500, 3, 0, 80] * 10, [60, 300, 129, 65] * 10, 8, 2, 64, 16),  # requests of several parts, one behind the other
+])
+def test_every_key_counts(sdamd, old, new, hq, hk, hd, depth):
+    spotted(sdamd, old, new, hq, hk, hd, depth)
+
+
+@pytest.mark.parametrize("old,new,hq,depth", [(300000, 40, 8, 4), (266000, 4200, 32, 516)])
+@pytest.mark.parametrize("bound", [None, 2200000])
+def test_more_key_tiles_than_workgroups(sdamd, old, new, hq, depth, bound):
+    """2344 tiles of 8 heads, with one part of the rows and with two; under the far bound a workgroup takes several."""
+    spotted(sdamd, [old], [new], hq, 8, 64, depth, max_kv=bound)
+
+
+def test_chunks_of_many_requests_under_a_far_bound(sdamd):
+    """2048 requests with a few rows each, bounds of 4096 rows and 131072 keys for any of them."""
+    rng = np.random.default_rng(2)
+    old = rng.integers(0, 60, 2048)
+    old[[0, 1000, 2047]] = 1500, 9000, 20000
+    kw = dict(max_new=4096, max_kv=131072)
+    new = rng.integers(1, 8, 2048).tolist()
+    least = 34 * 131072 * 8 * 4 + (64 << 20)
+    spotted(sdamd, old.tolist(), new, 32, 8, 64, 8, ws=torch.zeros(least, dtype=torch.uint8, device="cuda"), **kw)
