@@ -351,7 +351,7 @@ enum { SD_ROPE_HALF = 0, SD_ROPE_PAIRS = 1 };
 enum { SD_ROPE_PLAIN = 0, SD_ROPE_LINEAR = 1, SD_ROPE_BASE = 2, SD_ROPE_PARTS = 3 };
 
 /* freqs [RD/2] f64, on the host: the pairs' frequencies in radians per position.  RD even, 2 to 256 (4 for SD_ROPE_BASE),
- * theta and s at least 1; length, low and high of SD_ROPE_PARTS alone: length > 0, 0 <= low < high.  The calls below take
+ * theta (as scaled, too) and s at least 1 and finite; length, low and high of SD_ROPE_PARTS alone: length > 0, 0 <= low < high.  The calls below take
  * such an array on the device, or any other frequencies. */
 int sd_rope_freqs(int RD, double theta, int scaling, double factor, double length, double low, double high, double* freqs,
                   char* err, size_t errlen);

@@ -813,6 +813,7 @@ int sd_rope_freqs(int RD, double theta, int scaling, double factor, double lengt
         if (scaling == SD_ROPE_PARTS && (!(length > 0) || !std::isfinite(length) || !(low >= 0) || !(high > low) || !std::isfinite(high)))
             throw sd::Error(who + ": scaling in parts needs a length above 0 and 0 <= low < high");
         if (scaling == SD_ROPE_BASE) theta *= std::pow(factor, RD / (RD - 2.0));
+        if (!std::isfinite(theta)) throw sd::Error(who + ": theta scaled by the factor must be finite");
         for (int j = 0; j < RD / 2; j++) {
             double f = std::pow(theta, -2.0 * j / RD);
             if (scaling == SD_ROPE_LINEAR) f /= factor;

@@ -27,6 +27,12 @@ def test_freqs_refuses(sdamd, kw, message):
     refuses(sdamd, sdamd.rope_freqs, dict(RD=64, theta=1e4, scaling=1, factor=2.0), kw, "sd_rope_freqs", message)
 
 
+@pytest.mark.parametrize("rd,theta,factor", [(4, 1e4, 1e160), (64, 1e300, 1e9)])
+def test_freqs_refuses_a_base_past_all_numbers(sdamd, rd, theta, factor):
+    """(All frequencies but the first would be 0.)"""
+    refuses(sdamd, sdamd.rope_freqs, dict(RD=rd, theta=theta, scaling=2, factor=factor), {}, "sd_rope_freqs", "theta scaled")
+
+
 @pytest.mark.parametrize("rd,theta,kw", [
     (64, 1e7, {}), (2, 1e4, {}), (256, 1e6, dict(scaling="linear", factor=8.0)), (24, 1e4, dict(scaling="base", factor=4.0)),
     (4, 1e4, dict(scaling="base", factor=1.0)), (128, 5e5, dict(scaling="parts", factor=8.0, length=8192.0, low=1.0, high=4.0)),
