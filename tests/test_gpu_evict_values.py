@@ -1,5 +1,5 @@
 """The weight that every cached key receives where scores are far from 1, sums are long, and work is cut: keys and rows are
-chosen so that every weight is known."""
+chosen so that every weight is known.  Rows that go among infinite scores.  Calls on two streams at once."""
 import math
 
 import numpy as np
@@ -8,7 +8,7 @@ import torch
 
 import evict_ref as er
 import paged_ref as pr
-from test_gpu_evict import Step
+from test_gpu_evict import KIND, Step, run_evict
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,113 @@ def test_chunks_of_many_requests_under_a_far_bound(sdamd):
     new = rng.integers(1, 8, 2048).tolist()
     least = 34 * 131072 * 8 * 4 + (64 << 20)
     spotted(sdamd, old.tolist(), new, 32, 8, 64, 8, ws=torch.zeros(least, dtype=torch.uint8, device="cuda"), **kw)
+
+
+# ---- rows that go, among infinite scores ------------------------------------------------------------
+
+@pytest.mark.parametrize("n,m", [(2, 1), (300, 40), (5000, 1200), (20000, 3000), (40000, 9000)])
+@pytest.mark.parametrize("sink,recent", [(0, 0), (1, 0), (20, 300), (0, 5000)])
+def test_protected_rows_come_before_infinite_scores(sdamd, n, m, sink, recent):
+    """Protected rows, then +inf, then numbers, -inf, NaN: with more protected and infinite rows than the budget, too."""
+    rng = np.random.default_rng(n + sink + recent)
+    ps, hk = 128, 2
+    table, n_pages = pr.tables(rng, [n], ps)
+    scores = rng.choice(np.array([math.inf, math.inf, 1.0, 2.0, -math.inf, math.nan], np.float32), (n_pages, hk, ps))
+    kpos = rng.integers(0, 2 * n, (n_pages, hk, ps)).astype(np.int32)
+    new, moves, counts = run_evict(sdamd, torch.from_numpy(scores).cuda(), torch.from_numpy(kpos).cuda(), table, [n], [m], hk, ps, n_pages, sink, recent)
+    assert new == [m]
+    j = np.arange(n)
+    for h in range(hk):
+        x, p = scores[table[0, j // ps], h, j % ps].astype(np.float64), kpos[table[0, j // ps], h, j % ps]
+        safe = (p < sink) | (p > int(p.max()) - recent)
+        order = np.lexsort((j, -np.nan_to_num(x, nan=0.0, posinf=math.inf, neginf=-math.inf), np.where(safe, 0, np.where(np.isnan(x), 2, 1))))
+        # (nothing else decides between protected rows, or between NaN, than their order)
+        order = np.concatenate([j[safe], order[~safe[order] & ~np.isnan(x[order])], j[~safe & np.isnan(x)]])
+        kept = np.zeros(n, bool)
+        kept[order[:m]] = True
+        want = np.stack([j[:m][~kept[:m]], j[m:][kept[m:]]], 1)
+        assert counts[0, h] == len(want) and (moves[0, h, :len(want)] == want).all()
+
+
+# ---- calls on two streams at once -------------------------------------------------------------------
+
+def on_two_streams(calls, outs, again):
+    """calls[i](stream) fills outs[i]; each of them in turn on a stream of its own, without a wait between, ends as it does alone."""
+    want = []
+    for call, out in zip(calls, outs):
+        again()
+        torch.cuda.synchronize()
+        call(None)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in out])
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        again()
+        for st in streams:
+            st.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):  # (each call's outputs are the same every time)
+            for call, st in zip(calls, streams):
+                call(st.cuda_stream)
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
+@pytest.mark.parametrize("new,old", [(([1, 1], [31, 1]), [4000, 900]), (([60, 1], [200, 90]), [9000, 3000]), (([1] * 40, [1] * 40), [2000] * 40)])
+def test_weights_on_two_streams(sdamd, new, old):
+    steps = [Step(30 + i, old, n, 8, 2, 128, 64, "f16") for i, n in enumerate(new)]
+    outs, calls = [], []
+    for s in steps:
+        s.run(sdamd)
+        s.check()
+        outs.append([s.out, s.kpos])
+
+        def call(stream, s=s):
+            B = len(s.old)
+            sdamd.op_paged_weights(s.q.data_ptr(), s.cache.k.data_ptr(), s.dtable.data_ptr(), s.dtable.shape[1], s.cu.data_ptr(), s.lens.data_ptr(), B,
+                                   s.T, max(s.new), max(s.kv), s.hq, s.hk, s.hd, s.ps, s.n_pages, s.scores.data_ptr(), s.out.data_ptr(),
+                                   s.ws.data_ptr(), s.ws.numel(), KIND[s.kind], pos=s.pos.data_ptr(), kpos=s.kpos.data_ptr(), stream=stream)
+
+        calls.append(call)
+
+    def again():
+        for s in steps:
+            s.out.fill_(-7.0), s.kpos.fill_(-9), s.ws.fill_(0xFF)
+
+    on_two_streams(calls, outs, again)
+
+
+@pytest.mark.parametrize("n", [3000, 40000])
+def test_eviction_and_moves_on_two_streams(sdamd, n):
+    rng = np.random.default_rng(n)
+    ps, hk, hd, m = 64, 2, 64, n // 3
+    i32 = dict(dtype=torch.int32, device="cuda")
+    p = lambda t: t.data_ptr()
+    calls, outs, keep = [], [], []
+    for _ in range(2):
+        table, n_pages = pr.tables(rng, [n, n - 7], ps)
+        tb, kv, budgets = pr.dev(table), pr.dev([n, n - 7]), pr.dev([m, m + 5])
+        scores, kpos = torch.rand(n_pages, hk, ps, device="cuda"), torch.randint(0, n, (n_pages, hk, ps), **i32)
+        first = [torch.randn(n_pages * hk * ps * hd, device="cuda").half() for _ in range(2)]
+        caches = [t.clone() for t in first]
+        out = [torch.zeros(2, **i32), torch.zeros(2, hk, n // 2, 2, **i32), torch.zeros(2, hk, **i32)]
+        ws = torch.zeros(max(sdamd.page_evict_ws(2, n, hk), 16), dtype=torch.uint8, device="cuda")
+        keep.append((out, ws, first, caches))
+
+        def call(stream, tb=tb, kv=kv, budgets=budgets, scores=scores, kpos=kpos, out=out, ws=ws, caches=caches, n_pages=n_pages):
+            sdamd.op_page_evict(p(scores), p(kpos), p(tb), tb.shape[1], p(kv), p(budgets), 2, n, hk, ps, n_pages, 3, 20, p(out[0]), p(out[1]), p(out[2]),
+                                p(ws), ws.numel(), stream=stream)
+            sdamd.op_paged_move(p(out[1]), p(out[2]), p(tb), tb.shape[1], 2, n, hk, hd, ps, n_pages, p(caches[0]), p(caches[1]), None, None, 0, stream=stream)
+
+        calls.append(call)
+        outs.append(out + caches)
+
+    def again():
+        for out, ws, first, caches in keep:
+            ws.fill_(0xFF)
+            for t in out:
+                t.fill_(-4)
+            for a, b in zip(caches, first):
+                a.copy_(b)
+
+    on_two_streams(calls, outs, again)
