@@ -780,6 +780,19 @@ struct HeadRows {
     bool same(const HeadRows& o, int T) const { return p == o.p && (T == 1 || stride == o.stride) && (heads == 1 || step == o.step); }
 };
 
+// Whether rows `s` apart, up to `most` of them either way, bring a head within HD of one that begins d elements on.
+bool rows_meet(long long d, long long s, long long most, int HD) {  // -HD < d + t s < HD for some t
+    auto down = [](long long n, long long by) { return n / by - (n % by < 0); };
+    return std::max(-most, -down(HD - 1 + d, s)) <= std::min(most, down(HD - 1 - d, s));
+}
+// Whether two heads of x overlap.
+bool heads_overlap(const HeadRows& x, int T, int HD) {
+    if ((x.heads > 1 && x.step < (size_t)HD) || (T > 1 && x.stride < (size_t)HD)) return true;
+    for (int h = 1; h < x.heads && T > 1; h++)
+        if (rows_meet(h * (long long)x.step, (long long)x.stride, T - 1, HD)) return true;
+    return false;
+}
+
 // Whether a head of x overlaps one of y.  Both may lie in turn in one buffer, a row's heads behind another's, at one stride.
 bool heads_meet(const HeadRows& x, const HeadRows& y, int T, int HD, size_t size) {
     const Span a = x.span(T, HD, size), b = y.span(T, HD, size);
@@ -789,12 +802,9 @@ bool heads_meet(const HeadRows& x, const HeadRows& y, int T, int HD, size_t size
     const long long s = T > 1 ? (long long)x.stride : 1, most = T - 1;
     const long long wide = (x.heads - 1) * (long long)x.step + HD, wide2 = (y.heads - 1) * (long long)y.step + HD, at = ((apart % s) + s) % s;
     if (T > 1 && wide <= at && at + wide2 <= s) return false;  // (rows side by side)
-    auto down = [](long long n, long long d) { return n / d - (n % d < 0); };
     for (int i = 0; i < x.heads; i++)
-        for (int j = 0; j < y.heads; j++) {  // -HD < d + t s < HD for some t within the rows
-            const long long d = apart + j * (long long)y.step - i * (long long)x.step;
-            if (std::max(-most, -down(HD - 1 + d, s)) <= std::min(most, down(HD - 1 - d, s))) return true;
-        }
+        for (int j = 0; j < y.heads; j++)
+            if (rows_meet(apart + j * (long long)y.step - i * (long long)x.step, s, most, HD)) return true;
     return false;
 }
 
@@ -865,10 +875,7 @@ int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inve
             if (!x.p) continue;
             if (x.stride % 8 || x.step % 8 || x.stride > UINT32_MAX || x.step > UINT32_MAX)
                 throw sd::Error(who + ": strides must be multiples of 8 below 2^32");
-            const size_t wide = (x.heads - 1) * x.step + HD, tall = (T - 1) * x.stride + HD;
-            if ((x.heads > 1 && x.step < (size_t)HD) || (T > 1 && x.stride < (size_t)HD) ||
-                (x.heads > 1 && T > 1 && x.stride < wide && x.step < tall))
-                throw sd::Error(who + ": two heads overlap");
+            if (heads_overlap(x, T, HD)) throw sd::Error(who + ": two heads overlap");
             if (!aligned(x.p, 16)) throw sd::Error(who + ": the rows must be aligned to 16 bytes");
         }
         if (!aligned(freqs, 8) || !aligned(pos, 4)) throw sd::Error(who + ": the frequencies must be aligned to 8 bytes, the positions to 4");

@@ -268,3 +268,18 @@ def test_rows_of_one_buffer(sdamd, layout, t, kind):
         for b in (here, named, out):
             assert torch.equal(rows(b, 0), q1) and torch.equal(rows(b, second), k1)
         assert torch.equal(rows(half, 0), q1) and torch.equal(k2, k1) and torch.equal(rows(half, second), rows(x, second))
+
+
+def test_heads_between_other_rows_heads(sdamd):
+    """Heads two steps apart and rows three: every row's later heads lie between the next row's."""
+    t, heads, hd, rd = 4, 6, 16, 16
+    f, x = freqs_on(er.freqs(rd, 1e4)), torch.randn(2 * hd * (heads - 1) + 3 * hd * (t - 1) + hd, device="cuda")
+    rows = torch.as_strided(x, (2, heads, hd), (3 * hd, 2 * hd, 1)).clone()
+    y, z = torch.zeros(2, heads, hd, device="cuda"), x.clone()
+    sdamd.op_rope(f.data_ptr(), rd, 0, None, 2, hd, x.data_ptr(), 3 * hd, 2 * hd, heads, None, 0, 0, 0, 2, Qo=y.data_ptr())
+    sdamd.op_rope(f.data_ptr(), rd, 0, None, 2, hd, z.data_ptr(), 3 * hd, 2 * hd, heads, None, 0, 0, 0, 2)
+    want, mag = er.rope(rows.cpu().double(), np.arange(2), er.freqs(rd, 1e4), 1.0, "half", False)
+    check_rows(y.cpu(), want, mag, er.freqs(rd, 1e4), np.arange(2), "f32", 1.0)
+    assert torch.equal(torch.as_strided(z, (2, heads, hd), (3 * hd, 2 * hd, 1)), y)
+    with pytest.raises(sdamd.EngineError, match="two heads overlap"):  # (row 2's first head is row 0's fourth)
+        sdamd.op_rope(f.data_ptr(), rd, 0, None, t, hd, x.data_ptr(), 3 * hd, 2 * hd, heads, None, 0, 0, 0, 2)
