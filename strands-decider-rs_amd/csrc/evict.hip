@@ -912,6 +912,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 3 : 4) void k_weights_keys(const T
 // Adds up the parts of 128 keys, in their order: every fourth by a group of 128 threads, then the groups' sums.  (64 parts of
 // 4096 keys, 2 heads: 5.3 us; by one group 6.5)
 constexpr int SUM_G = 4;
+template <bool LOOP>
 __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a, int units) {
     __shared__ float part[SUM_G][KEY_TILE];
     const int kh = blockIdx.x % a.HK, i = threadIdx.x % KEY_TILE, grp = threadIdx.x / KEY_TILE;
@@ -921,7 +922,10 @@ __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a, 
         const Req rq = request(a.cu, a.kv_lens, tl.b, a.rows, a.max_new, a.kcap);
         const Seen ob = observed(rq, a.observers);
         const int parts = parts_of(a, ob.n), j0 = tl.i * KEY_TILE, j = j0 + i, slot = slot_of(a, rq, tl.b);
-        if (slot + parts > a.slots) continue;  // (row starts that do not ascend)
+        if (slot + parts > a.slots) {  // (row starts that do not ascend)
+            if (LOOP) continue;
+            return;
+        }
         const int page = a.table[(size_t)tl.b * a.max_blocks + min(j >> a.lps, a.max_blocks - 1)];
         int t0, t1;
         tokens_of(a, rq, ob, j0, t0, t1);
@@ -938,6 +942,7 @@ __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a, 
             for (int g = 1; g < SUM_G; g++) w += part[g][i];
             put_weight(a, rq, mark_at(page, a.HK, kh, j, a.lps), j, w);
         }
+        if (!LOOP) return;
         __syncthreads();
     }
 }
@@ -1787,7 +1792,8 @@ void weights_as(const PagedShape& s, const PagedWeights& a, hipStream_t st) {
         if (p.parts > 1) {
             const long long nkb = ((long long)a.max_kv + KEY_TILE - 1) / KEY_TILE;
             const int tiles = (int)std::min<long long>(std::min(a.B, p.slots) * nkb, p.units);
-            launch(k_weights_sum, dim3(std::min(tiles, 2 * looping) * s.HK), SUM_G * KEY_TILE, g, tiles);
+            if (tiles > 2 * looping) launch(k_weights_sum<true>, dim3(2 * looping * s.HK), SUM_G * KEY_TILE, g, tiles);
+            else launch(k_weights_sum<false>, dim3(tiles * s.HK), SUM_G * KEY_TILE, g, tiles);
         }
     }
     if (p.nr) {
