@@ -347,7 +347,8 @@ enum { SD_F32 = 2 };
 enum { SD_ROPE_HALF = 0, SD_ROPE_PAIRS = 1 };
 /* How the frequencies f_j = theta^(-2j/RD) are scaled by factor s: not at all; f_j / s; theta s^(RD/(RD-2)) in the place
  * of theta; or f_j (k + (1 - k) / s) with k = (length f_j / (2 pi) - low) / (high - low) within [0, 1]: pairs that make
- * fewer than `low` turns over the trained length are slowed down, those that make more than `high` are left. */
+ * fewer than `low` turns over the trained length are slowed down, those that make more than `high` are left.  (Not a ramp by the
+ * pair's number j between two numbers: frequencies of that, or any other, form are the caller's to make.) */
 enum { SD_ROPE_PLAIN = 0, SD_ROPE_LINEAR = 1, SD_ROPE_BASE = 2, SD_ROPE_PARTS = 3 };
 
 /* freqs [RD/2] f64, on the host: the pairs' frequencies in radians per position.  RD even, 2 to 256 (4 for SD_ROPE_BASE),
@@ -427,6 +428,7 @@ int sd_op_page_evict_ws(int B, int max_kv, int HK, size_t* bytes, char* err, siz
  * m < n <= max_kv, m rows of each kv head: first those whose position is below `sink` or among the latest `recent` (above
  * the head's largest less `recent`), then those of the largest scores; equal ones in row order; NaN, and rows in a hole,
  * come last.  kpos null: positions are row numbers (nothing dropped yet).
+ * (A place below m in a hole counts among those whose rows go; the row that is to move there has no place and is lost.)
  *   new_lens [B]: m where rows go, kv_lens[b] elsewhere
  *   counts   [B][HK], moves [B][HK][max(max_kv / 2, 1)][2]: the head's moves, pairs (place, row): the places below m whose
  *            rows go, ascending, and the rows from m on that stay, ascending; entries behind the count are left as they are

@@ -952,8 +952,9 @@ __global__ __launch_bounds__(SUM_G * KEY_TILE) void k_weights_sum(WeightArgs a, 
 // Of a (request, kv head)'s n rows the m of the highest ranks stay: a rank is 32 bits, its order the scores', protected
 // rows above all.  The m-th is found by digits of 11, 11 and 10 bits from the highest down: a histogram in LDS of the rows
 // whose digits above match, and a scan of its counts.  Rows above that rank stay, and of those that have it the first.
-// Up to 32768 rows one workgroup does it all, with every row's rank in registers, read once.  512 heads of 4113 rows: 11.5 us,
-// 17 MB; a chain of 16 barriers, two workgroups to a CU.
+// Up to 32768 rows one workgroup does it all, with every row's rank in registers, read once.  512 heads of 4113 rows under a
+// bound of 8192, 17 MB without positions: 8.5 us in a row of calls (8.7 with them), 11 to 12 by itself; a chain of 16 barriers, two
+// workgroups to a CU.
 
 // A score's place in the order, ascending: NaN, and a row in a hole, before all numbers; -0 is 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
