@@ -370,8 +370,8 @@ int sd_op_rope_table(const void* freqs, int pairs, double magnitude, const void*
  * freqs [RD/2] f64 on the device), RD even, 2 to 256; `inverse` turns back (-a: with magnitude 1 the inverse, with any the
  * gradient).  Angles in f64, products in f32, rounded once; other dims are copied as they are.  type SD_F16, SD_BF16 or
  * SD_F32.  Qo null: in place, and K in place too; else Qo (and Ko) receive the heads at their own strides: Q's (K's) own rows
- * at the same strides (in place), or rows that overlap no input's.  q's and k's heads that are written may lie in turn in one
- * buffer, at one row stride, but none may overlap another.  All aligned to 16 bytes. */
+ * at the same strides (in place), or heads that overlap no input's.  Heads of several of the four may lie in turn in one buffer, at
+ * one row stride; none that is written may overlap another.  All aligned to 16 bytes. */
 int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inverse, const void* pos, int T, int HD, void* Q,
                size_t q_stride, size_t q_step, int HQ, void* K, size_t k_stride, size_t k_step, int HK, void* Qo,
                size_t qo_stride, size_t qo_step, void* Ko, size_t ko_stride, size_t ko_step, int type, void* stream, char* err,

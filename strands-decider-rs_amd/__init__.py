@@ -580,7 +580,8 @@ def paged_weights_ws(B, T, max_new, max_kv, HQ, HK, HD, observers=0) -> int:
 def op_paged_weights(Q, Kp, table, max_blocks, cu, kv_lens, B, T, max_new, max_kv, HQ, HK, HD, page_size, n_pages, scores, out,
                      ws, ws_bytes, type, decay=1.0, observers=0, window=0, scale=None, pos=None, kpos=None, page_stride=0,
                      stream=None):
-    """sd_op_paged_weights: the attention weight that every cached key receives (scale None: 1/sqrt(HD))."""
+    """sd_op_paged_weights: the attention weight that every cached key receives (scale None: 1/sqrt(HD); ws: what paged_weights_ws
+    says, or less, down to one request's scores)."""
     _call(lib().sd_op_paged_weights, Q, Kp, table, max_blocks, cu, kv_lens, pos, B, T, max_new, max_kv, HQ, HK, HD, page_size,
           n_pages, page_stride, window, HD ** -0.5 if scale is None else scale, observers, decay, scores, out, kpos, ws,
           ws_bytes, type, stream)

@@ -879,13 +879,13 @@ int sd_op_rope(const void* freqs, int RD, double magnitude, int layout, int inve
             if (!aligned(x.p, 16)) throw sd::Error(who + ": the rows must be aligned to 16 bytes");
         }
         if (!aligned(freqs, 8) || !aligned(pos, 4)) throw sd::Error(who + ": the frequencies must be aligned to 8 bytes, the positions to 4");
-        const Span f{freqs, (size_t)RD * 4}, p{pos, (size_t)T * 4}, qs = q.span(T, HD, size), ks = k.span(T, HD, size);
-        // A side is in place where its output is its input; else its output lies apart from both inputs.
+        const Span f{freqs, (size_t)RD * 4}, p{pos, (size_t)T * 4};
+        // A side is in place where its output is its input; else its output's heads lie apart from both inputs'.
         const bool q_here = qo.same(q, T), k_here = ko.same(k, T);
         for (const auto& side : {std::make_pair(qo, q_here), std::make_pair(ko, k_here)}) {
-            const Span out = side.first.span(T, HD, size);
-            if (side.second) apart(who, {f, p}, {out});
-            else apart(who, {qs, ks, f, p}, {out});
+            apart(who, {f, p}, {side.first.span(T, HD, size)});
+            if (!side.second && (heads_meet(side.first, q, T, HD, size) || heads_meet(side.first, k, T, HD, size)))
+                throw sd::Error(who + ": an output overlaps an input");
         }
         if (heads_meet(qo, ko, T, HD, size) || (q_here != k_here && heads_meet(q, k, T, HD, size)))
             throw sd::Error(who + ": a q head overlaps a k head");

@@ -283,3 +283,20 @@ def test_heads_between_other_rows_heads(sdamd):
     assert torch.equal(torch.as_strided(z, (2, heads, hd), (3 * hd, 2 * hd, 1)), y)
     with pytest.raises(sdamd.EngineError, match="two heads overlap"):  # (row 2's first head is row 0's fourth)
         sdamd.op_rope(f.data_ptr(), rd, 0, None, t, hd, x.data_ptr(), 3 * hd, 2 * hd, heads, None, 0, 0, 0, 2)
+
+
+@pytest.mark.parametrize("t", [1, 50])
+def test_outputs_between_the_inputs_rows(sdamd, t):
+    """q, k and both outputs side by side in every row of one buffer."""
+    hq, hk, hd, rd = 3, 2, 64, 64
+    f = freqs_on(er.freqs(rd, 1e4))
+    x = torch.randn(t, 2, hq + hk, hd, device="cuda").half()
+    x[:, 1] = 7.0
+    q, k = (torch.zeros(t, n, hd, device="cuda").half() for n in (hq, hk))
+    first = x[:, 0].clone()
+    row, at = 2 * (hq + hk) * hd, x.data_ptr()
+    args = (f.data_ptr(), rd, 0, None, t, hd, at, row, hd, hq, at + hq * hd * 2, row, hd, hk, 0)
+    sdamd.op_rope(*args, Qo=q.data_ptr(), Ko=k.data_ptr())
+    out = at + (hq + hk) * hd * 2
+    sdamd.op_rope(*args, Qo=out, Ko=out + hq * hd * 2, qo_stride=row, qo_step=hd, ko_stride=row, ko_step=hd)
+    assert torch.equal(x[:, 0], first) and torch.equal(x[:, 1], torch.cat([q, k], 1))
